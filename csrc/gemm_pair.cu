@@ -33,7 +33,7 @@
 // In the reference's place: linear_fp4_fp8 / linear_fp4_mma8 (packages/tilerl-kernels/src/tilerl_kernels/kernels_linear.py:924-1687).
 #include <cuda.h>
 #include "common.cuh"
-#include "tcgen05.cuh"
+#include "tcgen05_pair.cuh"
 #include "gemm_pair.cuh"
 
 namespace {
@@ -74,41 +74,14 @@ struct PairParams {
   int parts;             // pairs that share a tile (a cluster), each a part of K; 1: a pair goes through whole tiles
 };
 
-__device__ __forceinline__ uint32_t gp_map(uint32_t addr, int cta) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
-  return r;
-}
 __device__ __forceinline__ float4 gp_ld_cluster(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-// What a CTA waits for without a limit, and why it ends.  A cluster barrier takes the place of __syncthreads for two to six CTAs
-// that the hardware starts together; shared memory of another CTA may only be touched once one has been passed, and no CTA may
-// leave before the last access to its own, so an mbarrier with a limit can stand in for neither the first nor the last.  Every thread
-// comes to each of them: no path returns early, and all waits in between (the ring, the accumulators, the producers' tail) have
-// a limit, after which they leave their loop.  The allocation of TMEM waits for the other CTA's, right behind the first barrier, and
-// for columns to be free: a CTA leaves too little shared memory on its SM for any other kernel that holds some (each takes
-// 190 KB or more, and gives its columns back on every path).  The release waits for the other CTA's, behind a barrier too.
-// Not the .aligned forms: the warps come here from loops and branches that their lanes left at different times, and a warp
-// that is not converged would count more than once.
-__device__ __forceinline__ void gp_cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-  __syncwarp();
-}
-__device__ __forceinline__ void gp_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void gp_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void gp_commit(uint32_t bar, uint16_t both) {       // on this barrier of both SMs
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"(both) : "memory");
 }
 __device__ __forceinline__ void gp_cp_sf(uint32_t taddr, uint32_t lo, uint32_t hi) {
   asm volatile("{ .reg .b64 d; mov.b64 d, {%1, %2}; tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d; }"

@@ -1,0 +1,410 @@
+// Log-probabilities of given tokens (and entropies) from hidden rows and the head, without the logits: x = h W^T stays in TMEM.
+//
+//   of a tile of 256 rows by 256 words, a row's (m, s[, u]) = (max x, sum e^(x - m)[, sum e^(x - m) (x - m)]), and x[t] where the target is
+//   among them;  then over a row's tiles  M = max m, S = sum s e^(m - M), lp = x[t] - M - log S, entropy = log S - U / S
+//
+// A product of matrices with an epilogue that gives back 8 bytes (12 with entropies) for 128 logits: bound by the tensor cores from a
+// few hundred rows on, by the reading of W below.  Pairs of SMs (`cta_group::2`) share a tile: 128 hidden rows each as the MMA's A, half of the
+// 256 words each as its B, so that a k-block of 64 brings 32 KB to an SM for 512 clocks of MMAs (one SM alone: 48 KB, more than L2
+// gives to all of them).  Two accumulators of 256 columns fill TMEM: a tile's epilogue runs beside the next one's products.  Rows are the
+// TMEM lanes, so a thread has a row's values and no two threads meet.  The tiles go round the pairs words by words over up to 2048
+// rows at a time: pairs that run together read the same words, and W comes from memory once for 2048 rows.
+//
+// Exponentials are ex2.approx of (x - m) log2(e): its 2^-22 and the rounding of far arguments are averages over the words of a row, below
+// fp32's rounding of lp.  (One fused x log2(e) - m log2(e) would carry the rounding of the second product into every word: 1e-6 of lp at
+// logits of 30, infinity at 1e38.)  Sums of a row's tiles are fp32, their logarithm fp64.
+//
+// Only scored rows are worked on: their indices are gathered first, on the device.  Roles (10 warps): warp 0 = TMA producer, warp 1 = TMEM
+// owner and MMA issuer (even SM), warps 2-9 = epilogue, two groups of four with 128 columns each.  Waits: see tcgen05_pair.cuh.
+// In the place of the reference's log-probabilities over full logits (tilerl_kernels/reference.py:1511-1603).
+#include "tcgen05_pair.cuh"
+
+namespace {
+
+constexpr int SC_ROWS = 128, SC_WORDS = 256, SC_KT = 64;       // rows an SM, words a tile, k a stage
+constexpr int SC_THREADS = 320, SC_STAGES = 7, SC_STAGE = 2 * SC_ROWS * SC_KT * 2;
+constexpr int SC_SMEM = SC_STAGES * SC_STAGE + 1024 + 256;
+constexpr int SC_GROUP = 8;                                     // tiles of 256 rows that go through the words together
+static_assert(SC_SMEM >= 208 * 1024 && SC_SMEM <= 227 * 1024, "no other kernel with TMEM fits beside it on an SM");
+constexpr int SC_SITE = 17;                                     // of trl_set_error
+
+struct ScoreArgs {
+  const int* count;            // scored rows, on the device (null: n of them)
+  const int* index;            // of a scored row among all (null: itself)
+  const long long* target;     // of all rows
+  float2* part;                // [n, parts] (m, s)
+  float* part_u;               // [n, parts], or null
+  float* xt;                   // [n]
+  int n, V, nk, v_tiles, parts;
+};
+
+__device__ __forceinline__ void sc_mma(uint32_t d, uint32_t alo, uint32_t blo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 da, db;\n"
+      "  mov.b64 da, {%1, %3}; mov.b64 db, {%2, %3};\n"
+      "  setp.ne.b32 p, %5, 0;\n"
+      "  tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p; }\n"
+      ::"r"(d), "r"(alo), "r"(blo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ float sc_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The tile of unit u: words fastest over rows of a group.
+__device__ __forceinline__ void sc_unit(int u, int r_tiles, int v_tiles, int& rt, int& vt) {
+  const int whole = SC_GROUP * v_tiles, g = u / whole, left = u - g * whole, rows = min(SC_GROUP, r_tiles - g * SC_GROUP);
+  vt = left / rows, rt = g * SC_GROUP + left - vt * rows;
+}
+
+template <bool ENTROPY>
+__global__ void __launch_bounds__(SC_THREADS, 1)
+score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const ScoreArgs p) {
+  constexpr int S = SC_STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * SC_STAGE);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };                              // the even SM's counts both SMs' copies
+  auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * S + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * S + 2 + b); };           // of the even SM: both SMs' epilogue warps
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 16);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  gp_cluster_sync();                                // both CTAs run, before TMEM is asked for
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  gp_cluster_sync();                                // both halves are allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int n = p.count ? min(*p.count, p.n) : p.n, r_tiles = (n + 2 * SC_ROWS - 1) / (2 * SC_ROWS), units = r_tiles * p.v_tiles;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (elect_one()) {
+      const uint32_t smem0 = smem_u32(smem);
+      int st = 0, issued = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs) {
+        int rt, vt;
+        sc_unit(u, r_tiles, p.v_tiles, rt, vt);
+        for (int kt = 0; kt < p.nk; ++kt, ++issued) {
+          if (issued >= S && !(ok = mbar_wait(empty(st), ph ^ 1u, abort_flag))) break;
+          const uint32_t dst = smem0 + (uint32_t)st * SC_STAGE, bar = gp_map(full(st), 0);
+          if (rank == 0) mbar_expect_tx(full(st), 2u * SC_STAGE);
+          gp_load_2d(dst, &map_h, kt * SC_KT, (rt * 2 + rank) * SC_ROWS, bar);
+          gp_load_2d(dst + SC_STAGE / 2, &map_w, kt * SC_KT, vt * SC_WORDS + rank * (SC_WORDS / 2), bar);
+          if (++st == S) st = 0, ph ^= 1u;
+        }
+      }
+      // the last arrivals of the even SM's MMAs on this CTA's barriers, before its memory goes away
+      const int pre = min(S, issued);
+      for (int s = 0; ok && s < pre; ++s) {
+        const int i = issued - pre + s;             // the last use of its stage
+        ok = mbar_wait(empty(i % S), (uint32_t)(i / S) & 1u, abort_flag);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (for both SMs) ----------------
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(SC_WORDS >> 3) << 17) | ((uint32_t)((2 * SC_ROWS) >> 4) << 24);
+      const uint64_t d0 = desc_sw128(smem_u32(smem));
+      const uint32_t lo0 = (uint32_t)d0, hi = (uint32_t)(d0 >> 32);
+      int st = 0, count = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs, ++count) {
+        const int buf = count & 1;
+        if (count >= 2) {
+          if (!(ok = mbar_wait(acc_empty(buf), (uint32_t)((count >> 1) - 1) & 1u, abort_flag))) break;
+          tc_fence_after();
+        }
+        const uint32_t acc = tmem_base + (uint32_t)buf * SC_WORDS;
+        for (int kt = 0; kt < p.nk; ++kt) {
+          if (!(ok = mbar_wait(full(st), ph, abort_flag))) break;
+          tc_fence_after();
+          const uint32_t a = lo0 + (uint32_t)st * (uint32_t)(SC_STAGE >> 4), b = a + (uint32_t)(SC_STAGE / 2 >> 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc_mma(acc, a + i * 2, b + i * 2, hi, idesc, kt || i ? 1u : 0u);
+          gp_commit(empty(st), 3);
+          if (++st == S) st = 0, ph ^= 1u;
+        }
+        if (ok) gp_commit(acc_full(buf), 3);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue (warps 2..9): a thread a row, 128 words ----------------
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    constexpr float L2E = 1.4426950408889634f;
+    const uint32_t even_empty = gp_map(acc_empty(0), 0);
+    int count = 0;
+    for (int u = pair; u < units; u += pairs, ++count) {
+      int rt, vt;
+      sc_unit(u, r_tiles, p.v_tiles, rt, vt);
+      const int buf = count & 1, row = (rt * 2 + rank) * SC_ROWS + quad * 32 + lane, col0 = vt * SC_WORDS + half * (SC_WORDS / 2);
+      const bool mine = row < n;
+      const long long t = mine ? p.target[p.index ? p.index[row] : row] : -1;
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full(buf), (uint32_t)(count >> 1) & 1u, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * SC_WORDS + half * (SC_WORDS / 2));
+      float m = -INFINITY, s = 0.f, w = 0.f;
+#pragma unroll
+      for (int c = 0; c < SC_WORDS / 2; c += 32) {
+        uint32_t r[32];
+        __syncwarp();                               // (the branches below part the lanes)
+        tc_ld32(taddr + (uint32_t)c, r);
+        tc_wait_ld();
+        if (c + 32 == SC_WORDS / 2) {               // read out: the accumulator goes back
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_empty + 8u * buf) : "memory");
+        }
+        if (col0 + c + 32 > p.V) {                  // past the last word
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col0 + c + i >= p.V) r[i] = 0xff800000u;
+        }
+        const long long at = t - col0 - c;
+        if (at >= 0 && at < 32 && t < p.V) {
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (at == i) x = __uint_as_float(r[i]);
+          p.xt[row] = x;
+        }
+        float best = m;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) best = fmaxf(best, __uint_as_float(r[i]));
+        const float base = best == -INFINITY ? 0.f : best;
+        if (best > m) {
+          const float f = sc_exp2((m - base) * L2E);       // (0 for the first)
+          if (ENTROPY) w = s > 0.f ? f * (w + s * (m - base)) : w;
+          s *= f, m = best;
+        }
+        float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float x = __uint_as_float(r[i]) - base, y = __uint_as_float(r[i + 1]) - base, e = sc_exp2(x * L2E), f = sc_exp2(y * L2E);
+          a0 += e, a1 += f;
+          if (ENTROPY) b0 += e > 0.f ? e * x : 0.f, b1 += f > 0.f ? f * y : 0.f;     // (no -inf times 0)
+        }
+        s += a0 + a1;
+        if (ENTROPY) w += b0 + b1;
+      }
+      if (mine) {
+        const size_t o = (size_t)row * p.parts + vt * 2 + half;
+        p.part[o] = make_float2(m, s);
+        if (ENTROPY) p.part_u[o] = w;
+      }
+      __syncwarp();
+    }
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // give copies that are still in flight time to land before the CTAs' memory goes away
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {
+    }
+  }
+  gp_cluster_sync();                                // nothing of the pair is in flight towards the other SM any more
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  gp_cluster_sync();                                // no CTA leaves while the other's half is being given back
+}
+
+// A block a scored row: its tiles together.
+__global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, float* lp, float* entropy) {
+  __shared__ float red[32];
+  const int row = blockIdx.x, n = p.count ? *p.count : p.n;
+  if (row >= n) return;
+  const float2* part = p.part + (size_t)row * p.parts;
+  float m = -INFINITY, s = 0.f, u = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < p.parts; i += 128) m = fmaxf(m, part[i].x);
+  m = block_max(m, red);
+  for (int i = threadIdx.x; i < p.parts; i += 128) {
+    const float2 v = part[i];
+    const float f = expf(v.x - m);
+    s += v.y * f;
+    if (entropy && v.y != 0.f) u += f * (p.part_u[(size_t)row * p.parts + i] + v.y * (v.x - m));
+  }
+  s = block_sum(s, red);
+  if (entropy) u = block_sum(u, red);
+  if (threadIdx.x) return;
+  const int to = p.index ? p.index[row] : row;
+  const long long t = p.target[to];
+  const double log_s = log((double)s);
+  if (t < 0 || t >= p.V) {
+    trl_set_error(TRL_ERR_BOUNDS, SC_SITE, (int)t, p.V);
+    lp[to] = NAN;
+  } else {
+    lp[to] = (float)((double)p.xt[row] - (double)m - log_s);
+  }
+  if (entropy) entropy[to] = (float)(log_s - (double)u / (double)s);
+}
+
+// Indices of the scored rows in order, and their number; results of the others are 0.  One block.
+__global__ void __launch_bounds__(1024) score_rows_kernel(const unsigned char* mask, int n, int* index, int* count, float* lp, float* entropy) {
+  __shared__ int sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += 1024) {
+    const int i = i0 + threadIdx.x;
+    const bool on = i < n && mask[i];
+    if (i < n && !on) {
+      lp[i] = 0.f;
+      if (entropy) entropy[i] = 0.f;
+    }
+    const unsigned vote = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) sums[warp] = __popc(vote);
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
+    }
+    if (on) index[base + before + __popc(vote & ((1u << lane) - 1u))] = i;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+// The scored rows in bf16, one behind the other.
+template <typename T>
+__global__ void __launch_bounds__(256) score_pack_kernel(const T* h, bf16* out, int n, int H, const int* index, const int* count) {
+  const int row = blockIdx.x;
+  if (count && row >= *count) return;
+  const T* src = h + (size_t)(index ? index[row] : row) * H;
+  bf16* dst = out + (size_t)row * H;
+  for (int c = threadIdx.x * 8; c < H; c += 2048) {
+    uint4 v;
+    if (sizeof(T) == 2) {
+      v = *reinterpret_cast<const uint4*>(src + c);
+    } else {
+      const float4 a = reinterpret_cast<const float4*>(src + c)[0], b = reinterpret_cast<const float4*>(src + c)[1];
+      v = make_uint4(f2_to_bf162_bits(a.x, a.y), f2_to_bf162_bits(a.z, a.w), f2_to_bf162_bits(b.x, b.y), f2_to_bf162_bits(b.z, b.w));
+    }
+    *reinterpret_cast<uint4*>(dst + c) = v;
+  }
+}
+
+typedef CUresult (*EncodeTiledFnS)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// [rows, K] bf16, boxes of 64 values x 128 rows; what lies past either end reads as zero
+bool score_map(CUtensorMap* m, const void* base, long rows, long K) {
+  static EncodeTiledFnS encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn) return false;
+    encode = (EncodeTiledFnS)fn;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)K * 2};
+  const cuuint32_t b[2] = {SC_KT, SC_ROWS}, estr[2] = {1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Pairs of SMs that run at a time.
+template <bool ENTROPY>
+int score_pairs() {
+  static TrlPerDevice<int> counts;
+  int& known = counts.here();
+  if (known == 0) {
+    auto kern = score_kernel<ENTROPY>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2), cfg.blockDim = dim3(SC_THREADS), cfg.dynamicSmemBytes = SC_SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SC_SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    known = n > 0 ? n : -1;
+  }
+  return known;
+}
+
+template <bool ENTROPY>
+int score_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& p, cudaStream_t st) {
+  const int most = score_pairs<ENTROPY>();
+  if (most < 1) return (int)cudaErrorInvalidConfiguration;
+  const long units = (long)((p.n + 2 * SC_ROWS - 1) / (2 * SC_ROWS)) * p.v_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)(units < most ? units : most)), cfg.blockDim = dim3(SC_THREADS), cfg.dynamicSmemBytes = SC_SMEM, cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, score_kernel<ENTROPY>, mh, mw, p);
+}
+
+int score_parts(int V) { return (V + SC_WORDS - 1) / SC_WORDS * 2; }
+
+}  // namespace
+
+// Bytes of workspace for n rows (of which the scored ones are gathered, `packed`), a multiple of 256.
+TRL_API long trl_score_workspace(int n, int H, int V, int packed, int entropy) {
+  long b = (long)n * score_parts(V) * (entropy ? 12 : 8) + 4l * n * 2 + 512;
+  if (packed) b += 2l * n * H + 512;
+  return (b + 255) / 256 * 256;
+}
+// h [n, H] (type 0: fp32, 1: bf16), w [V, H] bf16, both contiguous and 16-byte aligned, H % 8 == 0; target int64 [n]; mask bytes [n] or null; lp and entropy
+// (or null) fp32 [n]; n * parts of the words' tiles below 2^31.
+TRL_API int trl_score(const void* h, int type, const void* w, const void* target, const void* mask, int n, int H, int V, void* lp, void* entropy, void* work,
+                      void* stream) {
+  if (n < 1 || V < 1 || H < 8 || H % 8 || ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(work)) & 15))
+    return (int)cudaErrorInvalidValue;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool packed = mask || type == 0;
+  const int v_tiles = (V + SC_WORDS - 1) / SC_WORDS, parts = 2 * v_tiles;
+  if ((long)n * parts >= 1l << 31) return (int)cudaErrorInvalidValue;
+  unsigned char* at = (unsigned char*)work;
+  auto take = [&](long bytes) {
+    void* r = at;
+    at += (bytes + 15) / 16 * 16;
+    return r;
+  };
+  float2* part = (float2*)take(8l * n * parts);
+  float* part_u = entropy ? (float*)take(4l * n * parts) : nullptr;
+  float* xt = (float*)take(4l * n);
+  int* index = mask ? (int*)take(4l * n) : nullptr;
+  int* count = mask ? (int*)take(4) : nullptr;
+  bf16* rows = packed ? (bf16*)take(2l * n * H) : nullptr;
+  if (mask) score_rows_kernel<<<1, 1024, 0, st>>>((const unsigned char*)mask, n, index, count, (float*)lp, (float*)entropy);
+  if (packed) {
+    if (type == 0) score_pack_kernel<float><<<n, 256, 0, st>>>((const float*)h, rows, n, H, index, count);
+    else score_pack_kernel<bf16><<<n, 256, 0, st>>>((const bf16*)h, rows, n, H, index, count);
+  }
+  CUtensorMap mh, mw;
+  if (!score_map(&mh, packed ? rows : h, n, H) || !score_map(&mw, w, V, H)) return (int)cudaErrorInvalidValue;
+  const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, (H + SC_KT - 1) / SC_KT, v_tiles, parts};
+  const int rc = entropy ? score_launch<true>(mh, mw, p, st) : score_launch<false>(mh, mw, p, st);
+  if (rc) return rc;
+  score_join_kernel<<<n, 128, 0, st>>>(p, (float*)lp, (float*)entropy);
+  return (int)cudaGetLastError();
+}

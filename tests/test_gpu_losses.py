@@ -1,0 +1,261 @@
+"""Policy and preference losses on a B200 against their torch form in 64 bits on the CPU."""
+import math
+
+import pytest
+import torch
+
+from tilerl_b200 import tape as T
+from tilerl_b200.ops import native
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+NAN = float("nan")
+
+
+def _inputs(rows, v, dtype, seed, offset=0):
+    """Logits (on the GPU ``offset`` values off a 16-byte boundary), and what goes with them, fp32."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    logits, targets = (r(*rows, v) * 2), torch.randint(0, v, rows, generator=g)
+    logits.scatter_(-1, targets[..., None], math.log(v) + r(*rows, 1))
+    logits = logits.to(dtype)
+    lp = torch.log_softmax(logits.double(), -1).gather(-1, targets[..., None])[..., 0]
+    mask = torch.rand(rows, generator=g) < 0.7
+    mask.view(-1)[0] = True
+    here = torch.empty(logits.numel() + offset, dtype=dtype, device=DEV)[offset:].view(logits.shape).copy_(logits)
+    return logits, here, targets, mask, r(rows[0]), (lp + 0.3 * r(*rows)).float(), (lp + 0.2 * r(*rows)).float()
+
+
+def _adds(v):
+    """fp32 roundings behind a sum of v exponentials: a thread's own sums (no form has fewer than 32 threads a row), the reductions over
+    them, an exponential's own (2 ulp) and its argument's."""
+    return min(v, v / 32 + 80) + 24
+
+
+def _grad_bounds(lg, w, dw, v):
+    """Of a gradient w (p - onehot): the weight's error, the probability's, the products' roundings."""
+    p = torch.softmax(lg.double(), -1)
+    half = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2}[lg.dtype]
+    b = dw[..., None] + w.abs()[..., None] * (p * _adds(v) * 2 ** -24 + 2 ** -22)
+    return b + half * (w.abs()[..., None] * 2 + b)
+
+
+SHAPES = [((1,), 1, 0), ((3,), 2, 1), ((2, 5), 7, 0), ((4, 9), 320, 0), ((3, 3), 1023, 3), ((2, 2), 1024, 0), ((2, 2), 1025, 1), ((5,), 4099, 2), ((2, 3), 16384, 0),
+          ((3,), 16391, 1), ((2, 2), 32768, 0), ((2,), 49999, 1), ((3,), 65540, 2), ((2, 2), 131072, 0), ((3,), 150001, 3), ((2,), 248320, 0), ((2,), 262144, 0), ((2,), 262145, 0),
+          ((2,), 300007, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,v,offset", SHAPES)
+def test_policy_loss(rows, v, offset, dtype):
+    """Vocabularies of every form of the kernels and one value to either side of their borders, rows that begin anywhere, rows that are not scored."""
+    logits, here, targets, mask, adv, old, refs = _inputs(rows, v, dtype, v, offset)
+    before = native.launch_count
+    for kw in (dict(mask=mask, old_logprobs=old, ref_logprobs=refs, kl_coef=0.1, clip_eps_high=0.3), dict(old_logprobs=old), dict(mask=mask)):
+        tape = T.Tape()
+        tape.watch(here)
+        dev = {k: t.to(DEV) if isinstance(t, torch.Tensor) else t for k, t in kw.items()}
+        loss, terms = T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=0.25, **dev)
+        grad = tape.backward(loss)[id(here)].cpu()
+        cpu = T.Tape()
+        wide = logits.double()
+        cpu.watch(wide)
+        want, wants = T.policy_loss(cpu, wide, targets, adv, scale=0.25, **kw)
+        wgrad = cpu.backward(want)[id(wide)]
+        dlp = _adds(v) * 2 ** -24                        # a log-probability's error: the sum's relative one (and its rounding below)
+        a = adv.double().abs().view(-1, *[1] * (len(rows) - 1)).expand(rows)
+        slope = a * wants.ratio.double() + (0.1 * torch.exp(refs.double() - wants.logprobs.double()) if "kl_coef" in kw else 0.0)
+        tol = lambda t: t.double().abs() * 2 ** -23 + 1e-30
+        assert ((terms.logprobs.cpu() - wants.logprobs).abs() <= dlp + tol(wants.logprobs)).all()
+        assert ((terms.ratio.cpu() - wants.ratio).abs() <= wants.ratio * dlp + tol(wants.ratio)).all()
+        d = (refs.double() - wants.logprobs).abs()
+        assert ((terms.kl.cpu() - wants.kl).abs() <= torch.expm1(d) * dlp + dlp * dlp + tol(wants.kl)).all()
+        assert torch.equal(terms.clipped.cpu(), wants.clipped)
+        assert abs(float(loss) - float(want)) <= float(0.25 * (slope * dlp).sum()) + abs(float(want)) * 2 ** -23
+        assert grad.dtype == dtype and grad.shape == logits.shape
+        dw = 0.25 * slope * dlp + wants.weights.double().abs() * 2 ** -23
+        assert ((grad.double() - wgrad).abs() <= _grad_bounds(logits, wants.weights.double(), dw, v)).all()
+        if "mask" in kw:
+            assert not grad[~mask].any()
+    assert native.launch_count > before and native.read_error()[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairs,t,v,offset", [(1, 1, 1, 0), (2, 3, 5, 1), (3, 70, 320, 0), (1, 7, 4099, 1), (2, 5, 32768, 0), (1, 3, 49999, 3), (1, 2, 248320, 0)])
+def test_preference_loss(pairs, t, v, offset, dtype):
+    logits, here, targets, mask, _, _, refs = _inputs((2 * pairs, t), v, dtype, v + t, offset)
+    mask[-1] = False                                     # a sequence without a scored token
+    for kw in (dict(mask=mask, ref_logprobs=refs, beta=0.3, label_smoothing=0.1), dict(mask=mask, average=True, beta=2.0), dict(ref_logprobs=refs)):
+        tape = T.Tape()
+        tape.watch(here)
+        dev = {k: x.to(DEV) if isinstance(x, torch.Tensor) else x for k, x in kw.items()}
+        loss, terms = T.preference_loss(tape, here, targets.to(DEV), **dev)
+        up = torch.tensor(0.5, device=DEV)
+        grad = tape.backward(loss, up)[id(here)].cpu()
+        cpu, wide = T.Tape(), logits.double()
+        cpu.watch(wide)
+        want, wants = T.preference_loss(cpu, wide, targets, **kw)
+        wgrad = cpu.backward(want, torch.tensor(0.5, dtype=torch.float64))[id(wide)]
+        beta, dlp = kw.get("beta", 0.1), _adds(v) * 2 ** -24
+        dsum = t * dlp
+        assert ((terms.logprobs.cpu() - wants.logprobs).abs() <= dsum + wants.logprobs.abs() * 2 ** -23).all()
+        assert ((terms.margins.cpu() - wants.margins).abs() <= 2 * beta * dsum + wants.margins.abs() * 2 ** -23).all()
+        assert abs(float(loss) - float(want)) <= 2 * beta * dsum + abs(float(want)) * 2 ** -23
+        # a weight is beta / pairs times a sigmoid (halved), whose slope is a quarter at most
+        most = 0.5 * beta / pairs
+        w = torch.full(targets.shape, most, dtype=torch.float64)
+        bound = _grad_bounds(logits, w, w * (beta * dsum + 2 ** -22), v)
+        if dtype == torch.bfloat16:
+            bound = bound * 2 + 2 * most * 2 ** -8       # (the gradient is rounded before and after it is halved)
+        assert ((grad.double() - wgrad).abs() <= bound).all()
+    assert native.read_error()[0] == 0
+
+
+def test_rows_that_are_not_scored_are_not_looked_at():
+    logits, here, targets, mask, adv, old, refs = _inputs((40,), 1003, torch.float32, 5)
+    mask[20:] = False
+    for at, x in ((21, NAN), (22, float("-inf")), (23, torch.finfo(torch.float32).min), (24, float("inf"))):
+        here[at] = x
+    old[20:], refs[20:], adv[20:], targets[20:] = NAN, float("inf"), NAN, 10 ** 12
+    mask = mask.to(DEV)
+    tape = T.Tape()
+    tape.watch(here)
+    loss, terms = T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=1.0, mask=mask, old_logprobs=old.to(DEV), ref_logprobs=refs.to(DEV), kl_coef=0.1)
+    grad = tape.backward(loss)[id(here)]
+    assert torch.isfinite(loss) and torch.isfinite(grad).all() and not grad[20:].any() and not any(t[20:].any() for t in terms)
+    loss, terms = T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=1.0, mask=torch.zeros_like(mask))
+    assert float(loss) == 0.0 and not tape.backward(loss)[id(here)].any()
+    assert native.read_error()[0] == 0
+
+
+@pytest.mark.parametrize("v", [40, 5000, 20000, 150000, 270000])
+def test_infinities_and_nan_in_scored_rows(v):
+    """As the torch form: words that cannot be (-inf, the type's lowest) count nothing, a NaN or +inf makes its row NaN and no other."""
+    x = torch.randn(8, v, generator=torch.Generator().manual_seed(0))
+    low = torch.finfo(torch.float32).min
+    x[0, 1:], x[1, : v // 2], x[2, 3], x[3, v - 1], x[4], x[5, : v - 1] = float("-inf"), low, NAN, float("inf"), float("-inf"), low
+    targets = torch.tensor([0, v - 1, 0, 0, 0, v - 1, 5, 6])
+    sides = []
+    for dev in ("cpu", DEV):
+        lg, tape = x.to(dev), T.Tape()
+        tape.watch(lg)
+        loss, terms = T.policy_loss(tape, lg, targets.to(dev), torch.ones(8, device=dev), scale=1.0)
+        sides.append([terms.logprobs.cpu(), terms.weights.cpu(), tape.backward(loss)[id(lg)].cpu(), loss.cpu()])
+    for want, got in zip(*sides):
+        assert torch.equal(want.isnan(), got.isnan())
+        assert torch.allclose(want, got, rtol=1e-4, atol=1e-6, equal_nan=True)
+    assert sides[1][0].isnan().tolist() == [False, False, True, True, True, False, False, False]
+
+
+@pytest.mark.parametrize("v", [40, 5000, 20000, 150000, 270000])
+def test_targets_outside_of_the_vocabulary(v):
+    lg = torch.randn(4, v, generator=torch.Generator().manual_seed(0)).to(DEV)
+    for t in (-1, v, 1 << 40):
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.policy_loss(tape, lg, torch.tensor([0, t, 1, 2], device=DEV), torch.ones(4, device=DEV), scale=1.0)
+        grad = tape.backward(loss)[id(lg)]
+        assert loss.isnan() and terms.logprobs.isnan().tolist() == [False, True, False, False] and grad.isnan().any(-1).tolist() == [False, True, False, False]
+        code, site, _, n = native.read_error()
+        assert (code, site, n) == (2, 16, v)
+    tape.watch(lg)
+    pair = lg.view(4, 1, v)
+    loss, _ = T.preference_loss(T.Tape(), pair, torch.tensor([[0], [v], [1], [2]], device=DEV))
+    assert loss.isnan() and native.read_error()[0] == 2
+
+
+def test_upstream_gradient_strides_streams_and_graphs():
+    """A loss that is scaled further, logits that are a view, work on another stream, and a captured pass replayed on new inputs."""
+    logits, here, targets, mask, adv, old, refs = _inputs((3, 6), 700, torch.float32, 9)
+    dev = [t.to(DEV) for t in (targets, mask, adv, old, refs)]
+
+    def run(lg, factor=None):
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.policy_loss(tape, lg, dev[0], dev[2], scale=0.1, mask=dev[1], old_logprobs=dev[3], ref_logprobs=dev[4], kl_coef=0.1)
+        if factor is not None:
+            loss = T.scale(tape, loss, factor)
+        return loss, tape.backward(loss)[id(lg)], terms.logprobs
+
+    loss, grad, lp = run(here)
+    assert torch.allclose(run(here, 3.0)[1], grad * 3, rtol=1e-6)
+    wide = torch.zeros(3, 6, 800, device=DEV)
+    wide[..., :700] = here
+    view = wide[..., :700]
+    assert not view.is_contiguous() and torch.equal(run(view)[1], grad)
+    assert torch.equal(run(here.transpose(0, 1).contiguous().transpose(0, 1))[1], grad)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run(here)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, (loss, grad, lp)))
+    static = here.clone()
+    with torch.cuda.stream(side):
+        run(static)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static, 2.0)
+    static.copy_(here.flip(-1))
+    graph.replay()
+    again = run(here.flip(-1).contiguous(), 2.0)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
+    kept = grad.clone()
+    here.zero_()                                          # the logits may be written into: the gradient is there
+    assert torch.equal(grad, kept)
+
+
+def test_the_same_bits_twice():
+    for v in (320, 9000, 32768, 150000, 270000):
+        logits, here, targets, mask, adv, old, refs = _inputs((2, 4), v, torch.bfloat16, 1)
+        outs = []
+        for _ in range(2):
+            tape = T.Tape()
+            tape.watch(here)
+            loss, terms = T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=0.1, mask=mask.to(DEV), old_logprobs=old.to(DEV))
+            pair, _ = T.preference_loss(tape, here, targets.to(DEV), mask.to(DEV), refs.to(DEV))
+            outs.append([loss, pair, tape.backward(loss)[id(here)], *terms])
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_more_rows_than_blocks_run_at_a_time():
+    """Persistent forms go through their rows in turn: every row as it is on its own, scored ones and others in any order."""
+    for n, v in ((900, 1500), (700, 20001), (200, 66000)):
+        g = torch.Generator(device=DEV).manual_seed(n)
+        lg = torch.randn(n, v, generator=g, device=DEV)
+        tg = torch.randint(0, v, (n,), generator=g, device=DEV)
+        mask = torch.rand(n, generator=g, device=DEV) < 0.6
+        adv = torch.randn(n, generator=g, device=DEV)
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.policy_loss(tape, lg, tg, adv, scale=1.0, mask=mask)
+        grad = tape.backward(loss)[id(lg)]
+        assert torch.equal(terms.logprobs == 0, ~mask) and not grad[~mask].any()
+        for i in range(0, n, 61):
+            one = T.Tape()
+            row = lg[i:i + 1]
+            one.watch(row)
+            l1, t1 = T.policy_loss(one, row, tg[i:i + 1], adv[i:i + 1], scale=1.0, mask=mask[i:i + 1])
+            assert torch.allclose(t1.logprobs, terms.logprobs[i:i + 1], rtol=1e-6) and torch.allclose(one.backward(l1)[id(row)][0], grad[i], rtol=1e-4, atol=1e-9)
+        want = torch.log_softmax(lg[mask].double(), -1).gather(-1, tg[mask][:, None])[:, 0]
+        assert torch.allclose(terms.logprobs[mask].double(), want, atol=1e-5)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs in one process")
+def test_losses_on_a_gpu_that_is_not_the_current_one():
+    logits, here, targets, mask, adv, old, refs = _inputs((2, 4), 40000, torch.float32, 1)
+    outs = []
+    for dev in ("cuda:0", "cuda:1"):
+        lg, tape = here.to(dev), T.Tape()
+        tape.watch(lg)
+        loss, _ = T.policy_loss(tape, lg, targets.to(dev), adv.to(dev), scale=0.1, mask=mask.to(dev))
+        outs.append([loss.cpu(), tape.backward(loss)[id(lg)].cpu()])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+def test_inputs_on_unlike_devices_are_refused():
+    lg = torch.zeros(2, 5, device=DEV)
+    for kw in (dict(targets=torch.zeros(2, dtype=torch.long)), dict(mask=torch.ones(2, dtype=torch.bool)), dict(advantages=torch.zeros(2)), dict(old_logprobs=torch.zeros(2))):
+        with pytest.raises(ValueError):
+            T.policy_loss(T.Tape(), **{**dict(logits=lg, targets=torch.zeros(2, dtype=torch.long, device=DEV), advantages=torch.zeros(2, device=DEV), scale=1.0), **kw})

@@ -516,6 +516,78 @@ def cross_entropy_sharded(logits_shards, targets, weights, vocab_starts):
     return loss, grads
 
 
+# ---- losses of policy and preference training ---------------------------------------------------------
+def _scored_rows(logits, targets, mask):
+    """``(e, s, log-probabilities in 64 bits)`` of rows of logits: exponentials below the largest and their sum.  Rows that are not scored are
+    taken as zeros, so that nothing in them is seen."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    targets = targets.long()[:, None]
+    if mask is not None:
+        x, targets = torch.where(mask[:, None], x, 0.0), torch.where(mask[:, None], targets, 0)
+    m = x.amax(-1, keepdim=True)
+    e = torch.exp(x - m)
+    s = e.sum(-1, keepdim=True)
+    lp = (x.gather(-1, targets).double() - m.double() - torch.log(s.double()))[:, 0]
+    return e, s, targets, lp if mask is None else torch.where(mask, lp, 0.0)
+
+
+def _logits_grad(e, s, targets, weight, dtype):
+    g = e / s
+    g.scatter_add_(-1, targets, torch.full_like(s, -1.0))
+    return (g * weight.to(g.dtype)[:, None]).to(dtype)
+
+
+def policy_loss(logits, targets, mask, adv, old, ref, *, lo, hi, kl, scale, want_grad=True):
+    """``scale * sum over scored rows of (-min(rho A, clip(rho, lo, hi) A) + kl * k3)`` with ``rho = exp(lp - old)`` and
+    ``k3 = e^d - d - 1``, ``d = ref - lp``.  Returns the loss, terms ``[4, rows]`` (log-probability, ratio, k3, weight), which rows were clipped
+    and the logits' gradient ``weight * (softmax - onehot)``.  A row's terms are formed in 64 bits: d and k3 are small differences of
+    large numbers, and the clipping's border decides about a whole row."""
+    e, s, tg, lp = _scored_rows(logits, targets, mask)
+    a = adv.double().repeat_interleave(targets.numel() // max(1, adv.numel()))
+    rho = torch.ones_like(lp) if old is None else torch.exp(lp - old.double())
+    clipped = ((rho > hi) & (a > 0)) | ((rho < lo) & (a < 0))
+    held = torch.where(a > 0, torch.full_like(a, hi), torch.full_like(a, lo))
+    gain = torch.where(a == 0, 0.0, a * torch.where(clipped, held, rho))
+    w = torch.where((a == 0) | clipped, 0.0, a * rho)
+    gain, w = torch.where(lp.isnan(), lp, gain), torch.where(lp.isnan(), lp, w)
+    k3 = torch.zeros_like(lp)
+    if ref is not None:
+        d = ref.double() - lp
+        k3 = torch.expm1(d) - d
+        if kl:
+            w, gain = w + kl * torch.expm1(d), gain - kl * k3
+    keep = (lambda t: t) if mask is None else (lambda t: torch.where(mask, t, torch.zeros_like(t)))
+    w = keep(w) * scale
+    loss = -(keep(gain).sum() * scale)
+    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    terms = torch.stack([lp, keep(rho), keep(k3), w]).to(wide)
+    return loss.to(wide), terms, keep(clipped), _logits_grad(e, s, tg, w, logits.dtype) if want_grad else None
+
+
+def preference_loss(logits, targets, mask, ref, *, beta, smooth, average, scale, want_grad=True):
+    """Sequences ``targets [2P, T]``, chosen and rejected in turn: ``z = beta * ((S - R)_chosen - (S - R)_rejected)`` over sums (or means) S of
+    log-probabilities and R of ``ref`` at scored rows, ``scale * sum((1 - smooth) softplus(-z) + smooth softplus(z))``.  Returns the loss, S, z and
+    the logits' gradient."""
+    n, t = targets.shape
+    flat = None if mask is None else mask.reshape(-1)
+    e, s, tg, lp = _scored_rows(logits, targets.reshape(-1), flat)
+    gap = lp if ref is None else lp - ref.reshape(-1).double()
+    if flat is not None:
+        gap = torch.where(flat, gap, 0.0)
+    count = torch.ones(n, dtype=torch.float64, device=lp.device)
+    if average:
+        count = count * t if mask is None else mask.sum(-1).clamp_min(1).double()
+    total, gap = lp.view(n, t).sum(-1) / count, gap.view(n, t).sum(-1) / count
+    z = beta * (gap[0::2] - gap[1::2])
+    loss = ((1 - smooth) * F.softplus(-z) + smooth * F.softplus(z)).sum() * scale
+    dz = (smooth * torch.sigmoid(z) - (1 - smooth) * torch.sigmoid(-z)) * scale
+    w = (torch.stack([-dz, dz], -1).reshape(-1) * beta / count)[:, None].expand(n, t).reshape(-1)
+    if flat is not None:
+        w = torch.where(flat, w, 0.0)
+    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    return loss.to(wide), total.to(wide), z.to(wide), _logits_grad(e, s, tg, w, logits.dtype) if want_grad else None
+
+
 def token_logprobs(logits, targets):
     lg = _f(logits)
     return lg.gather(-1, targets.long()[:, None]).squeeze(-1) - torch.logsumexp(lg, -1)

@@ -168,6 +168,12 @@ register("any", "sm100", {
     "train_attention": Kernel("tr_attn_prep_kernel + tr_softmax_kernel + tr_attn_gate_kernel", "csrc/train.cu", "trl_train_attn_prep", "tilerl_b200.ops.train_kernels",
                               note="norms, rotation, masked softmax, gate and their gradients; the products are library GEMMs"),
     "train_cross_entropy": Kernel("tr_lse_kernel + tr_ce_grad_kernel", "csrc/train.cu", "trl_train_lse", "tilerl_b200.ops.train_kernels"),
+    "train_policy_loss": Kernel("pl_stats_kernel + pl_grad_kernel + pl_sum_kernel", "csrc/policy.cu", "trl_policy_loss", "tilerl_b200.ops.loss_kernels",
+                                note="clipped policy loss with a KL term, fp32 or bf16 logits"),
+    "train_preference_loss": Kernel("pl_stats_kernel + pl_pairs_kernel + pl_grad_kernel", "csrc/policy.cu", "trl_preference_loss", "tilerl_b200.ops.loss_kernels"),
+    "score_tokens": Kernel("score_kernel + score_join_kernel", "csrc/score.cu", "trl_score", "tilerl_b200.ops.score",
+                           note="log-probabilities and entropies from hidden rows and the head, logits in TMEM; only scored rows"),
+    "keep_8bit": Kernel("kp_kernel", "csrc/keep.cu", "trl_keep_pack", "tilerl_b200.ops.keep", note="activations in 8 bits, groups of 128; SwiGLU from and to them"),
     "train_gdn": Kernel("gt_prep_kernel + gt_chunk_kernel + gt_scan_kernel + gt_norm_kernel", "csrc/gdn_train.cu", "trl_gdn_train_forward", "tilerl_b200.ops.gdn_train",
                         note="forward and gradient of the block, fp32, chunks of 32, heads of 128"),
     "decode_advance": Kernel("decode_advance_kernel", "csrc/misc.cu", "trl_decode_advance"),

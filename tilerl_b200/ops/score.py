@@ -1,0 +1,67 @@
+"""Log-probabilities of given tokens from hidden rows and the head, on the kernels of ``csrc/score.cu`` (tcgen05) or in torch."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import native as N
+
+N.register("trl_score_workspace", [N.I] * 5, N.L)
+N.register("trl_score", [N.P, N.I, N.P, N.P, N.P] + [N.I] * 3 + [N.P] * 4)
+
+ROWS = 8192               # a call: the tiles' parts of as many rows over 248 320 words are 127 MB
+CHUNK = 256               # rows of logits that the torch form has at a time
+
+
+def takes(h: torch.Tensor, w: torch.Tensor) -> bool:
+    """Rows of a multiple of eight values (a copy's rows begin on 16 bytes) and a head in bf16, as the training head is."""
+    return (h.is_cuda and h.numel() > 0 and h.shape[-1] % 8 == 0 and h.dtype in (torch.float32, torch.bfloat16) and w.dtype == torch.bfloat16
+            and w.shape[0] < 1 << 24 and N.has("trl_score"))
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def score(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``h [rows, H]``, ``targets`` int64 and ``mask`` (bool or None) ``[rows]``."""
+    lib, (v, hidden) = N.lib(), w.shape
+    with torch.cuda.device(h.device):
+        h, w = _aligned(h), _aligned(w)
+        n, kind = h.shape[0], int(h.dtype == torch.bfloat16)
+        lp = torch.empty(n, dtype=torch.float32, device=h.device)
+        ent = torch.empty_like(lp) if entropy else None
+        for a in range(0, n, ROWS):
+            some = slice(a, min(n, a + ROWS))
+            m = some.stop - a
+            packed = int(mask is not None or not kind)
+            work = torch.empty(lib.trl_score_workspace(m, hidden, v, packed, int(entropy)), dtype=torch.uint8, device=h.device)
+            N.check(lib.trl_score(h[some].data_ptr(), kind, w.data_ptr(), targets[some].data_ptr(), None if mask is None else mask[some].data_ptr(), m, hidden, v,
+                                  lp[some].data_ptr(), ent[some].data_ptr() if entropy else None, work.data_ptr(), N.stream()), "score")
+            N.count(2 + packed + int(mask is not None))
+    return lp, ent
+
+
+def score_torch(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The same in torch, a few rows of logits at a time; on the GPU with bf16 operands and fp32 results, on the CPU in fp32."""
+    cd = torch.bfloat16 if h.is_cuda else torch.float64 if h.dtype == torch.float64 else torch.float32
+    wide = torch.float64 if cd == torch.float64 else torch.float32
+    wc = w.to(cd)
+    lp = torch.zeros(h.shape[0], dtype=wide, device=h.device)
+    ent = torch.zeros_like(lp) if entropy else None
+    for a in range(0, h.shape[0], CHUNK):
+        some = slice(a, a + CHUNK)
+        x = h[some].to(cd).to(wide) @ wc.t().to(wide)
+        tg = targets[some] if mask is None else torch.where(mask[some], targets[some], 0)
+        m = x.amax(-1, keepdim=True)
+        low = x - m
+        e = torch.exp(low)
+        s = e.sum(-1).double()
+        got = low.gather(-1, tg[:, None])[:, 0].double() - torch.log(s)
+        lp[some] = (got if mask is None else torch.where(mask[some], got, 0.0)).to(wide)
+        if entropy:
+            got = torch.log(s) - torch.where(e > 0, e * low, 0.0).sum(-1).double() / s
+            ent[some] = (got if mask is None else torch.where(mask[some], got, 0.0)).to(wide)
+    return lp, ent

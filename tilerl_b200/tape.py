@@ -20,12 +20,14 @@ table ``_BWD:275-301``, ``Tape:304``, ``backward:360``, streaming release
 from __future__ import annotations
 
 import math
-from typing import Callable, Dict, List, Optional, Sequence, Tuple
+import weakref
+from typing import Callable, Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
 
-from .ops import ref
+from .ops import keep, ref, score
+from .ops.keep import Kept8, keep8
 
 
 class _Node:
@@ -35,34 +37,69 @@ class _Node:
         self.name, self.inputs, self.outputs, self.bwd = name, inputs, outputs, bwd
 
 
+class _StandIn:
+    """In the nodes, for a tensor that the tape has let go of."""
+    __slots__ = ()
+
+
 class Tape:
     def __init__(self, tp_group=None, tp_world: int = 1):
         self.nodes: List[_Node] = []
         self.leaves: Dict[int, torch.Tensor] = {}
         self.made: set = set()            # ids of the recorded ops' outputs
+        self.gone: Dict[int, tuple] = {}  # id of a tensor let go of: (weak reference, its stand-in)
         self.tp_group, self.tp_world = tp_group, tp_world
         self.enabled = True
 
     # ---- recording -------------------------------------------------------------
     def watch(self, *tensors: torch.Tensor) -> None:
         for t in tensors:
+            key = self._key(t)
+            if key is not t:              # let go of before: back in its place
+                self._swap(key, t)
+                del self.gone[id(t)]
             self.leaves[id(t)] = t
 
     def record(self, name: str, inputs: Sequence[torch.Tensor], outputs: Sequence[torch.Tensor],
                bwd: Callable) -> None:
         if self.enabled:
+            if self.gone:
+                inputs, outputs = map(self._key, inputs), map(self._key, outputs)
             self.nodes.append(_Node(name, tuple(inputs), tuple(outputs), bwd))
-            self.made.update(map(id, outputs))
+            self.made.update(map(id, self.nodes[-1].outputs))
 
     def wants(self, t: torch.Tensor) -> bool:
         """Whether a gradient of ``t`` goes anywhere: it is watched, or an op on this tape made it."""
+        t = self._key(t)
         return id(t) in self.leaves or id(t) in self.made
+
+    def _key(self, t):
+        """What stands for ``t`` in the nodes (an id alone may be another tensor's by now)."""
+        known = self.gone.get(id(t))
+        return known[1] if known is not None and known[0]() is t else t
+
+    def _swap(self, old, new) -> None:
+        for n in reversed(self.nodes):
+            n.inputs = tuple(new if t is old else t for t in n.inputs)
+            if any(t is old for t in n.outputs):
+                n.outputs = tuple(new if t is old else t for t in n.outputs)
+                if id(old) in self.made:
+                    self.made.discard(id(old)), self.made.add(id(new))
+                break
+
+    def let_go(self, t: torch.Tensor) -> None:
+        """Hold ``t`` no longer, for ops that keep another form of what they need of it; gradients still pass.  (A watched tensor stays.)"""
+        if id(t) in self.leaves or self._key(t) is not t:
+            return
+        stand_in = _StandIn()
+        self._swap(t, stand_in)
+        self.gone[id(t)] = (weakref.ref(t), stand_in)
 
     # ---- backward ----------------------------------------------------------------
     def backward(self, root: torch.Tensor, grad: Optional[torch.Tensor] = None,
                  on_grad: Optional[Callable[[torch.Tensor, torch.Tensor], None]] = None
                  ) -> Dict[int, torch.Tensor]:
-        grads: Dict[int, torch.Tensor] = {id(root): torch.ones_like(root) if grad is None else grad}
+        grads: Dict[int, torch.Tensor] = {id(self._key(root)): torch.ones_like(root) if grad is None else grad}
         # first node (in forward order) that reads each leaf = last to contribute in reverse
         first_use: Dict[int, int] = {}
         for idx, n in enumerate(self.nodes):
@@ -89,6 +126,7 @@ class Tape:
                         on_grad(t, grads.pop(k))
         self.nodes.clear()
         self.made.clear()
+        self.gone.clear()
         return {k: g for k, g in grads.items() if k in self.leaves}
 
     def grad_of(self, grads: Dict[int, torch.Tensor], t: torch.Tensor) -> Optional[torch.Tensor]:
@@ -96,10 +134,14 @@ class Tape:
 
     # ---- checkpoint -----------------------------------------------------------------
     def checkpoint(self, fn: Callable, *inputs: torch.Tensor,
-                   params: Sequence[torch.Tensor] = ()) -> torch.Tensor:
+                   params: Sequence[torch.Tensor] = (), bits: int = 32) -> torch.Tensor:
         """Run ``fn(tape, *inputs)`` without recording and keep only its inputs;
         backward replays it on a private tape.  ``params`` lists the watched leaves
-        ``fn`` reads through its closure so their gradients flow out of the segment."""
+        ``fn`` reads through its closure so their gradients flow out of the segment.
+        ``bits=8``: fp32 inputs that are not watched are kept in 8 bits (``ops/keep.py``) and the tape
+        lets go of them; the replay, and so the gradients, start from what those stand for."""
+        if bits not in (8, 32):
+            raise ValueError(f"checkpoint: inputs are kept in 8 or 32 bits, not {bits}")
         was = self.enabled
         self.enabled = False
         try:
@@ -107,16 +149,24 @@ class Tape:
         finally:
             self.enabled = was
         params = tuple(params)
+        kept: tuple = inputs
+        if bits == 8 and self.enabled:
+            small = lambda t: t.dtype == torch.float32 and t.dim() > 0 and id(t) not in self.leaves
+            kept = tuple(keep8(t) if small(t) else t for t in inputs)
 
         def bwd(g):
             sub = Tape(self.tp_group, self.tp_world)
-            for t in inputs + params:
+            again = tuple(t.rows() if isinstance(t, Kept8) else t for t in kept)
+            for t in again + params:
                 sub.leaves[id(t)] = t
-            y = fn(sub, *inputs)
+            y = fn(sub, *again)
             gs = sub.backward(y, g)
-            return tuple(gs.get(id(t)) for t in inputs + params)
+            return tuple(gs.get(id(t)) for t in again + params)
 
         self.record("checkpoint", inputs + params, (out,), bwd)
+        for t, k in zip(inputs, kept):
+            if isinstance(k, Kept8):
+                self.let_go(t)
         return out
 
 
@@ -147,6 +197,12 @@ def _unchanged(*kept: torch.Tensor) -> Callable[[], None]:
         if any(t._version != v for t, v in kept):
             raise RuntimeError("a tensor that the backward pass needs was changed in place after the forward pass")
     return check
+
+
+class _Like(NamedTuple):
+    """Of an output that a gradient is checked against: no op needs its values."""
+    shape: torch.Size
+    device: torch.device
 
 
 @_nograd
@@ -267,10 +323,11 @@ def linear_lora(tape: Tape, x: torch.Tensor, w, frozen: bool, a: torch.Tensor, b
         return lora(tape, linear(tape, x, w, frozen=frozen), x, a, b, s)
     wf = DEQUANT_BF16(w) if hasattr(w, "wq") else w.to(torch.bfloat16)
     out, xa = K.lora(x.to(torch.bfloat16) @ wf.t(), x, a, b, s)
+    like = _Like(out.shape, out.device)
 
     def bwd(g):
-        if not K.grad_takes(g, out):
-            _, dx, da, db = _lora_torch(out, x, a, b, s)[1](g)
+        if not K.grad_takes(g, like):
+            _, dx, da, db = _lora_torch(0.0, x, a, b, s)[1](g)
             return dx + (g.to(torch.bfloat16) @ wf).float(), da, db
         g = K._grad(g)
         return K.lora_grad(x, xa, a, b, s, g, g.to(torch.bfloat16) @ wf)
@@ -306,7 +363,13 @@ def _swiglu_torch(gu: torch.Tensor):
 
 
 @_nograd
-def swiglu(tape: Tape, gu: torch.Tensor) -> torch.Tensor:
+def swiglu(tape: Tape, gu: torch.Tensor, bits: int = 32) -> torch.Tensor:
+    """``silu(gate) * up`` of interleaved pairs.  ``bits=8``: the pairs are kept in 8 bits for the gradient (``ops/keep.py``), which is
+    that at the values that they stand for, and the tape lets go of ``gu``."""
+    if bits not in (8, 32):
+        raise ValueError(f"swiglu: its input is kept in 8 or 32 bits, not {bits}")
+    if bits == 8 and tape.enabled:
+        return _swiglu_kept(tape, gu)
     K = _kernels(gu)
     if K is not None and K.swiglu_takes(gu):
         out = K.swiglu(gu)
@@ -314,6 +377,23 @@ def swiglu(tape: Tape, gu: torch.Tensor) -> torch.Tensor:
         return out
     out, bwd = _swiglu_torch(gu)
     tape.record("swiglu", (gu,), (out,), bwd)
+    return out
+
+
+def _swiglu_kept(tape: Tape, gu: torch.Tensor) -> torch.Tensor:
+    if gu.dtype != torch.float32 or gu.shape[-1] % 2:
+        raise ValueError(f"swiglu: pairs kept in 8 bits are fp32, got {tuple(gu.shape)} {gu.dtype}")
+    takes = keep.swiglu_takes(gu)
+    out, kept = keep.swiglu(gu) if takes else (_swiglu_torch(gu)[0], keep8(gu))
+    like = _Like(out.shape, out.device)
+
+    def bwd(g):
+        if takes and g.shape == like.shape and g.device == like.device:
+            return (keep.swiglu_grad(kept, g),)
+        return _swiglu_torch(kept.rows())[1](g)
+
+    tape.record("swiglu", (gu,), (out,), bwd)
+    tape.let_go(gu)
     return out
 
 
@@ -566,6 +646,122 @@ def cross_entropy(tape: Tape, logits: torch.Tensor, targets: torch.Tensor,
     return loss
 
 
+class PolicyTerms(NamedTuple):
+    """Of every row, in the targets' shape; all zero (False) where a row is not scored."""
+    logprobs: torch.Tensor      # log-probability of the target
+    ratio: torch.Tensor         # exp(logprobs - old_logprobs), 1 without the latter
+    kl: torch.Tensor            # e^d - d - 1 with d = ref_logprobs - logprobs, 0 without a reference
+    weights: torch.Tensor       # of the row's cross-entropy gradient: minus the loss's derivative by the log-probability
+    clipped: torch.Tensor       # bool: the clipping took the row's gradient
+
+
+class PreferenceTerms(NamedTuple):
+    logprobs: torch.Tensor      # [2P] of a sequence's scored tokens: their sum, or mean
+    margins: torch.Tensor       # [P] beta times the difference of the log ratios: positive where the chosen one is preferred
+
+
+def _loss_kernels(logits: torch.Tensor):
+    """The kernels of the two losses below for logits on the GPU."""
+    if not logits.is_cuda or not logits.numel():
+        return None
+    from .ops import loss_kernels
+    return loss_kernels if logits.dtype in loss_kernels.TYPES and loss_kernels.there() else None
+
+
+def _loss_inputs(what: str, logits, targets, mask, **floats):
+    """Shapes, types and devices of what a loss over rows of logits takes; the tensors as its kernels read them."""
+    if not logits.is_floating_point() or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{what}: logits are [..., vocab] in floating point, got {tuple(logits.shape)} {logits.dtype}")
+    rows = tuple(logits.shape[:-1])
+    if tuple(targets.shape) != rows or targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"{what}: targets are token ids {rows}, got {tuple(targets.shape)} {targets.dtype}")
+    if mask is not None and (tuple(mask.shape) != rows or mask.dtype != torch.bool):
+        raise ValueError(f"{what}: the mask is bool {rows}, got {tuple(mask.shape)} {mask.dtype}")
+    for name, t in floats.items():
+        if t is not None and (tuple(t.shape) != rows or not t.is_floating_point()):
+            raise ValueError(f"{what}: {name} is floating point {rows}, got {tuple(t.shape)} {t.dtype}")
+    for t in (targets, mask, *floats.values()):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{what}: logits are on {logits.device}, another input on {t.device}")
+    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    flat = lambda t, dtype: None if t is None else t.reshape(-1).to(dtype).contiguous()
+    return (flat(targets, torch.int64), flat(mask, torch.bool)) + tuple(flat(t, wide) for t in floats.values())
+
+
+def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
+    if grad is None:
+        return
+    grad = grad.view(logits.shape)
+
+    def bwd(g):
+        if K is not None and g.numel() == 1 and g.device == loss.device:
+            return (K.scale_grad(grad, g),)
+        return (grad * g,)
+
+    tape.record(name, (logits,), (loss,), bwd)
+
+
+@_nograd
+def policy_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, advantages: torch.Tensor, *, scale: float,
+                mask: Optional[torch.Tensor] = None, old_logprobs: Optional[torch.Tensor] = None, ref_logprobs: Optional[torch.Tensor] = None,
+                clip_eps: float = 0.2, clip_eps_high: Optional[float] = None, kl_coef: float = 0.0) -> Tuple[torch.Tensor, PolicyTerms]:
+    """Clipped policy loss with a KL term over rows of logits ``[..., vocab]``:
+    ``scale * sum over scored rows of (-min(rho A, clip(rho, 1 - clip_eps, 1 + clip_eps_high) A) + kl_coef * (e^d - d - 1))`` with
+    ``rho = exp(logp(target) - old_logprobs)`` (1 without old ones) and ``d = ref_logprobs - logp(target)``.
+
+    ``targets``, ``mask`` (bool: scored rows), ``old_logprobs`` and ``ref_logprobs`` have the logits' shape without the vocabulary;
+    ``advantages`` too, or one value for each of the first dimension.  ``clip_eps_high`` defaults to ``clip_eps``; ``scale`` is mostly one over the
+    number of scored tokens of the whole batch.  A reference with ``kl_coef`` 0 is measured only.  An advantage of 0 contributes nothing.
+
+    The logits' gradient has their type (fp32, bf16) and is formed here, so they may be written into afterwards.  Rows that are not scored get zeros, whatever
+    their logits (NaN among them) and targets are.  A target outside of the vocabulary in a scored row makes the loss and the row's gradient NaN and
+    sets the device's error word; on the CPU it is an error."""
+    if clip_eps < 0 or (clip_eps_high is not None and clip_eps_high < 0) or not math.isfinite(scale) or not math.isfinite(kl_coef):
+        raise ValueError("policy_loss: clip_eps is not negative, scale and kl_coef are finite")
+    if kl_coef and ref_logprobs is None:
+        raise ValueError("policy_loss: kl_coef needs ref_logprobs")
+    if tape.tp_world > 1:
+        raise ValueError("policy_loss takes whole rows of logits: with a sharded vocabulary use cross_entropy_tp")
+    tg, mk, old, refs = _loss_inputs("policy_loss", logits, targets, mask, old_logprobs=old_logprobs, ref_logprobs=ref_logprobs)
+    if tuple(advantages.shape) not in (tuple(targets.shape), tuple(targets.shape[:1])) or not advantages.is_floating_point() or advantages.device != logits.device:
+        raise ValueError(f"policy_loss: advantages are floating point {tuple(targets.shape)} or {tuple(targets.shape[:1])} on {logits.device}, "
+                         f"got {tuple(advantages.shape)} {advantages.dtype} on {advantages.device}")
+    adv = advantages.reshape(-1).to(torch.float64 if logits.dtype == torch.float64 else torch.float32).contiguous()
+    K = _loss_kernels(logits)
+    args = dict(lo=1.0 - clip_eps, hi=1.0 + (clip_eps if clip_eps_high is None else clip_eps_high), kl=float(kl_coef), scale=float(scale),
+                want_grad=tape.enabled and tape.wants(logits))
+    loss, terms, clipped, grad = (K.policy if K is not None else ref.policy_loss)(logits.reshape(-1, logits.shape[-1]), tg, mk, adv, old, refs, **args)
+    _record_loss(tape, "policy_loss", logits, loss, grad, K)
+    return loss, PolicyTerms(*terms.view(4, *targets.shape), clipped.view(targets.shape))
+
+
+@_nograd
+def preference_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                    ref_logprobs: Optional[torch.Tensor] = None, *, beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False,
+                    scale: Optional[float] = None) -> Tuple[torch.Tensor, PreferenceTerms]:
+    """Preference loss of pairs of sequences: ``logits [2P, T, vocab]``, ``targets [2P, T]``, chosen and rejected in turn.  With a sequence's log
+    ratio ``S`` = sum over its scored tokens of ``logp(target) - ref_logprobs`` (``average``: their mean; no reference: the log-probabilities alone)
+    and ``z = beta * (S_chosen - S_rejected)``:
+    ``scale * sum over pairs of (-(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z))``; ``scale`` is one over P unless given.
+
+    A sequence without scored tokens has a ratio of 0.  Gradient, rows that are not scored and targets out of range: as in :func:`policy_loss`."""
+    if logits.dim() != 3 or logits.shape[0] % 2:
+        raise ValueError(f"preference_loss: logits are [2 * pairs, tokens, vocab], got {tuple(logits.shape)}")
+    if not 0.0 <= label_smoothing <= 1.0 or not math.isfinite(beta) or (scale is not None and not math.isfinite(scale)):
+        raise ValueError("preference_loss: label_smoothing is within [0, 1], beta and scale are finite")
+    if tape.tp_world > 1:
+        raise ValueError("preference_loss takes whole rows of logits, not a sharded vocabulary")
+    tg, mk, refs = _loss_inputs("preference_loss", logits, targets, mask, ref_logprobs=ref_logprobs)
+    K, shape = _loss_kernels(logits), targets.shape
+    args = dict(beta=float(beta), smooth=float(label_smoothing), average=bool(average), want_grad=tape.enabled and tape.wants(logits),
+                scale=1.0 / max(1, shape[0] // 2) if scale is None else float(scale))
+    view = lambda t: None if t is None else t.view(shape)
+    loss, totals, margins, grad = (K.preference if K is not None else ref.preference_loss)(logits.reshape(-1, logits.shape[-1]), tg.view(shape), view(mk),
+                                                                                          view(refs), **args)
+    _record_loss(tape, "preference_loss", logits, loss, grad, K)
+    return loss, PreferenceTerms(totals, margins)
+
+
 @_nograd
 def cross_entropy_tp(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, lp_weights_fn: Callable):
     """Vocab-parallel weighted cross-entropy: ``logits [.., V / tp]`` is this rank's shard.  Three
@@ -645,6 +841,30 @@ def linear_cross_entropy(tape: Tape, h: torch.Tensor, w: torch.Tensor, targets: 
 
 
 @_nograd
+def linear_logprobs(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, mask: Optional[torch.Tensor] = None, entropy: bool = False):
+    """Log-probabilities of ``targets [...]`` under ``softmax(h W^T)`` from hidden rows ``h [..., H]`` and a dense head ``w [vocab, H]``, without the
+    logits: how a frozen policy (a reference, the one that sampled) is scored.  ``mask`` (bool): the rows to score, the others give 0 whatever they
+    hold and cost nothing.  ``entropy``: also the entropies of the rows, as a second result.  fp32; on CUDA the product has bf16 operands and fp32
+    sums, as :func:`linear`'s.  It is no op of a tape: gradients through the head are :func:`linear_cross_entropy`'s.
+
+    A target outside of the vocabulary in a scored row gives NaN and sets the device's error word; on the CPU it is an error."""
+    if not isinstance(w, torch.Tensor) or w.dim() != 2 or not w.is_floating_point() or not h.is_floating_point() or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"linear_logprobs: h [..., H] and a dense w [vocab, H], got {tuple(h.shape)} and {tuple(w.shape)}")
+    rows = tuple(h.shape[:-1])
+    if tuple(targets.shape) != rows or targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"linear_logprobs: targets are token ids {rows}, got {tuple(targets.shape)} {targets.dtype}")
+    if mask is not None and (tuple(mask.shape) != rows or mask.dtype != torch.bool):
+        raise ValueError(f"linear_logprobs: the mask is bool {rows}, got {tuple(mask.shape)} {mask.dtype}")
+    if any(t is not None and t.device != h.device for t in (w, targets, mask)):
+        raise ValueError("linear_logprobs: all inputs are on one device")
+    tg, mk = targets.reshape(-1).long().contiguous(), None if mask is None else mask.reshape(-1).contiguous()
+    hf = h.reshape(-1, h.shape[-1])
+    wc = w.to(torch.bfloat16) if h.is_cuda else w
+    lp, ent = (score.score if score.takes(hf, wc) else score.score_torch)(hf, wc, tg, mk, entropy)
+    return (lp.view(rows), ent.view(rows)) if entropy else lp.view(rows)
+
+
+@_nograd
 def tp_fork(tape: Tape, x: torch.Tensor) -> torch.Tensor:
     """Identity forward; all-reduce of the gradient in backward (entry of a
     column-parallel region)."""
@@ -693,10 +913,11 @@ def lora(tape: Tape, y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch
     K = _kernels(y)
     if K is not None and K.lora_takes(y, x, a, b):
         out, xa = K.lora(y, x, a, b, s)
+        like = _Like(out.shape, out.device)
 
         def bwd_kernel(g):
-            if not K.grad_takes(g, out):
-                return _lora_torch(y, x, a, b, s)[1](g)
+            if not K.grad_takes(g, like):
+                return _lora_torch(0.0, x, a, b, s)[1](g)
             g = K._grad(g)
             return (g,) + K.lora_grad(x, xa, a, b, s, g)
 
