@@ -8,15 +8,16 @@
 //               loss = scale sum (-(1 - e) log sigmoid(z) - e log sigmoid(-z)), w = -+ beta dloss/dz
 //   gradient    dx[c] = w (exp(x[c] - m) / s - [c == t]);  rows that are not scored: zeros, and nothing of them is read
 //
-// Bound by memory: a row is read, and its gradient written, once each at best.  Sums over a row are fp32 in
-// short runs and fp64 over them; what follows from them is
-// a handful of operations a row, done in fp64: d is a difference of two log-probabilities near each other, kl the third-order rest
+// Bound by memory: a row is read, and its gradient written, once each at best.  Sums over a row are fp32, 16 values and more at a time in a
+// tree; what follows from them is a handful of operations a row, done in fp64: d is a difference of two log-probabilities near each other, kl the third-order rest
 // of an exponential, and the border of the clipping decides about a whole row.  Sums over rows are fp64, in a fixed order.  No atomics.
 //
 // Targets out of range: the row's loss and gradient are NaN and the error word says which.
 // In the place of the reference's weighted cross-entropy (tilerl_kernels/reference.py:1511-1603) and its per-token weights
 // (src/tilerl/train.py:805-864).
-#include "common.cuh"
+#include <cuda.h>
+
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -79,11 +80,26 @@ __device__ __forceinline__ uint4 pl_pack(const float (&x)[8]) {
   return make_uint4(f2_to_bf162_bits(x[0], x[1]), f2_to_bf162_bits(x[2], x[3]), f2_to_bf162_bits(x[4], x[5]), f2_to_bf162_bits(x[6], x[7]));
 }
 
-// exp(x - m) where m may still be -inf: values of -inf count nothing, NaN stays.
-__device__ __forceinline__ float pl_base(float m) { return m == -INFINITY ? 0.f : m; }
+// ---- exponentials ------------------------------------------------------------------------------------------------------------
+// Sums are of 2^(x log2 e - B) with a whole number B, the row's largest x log2 e rounded up: one fused multiply-add, rounded once, and
+// ex2.approx, where expf(x - m) has ten instructions; instructions were these kernels' time.  A whole B makes it no matter which B: the rounding
+// of a product m log2 e would go into every value of the row.  fp32's log2 e is off by 1.3e-8 of itself, as if all of x were; ex2.approx by 2^-22, and the
+// multiply-add's rounding moves a value at a distance of d by d 2^-24 of itself, both at random over a row.  (Logits above 2.3e38 count as infinite.)
+constexpr float PL_L2E = 1.4426950408889634f;
+__device__ __forceinline__ float pl_exp2(float y) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+  return e;
+}
+__device__ __forceinline__ float pl_exp(float x, float base) { return pl_exp2(fmaf(x, PL_L2E, -base)); }
+// B for a largest value; as what is taken away from an exponent (nothing has counted yet at -inf: values of -inf then count nothing, and NaN stays)
+__device__ __forceinline__ float pl_base(float most) { return ceilf(most * PL_L2E); }
+__device__ __forceinline__ float pl_less(float base) { return base == -INFINITY ? 0.f : base; }
+// a sum at base `from` at base `to` (not below it)
+__device__ __forceinline__ float pl_moved(float s, float from, float to) { return s * pl_exp2(from - pl_less(to)); }
+// x - B ln 2, with it the log-probability, in fp64 and from the same log2 e, so that its error comes in with x's distance from the row's mean only
+__device__ __forceinline__ double pl_low(float x, float base) { return ((double)x * (double)PL_L2E - (double)base) * 0.693147180559945309417; }
 
-// log-probability of the target, in fp64; NaN for a target out of range.
-__device__ __forceinline__ double pl_logprob(float xt, float m, double s) { return (double)xt - (double)m - log(s); }
 template <typename T>
 __device__ __forceinline__ float pl_target(const T* row, long long t, long V, long r) {
   if (t < 0 || t >= V) {
@@ -93,22 +109,32 @@ __device__ __forceinline__ float pl_target(const T* row, long long t, long V, lo
   return pl_float(row[t]);
 }
 
-// A scored row's terms from its log-probability; the weight of its gradient comes back.
-__device__ __forceinline__ float pl_policy(const PolicyRow& a, long r, double lp) {
-  const double A = (double)a.adv[r / a.adv_rows];
-  const double rho = a.old ? exp(lp - (double)a.old[r]) : 1.0;
+// What a scored row's terms need, and they from its target's logit, largest value and sum.  The exponentials do not wait for the logarithm.
+struct PolicyIn {
+  float adv, old, ref;
+  __device__ PolicyIn() {}
+  __device__ PolicyIn(const PolicyRow& a, long r) : adv(a.adv[a.adv_rows == 1 ? (unsigned)r : (unsigned)r / (unsigned)a.adv_rows]), old(a.old ? a.old[r] : 0.f), ref(a.ref ? a.ref[r] : 0.f) {}
+};
+struct PolicyOut {
+  float weight, target;                              // of the row's gradient, and its target's: weight (p - 1)
+  double part;                                       // 1 / sum
+};
+__device__ __forceinline__ PolicyOut pl_policy(const PolicyRow& a, const PolicyIn& in, long r, float xt, float base, double sum, bool write = true) {
+  const double A = (double)in.adv, low = pl_low(xt, base), part = 1.0 / sum;
+  const double lp = low - log(sum), p = exp(low) * part;
+  const double rho = a.old ? exp(low - (double)in.old) * part : 1.0;
   const bool clip = (rho > a.hi && A > 0.0) || (rho < a.lo && A < 0.0);
   // (an advantage of nothing has no part in the loss, whatever the ratio)
   double w = A == 0.0 ? 0.0 : clip ? 0.0 : A * rho, loss = A == 0.0 ? 0.0 : clip ? -A * (A > 0.0 ? a.hi : a.lo) : -A * rho, kl = 0.0;
   if (lp != lp) w = loss = lp;                       // (NaN stays where the advantage or the clipping would hide it)
   if (a.ref) {
-    const double d = (double)a.ref[r] - lp, e = expm1(d);
-    kl = e - d;
-    if (a.kl != 0.0) w += a.kl * e, loss += a.kl * kl;
+    const double d = (double)in.ref - lp, e = exp((double)in.ref - low) * sum;      // (1e-16 of cancellation in kl: d^2 / 2 from |d| of 1e-5 on)
+    kl = e - d - 1.0;
+    if (a.kl != 0.0) w += a.kl * (e - 1.0), loss += a.kl * kl;
   }
   const float weight = (float)(w * a.scale);
-  a.lp[r] = (float)lp, a.ratio[r] = (float)rho, a.klv[r] = (float)kl, a.weight[r] = weight, a.clipped[r] = clip, a.loss[r] = loss;
-  return weight;
+  if (write) a.lp[r] = (float)lp, a.ratio[r] = (float)rho, a.klv[r] = (float)kl, a.weight[r] = weight, a.clipped[r] = clip, a.loss[r] = loss;
+  return {weight, (float)((p - 1.0) * (double)weight), part};
 }
 __device__ __forceinline__ void pl_policy_skip(const PolicyRow& a, long r) {
   a.lp[r] = a.ratio[r] = a.klv[r] = a.weight[r] = 0.f, a.clipped[r] = 0, a.loss[r] = 0.0;
@@ -128,117 +154,304 @@ __device__ __forceinline__ double pl_block_sum(double v, double* red) {
   return t;
 }
 
-// ---- rows of any length, in two kernels -----------------------------------------------------------------------------------
-// A block a row: (m, s) into ms, and its log-probability (POLICY: its terms).
-template <typename T, bool POLICY>
-__global__ void __launch_bounds__(512) pl_stats_kernel(const T* x, const Rows rows, float2* ms, double* lps, const PolicyRow a) {
+// ---- the two passes over a row --------------------------------------------------------------------------------------------------
+// G vectors a thread at a time, NT threads apart: f(vectors, first one's place, whether all are there).  Those past the end are -inf.
+template <typename T, int NT, int G, typename F>
+__device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f) {
+  int i = threadIdx.x;
+  const uint4* p = body + i;
+  uint4 z[G];
+#pragma unroll 1
+  for (; i + (G - 1) * NT < cnt; i += G * NT, p += G * NT) {
+#pragma unroll
+    for (int k = 0; k < G; ++k) z[k] = p[k * NT];
+    f(z, i, true);
+  }
+  if (i < cnt) {
+    constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+#pragma unroll
+    for (int k = 0; k < G; ++k) z[k] = i + k * NT < cnt ? p[k * NT] : make_uint4(low, low, low, low);
+    f(z, i, false);
+  }
+}
+// A thread's part of a row: (B, sum of 2^(x log2 e - B)) of its vectors and the value xe at one of its ends (-inf: none).
+template <typename T, int NT, int G>
+__device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, float& base, float& s) {
+  constexpr int E = Span<T>::E, C = E == 4 ? G : G / 2 < 1 ? 1 : G / 2;        // vectors that are unpacked at a time
+  base = pl_base(xe == xe ? xe : -INFINITY), s = pl_exp(xe, pl_less(base));
+  pl_each<T, NT, G>(body, cnt, [&](const uint4 (&z)[G], int, bool) {
+#pragma unroll
+    for (int k0 = 0; k0 < G; k0 += C) {
+      float v[C][E], top = -INFINITY, q[4] = {};
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        pl_unpack(z[k0 + k], v[k]);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) top = fmaxf(top, fmaxf(v[k][e], v[k][e + 1]));
+      }
+      const float b = pl_base(top);
+      if (b > base) s = pl_moved(s, base, b), base = b;
+      const float less = pl_less(base);
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e & 3] += pl_exp(v[k][e], less);
+      s += (q[0] + q[1]) + (q[2] + q[3]);
+    }
+  });
+}
+// The gradients of a thread's vectors, c 2^(x log2 e - B).
+template <typename T, int NT, int G>
+__device__ __forceinline__ void pl_grads(const uint4* body, uint4* dst, int cnt, float base, float c) {
+  constexpr int E = Span<T>::E;
+  pl_each<T, NT, G>(body, cnt, [&](const uint4 (&z)[G], int i, bool whole) {
+    uint4* o = dst + i;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      float v[E];
+      pl_unpack(z[k], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = pl_exp(v[e], base) * c;
+      if (whole || i + k * NT < cnt) __stcs(o + k * NT, pl_pack(v));
+    }
+  });
+}
+__device__ __forceinline__ void pl_store_zero(uint4* p) { __stcs(p, make_uint4(0u, 0u, 0u, 0u)); }
+// Whether this thread wrote the target's gradient: it is at one of its ends, or among its vectors lo + k, lo + k + NT, ...
+__device__ __forceinline__ bool pl_wrote(long long t, long end, int head, int E, long lo, int cnt, int k, int NT) {
+  const long tv = (long)(t - head) / E - lo;
+  return t >= 0 && (t == end || (t >= head && tv >= 0 && tv < cnt && tv % NT == k));
+}
+
+// ---- policy loss -----------------------------------------------------------------------------------------------------------------
+// Up to 4096 values: NT threads a row, which waits in registers, 16 values a thread, as exponentials until its sum and weight are known; the rows of a
+// block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, logarithm and exponentials in fp64) is some 6 us, so what
+// counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us.)
+__device__ __noinline__ float3 pl_policy_row(const PolicyRow& a, const PolicyIn& in, long r, float xt, float base, double sum) {       // (apart: its fp64 registers beside a row's values would halve the warps)
+  const PolicyOut o = pl_policy(a, in, r, xt, base, sum);
+  return make_float3(base, (float)((double)o.weight * o.part), o.target);
+}
+template <typename T, int NT>
+__global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   using S = Span<T>;
-  __shared__ __align__(8) float red[32];
+  constexpr int E = S::E, VPT = 16 / E, N = 16, W = NT / 32, R = 256 / NT;
+  __shared__ float2 sums[8];
+  __shared__ float3 found[R];                        // base, weight over the sum, the target's gradient
+  const int k = threadIdx.x % NT, mine = threadIdx.x / NT, warp = threadIdx.x >> 5;
+  const long r0 = (long)blockIdx.x * R, r = r0 + mine;
+  const bool there = r < rows.n, scored = there && (!rows.mask || rows.mask[r]);
+  // thread i < R looks after row r0 + i
+  const long rw = r0 + threadIdx.x;
+  const bool forms = threadIdx.x < R && rw < rows.n, weighs = forms && (!rows.mask || rows.mask[rw]);
+  PolicyIn in;
+  float xt = 0.f;
+  if (weighs) in = PolicyIn(a, rw), xt = pl_target(x + (size_t)rw * rows.V, rows.target[rw], rows.V, rw);
+  else if (forms) pl_policy_skip(a, rw);
+  const T* row = x + (size_t)r * rows.V;
+  T* out = grad + (size_t)r * rows.V;
+  const S sp(row, rows.V);
+  const int nv = there ? (int)sp.nv : 0;
+  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
+  const long ie = there ? sp.end_of(k) : -1;
+  float v[N], end = scored && ie >= 0 ? pl_float(row[ie]) : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;       // -inf
+    float u[E];
+    pl_unpack(scored && k + i * NT < nv ? body[k + i * NT] : make_uint4(low, low, low, low), u);
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[i * E + j] = u[j];
+  }
+  float m = end, s[4] = {};
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = fmaxf(m, fmaxf(v[i], v[i + 1]));
+  const float base = pl_base(warp_max(m)), less = pl_less(base);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = pl_exp(v[i], less), s[i & 3] += v[i];
+  end = pl_exp(end, less);
+  const float sum = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end);
+  if (threadIdx.x % 32 == 0) sums[warp] = make_float2(base, sum);
+  __syncthreads();
+  if (weighs) {
+    float top = -INFINITY;
+    double all = 0.0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = fmaxf(top, sums[threadIdx.x * W + i].x);
+#pragma unroll
+    for (int i = 0; i < W; ++i) all += (double)pl_moved(sums[threadIdx.x * W + i].y, sums[threadIdx.x * W + i].x, top);
+    if (top == -INFINITY) all = NAN;                 // a row without a finite value
+    found[threadIdx.x] = pl_policy_row(a, in, rw, xt, pl_less(top), all);
+  }
+  if (!grad) return;
+  __syncthreads();
+  if (!there) return;
+  const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
+  const float c = scored ? pl_exp2(less - f.x) * f.y : 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float u[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) u[j] = scored ? v[i * E + j] * c : 0.f;
+    if (k + i * NT < nv) __stcs(dst + k + i * NT, pl_pack(u));
+  }
+  if (ie >= 0) out[ie] = pl_round<T>(scored ? end * c : 0.f);
+  if (scored) {
+    const long long t = rows.target[r];
+    if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>(f.z);
+  }
+}
+
+// Longer rows: a cluster of CL blocks goes through a row twice, for its sum and for its gradient; the second time the row is still in L2, as long as
+// those in work fit there.  Between the passes the blocks send each other their (B, sum); each adds them up in a fixed order and forms the row's weight for
+// itself.  The cluster's first barrier is passed before another block's shared memory is touched, no block's is after the second.  Both end:
+// every thread of a scored row's cluster comes to them, and nothing before them waits.
+__device__ __forceinline__ uint32_t pl_map(uint32_t addr, int cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ void pl_cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void pl_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  __syncwarp();
+}
+
+template <typename T, int CL, int NT, int G, int BLOCKS>
+__global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
+  using S = Span<T>;
+  constexpr int W = NT / 32;
+  __shared__ float2 sums[W], peers[CL];
+  __shared__ float4 found;                           // base, weight over the sum, the target's gradient
+  const long r = blockIdx.x / CL;
+  const int rank = CL > 1 ? blockIdx.x % CL : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* row = x + (size_t)r * rows.V;
+  T* out = grad + (size_t)r * rows.V;
+  const S sp(row, rows.V);
+  const long per = (sp.nv + CL - 1) / CL, lo = min(sp.nv, rank * per);
+  const int cnt = (int)(min(sp.nv, lo + per) - lo);
+  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head) + lo;
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head) + lo;
+  const long ie = rank == 0 ? sp.end_of(tid) : -1;
+  if (rows.mask && !rows.mask[r]) {
+    if (tid == 0 && rank == 0) pl_policy_skip(a, r);
+    if (grad) {
+      for (int i = tid; i < cnt; i += NT) pl_store_zero(dst + i);
+      if (ie >= 0) out[ie] = pl_round<T>(0.f);
+    }
+    return;
+  }
+  if (CL > 1) pl_cluster_arrive();
+  const long long t = rows.target[r];
+  PolicyIn in;
+  float xt = 0.f;
+  if (tid == 0) in = PolicyIn(a, r), xt = pl_target(row, t, rows.V, r);
+  const float xe = ie >= 0 ? pl_float(row[ie]) : -INFINITY;
+  float base, s;
+  pl_sums<T, NT, G>(body, cnt, xe, base, s);
+  const float top = warp_max(base);
+  s = warp_sum(pl_moved(s, base, top));
+  if (lane == 0) sums[warp] = make_float2(top, s);
+  __syncthreads();
+  if (CL > 1) pl_cluster_wait();
+  if (warp == 0) {
+    const float2 q = lane < W ? sums[lane] : make_float2(-INFINITY, 0.f);
+    const float mine = warp_max(q.x), sum = warp_sum(pl_moved(q.y, q.x, mine));
+    if (CL > 1) {
+      if (lane < CL)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(pl_map(smem_u32(&peers[rank]), lane)), "f"(mine), "f"(sum) : "memory");
+    } else if (lane == 0) {
+      peers[0] = make_float2(mine, sum);
+    }
+  }
+  if (CL > 1) pl_cluster_arrive(), pl_cluster_wait();
+  if (tid == 0) {
+    float all = -INFINITY;
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < CL; ++k) all = fmaxf(all, peers[k].x);
+#pragma unroll
+    for (int k = 0; k < CL; ++k) sum += (double)pl_moved(peers[k].y, peers[k].x, all);
+    if (all == -INFINITY) sum = NAN;                 // a row without a finite value
+    const PolicyOut o = pl_policy(a, in, r, xt, pl_less(all), sum, rank == 0);
+    found = make_float4(pl_less(all), (float)((double)o.weight * o.part), o.target, 0.f);
+  }
+  if (!grad) return;
+  __syncthreads();
+  pl_grads<T, NT, G>(body, dst, cnt, found.x, found.y);
+  if (ie >= 0) out[ie] = pl_round<T>(pl_exp(xe, found.x) * found.y);
+  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, tid, NT)) out[t] = pl_round<T>(found.z);
+}
+
+// ---- preference loss: a row's weight needs its whole sequence -------------------------------------------------------------------
+// A block a row: (B, sum) into ms, and its log-probability.
+template <typename T>
+__global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows rows, float2* ms, double* lps) {
+  using S = Span<T>;
+  constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
+  __shared__ float2 sums[NT / 32];
   const long r = blockIdx.x;
   if (rows.mask && !rows.mask[r]) {
-    if (threadIdx.x == 0) {
-      if (POLICY) pl_policy_skip(a, r);
-      else lps[r] = 0.0;
-    }
+    if (threadIdx.x == 0) lps[r] = 0.0;
     return;
   }
   const T* row = x + (size_t)r * rows.V;
   const S sp(row, rows.V);
-  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
-  float m = -INFINITY;
-  double s = 0.0;                                    // (a thread adds up to V / 512 values: fp32 would lose 1e-6 of 250 000)
-  const long e = sp.end_of(threadIdx.x);
-  if (e >= 0) {
-    m = pl_float(row[e]);
-    s = expf(m - pl_base(m));
-    if (m != m) m = -INFINITY;
-  }
-  constexpr int U = 16 / S::E;                        // vectors in flight: 16 values
-  auto add = [&](const uint4 (&u)[U], int cnt) {
-    float v[U][S::E], n = m, t = 0.f;
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (k >= cnt) break;
-      pl_unpack(u[k], v[k]);
-#pragma unroll
-      for (int j = 0; j < S::E; ++j) n = fmaxf(n, v[k][j]);
-    }
-    if (n > m) s *= (double)expf(m - n), m = n;
-    const float b = pl_base(m);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (k >= cnt) break;
-#pragma unroll
-      for (int j = 0; j < S::E; j += 2) t += expf(v[k][j] - b) + expf(v[k][j + 1] - b);
-    }
-    s += (double)t;
-  };
-  long i = threadIdx.x;
-  for (; i + (U - 1) * 512 < sp.nv; i += U * 512) {
-    uint4 u[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) u[k] = body[i + k * 512];
-    add(u, U);
-  }
-  for (; i < sp.nv; i += 512) {
-    uint4 u[U];
-    u[0] = body[i];
-    add(u, 1);
-  }
-  const float all = block_max(m, red);
-  s = pl_block_sum<16>(s * (double)expf(m - all), reinterpret_cast<double*>(red));
-  if (threadIdx.x == 0) {
-    const double lp = pl_logprob(pl_target(row, rows.target[r], rows.V, r), all, s);
-    ms[r] = make_float2(all, (float)s);
-    if (POLICY) pl_policy(a, r, lp);
-    else lps[r] = lp;
-  }
+  float xt = 0.f, base, s;
+  if (threadIdx.x == 0) xt = pl_target(row, rows.target[r], rows.V, r);
+  const long ie = sp.end_of(threadIdx.x);
+  pl_sums<T, NT, G>(reinterpret_cast<const uint4*>(row + sp.head), (int)sp.nv, ie >= 0 ? pl_float(row[ie]) : -INFINITY, base, s);
+  const float top = warp_max(base);
+  s = warp_sum(pl_moved(s, base, top));
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = make_float2(top, s);
+  __syncthreads();
+  if (threadIdx.x) return;
+  float all = -INFINITY;
+  double sum = 0.0;
+  for (int k = 0; k < NT / 32; ++k) all = fmaxf(all, sums[k].x);
+  for (int k = 0; k < NT / 32; ++k) sum += (double)pl_moved(sums[k].y, sums[k].x, all);
+  if (all == -INFINITY) sum = NAN;
+  ms[r] = make_float2(pl_less(all), (float)sum), lps[r] = pl_low(xt, pl_less(all)) - log(sum);
 }
 
 // Gradients: a block a slice of a row.  weight of row r: weight[r / per].  The last rows first: they are what L2 still holds.
-constexpr int PL_SLICE = 2048;                       // vectors a block
+constexpr int PL_SLICE = 4096;                       // vectors a block
 template <typename T>
-__global__ void __launch_bounds__(256) pl_grad_kernel(const T* x, const Rows rows, const float2* ms, const float* weight, long per, T* grad, int slices) {
+__global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows rows, const float2* ms, const float* weight, long per, T* grad, int slices) {
   using S = Span<T>;
-  const long r = rows.n - 1 - blockIdx.x / slices;
-  const int slice = blockIdx.x % slices;
+  constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
+  const long r = rows.n - 1 - blockIdx.x / slices, lo = (long)(blockIdx.x % slices) * PL_SLICE;
   T* out = grad + (size_t)r * rows.V;
   const T* row = x + (size_t)r * rows.V;
   const S sp(row, rows.V);                           // (the gradient lies as the logits do)
-  const bool scored = !rows.mask || rows.mask[r];
-  const float w = scored ? weight[r / per] : 0.f;
-  const float2 st = scored ? ms[r] : make_float2(0.f, 1.f);
-  const float inv = 1.f / st.y;
-  const long long t = scored ? rows.target[r] : -1;
-  if (slice == 0) {
-    const long e = sp.end_of(threadIdx.x);
-    if (e >= 0) out[e] = pl_round<T>(scored ? (expf(pl_float(row[e]) - st.x) * inv - (e == t ? 1.f : 0.f)) * w : 0.f);
+  const int cnt = (int)max(0l, min(sp.nv - lo, (long)PL_SLICE)), k = threadIdx.x;
+  const long ie = lo == 0 ? sp.end_of(k) : -1;
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head) + lo;
+  if (rows.mask && !rows.mask[r]) {
+    for (int i = k; i < cnt; i += NT) pl_store_zero(dst + i);
+    if (ie >= 0) out[ie] = pl_round<T>(0.f);
+    return;
   }
-  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
-  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
-  const long end = min(sp.nv, (long)(slice + 1) * PL_SLICE);
-#pragma unroll 4
-  for (long i = (long)slice * PL_SLICE + threadIdx.x; i < end; i += 256) {
-    float v[S::E] = {};
-    if (scored) {
-      pl_unpack(body[i], v);
-#pragma unroll
-      for (int j = 0; j < S::E; ++j) v[j] = expf(v[j] - st.x) * inv;
-      const long long at = t - sp.head - i * S::E;
-#pragma unroll
-      for (int j = 0; j < S::E; ++j) v[j] = (v[j] - (at == j ? 1.f : 0.f)) * w;
-    }
-    dst[i] = pl_pack(v);
-  }
+  const float w = weight[(unsigned)r / (unsigned)per];
+  const float2 st = ms[r];
+  const long long t = rows.target[r];
+  pl_grads<T, NT, G>(reinterpret_cast<const uint4*>(row + sp.head) + lo, dst, cnt, st.x, w / st.y);
+  if (ie >= 0) out[ie] = pl_round<T>(pl_exp(pl_float(row[ie]), st.x) * (w / st.y));
+  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, k, NT)) out[t] = pl_round<T>((pl_exp(pl_float(row[t]), st.x) / st.y - 1.f) * w);
 }
 
 // ---- sums over rows, and pairs of sequences ----------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) pl_sum_kernel(const double* v, long n, double scale, float* out) {
-  __shared__ double red[8];
+__global__ void __launch_bounds__(1024) pl_sum_kernel(const double* v, long n, double scale, float* out) {
+  __shared__ double red[32];
   double s = 0.0;
-#pragma unroll 4
-  for (long i = threadIdx.x; i < n; i += 256) s += v[i];
-  s = pl_block_sum<8>(s, red);
+  pdl_wait();                                        // (launched while the rows' kernel runs)
+#pragma unroll 8
+  for (long i = threadIdx.x; i < n; i += 1024) s += v[i];
+  s = pl_block_sum<32>(s, red);
   if (threadIdx.x == 0) *out = (float)(s * scale);
 }
 
@@ -285,12 +498,47 @@ int grad_launch(const void* x, const Rows& rows, const float2* ms, const float* 
   return (int)cudaGetLastError();
 }
 
+template <typename T, int CL, int NT, int G, int BLOCKS>
+int policy_launch(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaStream_t st) {
+  if (rows.n * CL >= 1l << 31) return (int)cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows.n * CL)), cfg.blockDim = dim3(NT), cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, pl_policy_kernel<T, CL, NT, G, BLOCKS>, x, rows, grad, a);
+}
+// The form by a row's length.
+template <typename T>
+int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaStream_t st) {
+  constexpr int E = Span<T>::E;
+  const long V = rows.V;
+  auto brief = [&](auto kern, int per_block) {
+    kern<<<(unsigned)((rows.n + per_block - 1) / per_block), 256, 0, st>>>(x, rows, grad, a);
+    return (int)cudaGetLastError();
+  };
+  if (V <= 512) return brief(pl_policy_short_kernel<T, 32>, 8);
+  if (V <= 1024) return brief(pl_policy_short_kernel<T, 64>, 4);
+  if (V <= 2048) return brief(pl_policy_short_kernel<T, 128>, 2);
+  if (V <= 4096) return brief(pl_policy_short_kernel<T, 256>, 1);
+  // By a row's bytes, since those in work have to stay in L2 (some 40 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
+  // us: 4096 x 8192 60 (256 threads 65), 2048 x 32 768 109 (one block of 512 a row 109, two of 256 112), 1024 x 65 536 113 (eight of 128 111), 1024 x
+  // 248 320 394 (four of 256 437, eight with four blocks an SM 437); bf16 2048 x 49 999 104, 1024 x 131 072 119, 1024 x 248 320 222.
+  constexpr int G = E == 4 ? 8 : 4;                  // 32 values a thread at a time
+  const long bytes = V * (long)sizeof(T);
+  if (bytes <= 64 << 10) return policy_launch<T, 1, 128, 8, 8>(x, rows, grad, a, st);
+  if (bytes <= 192 << 10) return policy_launch<T, E == 4 ? 4 : 2, 128, 8, 8>(x, rows, grad, a, st);
+  if (bytes <= 384 << 10) return policy_launch<T, 4, 256, 4, 5>(x, rows, grad, a, st);
+  return policy_launch<T, 8, 256, G, E == 4 ? 3 : 5>(x, rows, grad, a, st);
+}
+
 bool rows_ok(long n, long V) { return n >= 1 && n < 1l << 31 && V >= 1 && V < 1l << 31; }
 
 }  // namespace
 
 // n rows of V logits, contiguous (type 0: fp32, 1: bf16), anywhere; the gradient (null: not wanted) lies at the same offset from a 16-byte boundary.
-// terms: [4, n] floats: log-probability, ratio, kl, weight; work: n doubles, then (n float2) what the kernels keep.
+// terms: [4, n] floats: log-probability, ratio, kl, weight; work: n doubles.
 TRL_API int trl_policy_loss(const void* x, int type, long n, long V, const void* target, const void* mask, const void* adv, long adv_rows, const void* old,
                             const void* ref, double lo, double hi, double kl, double scale, void* terms, void* clipped, void* loss, void* grad, void* work,
                             void* stream) {
@@ -299,18 +547,12 @@ TRL_API int trl_policy_loss(const void* x, int type, long n, long V, const void*
   cudaStream_t st = (cudaStream_t)stream;
   float* f = (float*)terms;
   double* row_loss = (double*)work;
-  float2* ms = (float2*)(row_loss + n);
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
   const PolicyRow a{(const float*)adv, (const float*)old, (const float*)ref, (int)adv_rows, lo, hi, kl, scale, f, f + n, f + 2 * n, f + 3 * n,
                     (unsigned char*)clipped, row_loss};
-  if (type) pl_stats_kernel<bf16, true><<<(int)n, 512, 0, st>>>((const bf16*)x, rows, ms, nullptr, a);
-  else pl_stats_kernel<float, true><<<(int)n, 512, 0, st>>>((const float*)x, rows, ms, nullptr, a);
-  if (grad) {
-    const int rc = type ? grad_launch<bf16>(x, rows, ms, a.weight, 1, grad, st) : grad_launch<float>(x, rows, ms, a.weight, 1, grad, st);
-    if (rc) return rc;
-  }
-  pl_sum_kernel<<<1, 256, 0, st>>>(row_loss, n, scale, (float*)loss);
-  return (int)cudaGetLastError();
+  const int rc = type ? policy_rows((const bf16*)x, rows, (bf16*)grad, a, st) : policy_rows((const float*)x, rows, (float*)grad, a, st);
+  if (rc) return rc;
+  return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, row_loss, n, scale, (float*)loss);
 }
 
 // 2 pairs sequences of T rows, chosen and rejected in turn.  totals [2 pairs], margins [pairs]; work: 2 pairs T doubles, as many
@@ -326,16 +568,15 @@ TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, lon
   double* pair_loss = (double*)(ms + n);
   float* weight = (float*)(pair_loss + pairs);
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
-  if (type) pl_stats_kernel<bf16, false><<<(int)n, 512, 0, st>>>((const bf16*)x, rows, ms, lps, PolicyRow{});
-  else pl_stats_kernel<float, false><<<(int)n, 512, 0, st>>>((const float*)x, rows, ms, lps, PolicyRow{});
+  if (type) pl_stats_kernel<bf16><<<(int)n, 256, 0, st>>>((const bf16*)x, rows, ms, lps);
+  else pl_stats_kernel<float><<<(int)n, 256, 0, st>>>((const float*)x, rows, ms, lps);
   pl_pairs_kernel<<<(int)pairs, 256, 0, st>>>(lps, (const float*)ref, rows.mask, T, beta, smooth, average, scale, (float*)totals, (float*)margins, pair_loss,
                                               weight);
   if (grad) {
     const int rc = type ? grad_launch<bf16>(x, rows, ms, weight, T, grad, st) : grad_launch<float>(x, rows, ms, weight, T, grad, st);
     if (rc) return rc;
   }
-  pl_sum_kernel<<<1, 256, 0, st>>>(pair_loss, pairs, scale, (float*)loss);
-  return (int)cudaGetLastError();
+  return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, pair_loss, pairs, scale, (float*)loss);
 }
 
 TRL_API int trl_loss_scale(void* x, int type, const void* up, long n, void* stream) {

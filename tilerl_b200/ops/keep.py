@@ -67,7 +67,7 @@ class Kept8:
         q = self.q
         if not (q.is_cuda and q.numel() and N.has("trl_keep_unpack")):
             return unpack(q, self.scale)
-        with torch.cuda.device(q.device):
+        with N.on(q.device):
             out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
             N.check(N.lib().trl_keep_unpack(q.data_ptr(), self.scale.data_ptr(), out.data_ptr(), q.numel() // q.shape[-1], q.shape[-1], N.stream()), "keep_unpack")
         N.count()
@@ -81,7 +81,7 @@ def keep8(x: torch.Tensor) -> Kept8:
     if not _takes(x):
         return Kept8(*pack(x))
     x = x.contiguous()
-    with torch.cuda.device(x.device):
+    with N.on(x.device):
         kept = Kept8(*_empty(x))
         N.check(N.lib().trl_keep_pack(x.data_ptr(), kept.q.data_ptr(), kept.scale.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], N.stream()), "keep_pack")
     N.count()
@@ -95,7 +95,7 @@ def swiglu_takes(gu: torch.Tensor) -> bool:
 def swiglu(gu: torch.Tensor) -> Tuple[torch.Tensor, Kept8]:
     """SwiGLU of interleaved (gate, up) pairs, and the pairs in 8 bits."""
     gu = gu.contiguous()
-    with torch.cuda.device(gu.device):
+    with N.on(gu.device):
         out, kept = torch.empty(*gu.shape[:-1], gu.shape[-1] // 2, dtype=torch.float32, device=gu.device), Kept8(*_empty(gu))
         N.check(N.lib().trl_keep_swiglu(gu.data_ptr(), kept.q.data_ptr(), kept.scale.data_ptr(), out.data_ptr(), gu.numel() // gu.shape[-1], gu.shape[-1],
                                         N.stream()), "keep_swiglu")
@@ -105,7 +105,7 @@ def swiglu(gu: torch.Tensor) -> Tuple[torch.Tensor, Kept8]:
 
 def swiglu_grad(kept: Kept8, g: torch.Tensor) -> torch.Tensor:
     g, q = g.float().contiguous(), kept.q
-    with torch.cuda.device(q.device):
+    with N.on(q.device):
         d = torch.empty(q.shape, dtype=torch.float32, device=q.device)
         N.check(N.lib().trl_keep_swiglu_grad(q.data_ptr(), kept.scale.data_ptr(), g.data_ptr(), d.data_ptr(), q.numel() // q.shape[-1], q.shape[-1], N.stream()),
                 "keep_swiglu_grad")

@@ -8,6 +8,7 @@ the library on a machine where it cannot be loaded raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_float, c_int, c_long, c_longlong, c_void_p
@@ -238,6 +239,14 @@ def stream() -> int:
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda d: torch.cuda.current_stream(d).cuda_stream)
 _device = getattr(torch._C, "_cuda_getDevice", lambda: torch.cuda.current_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """``torch.cuda.device(device)``, which costs 4 us a time, where it is not the current one already."""
+    return _HERE if device.index == _device() else torch.cuda.device(device)
 
 
 def read_error(clear: bool = True):

@@ -539,11 +539,13 @@ def _logits_grad(e, s, targets, weight, dtype):
 
 def policy_loss(logits, targets, mask, adv, old, ref, *, lo, hi, kl, scale, want_grad=True):
     """``scale * sum over scored rows of (-min(rho A, clip(rho, lo, hi) A) + kl * k3)`` with ``rho = exp(lp - old)`` and
-    ``k3 = e^d - d - 1``, ``d = ref - lp``.  Returns the loss, terms ``[4, rows]`` (log-probability, ratio, k3, weight), which rows were clipped
+    ``k3 = e^d - d - 1``, ``d = ref - lp``.  Returns the loss, terms (log-probability, ratio, k3, weight), which rows were clipped
     and the logits' gradient ``weight * (softmax - onehot)``.  A row's terms are formed in 64 bits: d and k3 are small differences of
     large numbers, and the clipping's border decides about a whole row."""
+    shape, flat = targets.shape, lambda t: None if t is None else t.reshape(-1)
+    logits, targets, mask, old, ref = logits.reshape(-1, logits.shape[-1]), flat(targets), flat(mask), flat(old), flat(ref)
     e, s, tg, lp = _scored_rows(logits, targets, mask)
-    a = adv.double().repeat_interleave(targets.numel() // max(1, adv.numel()))
+    a = adv.reshape(-1).double().repeat_interleave(targets.numel() // max(1, adv.numel()))
     rho = torch.ones_like(lp) if old is None else torch.exp(lp - old.double())
     clipped = ((rho > hi) & (a > 0)) | ((rho < lo) & (a < 0))
     held = torch.where(a > 0, torch.full_like(a, hi), torch.full_like(a, lo))
@@ -560,8 +562,8 @@ def policy_loss(logits, targets, mask, adv, old, ref, *, lo, hi, kl, scale, want
     w = keep(w) * scale
     loss = -(keep(gain).sum() * scale)
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    terms = torch.stack([lp, keep(rho), keep(k3), w]).to(wide)
-    return loss.to(wide), terms, keep(clipped), _logits_grad(e, s, tg, w, logits.dtype) if want_grad else None
+    terms = tuple(t.to(wide).view(shape) for t in (lp, keep(rho), keep(k3), w))
+    return loss.to(wide), terms, keep(clipped).view(shape), _logits_grad(e, s, tg, w, logits.dtype) if want_grad else None
 
 
 def preference_loss(logits, targets, mask, ref, *, beta, smooth, average, scale, want_grad=True):
@@ -570,6 +572,7 @@ def preference_loss(logits, targets, mask, ref, *, beta, smooth, average, scale,
     the logits' gradient."""
     n, t = targets.shape
     flat = None if mask is None else mask.reshape(-1)
+    logits = logits.reshape(-1, logits.shape[-1])
     e, s, tg, lp = _scored_rows(logits, targets.reshape(-1), flat)
     gap = lp if ref is None else lp - ref.reshape(-1).double()
     if flat is not None:

@@ -168,7 +168,7 @@ register("any", "sm100", {
     "train_attention": Kernel("tr_attn_prep_kernel + tr_softmax_kernel + tr_attn_gate_kernel", "csrc/train.cu", "trl_train_attn_prep", "tilerl_b200.ops.train_kernels",
                               note="norms, rotation, masked softmax, gate and their gradients; the products are library GEMMs"),
     "train_cross_entropy": Kernel("tr_lse_kernel + tr_ce_grad_kernel", "csrc/train.cu", "trl_train_lse", "tilerl_b200.ops.train_kernels"),
-    "train_policy_loss": Kernel("pl_stats_kernel + pl_grad_kernel + pl_sum_kernel", "csrc/policy.cu", "trl_policy_loss", "tilerl_b200.ops.loss_kernels",
+    "train_policy_loss": Kernel("pl_policy_kernel + pl_policy_short_kernel + pl_sum_kernel", "csrc/policy.cu", "trl_policy_loss", "tilerl_b200.ops.loss_kernels",
                                 note="clipped policy loss with a KL term, fp32 or bf16 logits"),
     "train_preference_loss": Kernel("pl_stats_kernel + pl_pairs_kernel + pl_grad_kernel", "csrc/policy.cu", "trl_preference_loss", "tilerl_b200.ops.loss_kernels"),
     "score_tokens": Kernel("score_kernel + score_join_kernel", "csrc/score.cu", "trl_score", "tilerl_b200.ops.score",

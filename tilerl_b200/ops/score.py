@@ -28,7 +28,7 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def score(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``h [rows, H]``, ``targets`` int64 and ``mask`` (bool or None) ``[rows]``."""
     lib, (v, hidden) = N.lib(), w.shape
-    with torch.cuda.device(h.device):
+    with N.on(h.device):
         h, w = _aligned(h), _aligned(w)
         n, kind = h.shape[0], int(h.dtype == torch.bfloat16)
         lp = torch.empty(n, dtype=torch.float32, device=h.device)

@@ -48,6 +48,7 @@ class Tape:
         self.leaves: Dict[int, torch.Tensor] = {}
         self.made: set = set()            # ids of the recorded ops' outputs
         self.gone: Dict[int, tuple] = {}  # id of a tensor let go of: (weak reference, its stand-in)
+        self.one: Optional[torch.Tensor] = None       # in the backward pass: the root's own gradient, where none was given
         self.tp_group, self.tp_world = tp_group, tp_world
         self.enabled = True
 
@@ -99,7 +100,9 @@ class Tape:
     def backward(self, root: torch.Tensor, grad: Optional[torch.Tensor] = None,
                  on_grad: Optional[Callable[[torch.Tensor, torch.Tensor], None]] = None
                  ) -> Dict[int, torch.Tensor]:
-        grads: Dict[int, torch.Tensor] = {id(self._key(root)): torch.ones_like(root) if grad is None else grad}
+        if grad is None:
+            grad = self.one = torch.ones_like(root)
+        grads: Dict[int, torch.Tensor] = {id(self._key(root)): grad}
         # first node (in forward order) that reads each leaf = last to contribute in reverse
         first_use: Dict[int, int] = {}
         for idx, n in enumerate(self.nodes):
@@ -127,6 +130,7 @@ class Tape:
         self.nodes.clear()
         self.made.clear()
         self.gone.clear()
+        self.one = None
         return {k: g for k, g in grads.items() if k in self.leaves}
 
     def grad_of(self, grads: Dict[int, torch.Tensor], t: torch.Tensor) -> Optional[torch.Tensor]:
@@ -684,8 +688,8 @@ def _loss_inputs(what: str, logits, targets, mask, **floats):
         if t is not None and t.device != logits.device:
             raise ValueError(f"{what}: logits are on {logits.device}, another input on {t.device}")
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    flat = lambda t, dtype: None if t is None else t.reshape(-1).to(dtype).contiguous()
-    return (flat(targets, torch.int64), flat(mask, torch.bool)) + tuple(flat(t, wide) for t in floats.values())
+    ready = lambda t, dtype: t if t is None or (t.dtype == dtype and t.is_contiguous()) else t.to(dtype).contiguous()
+    return (ready(targets, torch.int64), ready(mask, torch.bool)) + tuple(ready(t, wide) for t in floats.values())
 
 
 def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
@@ -694,7 +698,9 @@ def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
     grad = grad.view(logits.shape)
 
     def bwd(g):
-        if K is not None and g.numel() == 1 and g.device == loss.device:
+        if g is tape.one:
+            return (grad,)
+        if K is not None and g.numel() == 1 and g.device == grad.device:
             return (K.scale_grad(grad, g),)
         return (grad * g,)
 
@@ -726,13 +732,13 @@ def policy_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, advanta
     if tuple(advantages.shape) not in (tuple(targets.shape), tuple(targets.shape[:1])) or not advantages.is_floating_point() or advantages.device != logits.device:
         raise ValueError(f"policy_loss: advantages are floating point {tuple(targets.shape)} or {tuple(targets.shape[:1])} on {logits.device}, "
                          f"got {tuple(advantages.shape)} {advantages.dtype} on {advantages.device}")
-    adv = advantages.reshape(-1).to(torch.float64 if logits.dtype == torch.float64 else torch.float32).contiguous()
+    adv = advantages.to(torch.float64 if logits.dtype == torch.float64 else torch.float32).contiguous()
     K = _loss_kernels(logits)
     args = dict(lo=1.0 - clip_eps, hi=1.0 + (clip_eps if clip_eps_high is None else clip_eps_high), kl=float(kl_coef), scale=float(scale),
                 want_grad=tape.enabled and tape.wants(logits))
-    loss, terms, clipped, grad = (K.policy if K is not None else ref.policy_loss)(logits.reshape(-1, logits.shape[-1]), tg, mk, adv, old, refs, **args)
+    loss, terms, clipped, grad = (K.policy if K is not None else ref.policy_loss)(logits, tg, mk, adv, old, refs, **args)
     _record_loss(tape, "policy_loss", logits, loss, grad, K)
-    return loss, PolicyTerms(*terms.view(4, *targets.shape), clipped.view(targets.shape))
+    return loss, PolicyTerms(*terms, clipped)
 
 
 @_nograd
@@ -752,12 +758,10 @@ def preference_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, mas
     if tape.tp_world > 1:
         raise ValueError("preference_loss takes whole rows of logits, not a sharded vocabulary")
     tg, mk, refs = _loss_inputs("preference_loss", logits, targets, mask, ref_logprobs=ref_logprobs)
-    K, shape = _loss_kernels(logits), targets.shape
+    K = _loss_kernels(logits)
     args = dict(beta=float(beta), smooth=float(label_smoothing), average=bool(average), want_grad=tape.enabled and tape.wants(logits),
-                scale=1.0 / max(1, shape[0] // 2) if scale is None else float(scale))
-    view = lambda t: None if t is None else t.view(shape)
-    loss, totals, margins, grad = (K.preference if K is not None else ref.preference_loss)(logits.reshape(-1, logits.shape[-1]), tg.view(shape), view(mk),
-                                                                                          view(refs), **args)
+                scale=1.0 / max(1, logits.shape[0] // 2) if scale is None else float(scale))
+    loss, totals, margins, grad = (K.preference if K is not None else ref.preference_loss)(logits, tg, mk, refs, **args)
     _record_loss(tape, "preference_loss", logits, loss, grad, K)
     return loss, PreferenceTerms(totals, margins)
 
