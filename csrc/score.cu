@@ -234,6 +234,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
 // A block a scored row: its tiles together.
 __global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, float* lp, float* entropy) {
   __shared__ float red[32];
+  pdl_wait();
   const int row = blockIdx.x, n = p.count ? *p.count : p.n;
   if (row >= n) return;
   const float2* part = p.part + (size_t)row * p.parts;
@@ -260,6 +261,45 @@ __global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, floa
     lp[to] = (float)((double)p.xt[row] - (double)m - log_s);
   }
   if (entropy) entropy[to] = (float)(log_s - (double)u / (double)s);
+}
+
+// Few rows: their logits [n, ldo] are there; a block a row and SC_PART words of it.
+constexpr int SC_PART = 4096;
+__global__ void __launch_bounds__(256) score_part_kernel(const float* x, long ldo, const ScoreArgs p) {
+  __shared__ float red[32];
+  pdl_wait();
+  const int row = blockIdx.y, n = p.count ? *p.count : p.n;
+  if (row >= n) return;
+  const int c0 = blockIdx.x * SC_PART + threadIdx.x * 4;
+  const float* at = x + (size_t)row * ldo + c0;
+  float4 v[4];
+  float m = -INFINITY, s = 0.f, u = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = c0 + k * 1024;
+    v[k] = c < p.V ? *reinterpret_cast<const float4*>(at + k * 1024) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (c + 1 >= p.V) v[k].y = -INFINITY;            // (the last vector of a row may reach past it)
+    if (c + 2 >= p.V) v[k].z = -INFINITY;
+    if (c + 3 >= p.V) v[k].w = -INFINITY;
+    m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+  }
+  m = block_max(m, red);
+  const float base = m == -INFINITY ? 0.f : m;
+  auto one = [&](float x) {
+    const float d = x - base, e = expf(d);
+    s += e;
+    if (e > 0.f) u += e * d;
+  };
+#pragma unroll
+  for (int k = 0; k < 4; ++k) one(v[k].x), one(v[k].y), one(v[k].z), one(v[k].w);
+  s = block_sum(s, red);
+  if (p.part_u) u = block_sum(u, red);
+  if (threadIdx.x) return;
+  const size_t o = (size_t)row * p.parts + blockIdx.x;
+  p.part[o] = make_float2(m, s);
+  if (p.part_u) p.part_u[o] = u;
+  const long long t = p.target[p.index ? p.index[row] : row];
+  if (t >= 0 && t < p.V && t / SC_PART == blockIdx.x) p.xt[row] = x[(size_t)row * ldo + t];
 }
 
 // Indices of the scored rows in order, and their number; results of the others are 0.  One block.
@@ -363,14 +403,21 @@ int score_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& 
   return (int)cudaLaunchKernelEx(&cfg, score_kernel<ENTROPY>, mh, mw, p);
 }
 
+// Up to so many rows the head's kernel for decode ticks streams the words (its MMA has them as rows, and as many columns as there are hidden rows), and
+// their logits, 1 MB a row of 248 320, go through L2: an MMA of 256 rows here, most of them empty, takes longer than the words from memory.  Pairs and
+// this, us: 248 320 x 5120 1 row 562, 388 (389 to read W), 32 rows 441, 411, 40 rows 445, 431, 64 rows 449, 445; 32 768 x 1024 1 row 40, 30, 33 rows 34, 34.
+constexpr int SC_FEW = 32;
 int score_parts(int V) { return (V + SC_WORDS - 1) / SC_WORDS * 2; }
 
 }  // namespace
+
+TRL_API int trl_head_bf16(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream);
 
 // Bytes of workspace for n rows (of which the scored ones are gathered, `packed`), a multiple of 256.
 TRL_API long trl_score_workspace(int n, int H, int V, int packed, int entropy) {
   long b = (long)n * score_parts(V) * (entropy ? 12 : 8) + 4l * n * 2 + 512;
   if (packed) b += 2l * n * H + 512;
+  if (n <= SC_FEW) b += 4l * n * ((V + 3) / 4 * 4) + 512;
   return (b + 255) / 256 * 256;
 }
 // h [n, H] (type 0: fp32, 1: bf16), w [V, H] bf16, both contiguous and 16-byte aligned, H % 8 == 0; target int64 [n]; mask bytes [n] or null; lp and entropy
@@ -400,11 +447,18 @@ TRL_API int trl_score(const void* h, int type, const void* w, const void* target
     if (type == 0) score_pack_kernel<float><<<n, 256, 0, st>>>((const float*)h, rows, n, H, index, count);
     else score_pack_kernel<bf16><<<n, 256, 0, st>>>((const bf16*)h, rows, n, H, index, count);
   }
+  if (n <= SC_FEW) {
+    const long ldo = (V + 3) / 4 * 4;
+    float* logits = (float*)take(4l * n * ldo);
+    const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, 0, 0, (V + SC_PART - 1) / SC_PART};
+    int rc = trl_head_bf16(packed ? rows : h, w, logits, ldo, n, V, H, stream);
+    if (!rc) rc = (int)trl_launch(score_part_kernel, dim3(p.parts, n), dim3(256), 0, st, (const float*)logits, ldo, p);
+    return rc ? rc : (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
+  }
   CUtensorMap mh, mw;
   if (!score_map(&mh, packed ? rows : h, n, H) || !score_map(&mw, w, V, H)) return (int)cudaErrorInvalidValue;
   const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, (H + SC_KT - 1) / SC_KT, v_tiles, parts};
   const int rc = entropy ? score_launch<true>(mh, mw, p, st) : score_launch<false>(mh, mw, p, st);
   if (rc) return rc;
-  score_join_kernel<<<n, 128, 0, st>>>(p, (float*)lp, (float*)entropy);
-  return (int)cudaGetLastError();
+  return (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
 }

@@ -11,6 +11,7 @@ N.register("trl_score_workspace", [N.I] * 5, N.L)
 N.register("trl_score", [N.P, N.I, N.P, N.P, N.P] + [N.I] * 3 + [N.P] * 4)
 
 ROWS = 8192               # a call: the tiles' parts of as many rows over 248 320 words are 127 MB
+FEW = 32                  # rows that go through the decode ticks' head and a pass over their logits
 CHUNK = 256               # rows of logits that the torch form has at a time
 
 
@@ -40,7 +41,7 @@ def score(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[to
             work = torch.empty(lib.trl_score_workspace(m, hidden, v, packed, int(entropy)), dtype=torch.uint8, device=h.device)
             N.check(lib.trl_score(h[some].data_ptr(), kind, w.data_ptr(), targets[some].data_ptr(), None if mask is None else mask[some].data_ptr(), m, hidden, v,
                                   lp[some].data_ptr(), ent[some].data_ptr() if entropy else None, work.data_ptr(), N.stream()), "score")
-            N.count(2 + packed + int(mask is not None))
+            N.count(2 + packed + int(mask is not None) + int(m <= FEW))
     return lp, ent
 
 
