@@ -7,7 +7,9 @@
 // few hundred rows on, by the reading of W below.  Pairs of SMs (`cta_group::2`) share a tile: 128 hidden rows each as the MMA's A, half of the
 // 256 words each as its B, so that a k-block of 64 brings 32 KB to an SM for 512 clocks of MMAs (one SM alone: 48 KB, more than L2
 // gives to all of them).  Two accumulators of 256 columns fill TMEM: a tile's epilogue runs beside the next one's products.  Rows are the
-// TMEM lanes, so a thread has a row's values and no two threads meet.  The tiles go round the pairs words by words over up to 2048
+// TMEM lanes, so a thread has a row's values and no two threads meet.  The tensor cores cut off what they add up, so that 5120 terms in one accumulator
+// lose 1e-6 of lp; an accumulator has at most 2048 of them, and the epilogue adds the accumulators in registers (1 to 3 % of the time; with 1024
+// 3 to 5 %).  Where there is one, it goes through a row's values as they come from TMEM.  The tiles go round the pairs words by words over up to 2048
 // rows at a time: pairs that run together read the same words, and W comes from memory once for 2048 rows.
 //
 // Exponentials are ex2.approx of (x - m) log2(e): its 2^-22 and the rounding of far arguments are averages over the words of a row, below
@@ -24,6 +26,7 @@ namespace {
 constexpr int SC_ROWS = 128, SC_WORDS = 256, SC_KT = 64;       // rows an SM, words a tile, k a stage
 constexpr int SC_THREADS = 320, SC_STAGES = 7, SC_STAGE = 2 * SC_ROWS * SC_KT * 2;
 constexpr int SC_SMEM = SC_STAGES * SC_STAGE + 1024 + 256;
+constexpr int SC_SEGMENT = 2048;                                // values of k whose products an accumulator adds up
 constexpr int SC_GROUP = 8;                                     // tiles of 256 rows that go through the words together
 static_assert(SC_SMEM >= 208 * 1024 && SC_SMEM <= 227 * 1024, "no other kernel with TMEM fits beside it on an SM");
 constexpr int SC_SITE = 17;                                     // of trl_set_error
@@ -35,7 +38,7 @@ struct ScoreArgs {
   float2* part;                // [n, parts] (m, s)
   float* part_u;               // [n, parts], or null
   float* xt;                   // [n]
-  int n, V, nk, v_tiles, parts;
+  int n, V, nk, v_tiles, parts, segments;
 };
 
 __device__ __forceinline__ void sc_mma(uint32_t d, uint32_t alo, uint32_t blo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
@@ -58,7 +61,8 @@ __device__ __forceinline__ void sc_unit(int u, int r_tiles, int v_tiles, int& rt
   vt = left / rows, rt = g * SC_GROUP + left - vt * rows;
 }
 
-template <bool ENTROPY>
+// WHOLE: one accumulator a tile.
+template <bool ENTROPY, bool WHOLE>
 __global__ void __launch_bounds__(SC_THREADS, 1)
 score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, const ScoreArgs p) {
   constexpr int S = SC_STAGES;
@@ -89,6 +93,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
   gp_cluster_sync();                                // both halves are allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();                                       // (the rows and their number come from the kernels before)
   const int n = p.count ? min(*p.count, p.n) : p.n, r_tiles = (n + 2 * SC_ROWS - 1) / (2 * SC_ROWS), units = r_tiles * p.v_tiles;
 
   if (warp == 0) {
@@ -127,23 +132,25 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
       int st = 0, count = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int u = pair; ok && u < units; u += pairs, ++count) {
-        const int buf = count & 1;
-        if (count >= 2) {
-          if (!(ok = mbar_wait(acc_empty(buf), (uint32_t)((count >> 1) - 1) & 1u, abort_flag))) break;
-          tc_fence_after();
-        }
-        const uint32_t acc = tmem_base + (uint32_t)buf * SC_WORDS;
-        for (int kt = 0; kt < p.nk; ++kt) {
-          if (!(ok = mbar_wait(full(st), ph, abort_flag))) break;
-          tc_fence_after();
-          const uint32_t a = lo0 + (uint32_t)st * (uint32_t)(SC_STAGE >> 4), b = a + (uint32_t)(SC_STAGE / 2 >> 4);
+      for (int u = pair; ok && u < units; u += pairs) {
+        for (int seg = 0; ok && seg < p.segments; ++seg, ++count) {
+          const int buf = count & 1, k0 = seg * p.nk / p.segments, k1 = (seg + 1) * p.nk / p.segments;
+          if (count >= 2) {
+            if (!(ok = mbar_wait(acc_empty(buf), (uint32_t)((count >> 1) - 1) & 1u, abort_flag))) break;
+            tc_fence_after();
+          }
+          const uint32_t acc = tmem_base + (uint32_t)buf * SC_WORDS;
+          for (int kt = k0; kt < k1; ++kt) {
+            if (!(ok = mbar_wait(full(st), ph, abort_flag))) break;
+            tc_fence_after();
+            const uint32_t a = lo0 + (uint32_t)st * (uint32_t)(SC_STAGE >> 4), b = a + (uint32_t)(SC_STAGE / 2 >> 4);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc_mma(acc, a + i * 2, b + i * 2, hi, idesc, kt || i ? 1u : 0u);
-          gp_commit(empty(st), 3);
-          if (++st == S) st = 0, ph ^= 1u;
+            for (int i = 0; i < 4; ++i) sc_mma(acc, a + i * 2, b + i * 2, hi, idesc, kt > k0 || i ? 1u : 0u);
+            gp_commit(empty(st), 3);
+            if (++st == S) st = 0, ph ^= 1u;
+          }
+          if (ok) gp_commit(acc_full(buf), 3);
         }
-        if (ok) gp_commit(acc_full(buf), 3);
       }
     }
     __syncwarp();
@@ -153,43 +160,31 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
     constexpr float L2E = 1.4426950408889634f;
     const uint32_t even_empty = gp_map(acc_empty(0), 0);
     int count = 0;
-    for (int u = pair; u < units; u += pairs, ++count) {
+    bool ok = true;
+    for (int u = pair; ok && u < units; u += pairs) {
       int rt, vt;
       sc_unit(u, r_tiles, p.v_tiles, rt, vt);
-      const int buf = count & 1, row = (rt * 2 + rank) * SC_ROWS + quad * 32 + lane, col0 = vt * SC_WORDS + half * (SC_WORDS / 2);
+      const int row = (rt * 2 + rank) * SC_ROWS + quad * 32 + lane, col0 = vt * SC_WORDS + half * (SC_WORDS / 2);
       const bool mine = row < n;
       const long long t = mine ? p.target[p.index ? p.index[row] : row] : -1;
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full(buf), (uint32_t)(count >> 1) & 1u, abort_flag))) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * SC_WORDS + half * (SC_WORDS / 2));
       float m = -INFINITY, s = 0.f, w = 0.f;
-#pragma unroll
-      for (int c = 0; c < SC_WORDS / 2; c += 32) {
-        uint32_t r[32];
-        __syncwarp();                               // (the branches below part the lanes)
-        tc_ld32(taddr + (uint32_t)c, r);
-        tc_wait_ld();
-        if (c + 32 == SC_WORDS / 2) {               // read out: the accumulator goes back
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_empty + 8u * buf) : "memory");
-        }
+      auto take = [&](float (&x)[32], int c) {      // 32 of the row's values, from word col0 + c on
         if (col0 + c + 32 > p.V) {                  // past the last word
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (col0 + c + i >= p.V) r[i] = 0xff800000u;
+            if (col0 + c + i >= p.V) x[i] = -INFINITY;
         }
         const long long at = t - col0 - c;
         if (at >= 0 && at < 32 && t < p.V) {
-          float x = 0.f;
+          float xt = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (at == i) x = __uint_as_float(r[i]);
-          p.xt[row] = x;
+            if (at == i) xt = x[i];
+          p.xt[row] = xt;
         }
         float best = m;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) best = fmaxf(best, __uint_as_float(r[i]));
+        for (int i = 0; i < 32; ++i) best = fmaxf(best, x[i]);
         const float base = best == -INFINITY ? 0.f : best;
         if (best > m) {
           const float f = sc_exp2((m - base) * L2E);       // (0 for the first)
@@ -199,12 +194,58 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
         float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float x = __uint_as_float(r[i]) - base, y = __uint_as_float(r[i + 1]) - base, e = sc_exp2(x * L2E), f = sc_exp2(y * L2E);
+          const float d = x[i] - base, g = x[i + 1] - base, e = sc_exp2(d * L2E), f = sc_exp2(g * L2E);
           a0 += e, a1 += f;
-          if (ENTROPY) b0 += e > 0.f ? e * x : 0.f, b1 += f > 0.f ? f * y : 0.f;     // (no -inf times 0)
+          if (ENTROPY) b0 += e > 0.f ? e * d : 0.f, b1 += f > 0.f ? f * g : 0.f;     // (no -inf times 0)
         }
         s += a0 + a1;
         if (ENTROPY) w += b0 + b1;
+      };
+      auto tmem = [&](int buf) { return tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * SC_WORDS + half * (SC_WORDS / 2)); };
+      auto wait = [&](int buf) {
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_full(buf), (uint32_t)(count >> 1) & 1u, abort_flag));
+        tc_fence_after();
+        return ok;
+      };
+      auto give_back = [&](int buf) {               // read out: the accumulator goes back
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_empty + 8u * buf) : "memory");
+      };
+      if (WHOLE) {
+        const int buf = count & 1;
+        if (!wait(buf)) break;
+#pragma unroll
+        for (int c = 0; c < SC_WORDS / 2; c += 32) {
+          uint32_t r[32];
+          float x[32];
+          __syncwarp();                             // (the branches in `take` part the lanes)
+          tc_ld32(tmem(buf) + (uint32_t)c, r);
+          tc_wait_ld();
+          if (c + 32 == SC_WORDS / 2) give_back(buf);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+          take(x, c);
+        }
+        ++count;
+      } else {
+        float x[SC_WORDS / 64][32] = {};            // the thread's logits: the sums of the accumulators, as they come
+        for (int seg = 0; seg < p.segments; ++seg, ++count) {
+          const int buf = count & 1;
+          if (!wait(buf)) break;
+#pragma unroll
+          for (int c = 0; c < SC_WORDS / 64; ++c) {
+            uint32_t r[32];
+            tc_ld32(tmem(buf) + (uint32_t)c * 32, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[c][i] += __uint_as_float(r[i]);
+          }
+          give_back(buf);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < SC_WORDS / 64; ++c) take(x[c], c * 32);
       }
       if (mine) {
         const size_t o = (size_t)row * p.parts + vt * 2 + half;
@@ -331,6 +372,7 @@ __global__ void __launch_bounds__(1024) score_rows_kernel(const unsigned char* m
 // The scored rows in bf16, one behind the other.
 template <typename T>
 __global__ void __launch_bounds__(256) score_pack_kernel(const T* h, bf16* out, int n, int H, const int* index, const int* count) {
+  pdl_wait();
   const int row = blockIdx.x;
   if (count && row >= *count) return;
   const T* src = h + (size_t)(index ? index[row] : row) * H;
@@ -366,12 +408,12 @@ bool score_map(CUtensorMap* m, const void* base, long rows, long K) {
 }
 
 // Pairs of SMs that run at a time.
-template <bool ENTROPY>
+template <bool ENTROPY, bool WHOLE>
 int score_pairs() {
   static TrlPerDevice<int> counts;
   int& known = counts.here();
   if (known == 0) {
-    auto kern = score_kernel<ENTROPY>;
+    auto kern = score_kernel<ENTROPY, WHOLE>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2), cfg.blockDim = dim3(SC_THREADS), cfg.dynamicSmemBytes = SC_SMEM;
     cudaLaunchAttribute attr[1];
@@ -389,18 +431,20 @@ int score_pairs() {
   return known;
 }
 
-template <bool ENTROPY>
+template <bool ENTROPY, bool WHOLE>
 int score_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& p, cudaStream_t st) {
-  const int most = score_pairs<ENTROPY>();
+  const int most = score_pairs<ENTROPY, WHOLE>();
   if (most < 1) return (int)cudaErrorInvalidConfiguration;
   const long units = (long)((p.n + 2 * SC_ROWS - 1) / (2 * SC_ROWS)) * p.v_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (unsigned)(units < most ? units : most)), cfg.blockDim = dim3(SC_THREADS), cfg.dynamicSmemBytes = SC_SMEM, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, score_kernel<ENTROPY>, mh, mw, p);
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = g_trl_use_pdl ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, score_kernel<ENTROPY, WHOLE>, mh, mw, p);
 }
 
 // Up to so many rows the head's kernel for decode ticks streams the words (its MMA has them as rows, and as many columns as there are hidden rows), and
@@ -444,21 +488,23 @@ TRL_API int trl_score(const void* h, int type, const void* w, const void* target
   bf16* rows = packed ? (bf16*)take(2l * n * H) : nullptr;
   if (mask) score_rows_kernel<<<1, 1024, 0, st>>>((const unsigned char*)mask, n, index, count, (float*)lp, (float*)entropy);
   if (packed) {
-    if (type == 0) score_pack_kernel<float><<<n, 256, 0, st>>>((const float*)h, rows, n, H, index, count);
-    else score_pack_kernel<bf16><<<n, 256, 0, st>>>((const bf16*)h, rows, n, H, index, count);
+    const cudaError_t rc = type == 0 ? trl_launch(score_pack_kernel<float>, dim3(n), dim3(256), 0, st, (const float*)h, rows, n, H, (const int*)index, (const int*)count)
+                                     : trl_launch(score_pack_kernel<bf16>, dim3(n), dim3(256), 0, st, (const bf16*)h, rows, n, H, (const int*)index, (const int*)count);
+    if (rc != cudaSuccess) return (int)rc;
   }
   if (n <= SC_FEW) {
     const long ldo = (V + 3) / 4 * 4;
     float* logits = (float*)take(4l * n * ldo);
-    const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, 0, 0, (V + SC_PART - 1) / SC_PART};
+    const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, 0, 0, (V + SC_PART - 1) / SC_PART, 0};
     int rc = trl_head_bf16(packed ? rows : h, w, logits, ldo, n, V, H, stream);
     if (!rc) rc = (int)trl_launch(score_part_kernel, dim3(p.parts, n), dim3(256), 0, st, (const float*)logits, ldo, p);
     return rc ? rc : (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
   }
   CUtensorMap mh, mw;
   if (!score_map(&mh, packed ? rows : h, n, H) || !score_map(&mw, w, V, H)) return (int)cudaErrorInvalidValue;
-  const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, (H + SC_KT - 1) / SC_KT, v_tiles, parts};
-  const int rc = entropy ? score_launch<true>(mh, mw, p, st) : score_launch<false>(mh, mw, p, st);
+  const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, (H + SC_KT - 1) / SC_KT, v_tiles, parts, (H + SC_SEGMENT - 1) / SC_SEGMENT};
+  const int rc = p.segments == 1 ? (entropy ? score_launch<true, true>(mh, mw, p, st) : score_launch<false, true>(mh, mw, p, st))
+                                 : (entropy ? score_launch<true, false>(mh, mw, p, st) : score_launch<false, false>(mh, mw, p, st));
   if (rc) return rc;
   return (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
 }
