@@ -96,6 +96,15 @@ def build_parser() -> argparse.ArgumentParser:
     t.add_argument("--reward", default=None)
     t.add_argument("--clip-eps", type=float, default=0.2)
     t.add_argument("--kl-coef", type=float, default=0.0)
+    t.add_argument("--kl-reference", default="none", choices=["none", "base"],
+                   help="what the KL term of --kl-coef holds to: base = the model without its adapters (none: no such term)")
+    t.add_argument("--preference", action="store_true",
+                   help="preference training on --data rows {prompt, chosen, rejected} (adapters: against the base model's log-probabilities)")
+    t.add_argument("--beta", type=float, default=0.1, help="--preference: factor of the log ratios")
+    t.add_argument("--label-smoothing", type=float, default=0.0, help="--preference: share of pairs taken to be the wrong way round")
+    t.add_argument("--checkpoint-layers", action="store_true", help="keep only the layers' inputs and run each again in the backward pass")
+    t.add_argument("--activation-bits", type=int, default=32, choices=[8, 32],
+                   help="8: keep the checkpointed layers' inputs, or without --checkpoint-layers the feed-forwards' gate and up rows, in 8 bits")
     t.add_argument("--prompts", default=None, help="jsonl of prompts (default: random token prompts)")
     t.add_argument("--prompt-len", type=int, default=16)
     t.add_argument("--save-model", default=None)
@@ -357,6 +366,10 @@ def cmd_train(args) -> int:
     if curve_every and not args.dry_run:
         from .ledger import refuse_blind_curve
         refuse_blind_curve(args.eval_curve_n, args.curve_target_pt)
+    if args.preference and (not args.data or flags.get("rl") or flags.get("opd")):
+        raise SystemExit("--preference trains on --data rows.jsonl with {prompt, chosen, rejected} rows, without --rl or --opd")
+    if args.kl_reference == "base" and not (flags.get("rl") and flags.get("lora_rank")):
+        raise SystemExit("--kl-reference base is the model without its adapters: give --rl and --lora-rank")
     if flags.get("allow_short_rollouts"):        # (a smoke recipe runs into its cap on purpose)
         args.allow_short_rollouts = True
     cfg = get_config(flags.get("model", args.model))
@@ -429,6 +442,10 @@ def cmd_train(args) -> int:
               "prompt_len": args.prompt_len, "eval_gsm8k": args.eval_gsm8k, "eval_mmlu": args.eval_mmlu,
               "eval_n": args.eval_n, "eval_every": args.eval_every, "eval_curve_n": args.eval_curve_n,
               "eval_curve_seed": args.eval_curve_seed}
+    # (inputs that came later are named only where they are set, so that earlier runs keep their ids)
+    inputs.update({k: getattr(args, k) for k, default in (("kl_reference", "none"), ("preference", False), ("beta", 0.1), ("label_smoothing", 0.0),
+                                                          ("checkpoint_layers", False), ("activation_bits", 32)) if getattr(args, k) != default})
+    fb = {k: getattr(args, k) for k, default in (("checkpoint_layers", False), ("activation_bits", 32)) if getattr(args, k) != default}
     if args.load_adapter and not args.lineage:
         # a run that starts from a saved adapter descends from the run that wrote it (looked up through the
         # manifests' artifacts, never guessed from the path)
@@ -463,7 +480,16 @@ def cmd_train(args) -> int:
             with open(path) as f:
                 rows = [json.loads(ln) for ln in f if ln.strip()]
             return [{"question": r.get("prompt", r.get("question")), "answer": str(r["answer"])} for r in rows]
-    if args.data:
+    pairs = None
+    if args.preference:
+        with open(args.data) as f:
+            rows = [json.loads(ln) for ln in f if ln.strip()]
+        bad = next((i for i, r in enumerate(rows) if not all(isinstance(r.get(k), str) for k in ("prompt", "chosen", "rejected"))), None)
+        if bad is not None or not rows:
+            raise SystemExit(f"--preference: row {bad} of {args.data} has no prompt, chosen and rejected text" if rows else f"--preference: {args.data} has no rows")
+        pairs = [tuple(tok.encode(r[k]) for k in ("prompt", "chosen", "rejected")) for r in rows]
+        prompts = [p for p, _, _ in pairs]
+    elif args.data:
         items = read_jsonl(args.data)
         prompts = [tok.encode(it["question"]) for it in items]
         reward_fn = evals.make_text_reward(tok, {it["question"]: it["answer"] for it in items},
@@ -535,25 +561,31 @@ def cmd_train(args) -> int:
         # adapter run with evals, early stop and best-adapter save
         kw = dict(max_tokens=flags["max_tokens"], prompts_per_step=flags["prompts_per_step"])
         if not flags.get("opd"):
-            kw.update(group=flags["group"], clip_eps=args.clip_eps, kl_coef=args.kl_coef, micro=flags.get("micro") or 0)
+            kw.update(group=flags["group"], clip_eps=args.clip_eps, kl_coef=args.kl_coef, micro=flags.get("micro") or 0,
+                      reference=None if args.kl_reference == "none" else args.kl_reference)
         out = rl.train_adapters(eng, model, prompts[:48], reward_fn, opt,
                                 steps=flags["steps"], eval_prompts=prompts[48:], eval_every=args.eval_every or flags["eval_every"],
                                 patience=flags.get("patience", args.patience), save_dir=args.save_model, run=run,
-                                opd=bool(flags.get("opd")), **kw)
+                                opd=bool(flags.get("opd")), **kw, **fb)
         say(json.dumps({k: v for k, v in out.items() if k != "history"}, default=str), flush=True)
         return done()
     if flags.get("opd"):
         loop = rl.opd_loop(eng, model, prompts, opt, steps=flags["steps"], max_tokens=flags["max_tokens"],
-                           prompts_per_step=flags["prompts_per_step"])
+                           prompts_per_step=flags["prompts_per_step"], **fb)
+    elif pairs is not None:
+        loop = rl.preference_loop(model, pairs, opt, steps=flags["steps"], pairs_per_step=flags["prompts_per_step"],
+                                  reference="base" if flags.get("lora_rank") else None, device=dev, micro=flags.get("micro") or 0, post_step=post,
+                                  beta=args.beta, label_smoothing=args.label_smoothing, **fb)
     elif flags.get("rl"):
         loop = rl.grpo_loop(eng, model, prompts, reward_fn, opt,
                             steps=flags["steps"], group=flags["group"], prompts_per_step=flags["prompts_per_step"],
                             max_tokens=flags["max_tokens"], clip_eps=args.clip_eps, kl_coef=args.kl_coef,
                             micro=flags.get("micro") or 0, post_step=post, length_penalty=args.length_penalty, judge=judge,
-                            max_think_tokens=args.max_think_tokens or None)
+                            max_think_tokens=args.max_think_tokens or None,
+                            reference=None if args.kl_reference == "none" else args.kl_reference, **fb)
     else:
         data = iter(lambda: torch.randint(0, cfg.vocab, (2, args.prompt_len), generator=g), None)
-        loop = iter(rl.pretrain(model, data, opt, steps=flags["steps"], lr=flags["lr"]))
+        loop = iter(rl.pretrain(model, data, opt, steps=flags["steps"], lr=flags["lr"], **fb))
     drift = rl.RolloutDrift(flags["max_tokens"]) if flags.get("rl") and not args.allow_short_rollouts else None
     if curve_items:
         curve_point(0)

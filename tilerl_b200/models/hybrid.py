@@ -25,6 +25,7 @@ Parity: reference ``src/tilerl/model.py`` -- ``param_specs:38``,
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -186,6 +187,15 @@ class HybridModel:
     def _lora(self, name: str):
         return self.lora.get(name)
 
+    @contextlib.contextmanager
+    def without_adapters(self):
+        """The base model while the block runs (training forward): the policy that adapters started from."""
+        kept, self.lora = self.lora, {}
+        try:
+            yield self
+        finally:
+            self.lora = kept
+
     # ---- serving forward ------------------------------------------------------------------
     def forward(self, batch, ops, kv_pool, state_pool, *, last_only: bool = True,
                 aux_layers: Sequence[int] = (), return_hidden: bool = False, rows=None):
@@ -294,7 +304,7 @@ class HybridModel:
 
     def forward_dense(self, tape, ids: torch.Tensor, *, checkpoint_layers: bool = False,
                       positions: Optional[torch.Tensor] = None, hook=None, cp=None,
-                      return_hidden: bool = False):
+                      return_hidden: bool = False, activation_bits: int = 32):
         """Full-sequence forward on dense ``ids [B, T]`` with every op recorded on
         ``tape``; no KV cache, zero initial GDN state.  Returns this rank's logits
         ``[B, T, vocab_local]`` (full vocab at TP=1).  ``hook`` (a parameter sharder) is told
@@ -302,12 +312,16 @@ class HybridModel:
         and again in its backward replay -- (``pre_layer``) and when a layer's forward is over
         (``post_layer``).  ``cp`` (a ``parallel.cp.CPContext``): ``ids`` and ``positions`` hold this
         rank's zigzag slice of the sequence; attention gathers K / V, the GDN layers exchange
-        chunk summaries and conv halos."""
+        chunk summaries and conv halos.  ``activation_bits=8``: what is kept for the backward pass of the
+        checkpointed layers' inputs, or without checkpointing of the feed-forwards' gate and up rows, is kept in
+        8 bits (``ops/keep.py``); the forward pass is the same, gradients are those at what that stands for."""
         from .. import tape as T
         cfg, P, d = self.cfg, self.params, self.dims
         eps = cfg.rms_eps
         b, t = ids.shape
         pos = positions if positions is not None else torch.arange(t, device=ids.device)
+        if activation_bits not in (8, 32):
+            raise ValueError(f"activations are kept in 8 or 32 bits, not {activation_bits}")
         if hook is not None:
             hook.pre_model()
         x = T.embedding(tape, P["embed"], ids)
@@ -339,7 +353,7 @@ class HybridModel:
             h = T.rmsnorm(tape, x, P[p + "norm2"], eps, own=True)
             if tp:
                 h = T.tp_fork(tape, h)
-            act = T.swiglu(tape, self._tlinear(tape, h, p + "gate_up"))
+            act = T.swiglu(tape, self._tlinear(tape, h, p + "gate_up"), bits=32 if checkpoint_layers else activation_bits)
             y = self._tlinear(tape, act, p + "down")
             if tp:
                 y = T.all_reduce(tape, y)
@@ -350,7 +364,7 @@ class HybridModel:
                 p = f"L{i}."
                 leaves = [v for k, v in self.params.items()
                           if (k.startswith(p) or k.startswith("master." + p)) and id(v) in tape.leaves]
-                x = tape.checkpoint(lambda tp_, x_, i=i: layer(tp_, x_, i), x, params=leaves)
+                x = tape.checkpoint(lambda tp_, x_, i=i: layer(tp_, x_, i), x, params=leaves, bits=activation_bits)
             else:
                 x = layer(tape, x, i)
             if hook is not None and checkpoint_layers:

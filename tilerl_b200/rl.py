@@ -1,4 +1,4 @@
-"""Training loops on the hand-written tape: SFT, GRPO, on-policy distillation.
+"""Training loops on the hand-written tape: SFT, GRPO, on-policy distillation, preference pairs.
 
 ``policy_step`` implements the clipped GRPO surrogate with the rollout
 log-probabilities as ``pi_old``:
@@ -7,8 +7,8 @@ log-probabilities as ``pi_old``:
 
 Its gradient w.r.t. the logits is a weighted cross-entropy gradient with
 per-token weight ``w_i = (A_i rho_i [unclipped_i] - beta (1 - exp(ref_i - logp_i))) / N``,
-so the tape's ``cross_entropy`` op (which emits loss and gradient together and
-never differentiates a softmax twice) is the whole objective.  With one
+formed with the objective by the tape's ``policy_loss`` op where whole logits are, and given to its
+cross-entropies over a chunked head or a sharded vocabulary.  With one
 on-policy update ``rho == 1`` and the weights reduce to ``A_i / N`` -- exactly the
 REINFORCE-with-baseline form of the reference.  ``N`` is the batch-wide scored
 token count, not the micro-batch's.
@@ -18,6 +18,9 @@ samples with per-sample seeds), scores, normalises advantages per group, runs
 ``policy_step``, re-quantises the served weights in place and invalidates the
 engine's caches.
 
+``preference_step`` trains on pairs (chosen, rejected) by the log ratios of both to a reference;
+``sequence_logprobs`` is how a reference, for it or for the KL term, is scored.
+
 Parity: reference ``src/tilerl/train.py`` -- ``_step:164-310``,
 ``train_step:716``, ``group_advantages:740``, ``rl_step:805``,
 ``_require_on_policy:864``, ``grpo_loop:936-1135``, ``opd_loop:1138``,
@@ -25,6 +28,7 @@ Parity: reference ``src/tilerl/train.py`` -- ``_step:164-310``,
 """
 from __future__ import annotations
 
+import contextlib
 import json
 import os
 import time
@@ -36,7 +40,6 @@ import torch
 from . import tape as T
 from .engine import Engine, SamplingParams
 from .optim import clip_grad_norm, cosine_warmup
-from .ops import ref
 
 
 def group_advantages(rewards: Sequence[float], group: int, live: Optional[Sequence[bool]] = None,
@@ -140,19 +143,21 @@ def _scored_mask(ids: torch.Tensor, prompt_lens, seq_lens) -> torch.Tensor:
 def forward_backward(model, ids: torch.Tensor, targets: torch.Tensor, weights_fn, *,
                      trainable: Dict[str, torch.Tensor], tp_group=None, tp_world: int = 1,
                      checkpoint_layers: bool = False, on_grad=None, hook=None, fused_ce: bool = False,
-                     lp_weights_fn=None):
+                     lp_weights_fn=None, loss_fn=None, activation_bits: int = 32):
     """One micro-batch: dense forward on a fresh tape, weights from ``weights_fn(logits)``,
     cross-entropy op, backward.  Returns (loss, named grads, logits).  With ``fused_ce`` the head
     and the loss run chunked (``tape.linear_cross_entropy``): ``lp_weights_fn(logprobs [B, T])``
-    gives the weights and the third return value is the target log-probabilities."""
+    gives the weights and the third return value is the target log-probabilities.  ``loss_fn(tape, logits)``
+    takes the place of weights and cross-entropy where whole logits are formed.  ``activation_bits``: of
+    what the forward pass keeps (``HybridModel.forward_dense``)."""
     tp = T.Tape(tp_group, tp_world)
     tp.watch(*trainable.values())
     if fused_ce and tp_world == 1:
-        h, w, frozen = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook, return_hidden=True)
+        h, w, frozen = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook, return_hidden=True, activation_bits=activation_bits)
         loss, lp = T.linear_cross_entropy(tp, h, w, targets, lp_weights_fn, frozen=frozen)
         grads = tp.backward(loss, on_grad=on_grad)
         return float(loss), _named_grads(trainable, grads), lp
-    logits = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook)
+    logits = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook, activation_bits=activation_bits)
     if tp_world > 1:
         # vocab-parallel logits: the loss and the weights come from the sharded CE
         if lp_weights_fn is None:
@@ -162,8 +167,7 @@ def forward_backward(model, ids: torch.Tensor, targets: torch.Tensor, weights_fn
         named = _named_grads(trainable, grads)
         tp_sync_replicated_grads(named, tp_group)
         return float(loss), named, lp
-    w = weights_fn(logits)
-    loss = T.cross_entropy(tp, logits, targets, w)
+    loss = loss_fn(tp, logits) if loss_fn is not None else T.cross_entropy(tp, logits, targets, weights_fn(logits))
     grads = tp.backward(loss, on_grad=on_grad)
     return float(loss), _named_grads(trainable, grads), logits
 
@@ -198,7 +202,9 @@ def policy_step(model, ids: torch.Tensor, prompt_lens, seq_lens, advantages: tor
                 max_norm: float = 1.0, lr: Optional[float] = None, micro: int = 0,
                 return_grads: bool = False, **fb) -> Dict[str, object]:
     """One GRPO update on padded ``ids [B, T]``.  ``old_logprobs [B, T]`` holds
-    log pi_old of token i+1 at position i (None: on-policy, rho = 1)."""
+    log pi_old of token i+1 at position i (None: on-policy, rho = 1), ``ref_logprobs`` the reference
+    policy's (:func:`sequence_logprobs`).  ``loss`` among the results is the weighted negative log-likelihood whose gradient the
+    objective's is; where whole logits are formed (``tape.policy_loss``), ``objective`` is its value and ``kl`` its mean KL term."""
     b, t = ids.shape
     mask = _scored_mask(ids, prompt_lens, seq_lens)
     n = max(1.0, float(mask.sum()))
@@ -226,13 +232,24 @@ def policy_step(model, ids: torch.Tensor, prompt_lens, seq_lens, advantages: tor
             stats["ratio_mean"] += float((rho * m).sum())
             return w * m / n
 
-        def weights(lg, sl=sl):
-            lp = ref.token_logprobs(lg.reshape(-1, lg.shape[-1]), targets[sl].reshape(-1)).view(lg.shape[:2])
-            return weights_lp(lp)
+        def objective(tape, lg, sl=sl, adv=adv):
+            on = lambda t: None if t is None else t[sl].to(lg.device)
+            refs = on(ref_logprobs)
+            loss, terms = T.policy_loss(tape, lg, on(targets), adv[:, 0].to(lg.device), scale=1.0 / n, mask=on(mask), old_logprobs=on(old_logprobs),
+                                        ref_logprobs=refs, clip_eps=clip_eps, kl_coef=kl_coef if refs is not None else 0.0)
+            nll, clipped, ratio, kl = torch.stack([-(terms.weights * terms.logprobs).sum(), terms.clipped.sum(), terms.ratio.sum(), terms.kl.sum()]).tolist()
+            stats["loss"] += nll
+            stats["clipped"] += clipped
+            stats["ratio_mean"] += ratio
+            stats["kl"] = stats.get("kl", 0.0) + kl / n
+            return loss
 
-        loss, grads, _ = forward_backward(model, ids[sl], targets[sl], weights, trainable=trainable,
-                                          lp_weights_fn=weights_lp, **fb)
-        stats["loss"] += loss
+        loss, grads, _ = forward_backward(model, ids[sl], targets[sl], None, trainable=trainable,
+                                          lp_weights_fn=weights_lp, loss_fn=objective, **fb)
+        if "kl" in stats:                           # whole logits
+            stats["objective"] = stats.get("objective", 0.0) + loss
+        else:
+            stats["loss"] += loss
         for k, g in grads.items():
             acc[k] = g if k not in acc else acc[k] + g
     stats["ratio_mean"] /= n
@@ -243,6 +260,100 @@ def policy_step(model, ids: torch.Tensor, prompt_lens, seq_lens, advantages: tor
     if return_grads:
         stats["grads"] = acc
     return stats
+
+
+def sequence_logprobs(model, ids: torch.Tensor, prompt_lens, seq_lens, *, adapters: bool = True, micro: int = 0,
+                      entropy: bool = False):
+    """Log-probabilities ``[B, T]`` that ``model`` gives token i+1 at position i, 0 at positions that are not scored (prompt, padding), and with
+    ``entropy`` the entropies there.  ``adapters=False``: of the base model, the usual reference of an adapter run.  Nothing is kept and
+    no logits are formed (``tape.linear_logprobs``)."""
+    if model.tp > 1:
+        raise ValueError("sequence_logprobs scores with whole vocabularies: give it a model that is not sharded")
+    mask, targets, out = _scored_mask(ids, prompt_lens, seq_lens).to(ids.device), torch.roll(ids, -1, 1), []
+    for s in range(0, len(ids), micro or max(1, len(ids))):
+        sl = slice(s, s + (micro or len(ids)))
+        tape = T.Tape()
+        tape.enabled = False
+        with contextlib.nullcontext() if adapters else model.without_adapters():
+            h, w, _ = model.forward_dense(tape, ids[sl], return_hidden=True)
+        out.append(T.linear_logprobs(h, w, targets[sl], mask=mask[sl], entropy=entropy))
+    if not out:
+        raise ValueError("sequence_logprobs: no sequences")
+    return tuple(torch.cat(o) for o in zip(*out)) if entropy else torch.cat(out)
+
+
+def _reference_logprobs(reference, model, ids, prompt_lens, seq_lens, micro: int = 0) -> Optional[torch.Tensor]:
+    """``reference``: None, ``"base"`` (``model`` without its adapters) or another model."""
+    if reference is None:
+        return None
+    if isinstance(reference, str):
+        if reference != "base":
+            raise ValueError(f"a reference is None, 'base' or a model, not {reference!r}")
+        if not model.lora:
+            raise ValueError("reference 'base' is the model without its adapters, and this one has none: give a frozen copy")
+        return sequence_logprobs(model, ids, prompt_lens, seq_lens, adapters=False, micro=micro)
+    return sequence_logprobs(reference, ids, prompt_lens, seq_lens, micro=micro)
+
+
+def preference_step(model, ids: torch.Tensor, prompt_lens, seq_lens, optimizer, *, ref_logprobs: Optional[torch.Tensor] = None,
+                    beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False, max_norm: float = 1.0,
+                    lr: Optional[float] = None, micro: int = 0, return_grads: bool = False, **fb) -> Dict[str, object]:
+    """One update by the preference loss (``tape.preference_loss``) on padded ``ids [2P, T]``, chosen and rejected sequences in turn; their
+    tokens from ``prompt_lens`` on are scored.  ``ref_logprobs [2P, T]``: the reference policy's (:func:`sequence_logprobs`).  ``micro``: pairs at
+    a time."""
+    b, _ = ids.shape
+    if b % 2 or b == 0:
+        raise ValueError(f"preference_step: chosen and rejected sequences come in pairs, got {b}")
+    if int(fb.get("tp_world", 1) or 1) > 1 or fb.get("fused_ce"):
+        raise ValueError("preference_step forms whole logits: neither tensor parallelism nor fused_ce")
+    mask, targets, trainable = _scored_mask(ids, prompt_lens, seq_lens), torch.roll(ids, -1, 1), model.trainable()
+    acc: Dict[str, torch.Tensor] = {}
+    stats: Dict[str, object] = dict(loss=0.0, margin=0.0, accuracy=0.0)
+    mb = 2 * micro or b
+    for s in range(0, b, mb):
+        sl = slice(s, s + mb)
+
+        def objective(tape, lg, sl=sl):
+            on = lambda t: None if t is None else t[sl].to(lg.device)
+            loss, terms = T.preference_loss(tape, lg, on(targets), on(mask), on(ref_logprobs), beta=beta, label_smoothing=label_smoothing,
+                                            average=average, scale=2.0 / b)
+            stats["margin"] += float(terms.margins.sum()) * 2 / b
+            stats["accuracy"] += float((terms.margins > 0).sum()) * 2 / b
+            return loss
+
+        loss, grads, _ = forward_backward(model, ids[sl], targets[sl], None, trainable=trainable, loss_fn=objective, **fb)
+        stats["loss"] += loss
+        for k, g in grads.items():
+            acc[k] = g if k not in acc else acc[k] + g
+    stats["grad_norm"] = _clip(acc, max_norm, fb)
+    stats["tokens"] = float(mask.sum())
+    if optimizer is not None:
+        optimizer.step(acc, lr)
+    if return_grads:
+        stats["grads"] = acc
+    return stats
+
+
+def preference_loop(model, pairs: Sequence[tuple], optimizer, *, steps: int, pairs_per_step: int = 2, reference="base", device=None,
+                    micro: int = 0, post_step: Optional[Callable] = None, **kw) -> Iterator[Dict[str, object]]:
+    """Preference training on ``pairs`` of token lists (prompt, chosen, rejected), ``pairs_per_step`` of them in turn a step; yields a
+    step's metrics.  ``reference``: None, ``"base"`` (the model without its adapters) or a frozen model; ``kw`` goes to :func:`preference_step`."""
+    if not pairs:
+        raise ValueError("preference_loop: no pairs")
+    cursor = 0
+    for step in range(steps):
+        t0 = time.perf_counter()
+        some = [pairs[(cursor + i) % len(pairs)] for i in range(pairs_per_step)]
+        cursor += pairs_per_step
+        seqs = [list(p) + list(c) for p, good, bad in some for c in (good, bad)]
+        plens, slens = [len(p) for p, _, _ in some for _ in range(2)], [len(s) for s in seqs]
+        ids = pad_batch(seqs)
+        ids = ids if device is None else ids.to(device)
+        refs = _reference_logprobs(reference, model, ids, plens, slens, 2 * micro)
+        m = preference_step(model, ids, plens, slens, optimizer, ref_logprobs=refs, micro=micro, **kw)
+        if post_step is not None:
+            post_step(model)
+        yield dict(step=step, **m, seconds=time.perf_counter() - t0)
 
 
 def drain(engine: Engine, rids: Sequence[int], max_ticks: int = 1 << 30) -> List:
@@ -305,10 +416,11 @@ def grpo_loop(engine: Engine, model, prompts: Sequence[Sequence[int]], reward_fn
               max_tokens: int = 16, clip_eps: float = 0.2, kl_coef: float = 0.0, lr: Optional[float] = None,
               micro: int = 0, seed: int = 0, on_policy_updates: int = 1, post_step: Optional[Callable] = None,
               length_penalty: float = 0.0, judge: Optional[Callable] = None,
-              max_think_tokens: Optional[int] = None, **fb) -> Iterator[Dict[str, object]]:
+              max_think_tokens: Optional[int] = None, reference=None, **fb) -> Iterator[Dict[str, object]]:
     """Yields one metrics dict per RL step (mean reward, loss, seconds by phase).  ``judge(prompt,
     completions, rewards) -> rewards``: called per group after the rule-based reward, it may order the
-    completions that tie (the rule decides first; see ``evals.judge_tiebreak``)."""
+    completions that tie (the rule decides first; see ``evals.judge_tiebreak``).  ``reference``: the policy that the KL term
+    (``kl_coef``) holds to: None (no such term), ``"base"`` (the model without its adapters) or a frozen model."""
     engine.invalidate_weights()
     cursor = 0
     for step in range(steps):
@@ -345,11 +457,13 @@ def grpo_loop(engine: Engine, model, prompts: Sequence[Sequence[int]], reward_fn
             for i, r in enumerate(results):
                 if r is not None and r.logprobs:
                     old[i, plens[i] - 1:plens[i] - 1 + len(r.logprobs)] = torch.tensor(r.logprobs)
+        ids = ids.to(engine.device)
+        refs = _reference_logprobs(reference, model, ids, plens, slens, micro)
         t2 = time.perf_counter()
         stats = {}
         for _ in range(on_policy_updates):
-            stats = policy_step(model, ids.to(engine.device), plens, slens, adv, optimizer,
-                                old_logprobs=old, clip_eps=clip_eps, kl_coef=kl_coef, lr=lr,
+            stats = policy_step(model, ids, plens, slens, adv, optimizer,
+                                old_logprobs=old, ref_logprobs=refs, clip_eps=clip_eps, kl_coef=kl_coef, lr=lr,
                                 micro=micro, **fb)
         t3 = time.perf_counter()
         if post_step is not None:
@@ -360,6 +474,7 @@ def grpo_loop(engine: Engine, model, prompts: Sequence[Sequence[int]], reward_fn
                      if len(set(rewards[g0:g0 + group])) == 1)
         yield dict(step=step, reward=sum(rewards) / len(rewards), loss=stats.get("loss", 0.0),
                    grad_norm=stats.get("grad_norm", 0.0), tokens=stats.get("tokens", 0),
+                   **({"kl": stats["kl"]} if refs is not None and "kl" in stats else {}),
                    tied_groups=n_tied, completion_tokens=sum(len(c) for c in comps),
                    mean_completion_tokens=sum(len(c) for c in comps) / max(1, len(comps)),
                    # one row per completion, so that length and reward stay paired (group means per step
