@@ -84,7 +84,7 @@ __device__ __forceinline__ uint4 pl_pack(const float (&x)[8]) {
 // Sums are of 2^(x log2 e - B) with a whole number B, the row's largest x log2 e rounded up: one fused multiply-add, rounded once, and
 // ex2.approx, where expf(x - m) has ten instructions; instructions were these kernels' time.  A whole B makes it no matter which B: the rounding
 // of a product m log2 e would go into every value of the row.  fp32's log2 e is off by 1.3e-8 of itself, as if all of x were; ex2.approx by 2^-22, and the
-// multiply-add's rounding moves a value at a distance of d by d 2^-24 of itself, both at random over a row.  (Logits above 2.3e38 count as infinite.)
+// multiply-add's rounding moves a value at a distance of d by d 2^-24 of itself, both at random over a row.
 constexpr float PL_L2E = 1.4426950408889634f;
 __device__ __forceinline__ float pl_exp2(float y) {
   float e;
@@ -92,11 +92,13 @@ __device__ __forceinline__ float pl_exp2(float y) {
   return e;
 }
 __device__ __forceinline__ float pl_exp(float x, float base) { return pl_exp2(fmaf(x, PL_L2E, -base)); }
-// B for a largest value; as what is taken away from an exponent (nothing has counted yet at -inf: values of -inf then count nothing, and NaN stays)
-__device__ __forceinline__ float pl_base(float most) { return ceilf(most * PL_L2E); }
-__device__ __forceinline__ float pl_less(float base) { return base == -INFINITY ? 0.f : base; }
+// B for a largest value.  From below it is bounded: threads that see nothing but masked words (-inf, -1e30) have sums of 0 there.  A row whose B is
+// that bound, or so large that whole numbers near it have gaps, is far: gone through once more, slowly, with x - m.
+constexpr float PL_FAR = 2097152.f;
+__device__ __forceinline__ float pl_base(float most) { return fmaxf(ceilf(most * PL_L2E), -PL_FAR); }
+__device__ __forceinline__ bool pl_far(float base) { return !(fabsf(base) < PL_FAR); }
 // a sum at base `from` at base `to` (not below it)
-__device__ __forceinline__ float pl_moved(float s, float from, float to) { return s * pl_exp2(from - pl_less(to)); }
+__device__ __forceinline__ float pl_moved(float s, float from, float to) { return s * pl_exp2(from - to); }
 // x - B ln 2, with it the log-probability, in fp64 and from the same log2 e, so that its error comes in with x's distance from the row's mean only
 __device__ __forceinline__ double pl_low(float x, float base) { return ((double)x * (double)PL_L2E - (double)base) * 0.693147180559945309417; }
 
@@ -109,7 +111,7 @@ __device__ __forceinline__ float pl_target(const T* row, long long t, long V, lo
   return pl_float(row[t]);
 }
 
-// What a scored row's terms need, and they from its target's logit, largest value and sum.  The exponentials do not wait for the logarithm.
+// What a scored row's terms need, and they from its target's logit, less what the sum's exponentials have less, and the sum.  The exponentials do not wait for the logarithm.
 struct PolicyIn {
   float adv, old, ref;
   __device__ PolicyIn() {}
@@ -119,8 +121,8 @@ struct PolicyOut {
   float weight, target;                              // of the row's gradient, and its target's: weight (p - 1)
   double part;                                       // 1 / sum
 };
-__device__ __forceinline__ PolicyOut pl_policy(const PolicyRow& a, const PolicyIn& in, long r, float xt, float base, double sum, bool write = true) {
-  const double A = (double)in.adv, low = pl_low(xt, base), part = 1.0 / sum;
+__device__ __forceinline__ PolicyOut pl_policy(const PolicyRow& a, const PolicyIn& in, long r, double low, double sum, bool write = true) {
+  const double A = (double)in.adv, part = 1.0 / sum;
   const double lp = low - log(sum), p = exp(low) * part;
   const double rho = a.old ? exp(low - (double)in.old) * part : 1.0;
   const bool clip = (rho > a.hi && A > 0.0) || (rho < a.lo && A < 0.0);
@@ -178,7 +180,7 @@ __device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f) {
 template <typename T, int NT, int G>
 __device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, float& base, float& s) {
   constexpr int E = Span<T>::E, C = E == 4 ? G : G / 2 < 1 ? 1 : G / 2;        // vectors that are unpacked at a time
-  base = pl_base(xe == xe ? xe : -INFINITY), s = pl_exp(xe, pl_less(base));
+  base = pl_base(xe == xe ? xe : -INFINITY), s = pl_exp(xe, base);
   pl_each<T, NT, G>(body, cnt, [&](const uint4 (&z)[G], int, bool) {
 #pragma unroll
     for (int k0 = 0; k0 < G; k0 += C) {
@@ -191,11 +193,10 @@ __device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, fl
       }
       const float b = pl_base(top);
       if (b > base) s = pl_moved(s, base, b), base = b;
-      const float less = pl_less(base);
 #pragma unroll
       for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e & 3] += pl_exp(v[k][e], less);
+        for (int e = 0; e < E; ++e) q[e & 3] += pl_exp(v[k][e], base);
       s += (q[0] + q[1]) + (q[2] + q[3]);
     }
   });
@@ -216,6 +217,36 @@ __device__ __forceinline__ void pl_grads(const uint4* body, uint4* dst, int cnt,
     }
   });
 }
+// Of far rows: a thread's largest value, its sum of e^(x - m), its gradients c e^(x - m).
+template <typename T, int NT>
+__device__ float pl_far_most(const uint4* body, int cnt, float xe) {
+  float m = xe;
+  pl_each<T, NT, 1>(body, cnt, [&](const uint4 (&z)[1], int, bool) {
+    float v[Span<T>::E];
+    pl_unpack(z[0], v);
+    for (int e = 0; e < Span<T>::E; ++e) m = fmaxf(m, v[e]);
+  });
+  return m;
+}
+template <typename T, int NT>
+__device__ float pl_far_sum(const uint4* body, int cnt, float xe, bool end, float m) {
+  float s = end ? expf(xe - m) : 0.f;
+  pl_each<T, NT, 1>(body, cnt, [&](const uint4 (&z)[1], int i, bool) {
+    float v[Span<T>::E];
+    pl_unpack(z[0], v);
+    for (int e = 0; e < Span<T>::E; ++e) s += expf(v[e] - m);
+  });
+  return s;
+}
+template <typename T, int NT>
+__device__ void pl_far_grads(const uint4* body, uint4* dst, int cnt, float m, float c) {
+  pl_each<T, NT, 1>(body, cnt, [&](const uint4 (&z)[1], int i, bool) {
+    float v[Span<T>::E];
+    pl_unpack(z[0], v);
+    for (int e = 0; e < Span<T>::E; ++e) v[e] = expf(v[e] - m) * c;
+    dst[i] = pl_pack(v);
+  });
+}
 __device__ __forceinline__ void pl_store_zero(uint4* p) { __stcs(p, make_uint4(0u, 0u, 0u, 0u)); }
 // Whether this thread wrote the target's gradient: it is at one of its ends, or among its vectors lo + k, lo + k + NT, ...
 __device__ __forceinline__ bool pl_wrote(long long t, long end, int head, int E, long lo, int cnt, int k, int NT) {
@@ -227,16 +258,16 @@ __device__ __forceinline__ bool pl_wrote(long long t, long end, int head, int E,
 // Up to 4096 values: NT threads a row, which waits in registers, 16 values a thread, as exponentials until its sum and weight are known; the rows of a
 // block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, logarithm and exponentials in fp64) is some 6 us, so what
 // counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us.)
-__device__ __noinline__ float3 pl_policy_row(const PolicyRow& a, const PolicyIn& in, long r, float xt, float base, double sum) {       // (apart: its fp64 registers beside a row's values would halve the warps)
-  const PolicyOut o = pl_policy(a, in, r, xt, base, sum);
-  return make_float3(base, (float)((double)o.weight * o.part), o.target);
+__device__ __noinline__ float2 pl_policy_row(const PolicyRow& a, const PolicyIn& in, long r, double low, double sum) {       // (apart: its fp64 registers beside a row's values would halve the warps)
+  const PolicyOut o = pl_policy(a, in, r, low, sum);
+  return make_float2((float)((double)o.weight * o.part), o.target);
 }
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   using S = Span<T>;
   constexpr int E = S::E, VPT = 16 / E, N = 16, W = NT / 32, R = 256 / NT;
   __shared__ float2 sums[8];
-  __shared__ float3 found[R];                        // base, weight over the sum, the target's gradient
+  __shared__ float3 found[R];                        // the largest value, weight over the sum, the target's gradient
   const int k = threadIdx.x % NT, mine = threadIdx.x / NT, warp = threadIdx.x >> 5;
   const long r0 = (long)blockIdx.x * R, r = r0 + mine;
   const bool there = r < rows.n, scored = there && (!rows.mask || rows.mask[r]);
@@ -266,12 +297,13 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   float m = end, s[4] = {};
 #pragma unroll
   for (int i = 0; i < N; i += 2) m = fmaxf(m, fmaxf(v[i], v[i + 1]));
-  const float base = pl_base(warp_max(m)), less = pl_less(base);
+  // (the largest value is known before the first exponential here, and the two more instructions of (x - m) log2 e are not what counts)
+  const float most = warp_max(m), less = most == -INFINITY ? 0.f : most;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = pl_exp(v[i], less), s[i & 3] += v[i];
-  end = pl_exp(end, less);
+  for (int i = 0; i < N; ++i) v[i] = pl_exp2((v[i] - less) * PL_L2E), s[i & 3] += v[i];
+  end = pl_exp2((end - less) * PL_L2E);
   const float sum = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end);
-  if (threadIdx.x % 32 == 0) sums[warp] = make_float2(base, sum);
+  if (threadIdx.x % 32 == 0) sums[warp] = make_float2(most, sum);
   __syncthreads();
   if (weighs) {
     float top = -INFINITY;
@@ -279,15 +311,15 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
 #pragma unroll
     for (int i = 0; i < W; ++i) top = fmaxf(top, sums[threadIdx.x * W + i].x);
 #pragma unroll
-    for (int i = 0; i < W; ++i) all += (double)pl_moved(sums[threadIdx.x * W + i].y, sums[threadIdx.x * W + i].x, top);
-    if (top == -INFINITY) all = NAN;                 // a row without a finite value
-    found[threadIdx.x] = pl_policy_row(a, in, rw, xt, pl_less(top), all);
+    for (int i = 0; i < W; ++i) all += (double)(sums[threadIdx.x * W + i].y * pl_exp2((sums[threadIdx.x * W + i].x - top) * PL_L2E));      // (NaN without a finite value)
+    const float2 f = pl_policy_row(a, in, rw, (double)xt - (double)top, all);
+    found[threadIdx.x] = make_float3(top, f.x, f.y);
   }
   if (!grad) return;
   __syncthreads();
   if (!there) return;
   const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
-  const float c = scored ? pl_exp2(less - f.x) * f.y : 0.f;
+  const float c = scored ? pl_exp2((less - f.x) * PL_L2E) * f.y : 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float u[E];
@@ -321,27 +353,82 @@ __device__ __forceinline__ void pl_cluster_wait() {
   __syncwarp();
 }
 
+// What a block works on: its vectors of a row, and its threads' values at the row's ends.
+template <typename T, int CL>
+struct PolicyPart {
+  const T* row;
+  T* out;
+  Span<T> sp;
+  long lo, ie;
+  int rank, cnt;
+  const uint4* body;
+  uint4* dst;
+  __device__ PolicyPart(const T* x, T* grad, long r, long V)
+      : row(x + (size_t)r * V), out(grad + (size_t)r * V), sp(row, V), rank(CL > 1 ? blockIdx.x % CL : 0) {
+    const long per = (sp.nv + CL - 1) / CL;
+    lo = min(sp.nv, rank * per), cnt = (int)(min(sp.nv, lo + per) - lo);
+    body = reinterpret_cast<const uint4*>(row + sp.head) + lo, dst = reinterpret_cast<uint4*>(out + sp.head) + lo;
+    ie = rank == 0 ? sp.end_of(threadIdx.x) : -1;
+  }
+};
+
+// A far row.  All blocks of its cluster come here, behind the same barriers.
+template <typename T, int CL, int NT>
+__device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad, const PolicyRow& a, long r, float2* sums, float2* peers, float4* found) {
+  const PolicyPart<T, CL> p(x, grad, r, rows.V);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto meet = [&] {
+    if (CL > 1) pl_cluster_arrive(), pl_cluster_wait();
+    else __syncthreads();
+  };
+  auto join = [&](float v, auto warps, auto op, float none) {       // of all threads of the cluster
+    v = warps(v);
+    meet();                                          // (what was there before has been read)
+    if (lane == 0) sums[warp].x = v;
+    __syncthreads();
+    if (warp == 0) {
+      v = warps(lane < NT / 32 ? sums[lane].x : none);
+      if (CL > 1) {
+        if (lane < CL) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(pl_map(smem_u32(&peers[p.rank]), lane)), "f"(v) : "memory");
+      } else if (lane == 0) {
+        peers[0].x = v;
+      }
+    }
+    meet();
+    v = peers[0].x;
+    for (int k = 1; k < CL; ++k) v = op(v, peers[k].x);
+    return v;
+  };
+  const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
+  const float m = join(pl_far_most<T, NT>(p.body, p.cnt, xe), [](float v) { return warp_max(v); }, [](float v, float w) { return fmaxf(v, w); }, -INFINITY);
+  const float sum = join(pl_far_sum<T, NT>(p.body, p.cnt, xe, p.ie >= 0, m), [](float v) { return warp_sum(v); }, [](float v, float w) { return v + w; }, 0.f);
+  const long long t = rows.target[r];
+  if (tid == 0) {
+    const PolicyOut o = pl_policy(a, PolicyIn(a, r), r, (double)pl_target(p.row, t, rows.V, r) - (double)m, (double)sum, p.rank == 0);
+    *found = make_float4(0.f, (float)((double)o.weight * o.part), o.target, 0.f);
+  }
+  __syncthreads();
+  if (grad) {
+    pl_far_grads<T, NT>(p.body, p.dst, p.cnt, m, found->y);
+    if (p.ie >= 0) p.out[p.ie] = pl_round<T>(expf(xe - m) * found->y);
+    if (t < rows.V && pl_wrote(t, p.ie, p.sp.head, Span<T>::E, p.lo, p.cnt, tid, NT)) p.out[t] = pl_round<T>(found->z);
+  }
+  meet();                                            // (no block leaves while another reads what it sent)
+}
+
 template <typename T, int CL, int NT, int G, int BLOCKS>
-__global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
-  using S = Span<T>;
+__global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const __grid_constant__ Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   constexpr int W = NT / 32;
   __shared__ float2 sums[W], peers[CL];
-  __shared__ float4 found;                           // base, weight over the sum, the target's gradient
+  __shared__ float4 found;                           // base, weight over the sum, the target's gradient, whether the row is far
   const long r = blockIdx.x / CL;
-  const int rank = CL > 1 ? blockIdx.x % CL : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* row = x + (size_t)r * rows.V;
-  T* out = grad + (size_t)r * rows.V;
-  const S sp(row, rows.V);
-  const long per = (sp.nv + CL - 1) / CL, lo = min(sp.nv, rank * per);
-  const int cnt = (int)(min(sp.nv, lo + per) - lo);
-  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head) + lo;
-  uint4* dst = reinterpret_cast<uint4*>(out + sp.head) + lo;
-  const long ie = rank == 0 ? sp.end_of(tid) : -1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const PolicyPart<T, CL> p(x, grad, r, rows.V);
   if (rows.mask && !rows.mask[r]) {
-    if (tid == 0 && rank == 0) pl_policy_skip(a, r);
+    if (tid == 0 && p.rank == 0) pl_policy_skip(a, r);
     if (grad) {
-      for (int i = tid; i < cnt; i += NT) pl_store_zero(dst + i);
-      if (ie >= 0) out[ie] = pl_round<T>(0.f);
+      for (int i = tid; i < p.cnt; i += NT) pl_store_zero(p.dst + i);
+      if (p.ie >= 0) p.out[p.ie] = pl_round<T>(0.f);
     }
     return;
   }
@@ -349,51 +436,60 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   const long long t = rows.target[r];
   PolicyIn in;
   float xt = 0.f;
-  if (tid == 0) in = PolicyIn(a, r), xt = pl_target(row, t, rows.V, r);
-  const float xe = ie >= 0 ? pl_float(row[ie]) : -INFINITY;
+  if (tid == 0) in = PolicyIn(a, r), xt = pl_target(p.row, t, rows.V, r);
+  const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
   float base, s;
-  pl_sums<T, NT, G>(body, cnt, xe, base, s);
+  pl_sums<T, NT, G>(p.body, p.cnt, xe, base, s);
   const float top = warp_max(base);
   s = warp_sum(pl_moved(s, base, top));
   if (lane == 0) sums[warp] = make_float2(top, s);
   __syncthreads();
   if (CL > 1) pl_cluster_wait();
   if (warp == 0) {
-    const float2 q = lane < W ? sums[lane] : make_float2(-INFINITY, 0.f);
+    const float2 q = lane < W ? sums[lane] : make_float2(-PL_FAR, 0.f);
     const float mine = warp_max(q.x), sum = warp_sum(pl_moved(q.y, q.x, mine));
     if (CL > 1) {
       if (lane < CL)
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(pl_map(smem_u32(&peers[rank]), lane)), "f"(mine), "f"(sum) : "memory");
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(pl_map(smem_u32(&peers[p.rank]), lane)), "f"(mine), "f"(sum) : "memory");
     } else if (lane == 0) {
       peers[0] = make_float2(mine, sum);
     }
   }
   if (CL > 1) pl_cluster_arrive(), pl_cluster_wait();
   if (tid == 0) {
-    float all = -INFINITY;
+    float all = -PL_FAR;
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < CL; ++k) all = fmaxf(all, peers[k].x);
 #pragma unroll
     for (int k = 0; k < CL; ++k) sum += (double)pl_moved(peers[k].y, peers[k].x, all);
-    if (all == -INFINITY) sum = NAN;                 // a row without a finite value
-    const PolicyOut o = pl_policy(a, in, r, xt, pl_less(all), sum, rank == 0);
-    found = make_float4(pl_less(all), (float)((double)o.weight * o.part), o.target, 0.f);
+    if (pl_far(all)) {
+      found.w = 1.f;
+    } else {
+      const PolicyOut o = pl_policy(a, in, r, pl_low(xt, all), sum, p.rank == 0);
+      found = make_float4(all, (float)((double)o.weight * o.part), o.target, 0.f);
+    }
+  }
+  __syncthreads();
+  if (found.w != 0.f) {
+    pl_policy_far<T, CL, NT>(x, rows, grad, a, r, sums, peers, &found);
+    return;
   }
   if (!grad) return;
-  __syncthreads();
-  pl_grads<T, NT, G>(body, dst, cnt, found.x, found.y);
-  if (ie >= 0) out[ie] = pl_round<T>(pl_exp(xe, found.x) * found.y);
-  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, tid, NT)) out[t] = pl_round<T>(found.z);
+  pl_grads<T, NT, G>(p.body, p.dst, p.cnt, found.x, found.y);
+  if (p.ie >= 0) p.out[p.ie] = pl_round<T>(pl_exp(xe, found.x) * found.y);
+  if (t < rows.V && pl_wrote(t, p.ie, p.sp.head, Span<T>::E, p.lo, p.cnt, tid, NT)) p.out[t] = pl_round<T>(found.z);
 }
 
 // ---- preference loss: a row's weight needs its whole sequence -------------------------------------------------------------------
-// A block a row: (B, sum) into ms, and its log-probability.
+// A block a row: what its gradient needs into `rest` (base; of far rows the largest value; sum; whether the row is far), and its log-probability.
 template <typename T>
-__global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows rows, float2* ms, double* lps) {
+__global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows rows, float4* rest, double* lps) {
   using S = Span<T>;
   constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
   __shared__ float2 sums[NT / 32];
+  __shared__ float red[32];
+  __shared__ int far;
   const long r = blockIdx.x;
   if (rows.mask && !rows.mask[r]) {
     if (threadIdx.x == 0) lps[r] = 0.0;
@@ -401,27 +497,35 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   }
   const T* row = x + (size_t)r * rows.V;
   const S sp(row, rows.V);
+  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
   float xt = 0.f, base, s;
   if (threadIdx.x == 0) xt = pl_target(row, rows.target[r], rows.V, r);
   const long ie = sp.end_of(threadIdx.x);
-  pl_sums<T, NT, G>(reinterpret_cast<const uint4*>(row + sp.head), (int)sp.nv, ie >= 0 ? pl_float(row[ie]) : -INFINITY, base, s);
+  const float xe = ie >= 0 ? pl_float(row[ie]) : -INFINITY;
+  pl_sums<T, NT, G>(body, (int)sp.nv, xe, base, s);
   const float top = warp_max(base);
   s = warp_sum(pl_moved(s, base, top));
   if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = make_float2(top, s);
   __syncthreads();
-  if (threadIdx.x) return;
-  float all = -INFINITY;
-  double sum = 0.0;
-  for (int k = 0; k < NT / 32; ++k) all = fmaxf(all, sums[k].x);
-  for (int k = 0; k < NT / 32; ++k) sum += (double)pl_moved(sums[k].y, sums[k].x, all);
-  if (all == -INFINITY) sum = NAN;
-  ms[r] = make_float2(pl_less(all), (float)sum), lps[r] = pl_low(xt, pl_less(all)) - log(sum);
+  if (threadIdx.x == 0) {
+    float all = -PL_FAR;
+    double sum = 0.0;
+    for (int k = 0; k < NT / 32; ++k) all = fmaxf(all, sums[k].x);
+    for (int k = 0; k < NT / 32; ++k) sum += (double)pl_moved(sums[k].y, sums[k].x, all);
+    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all) - log(sum);
+    far = pl_far(all);
+  }
+  __syncthreads();
+  if (!far) return;
+  const float m = block_max(pl_far_most<T, NT>(body, (int)sp.nv, xe), red);
+  s = block_sum(pl_far_sum<T, NT>(body, (int)sp.nv, xe, ie >= 0, m), red);
+  if (threadIdx.x == 0) rest[r] = make_float4(0.f, m, s, 1.f), lps[r] = (double)xt - (double)m - log((double)s);
 }
 
 // Gradients: a block a slice of a row.  weight of row r: weight[r / per].  The last rows first: they are what L2 still holds.
 constexpr int PL_SLICE = 4096;                       // vectors a block
 template <typename T>
-__global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows rows, const float2* ms, const float* weight, long per, T* grad, int slices) {
+__global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows rows, const float4* rest, const float* weight, long per, T* grad, int slices) {
   using S = Span<T>;
   constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
   const long r = rows.n - 1 - blockIdx.x / slices, lo = (long)(blockIdx.x % slices) * PL_SLICE;
@@ -437,11 +541,15 @@ __global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows 
     return;
   }
   const float w = weight[(unsigned)r / (unsigned)per];
-  const float2 st = ms[r];
+  const float4 st = rest[r];
   const long long t = rows.target[r];
-  pl_grads<T, NT, G>(reinterpret_cast<const uint4*>(row + sp.head) + lo, dst, cnt, st.x, w / st.y);
-  if (ie >= 0) out[ie] = pl_round<T>(pl_exp(pl_float(row[ie]), st.x) * (w / st.y));
-  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, k, NT)) out[t] = pl_round<T>((pl_exp(pl_float(row[t]), st.x) / st.y - 1.f) * w);
+  const uint4* body = reinterpret_cast<const uint4*>(row + sp.head) + lo;
+  const float c = w / st.z;
+  auto one = [&](float x) { return st.w != 0.f ? expf(x - st.y) : pl_exp(x, st.x); };
+  if (st.w != 0.f) pl_far_grads<T, NT>(body, dst, cnt, st.y, c);
+  else pl_grads<T, NT, G>(body, dst, cnt, st.x, c);
+  if (ie >= 0) out[ie] = pl_round<T>(one(pl_float(row[ie])) * c);
+  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, k, NT)) out[t] = pl_round<T>((one(pl_float(row[t])) / st.z - 1.f) * w);
 }
 
 // ---- sums over rows, and pairs of sequences ----------------------------------------------------------------------------------
@@ -491,10 +599,10 @@ __global__ void __launch_bounds__(256) pl_scale_kernel(T* x, const float* up, lo
 }
 
 template <typename T>
-int grad_launch(const void* x, const Rows& rows, const float2* ms, const float* weight, long per, void* grad, cudaStream_t st) {
+int grad_launch(const void* x, const Rows& rows, const float4* rest, const float* weight, long per, void* grad, cudaStream_t st) {
   const long nv = rows.V / Span<T>::E, slices = nv < PL_SLICE ? 1 : (nv + PL_SLICE - 1) / PL_SLICE;
   if (rows.n * slices >= 1l << 31) return (int)cudaErrorInvalidValue;
-  pl_grad_kernel<T><<<(unsigned)(rows.n * slices), 256, 0, st>>>((const T*)x, rows, ms, weight, per, (T*)grad, (int)slices);
+  pl_grad_kernel<T><<<(unsigned)(rows.n * slices), 256, 0, st>>>((const T*)x, rows, rest, weight, per, (T*)grad, (int)slices);
   return (int)cudaGetLastError();
 }
 
@@ -555,25 +663,25 @@ TRL_API int trl_policy_loss(const void* x, int type, long n, long V, const void*
   return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, row_loss, n, scale, (float*)loss);
 }
 
-// 2 pairs sequences of T rows, chosen and rejected in turn.  totals [2 pairs], margins [pairs]; work: 2 pairs T doubles, as many
-// float2, then pairs doubles and 2 pairs floats.
+// 2 pairs sequences of T rows, chosen and rejected in turn.  totals [2 pairs], margins [pairs]; work: 2 pairs T float4, as many
+// doubles, then pairs doubles and 2 pairs floats.
 TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, long V, const void* target, const void* mask, const void* ref, double beta,
                                 double smooth, int average, double scale, void* totals, void* margins, void* loss, void* grad, void* work, void* stream) {
   const long n = 2 * pairs * T;
   if (pairs < 1 || T < 1 || pairs >= 1l << 30 || T >= 1l << 31 || !rows_ok(n, V)) return (int)cudaErrorInvalidValue;
   if (grad && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(grad)) & 15)) return (int)cudaErrorInvalidValue;
   cudaStream_t st = (cudaStream_t)stream;
-  double* lps = (double*)work;
-  float2* ms = (float2*)(lps + n);
-  double* pair_loss = (double*)(ms + n);
+  float4* rest = (float4*)work;
+  double* lps = (double*)(rest + n);
+  double* pair_loss = lps + n;
   float* weight = (float*)(pair_loss + pairs);
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
-  if (type) pl_stats_kernel<bf16><<<(int)n, 256, 0, st>>>((const bf16*)x, rows, ms, lps);
-  else pl_stats_kernel<float><<<(int)n, 256, 0, st>>>((const float*)x, rows, ms, lps);
+  if (type) pl_stats_kernel<bf16><<<(int)n, 256, 0, st>>>((const bf16*)x, rows, rest, lps);
+  else pl_stats_kernel<float><<<(int)n, 256, 0, st>>>((const float*)x, rows, rest, lps);
   pl_pairs_kernel<<<(int)pairs, 256, 0, st>>>(lps, (const float*)ref, rows.mask, T, beta, smooth, average, scale, (float*)totals, (float*)margins, pair_loss,
                                               weight);
   if (grad) {
-    const int rc = type ? grad_launch<bf16>(x, rows, ms, weight, T, grad, st) : grad_launch<float>(x, rows, ms, weight, T, grad, st);
+    const int rc = type ? grad_launch<bf16>(x, rows, rest, weight, T, grad, st) : grad_launch<float>(x, rows, rest, weight, T, grad, st);
     if (rc) return rc;
   }
   return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, pair_loss, pairs, scale, (float*)loss);

@@ -40,7 +40,7 @@ def _grad_bounds(lg, w, dw, v):
     return b + half * (w.abs()[..., None] * 2 + b)
 
 
-SHAPES = [((1,), 1, 0), ((3,), 2, 1), ((2, 5), 7, 0), ((4, 9), 320, 0), ((3, 3), 1023, 3), ((2, 2), 1024, 0), ((2, 2), 1025, 1), ((5,), 4099, 2), ((2, 3), 16384, 0),
+SHAPES = [((1,), 1, 0), ((3,), 2, 1), ((2, 5), 7, 0), ((4, 9), 320, 0), ((9,), 512, 0), ((5,), 513, 1), ((3,), 2049, 0), ((2,), 4096, 0), ((3, 3), 1023, 3), ((2, 2), 1024, 0), ((2, 2), 1025, 1), ((5,), 4099, 2), ((2, 3), 16384, 0),
           ((3,), 16391, 1), ((2, 2), 32768, 0), ((2,), 49999, 1), ((3,), 65540, 2), ((2, 2), 131072, 0), ((3,), 150001, 3), ((2,), 248320, 0), ((2,), 262144, 0), ((2,), 262145, 0),
           ((2,), 300007, 1)]
 
@@ -147,6 +147,49 @@ def test_infinities_and_nan_in_scored_rows(v):
     assert sides[1][0].isnan().tolist() == [False, False, True, True, True, False, False, False]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [40, 900, 5000, 20001, 50000, 150000, 270000])
+def test_rows_far_from_zero(v, dtype):
+    """Logits of any finite size: masked words of -1e4 to the type's lowest in long runs, rows that lie at 1e6 or -1e30 as a whole, rows of nothing but the lowest
+    value (all words alike).  Against 64 bits: a log-probability is off by its own rounding and that of the row's differences, 2^-22 of them, and by
+    the sum's roundings."""
+    g = torch.Generator().manual_seed(v)
+    x = torch.randn(12, v, generator=g)
+    low = torch.finfo(dtype).min
+    x[0, : v - 3], x[1, 3:], x[2], x[3, : v // 2], x[4, : v // 2] = -1e10, low, low, -1e4, -1e30
+    x[5] += 1e6
+    x[6] -= 1e6
+    x[7] = x[7] * 1e9
+    x[8] = -1e30
+    x[8, v // 3] = -1e30 * (1 - 2 ** -6)
+    x[9] = 3e38
+    x[10, : v - 1], x[10, v - 1] = low, -low
+    x = x.to(dtype)
+    targets = torch.tensor([v - 1, 2, 5, v - 1, v - 1, 7, 7, int(x[7].float().argmax()), v // 3, 1, v - 1, 3])
+    wide, tape64 = x.double(), T.Tape()
+    tape64.watch(wide)
+    want, terms64 = T.policy_loss(tape64, wide, targets, torch.ones(12), scale=1.0)
+    wgrad = tape64.backward(want)[id(wide)]
+    here, tape = x.to(DEV), T.Tape()
+    tape.watch(here)
+    loss, terms = T.policy_loss(tape, here, targets.to(DEV), torch.ones(12, device=DEV), scale=1.0)
+    grad = tape.backward(loss)[id(here)].cpu()
+    spread = (wide.amax(-1) - wide.gather(-1, targets[:, None])[:, 0]).abs()
+    assert ((terms.logprobs.cpu() - terms64.logprobs).abs() <= spread * 2 ** -22 + _adds(v) * 2 ** -24 + terms64.logprobs.abs() * 2 ** -23).all()
+    bound = _grad_bounds(x, terms64.weights.double(), torch.zeros(12, dtype=torch.float64), v)
+    assert torch.isfinite(grad).all() and ((grad.double() - wgrad).abs() <= bound).all()
+    chosen = here.view(12, 1, v)
+    tape.watch(chosen)
+    pref, seen = T.preference_loss(tape, chosen, targets.to(DEV)[:, None])
+    assert torch.allclose(seen.logprobs, terms.logprobs, rtol=2 ** -22, atol=_adds(v) * 2 ** -24)
+    pgrad = tape.backward(pref)[id(chosen)].cpu().view(12, v).double()
+    # the same rows with other weights (a sequence of one row each): their gradients are in the same proportion
+    tg = torch.arange(12), targets
+    share = pgrad[tg] / torch.where(wgrad[tg] == 0, 1.0, wgrad[tg])
+    assert torch.isfinite(pgrad).all() and ((pgrad - wgrad * share[:, None]).abs() <= 2 * bound * share.abs()[:, None] + 2 ** -20 * (wgrad * share[:, None]).abs()
+                                            + (wgrad[tg] == 0)[:, None]).all()
+
+
 @pytest.mark.parametrize("v", [40, 5000, 20000, 150000, 270000])
 def test_targets_outside_of_the_vocabulary(v):
     lg = torch.randn(4, v, generator=torch.Generator().manual_seed(0)).to(DEV)
@@ -221,7 +264,7 @@ def test_the_same_bits_twice():
 
 def test_more_rows_than_blocks_run_at_a_time():
     """Persistent forms go through their rows in turn: every row as it is on its own, scored ones and others in any order."""
-    for n, v in ((900, 1500), (700, 20001), (200, 66000)):
+    for n, v in ((5000, 400), (900, 1500), (700, 20001), (200, 66000)):
         g = torch.Generator(device=DEV).manual_seed(n)
         lg = torch.randn(n, v, generator=g, device=DEV)
         tg = torch.randint(0, v, (n,), generator=g, device=DEV)

@@ -44,7 +44,7 @@ def policy(logits, targets, mask, adv, old, ref, *, lo: float, hi: float, kl: fl
 def preference(logits, targets, mask, ref: Optional[torch.Tensor], *, beta: float, smooth: float, average: bool, scale: float, want_grad: bool):
     """Loss, log-probabilities of the sequences, margins of the pairs and the gradient (or None); tensors as for :func:`policy`."""
     x, n, (seqs, t) = logits.contiguous(), targets.numel(), targets.shape
-    keep = 4 * n + 2 * seqs                             # floats that the kernels keep: a row's log-probability (fp64) and (base, sum), a pair's loss (fp64) and weights
+    keep = 6 * n + 2 * seqs                             # floats that the kernels keep: of a row four for its gradient and its log-probability (fp64), of a pair its loss (fp64) and weights
     with N.on(x.device):
         some = torch.empty(keep + seqs + seqs // 2 + 1, dtype=torch.float32, device=x.device)
         grad, at = _like(x) if want_grad else None, some.data_ptr()
