@@ -158,30 +158,46 @@ __device__ __forceinline__ double pl_block_sum(double v, double* red) {
 
 // ---- the two passes over a row --------------------------------------------------------------------------------------------------
 // G vectors a thread at a time, NT threads apart: f(vectors, first one's place, whether all are there).  Those past the end are -inf.
-template <typename T, int NT, int G, typename F>
-__device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f) {
+// HINT: L2 is told whether it should keep them (the second pass reads them again: 1024 x 248 320 388 -> 382 us, bf16 217 -> 213) or they are not needed
+// any more.
+__device__ __forceinline__ uint64_t pl_policy_of(bool keep) {
+  uint64_t last, first;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(last));
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  return keep ? last : first;
+}
+template <bool HINT>
+__device__ __forceinline__ uint4 pl_load(const uint4* p, uint64_t policy) {
+  if (!HINT) return *p;
+  uint4 v;
+  asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
+  return v;
+}
+template <typename T, int NT, int G, bool HINT = false, typename F>
+__device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f, bool keep = false) {
+  const uint64_t policy = HINT ? pl_policy_of(keep) : 0;
   int i = threadIdx.x;
   const uint4* p = body + i;
   uint4 z[G];
 #pragma unroll 1
   for (; i + (G - 1) * NT < cnt; i += G * NT, p += G * NT) {
 #pragma unroll
-    for (int k = 0; k < G; ++k) z[k] = p[k * NT];
+    for (int k = 0; k < G; ++k) z[k] = pl_load<HINT>(p + k * NT, policy);
     f(z, i, true);
   }
   if (i < cnt) {
     constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-    for (int k = 0; k < G; ++k) z[k] = i + k * NT < cnt ? p[k * NT] : make_uint4(low, low, low, low);
+    for (int k = 0; k < G; ++k) z[k] = i + k * NT < cnt ? pl_load<HINT>(p + k * NT, policy) : make_uint4(low, low, low, low);
     f(z, i, false);
   }
 }
 // A thread's part of a row: (B, sum of 2^(x log2 e - B)) of its vectors and the value xe at one of its ends (-inf: none).
-template <typename T, int NT, int G>
-__device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, float& base, float& s) {
+template <typename T, int NT, int G, bool HINT = false>
+__device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, float& base, float& s, bool keep = false) {
   constexpr int E = Span<T>::E, C = E == 4 ? G : G / 2 < 1 ? 1 : G / 2;        // vectors that are unpacked at a time
   base = pl_base(xe == xe ? xe : -INFINITY), s = pl_exp(xe, base);
-  pl_each<T, NT, G>(body, cnt, [&](const uint4 (&z)[G], int, bool) {
+  pl_each<T, NT, G, HINT>(body, cnt, [&](const uint4 (&z)[G], int, bool) {
 #pragma unroll
     for (int k0 = 0; k0 < G; k0 += C) {
       float v[C][E], top = -INFINITY, q[4] = {};
@@ -199,13 +215,13 @@ __device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, fl
         for (int e = 0; e < E; ++e) q[e & 3] += pl_exp(v[k][e], base);
       s += (q[0] + q[1]) + (q[2] + q[3]);
     }
-  });
+  }, keep);
 }
 // The gradients of a thread's vectors, c 2^(x log2 e - B).
-template <typename T, int NT, int G>
+template <typename T, int NT, int G, bool HINT = false>
 __device__ __forceinline__ void pl_grads(const uint4* body, uint4* dst, int cnt, float base, float c) {
   constexpr int E = Span<T>::E;
-  pl_each<T, NT, G>(body, cnt, [&](const uint4 (&z)[G], int i, bool whole) {
+  pl_each<T, NT, G, HINT>(body, cnt, [&](const uint4 (&z)[G], int i, bool whole) {
     uint4* o = dst + i;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
@@ -439,7 +455,7 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   if (tid == 0) in = PolicyIn(a, r), xt = pl_target(p.row, t, rows.V, r);
   const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
   float base, s;
-  pl_sums<T, NT, G>(p.body, p.cnt, xe, base, s);
+  pl_sums<T, NT, G, true>(p.body, p.cnt, xe, base, s, grad != nullptr);
   const float top = warp_max(base);
   s = warp_sum(pl_moved(s, base, top));
   if (lane == 0) sums[warp] = make_float2(top, s);
@@ -476,7 +492,7 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
     return;
   }
   if (!grad) return;
-  pl_grads<T, NT, G>(p.body, p.dst, p.cnt, found.x, found.y);
+  pl_grads<T, NT, G, true>(p.body, p.dst, p.cnt, found.x, found.y);
   if (p.ie >= 0) p.out[p.ie] = pl_round<T>(pl_exp(xe, found.x) * found.y);
   if (t < rows.V && pl_wrote(t, p.ie, p.sp.head, Span<T>::E, p.lo, p.cnt, tid, NT)) p.out[t] = pl_round<T>(found.z);
 }
@@ -630,15 +646,15 @@ int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaS
   if (V <= 1024) return brief(pl_policy_short_kernel<T, 64>, 4);
   if (V <= 2048) return brief(pl_policy_short_kernel<T, 128>, 2);
   if (V <= 4096) return brief(pl_policy_short_kernel<T, 256>, 1);
-  // By a row's bytes, since those in work have to stay in L2 (some 40 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
-  // us: 4096 x 8192 60 (256 threads 65), 2048 x 32 768 109 (one block of 512 a row 109, two of 256 112), 1024 x 65 536 113 (eight of 128 111), 1024 x
-  // 248 320 394 (four of 256 437, eight with four blocks an SM 437); bf16 2048 x 49 999 104, 1024 x 131 072 119, 1024 x 248 320 222.
-  constexpr int G = E == 4 ? 8 : 4;                  // 32 values a thread at a time
+  // By a row's bytes, since those in work have to stay in L2 (some 50 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
+  // us (and the next): 4096 x 8192 57 (two blocks a row 68), 2048 x 32 768 107 (one block of 384 threads 110, two of 192 108), 1024 x 65 536 110 (two of 256 113),
+  // 1024 x 248 320 382 (four of 256 415, four blocks an SM in place of three 437); bf16 2048 x 49 999 99 (one of 128 107), 1024 x 131 072 116 (four of 128
+  // 118), 1024 x 248 320 213 (eight of 256 222).
   const long bytes = V * (long)sizeof(T);
   if (bytes <= 64 << 10) return policy_launch<T, 1, 128, 8, 8>(x, rows, grad, a, st);
   if (bytes <= 192 << 10) return policy_launch<T, E == 4 ? 4 : 2, 128, 8, 8>(x, rows, grad, a, st);
   if (bytes <= 384 << 10) return policy_launch<T, 4, 256, 4, 5>(x, rows, grad, a, st);
-  return policy_launch<T, 8, 256, G, E == 4 ? 3 : 5>(x, rows, grad, a, st);
+  return policy_launch<T, E == 4 ? 8 : 4, 256, 8, 3>(x, rows, grad, a, st);
 }
 
 bool rows_ok(long n, long V) { return n >= 1 && n < 1l << 31 && V >= 1 && V < 1l << 31; }
