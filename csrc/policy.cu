@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   constexpr int E = S::E, VPT = 16 / E, N = 16, W = NT / 32, R = 256 / NT;
   __shared__ float2 sums[8];
   __shared__ float3 found[R];                        // the largest value, weight over the sum, the target's gradient
+  pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const int k = threadIdx.x % NT, mine = threadIdx.x / NT, warp = threadIdx.x >> 5;
   const long r0 = (long)blockIdx.x * R, r = r0 + mine;
   const bool there = r < rows.n, scored = there && (!rows.mask || rows.mask[r]);
@@ -437,6 +438,7 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   constexpr int W = NT / 32;
   __shared__ float2 sums[W], peers[CL];
   __shared__ float4 found;                           // base, weight over the sum, the target's gradient, whether the row is far
+  pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const long r = blockIdx.x / CL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const PolicyPart<T, CL> p(x, grad, r, rows.V);
@@ -506,6 +508,7 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   __shared__ float2 sums[NT / 32];
   __shared__ float red[32];
   __shared__ int far;
+  pdl_launch_dependents();
   const long r = blockIdx.x;
   if (rows.mask && !rows.mask[r]) {
     if (threadIdx.x == 0) lps[r] = 0.0;
@@ -544,6 +547,8 @@ template <typename T>
 __global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows rows, const float4* rest, const float* weight, long per, T* grad, int slices) {
   using S = Span<T>;
   constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
+  pdl_launch_dependents();
+  pdl_wait();
   const long r = rows.n - 1 - blockIdx.x / slices, lo = (long)(blockIdx.x % slices) * PL_SLICE;
   T* out = grad + (size_t)r * rows.V;
   const T* row = x + (size_t)r * rows.V;
@@ -579,31 +584,45 @@ __global__ void __launch_bounds__(1024) pl_sum_kernel(const double* v, long n, d
   if (threadIdx.x == 0) *out = (float)(s * scale);
 }
 
-// log(1 + e^y)
-__device__ __forceinline__ double pl_softplus(double y) { return fmax(y, 0.0) + log1p(exp(-fabs(y))); }
 // A block a pair: rows [2p T, 2p T + T) chosen, the T behind them rejected.  Results: sums of log-probabilities, margins, a pair's
 // loss, and each sequence's weight for its rows' gradients.
 __global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const float* ref, const unsigned char* mask, long T, double beta, double smooth,
                                                        int average, double scale, float* totals, float* margins, double* loss, float* weight) {
-  __shared__ double red[8];
+  __shared__ double red[8][6];
+  pdl_launch_dependents();
+  pdl_wait();
   const long p = blockIdx.x;
-  double total[2], gap[2], div[2];
+  double v[6] = {};                                  // log-probabilities, their differences to the reference's, scored tokens; chosen, rejected
+#pragma unroll
   for (int k = 0; k < 2; ++k) {
     const long at = (2 * p + k) * T;
-    double a = 0.0, b = 0.0, c = 0.0;
+#pragma unroll 4
     for (long i = threadIdx.x; i < T; i += 256)
-      if (!mask || mask[at + i]) a += lps[at + i], b += lps[at + i] - (ref ? (double)ref[at + i] : 0.0), c += 1.0;
-    total[k] = pl_block_sum<8>(a, red), gap[k] = pl_block_sum<8>(b, red), c = pl_block_sum<8>(c, red);
-    div[k] = average ? fmax(c, 1.0) : 1.0;
+      if (!mask || mask[at + i]) v[3 * k] += lps[at + i], v[3 * k + 1] += lps[at + i] - (ref ? (double)ref[at + i] : 0.0), v[3 * k + 2] += 1.0;
   }
+#pragma unroll
+  for (int q = 0; q < 6; ++q) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32][q] = v[q];
+  }
+  __syncthreads();
   if (threadIdx.x) return;
-  const double z = beta * (gap[0] / div[0] - gap[1] / div[1]), e = smooth;
-  const double dz = e / (1.0 + exp(-z)) - (1.0 - e) / (1.0 + exp(z));
-  totals[2 * p] = (float)(total[0] / div[0]), totals[2 * p + 1] = (float)(total[1] / div[1]);
+#pragma unroll
+  for (int q = 0; q < 6; ++q) {
+    v[q] = 0.0;
+    for (int w = 0; w < 8; ++w) v[q] += red[w][q];
+  }
+  const double by0 = average ? 1.0 / fmax(v[2], 1.0) : 1.0, by1 = average ? 1.0 / fmax(v[5], 1.0) : 1.0;
+  const double z = beta * (v[1] * by0 - v[4] * by1), e = smooth;
+  // with u = e^-|z|: sigmoid(|z|) = 1 / (1 + u), -log of it log(1 + u), and |z| more the other way round
+  const double u = exp(-fabs(z)), l = log1p(u), near = 1.0 / (1.0 + u), up = z >= 0.0 ? near : u * near, down = z >= 0.0 ? u * near : near;
+  const double dz = z == z ? e * up - (1.0 - e) * down : z;
+  totals[2 * p] = (float)(v[0] * by0), totals[2 * p + 1] = (float)(v[3] * by1);
   margins[p] = (float)z;
-  loss[p] = (1.0 - e) * pl_softplus(-z) + (e != 0.0 ? e * pl_softplus(z) : 0.0);
+  loss[p] = (1.0 - e) * (l + fmax(-z, 0.0)) + (e != 0.0 ? e * (l + fmax(z, 0.0)) : 0.0);
   // (the row's gradient is weight (p - onehot): minus that of its log-probability)
-  weight[2 * p] = (float)(-dz * scale * beta / div[0]), weight[2 * p + 1] = (float)(dz * scale * beta / div[1]);
+  weight[2 * p] = (float)(-dz * scale * beta * by0), weight[2 * p + 1] = (float)(dz * scale * beta * by1);
 }
 
 // x times *up; no pass over the values where that is 1.
@@ -618,8 +637,7 @@ template <typename T>
 int grad_launch(const void* x, const Rows& rows, const float4* rest, const float* weight, long per, void* grad, cudaStream_t st) {
   const long nv = rows.V / Span<T>::E, slices = nv < PL_SLICE ? 1 : (nv + PL_SLICE - 1) / PL_SLICE;
   if (rows.n * slices >= 1l << 31) return (int)cudaErrorInvalidValue;
-  pl_grad_kernel<T><<<(unsigned)(rows.n * slices), 256, 0, st>>>((const T*)x, rows, rest, weight, per, (T*)grad, (int)slices);
-  return (int)cudaGetLastError();
+  return (int)trl_launch(pl_grad_kernel<T>, dim3((unsigned)(rows.n * slices)), dim3(256), 0, st, (const T*)x, rows, rest, weight, per, (T*)grad, (int)slices);
 }
 
 template <typename T, int CL, int NT, int G, int BLOCKS>
@@ -694,8 +712,9 @@ TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, lon
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
   if (type) pl_stats_kernel<bf16><<<(int)n, 256, 0, st>>>((const bf16*)x, rows, rest, lps);
   else pl_stats_kernel<float><<<(int)n, 256, 0, st>>>((const float*)x, rows, rest, lps);
-  pl_pairs_kernel<<<(int)pairs, 256, 0, st>>>(lps, (const float*)ref, rows.mask, T, beta, smooth, average, scale, (float*)totals, (float*)margins, pair_loss,
-                                              weight);
+  const cudaError_t paired = trl_launch(pl_pairs_kernel, dim3((unsigned)pairs), dim3(256), 0, st, (const double*)lps, (const float*)ref, rows.mask, T, beta, smooth,
+                                        average, scale, (float*)totals, (float*)margins, pair_loss, weight);
+  if (paired != cudaSuccess) return (int)paired;
   if (grad) {
     const int rc = type ? grad_launch<bf16>(x, rows, rest, weight, T, grad, st) : grad_launch<float>(x, rows, rest, weight, T, grad, st);
     if (rc) return rc;
