@@ -37,6 +37,9 @@ class _Node:
         self.name, self.inputs, self.outputs, self.bwd = name, inputs, outputs, bwd
 
 
+_ONE = object()           # the root's own gradient, to ops whose ``bwd.takes_one``
+
+
 class _StandIn:
     """In the nodes, for a tensor that the tape has let go of."""
     __slots__ = ()
@@ -48,7 +51,6 @@ class Tape:
         self.leaves: Dict[int, torch.Tensor] = {}
         self.made: set = set()            # ids of the recorded ops' outputs
         self.gone: Dict[int, tuple] = {}  # id of a tensor let go of: (weak reference, its stand-in)
-        self.one: Optional[torch.Tensor] = None       # in the backward pass: the root's own gradient, where none was given
         self.tp_group, self.tp_world = tp_group, tp_world
         self.enabled = True
 
@@ -100,9 +102,13 @@ class Tape:
     def backward(self, root: torch.Tensor, grad: Optional[torch.Tensor] = None,
                  on_grad: Optional[Callable[[torch.Tensor, torch.Tensor], None]] = None
                  ) -> Dict[int, torch.Tensor]:
+        key = self._key(root)
         if grad is None:
-            grad = self.one = torch.ones_like(root)
-        grads: Dict[int, torch.Tensor] = {id(self._key(root)): grad}
+            # (a loss that has its gradient already gets no tensor of ones to multiply with)
+            last = self.nodes[-1] if self.nodes else None
+            whole = last is not None and last.outputs and last.outputs[0] is key and getattr(last.bwd, "takes_one", False)
+            grad = _ONE if whole else torch.ones_like(root)
+        grads: Dict[int, torch.Tensor] = {id(key): grad}
         # first node (in forward order) that reads each leaf = last to contribute in reverse
         first_use: Dict[int, int] = {}
         for idx, n in enumerate(self.nodes):
@@ -130,7 +136,6 @@ class Tape:
         self.nodes.clear()
         self.made.clear()
         self.gone.clear()
-        self.one = None
         return {k: g for k, g in grads.items() if k in self.leaves}
 
     def grad_of(self, grads: Dict[int, torch.Tensor], t: torch.Tensor) -> Optional[torch.Tensor]:
@@ -684,8 +689,9 @@ def _loss_inputs(what: str, logits, targets, mask, **floats):
     for name, t in floats.items():
         if t is not None and (tuple(t.shape) != rows or not t.is_floating_point()):
             raise ValueError(f"{what}: {name} is floating point {rows}, got {tuple(t.shape)} {t.dtype}")
+    dev = logits.device
     for t in (targets, mask, *floats.values()):
-        if t is not None and t.device != logits.device:
+        if t is not None and t.device != dev:
             raise ValueError(f"{what}: logits are on {logits.device}, another input on {t.device}")
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
     ready = lambda t, dtype: t if t is None or (t.dtype == dtype and t.is_contiguous()) else t.to(dtype).contiguous()
@@ -698,12 +704,13 @@ def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
     grad = grad.view(logits.shape)
 
     def bwd(g):
-        if g is tape.one:
+        if g is _ONE:
             return (grad,)
         if K is not None and g.numel() == 1 and g.device == grad.device:
             return (K.scale_grad(grad, g),)
         return (grad * g,)
 
+    bwd.takes_one = True
     tape.record(name, (logits,), (loss,), bwd)
 
 
