@@ -191,7 +191,7 @@ bool head_map(CUtensorMap* m, const void* base, long rows, long K, int box) {
 }
 
 template <int BN>
-int launch_head(const CUtensorMap& mw, const CUtensorMap& mx, float* out, long ldo, int M, int N, int nk, int grid, cudaStream_t st) {
+int launch_head(const CUtensorMap& mw, const CUtensorMap& mx, float* out, long ldo, int M, int N, int nk, int grid, bool early, cudaStream_t st) {
   auto kern = head_bf16_kernel<BN>;
   static TrlPerDevice<bool> set;
   bool& configured = set.here();
@@ -199,13 +199,12 @@ int launch_head(const CUtensorMap& mw, const CUtensorMap& mx, float* out, long l
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, HeadCfg<BN>::SMEM) != cudaSuccess) return 3;
     configured = true;
   }
-  return (int)trl_launch(kern, dim3(grid), dim3(HT_THREADS), (size_t)HeadCfg<BN>::SMEM, st, mw, mx, out, ldo, M, N, nk);
+  if (early) return (int)trl_launch(kern, dim3(grid), dim3(HT_THREADS), (size_t)HeadCfg<BN>::SMEM, st, mw, mx, out, ldo, M, N, nk);
+  kern<<<grid, HT_THREADS, HeadCfg<BN>::SMEM, st>>>(mw, mx, out, ldo, M, N, nk);
+  return (int)cudaGetLastError();
 }
 
-}  // namespace
-
-// x [M, K] bf16 contiguous, w [N, K] bf16, out fp32 [M, ldo]; K % 8 == 0, both inputs 16-byte aligned, M up to 64.
-TRL_API int trl_head_bf16(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream) {
+int head_bf16(const void* x, const void* w, void* out, long ldo, int M, int N, int K, bool early, void* stream) {
   if (M < 1 || M > 64 || N < 1 || K < 8 || K % 8 || (reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15))
     return (int)cudaErrorInvalidValue;
   const int bn = M <= 16 ? 16 : M <= 32 ? 32 : 64, tiles = (N + HT_M - 1) / HT_M;
@@ -217,8 +216,19 @@ TRL_API int trl_head_bf16(const void* x, const void* w, void* out, long ldo, int
   const int grid = min(tiles, sms), nk = (K + 2 * HT_BOX - 1) / (2 * HT_BOX);
   cudaStream_t st = (cudaStream_t)stream;
   switch (bn) {
-    case 16: return launch_head<16>(mw, mx, (float*)out, ldo, M, N, nk, grid, st);
-    case 32: return launch_head<32>(mw, mx, (float*)out, ldo, M, N, nk, grid, st);
-    default: return launch_head<64>(mw, mx, (float*)out, ldo, M, N, nk, grid, st);
+    case 16: return launch_head<16>(mw, mx, (float*)out, ldo, M, N, nk, grid, early, st);
+    case 32: return launch_head<32>(mw, mx, (float*)out, ldo, M, N, nk, grid, early, st);
+    default: return launch_head<64>(mw, mx, (float*)out, ldo, M, N, nk, grid, early, st);
   }
+}
+
+}  // namespace
+
+// x [M, K] bf16 contiguous, w [N, K] bf16, out fp32 [M, ldo]; K % 8 == 0, both inputs 16-byte aligned, M up to 64.
+TRL_API int trl_head_bf16(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream) {
+  return head_bf16(x, w, out, ldo, M, N, K, true, stream);
+}
+// The same where the kernel before may have written the weights: their first copies wait for it too.
+TRL_API int trl_head_bf16_after(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream) {
+  return head_bf16(x, w, out, ldo, M, N, K, false, stream);
 }

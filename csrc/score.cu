@@ -455,7 +455,7 @@ int score_parts(int V) { return (V + SC_WORDS - 1) / SC_WORDS * 2; }
 
 }  // namespace
 
-TRL_API int trl_head_bf16(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream);
+TRL_API int trl_head_bf16_after(const void* x, const void* w, void* out, long ldo, int M, int N, int K, void* stream);
 
 // Bytes of workspace for n rows (of which the scored ones are gathered, `packed`), a multiple of 256.
 TRL_API long trl_score_workspace(int n, int H, int V, int packed, int entropy) {
@@ -496,7 +496,7 @@ TRL_API int trl_score(const void* h, int type, const void* w, const void* target
     const long ldo = (V + 3) / 4 * 4;
     float* logits = (float*)take(4l * n * ldo);
     const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, 0, 0, (V + SC_PART - 1) / SC_PART, 0};
-    int rc = trl_head_bf16(packed ? rows : h, w, logits, ldo, n, V, H, stream);
+    int rc = trl_head_bf16_after(packed ? rows : h, w, logits, ldo, n, V, H, stream);
     if (!rc) rc = (int)trl_launch(score_part_kernel, dim3(p.parts, n), dim3(256), 0, st, (const float*)logits, ldo, p);
     return rc ? rc : (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
   }

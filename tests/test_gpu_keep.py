@@ -114,3 +114,25 @@ def test_streams_and_graphs():
     static.copy_(x)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_offsets_past_32_bits():
+    rows, width = 70000, 32768
+    x = torch.zeros(rows, width, device=DEV)
+    x[-3:] = torch.randn(3, width, generator=torch.Generator(device=DEV).manual_seed(0), device=DEV)
+    x[0] = 2.0
+    kept = T.keep8(x)
+    q, scale = keep.pack(x[-3:].cpu())
+    assert torch.equal(kept.q[-3:].cpu(), q) and torch.equal(kept.scale[-3:].cpu(), scale) and not any(p.any() for p in kept.q[1:-3].split(10000))
+    back = kept.rows()
+    assert torch.equal(back[-3:].cpu(), keep.unpack(q, scale)) and torch.equal(back[0], x[0])
+    del back, kept
+    tape = T.Tape()
+    tape.watch(x)
+    y = T.swiglu(tape, x, bits=8)
+    grad = tape.backward(y, torch.ones_like(y))[id(x)]
+    small = x[-3:].clone()
+    one = T.Tape()
+    one.watch(small)
+    z = T.swiglu(one, small, bits=8)
+    assert torch.equal(y[-3:], z) and torch.equal(grad[-3:], one.backward(z, torch.ones_like(z))[id(small)])
