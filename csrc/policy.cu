@@ -83,24 +83,63 @@ __device__ __forceinline__ uint4 pl_pack(const float (&x)[8]) {
 // ---- exponentials ------------------------------------------------------------------------------------------------------------
 // Sums are of 2^(x log2 e - B) with a whole number B, the row's largest x log2 e rounded up: one fused multiply-add, rounded once, and
 // ex2.approx, where expf(x - m) has ten instructions; instructions were these kernels' time.  A whole B makes it no matter which B: the rounding
-// of a product m log2 e would go into every value of the row.  fp32's log2 e is off by 1.3e-8 of itself, as if all of x were; ex2.approx by 2^-22, and the
-// multiply-add's rounding moves a value at a distance of d by d 2^-24 of itself, both at random over a row.
+// of a product m log2 e would go into every value of the row.  ex2.approx is off by 2^-22, and the multiply-add's rounding moves a value at a distance
+// of d by d 2^-24 of itself, both at random over a row.  fp32's log2 e is off by PL_OFF of itself, as if all of x were: lp by PL_OFF times the distance
+// of x[t] from the row's mean, 1e-7 of the same sign in every row, which a sequence's sum or a divergence shows.  So the mean, u / s with
+// u = sum 2^y y, comes out of the pass over the row too (one multiply-add more), and lp without that.  ex2.approx is low by some 4e-8 in the mean
+// (measured against 64 bits: 2 to 5e-8, by the spread of the logits), which lp is given back.
 constexpr float PL_L2E = 1.4426950408889634f;
+constexpr double PL_LN2 = 0.693147180559945309417, PL_OFF = (double)PL_L2E * PL_LN2 - 1.0, PL_LESS = 3.5e-8;
 __device__ __forceinline__ float pl_exp2(float y) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
   return e;
 }
 __device__ __forceinline__ float pl_exp(float x, float base) { return pl_exp2(fmaf(x, PL_L2E, -base)); }
+// into s and u  (0 times -inf is not meant; 2^-256 is 0)
+__device__ __forceinline__ void pl_add(float x, float base, float& s, float& u) {
+  const float y = fmaf(x, PL_L2E, -base), e = pl_exp2(y);
+  s += e, u = fmaf(e, fmaxf(y, -256.f), u);
+}
 // B for a largest value.  From below it is bounded: threads that see nothing but masked words (-inf, -1e30) have sums of 0 there.  A row whose B is
 // that bound, or so large that whole numbers near it have gaps, is far: gone through once more, slowly, with x - m.
 constexpr float PL_FAR = 2097152.f;
 __device__ __forceinline__ float pl_base(float most) { return fmaxf(ceilf(most * PL_L2E), -PL_FAR); }
 __device__ __forceinline__ bool pl_far(float base) { return !(fabsf(base) < PL_FAR); }
-// a sum at base `from` at base `to` (not below it)
-__device__ __forceinline__ float pl_moved(float s, float from, float to) { return s * pl_exp2(from - to); }
-// x - B ln 2, with it the log-probability, in fp64 and from the same log2 e, so that its error comes in with x's distance from the row's mean only
-__device__ __forceinline__ double pl_low(float x, float base) { return ((double)x * (double)PL_L2E - (double)base) * 0.693147180559945309417; }
+// (B, s, u) of some of a row's values.
+struct Part {
+  float base, s, u;
+  // at a base that is not below its own
+  __device__ __forceinline__ void move(float to) {
+    const float d = base - to, f = pl_exp2(d);
+    u = fmaf(d, s, u) * f, s *= f, base = to;
+  }
+  __device__ __forceinline__ void join_warp() {
+    move(warp_max(base));
+    s = warp_sum(s), u = warp_sum(u);
+  }
+};
+// The log-probability of a value x but for the logarithm of the sum, in fp64.
+__device__ __forceinline__ double pl_low(float x, float base, float mean) {
+  const double y = (double)x * (double)PL_L2E - (double)base;
+  return (y - PL_OFF * (y - (double)mean)) * PL_LN2 - PL_LESS;
+}
+// N parts, in order: the sum and, through it, a value's pl_low.  base: at first one that the result's is not to be below.
+template <int N>
+__device__ __forceinline__ double pl_join(const Part* parts, float& base, float& mean) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) base = fmaxf(base, parts[k].base);
+  double sum = 0.0;
+  float u = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    Part q = parts[k];
+    q.move(base);
+    sum += (double)q.s, u += q.u;
+  }
+  mean = u / (float)sum;
+  return sum;
+}
 
 template <typename T>
 __device__ __forceinline__ float pl_target(const T* row, long long t, long V, long r) {
@@ -192,30 +231,41 @@ __device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f, bool ke
     f(z, i, false);
   }
 }
-// A thread's part of a row: (B, sum of 2^(x log2 e - B)) of its vectors and the value xe at one of its ends (-inf: none).
-template <typename T, int NT, int G, bool HINT = false>
-__device__ __forceinline__ void pl_sums(const uint4* body, int cnt, float xe, float& base, float& s, bool keep = false) {
+// A thread's part of a row: of its vectors and the value xe at one of its ends (-inf: none).  SKIP: without value `skip % E` of vector
+// `skip / E` of the row.
+template <typename T, int NT, int G, bool HINT = false, bool SKIP = false>
+__device__ __forceinline__ Part pl_sums(const uint4* body, int cnt, float xe, bool keep = false, int skip = -1) {
   constexpr int E = Span<T>::E, C = E == 4 ? G : G / 2 < 1 ? 1 : G / 2;        // vectors that are unpacked at a time
-  base = pl_base(xe == xe ? xe : -INFINITY), s = pl_exp(xe, base);
-  pl_each<T, NT, G, HINT>(body, cnt, [&](const uint4 (&z)[G], int, bool) {
+  Part p = {pl_base(xe == xe ? xe : -INFINITY), 0.f, 0.f};
+  pl_add(xe, p.base, p.s, p.u);
+  const int place = SKIP && skip >= 0 && skip / E % NT == threadIdx.x ? skip / E : -1;
+  pl_each<T, NT, G, HINT>(body, cnt, [&](const uint4 (&z)[G], int i, bool) {
 #pragma unroll
     for (int k0 = 0; k0 < G; k0 += C) {
-      float v[C][E], top = -INFINITY, q[4] = {};
+      float v[C][E], top = -INFINITY, q[4] = {}, w[2] = {};
+#pragma unroll
+      for (int k = 0; k < C; ++k) pl_unpack(z[k0 + k], v[k]);
+      if (SKIP && place >= i + k0 * NT && place < i + (k0 + C) * NT) {
+        const int which = (place - (i + k0 * NT)) / NT * E + skip % E;
+#pragma unroll
+        for (int k = 0; k < C * E; ++k)              // (written so that v stays in registers)
+          asm("{ .reg .pred p; setp.eq.s32 p, %1, %2; @p mov.b32 %0, 0fFF800000; }" : "+f"(v[k / E][k % E]) : "r"(which), "r"(k));
+      }
 #pragma unroll
       for (int k = 0; k < C; ++k) {
-        pl_unpack(z[k0 + k], v[k]);
 #pragma unroll
         for (int e = 0; e < E; e += 2) top = fmaxf(top, fmaxf(v[k][e], v[k][e + 1]));
       }
       const float b = pl_base(top);
-      if (b > base) s = pl_moved(s, base, b), base = b;
+      if (b > p.base) p.move(b);
 #pragma unroll
       for (int k = 0; k < C; ++k)
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e & 3] += pl_exp(v[k][e], base);
-      s += (q[0] + q[1]) + (q[2] + q[3]);
+        for (int e = 0; e < E; ++e) pl_add(v[k][e], p.base, q[e & 3], w[e & 1]);
+      p.s += (q[0] + q[1]) + (q[2] + q[3]), p.u += w[0] + w[1];
     }
   }, keep);
+  return p;
 }
 // The gradients of a thread's vectors, c 2^(x log2 e - B).
 template <typename T, int NT, int G, bool HINT = false>
@@ -282,7 +332,7 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   using S = Span<T>;
   constexpr int E = S::E, VPT = 16 / E, N = 16, W = NT / 32, R = 256 / NT;
-  __shared__ float2 sums[8];
+  __shared__ Part sums[8];                           // (at the base of the largest value itself)
   __shared__ float3 found[R];                        // the largest value, weight over the sum, the target's gradient
   pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const int k = threadIdx.x % NT, mine = threadIdx.x / NT, warp = threadIdx.x >> 5;
@@ -311,25 +361,34 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
 #pragma unroll
     for (int j = 0; j < E; ++j) v[i * E + j] = u[j];
   }
-  float m = end, s[4] = {};
+  float m = end, s[4] = {}, u[2] = {};
 #pragma unroll
   for (int i = 0; i < N; i += 2) m = fmaxf(m, fmaxf(v[i], v[i + 1]));
   // (the largest value is known before the first exponential here, and the two more instructions of (x - m) log2 e are not what counts)
   const float most = warp_max(m), less = most == -INFINITY ? 0.f : most;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = pl_exp2((v[i] - less) * PL_L2E), s[i & 3] += v[i];
-  end = pl_exp2((end - less) * PL_L2E);
-  const float sum = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end);
-  if (threadIdx.x % 32 == 0) sums[warp] = make_float2(most, sum);
+  for (int i = 0; i < N; ++i) {
+    const float y = (v[i] - less) * PL_L2E;
+    v[i] = pl_exp2(y), s[i & 3] += v[i], u[i & 1] = fmaf(v[i], fmaxf(y, -256.f), u[i & 1]);
+  }
+  const float y = (end - less) * PL_L2E;
+  end = pl_exp2(y);
+  const float sum = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end), sum_u = warp_sum(u[0] + u[1] + end * fmaxf(y, -256.f));
+  if (threadIdx.x % 32 == 0) sums[warp] = Part{most, sum, sum_u};
   __syncthreads();
   if (weighs) {
-    float top = -INFINITY;
+    const Part* q = sums + threadIdx.x * W;
+    float top = -INFINITY, all_u = 0.f;
     double all = 0.0;
 #pragma unroll
-    for (int i = 0; i < W; ++i) top = fmaxf(top, sums[threadIdx.x * W + i].x);
+    for (int i = 0; i < W; ++i) top = fmaxf(top, q[i].base);
 #pragma unroll
-    for (int i = 0; i < W; ++i) all += (double)(sums[threadIdx.x * W + i].y * pl_exp2((sums[threadIdx.x * W + i].x - top) * PL_L2E));      // (NaN without a finite value)
-    const float2 f = pl_policy_row(a, in, rw, (double)xt - (double)top, all);
+    for (int i = 0; i < W; ++i) {                    // (without a finite value nothing is a number here)
+      const float d = fmaxf((q[i].base - top) * PL_L2E, -256.f), f = pl_exp2(d);
+      all += (double)(q[i].s * f), all_u += fmaf(d, q[i].s, q[i].u) * f;
+    }
+    const float mean = all_u / (float)all, others = 1.f - 1.f / (float)all;        // (the largest value's is 1 exactly)
+    const float2 f = pl_policy_row(a, in, rw, (double)xt - (double)top + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)others, all);
     found[threadIdx.x] = make_float3(top, f.x, f.y);
   }
   if (!grad) return;
@@ -352,7 +411,7 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
 }
 
 // Longer rows: a cluster of CL blocks goes through a row twice, for its sum and for its gradient; the second time the row is still in L2, as long as
-// those in work fit there.  Between the passes the blocks send each other their (B, sum); each adds them up in a fixed order and forms the row's weight for
+// those in work fit there.  Between the passes the blocks send each other their (B, s, u); each adds them up in a fixed order and forms the row's weight for
 // itself.  The cluster's first barrier is passed before another block's shared memory is touched, no block's is after the second.  Both end:
 // every thread of a scored row's cluster comes to them, and nothing before them waits.
 __device__ __forceinline__ uint32_t pl_map(uint32_t addr, int cta) {
@@ -391,7 +450,7 @@ struct PolicyPart {
 
 // A far row.  All blocks of its cluster come here, behind the same barriers.
 template <typename T, int CL, int NT>
-__device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad, const PolicyRow& a, long r, float2* sums, float2* peers, float4* found) {
+__device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad, const PolicyRow& a, long r, Part* sums, Part* peers, float4* found) {
   const PolicyPart<T, CL> p(x, grad, r, rows.V);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto meet = [&] {
@@ -401,19 +460,19 @@ __device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad
   auto join = [&](float v, auto warps, auto op, float none) {       // of all threads of the cluster
     v = warps(v);
     meet();                                          // (what was there before has been read)
-    if (lane == 0) sums[warp].x = v;
+    if (lane == 0) sums[warp].s = v;
     __syncthreads();
     if (warp == 0) {
-      v = warps(lane < NT / 32 ? sums[lane].x : none);
+      v = warps(lane < NT / 32 ? sums[lane].s : none);
       if (CL > 1) {
-        if (lane < CL) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(pl_map(smem_u32(&peers[p.rank]), lane)), "f"(v) : "memory");
+        if (lane < CL) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(pl_map(smem_u32(&peers[p.rank].s), lane)), "f"(v) : "memory");
       } else if (lane == 0) {
-        peers[0].x = v;
+        peers[0].s = v;
       }
     }
     meet();
-    v = peers[0].x;
-    for (int k = 1; k < CL; ++k) v = op(v, peers[k].x);
+    v = peers[0].s;
+    for (int k = 1; k < CL; ++k) v = op(v, peers[k].s);
     return v;
   };
   const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
@@ -436,7 +495,7 @@ __device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad
 template <typename T, int CL, int NT, int G, int BLOCKS>
 __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const __grid_constant__ Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   constexpr int W = NT / 32;
-  __shared__ float2 sums[W], peers[CL];
+  __shared__ Part sums[W], peers[CL];
   __shared__ float4 found;                           // base, weight over the sum, the target's gradient, whether the row is far
   pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const long r = blockIdx.x / CL;
@@ -456,35 +515,31 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   float xt = 0.f;
   if (tid == 0) in = PolicyIn(a, r), xt = pl_target(p.row, t, rows.V, r);
   const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
-  float base, s;
-  pl_sums<T, NT, G, true>(p.body, p.cnt, xe, base, s, grad != nullptr);
-  const float top = warp_max(base);
-  s = warp_sum(pl_moved(s, base, top));
-  if (lane == 0) sums[warp] = make_float2(top, s);
+  Part part = pl_sums<T, NT, G, true>(p.body, p.cnt, xe, grad != nullptr);
+  part.join_warp();
+  if (lane == 0) sums[warp] = part;
   __syncthreads();
   if (CL > 1) pl_cluster_wait();
   if (warp == 0) {
-    const float2 q = lane < W ? sums[lane] : make_float2(-PL_FAR, 0.f);
-    const float mine = warp_max(q.x), sum = warp_sum(pl_moved(q.y, q.x, mine));
+    part = lane < W ? sums[lane] : Part{-PL_FAR, 0.f, 0.f};
+    part.join_warp();
     if (CL > 1) {
-      if (lane < CL)
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(pl_map(smem_u32(&peers[p.rank]), lane)), "f"(mine), "f"(sum) : "memory");
+      if (lane < CL) {
+        const uint32_t to = pl_map(smem_u32(&peers[p.rank]), lane);
+        asm volatile("st.shared::cluster.f32 [%0], %1; st.shared::cluster.f32 [%0 + 4], %2; st.shared::cluster.f32 [%0 + 8], %3;" ::"r"(to), "f"(part.base), "f"(part.s), "f"(part.u) : "memory");
+      }
     } else if (lane == 0) {
-      peers[0] = make_float2(mine, sum);
+      peers[0] = part;
     }
   }
   if (CL > 1) pl_cluster_arrive(), pl_cluster_wait();
   if (tid == 0) {
-    float all = -PL_FAR;
-    double sum = 0.0;
-#pragma unroll
-    for (int k = 0; k < CL; ++k) all = fmaxf(all, peers[k].x);
-#pragma unroll
-    for (int k = 0; k < CL; ++k) sum += (double)pl_moved(peers[k].y, peers[k].x, all);
+    float all = -PL_FAR, mean;
+    const double sum = pl_join<CL>(peers, all, mean);
     if (pl_far(all)) {
       found.w = 1.f;
     } else {
-      const PolicyOut o = pl_policy(a, in, r, pl_low(xt, all), sum, p.rank == 0);
+      const PolicyOut o = pl_policy(a, in, r, pl_low(xt, all, mean), sum, p.rank == 0);
       found = make_float4(all, (float)((double)o.weight * o.part), o.target, 0.f);
     }
   }
@@ -505,7 +560,7 @@ template <typename T>
 __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows rows, float4* rest, double* lps) {
   using S = Span<T>;
   constexpr int NT = 256, G = sizeof(T) == 4 ? 8 : 4;
-  __shared__ float2 sums[NT / 32];
+  __shared__ Part sums[NT / 32];
   __shared__ float red[32];
   __shared__ int far;
   pdl_launch_dependents();
@@ -517,27 +572,31 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   const T* row = x + (size_t)r * rows.V;
   const S sp(row, rows.V);
   const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
-  float xt = 0.f, base, s;
-  if (threadIdx.x == 0) xt = pl_target(row, rows.target[r], rows.V, r);
+  float xt = 0.f;
+  const long long t = rows.target[r];
+  if (threadIdx.x == 0) xt = pl_target(row, t, rows.V, r);
   const long ie = sp.end_of(threadIdx.x);
   const float xe = ie >= 0 ? pl_float(row[ie]) : -INFINITY;
-  pl_sums<T, NT, G>(body, (int)sp.nv, xe, base, s);
-  const float top = warp_max(base);
-  s = warp_sum(pl_moved(s, base, top));
-  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = make_float2(top, s);
+  // A sequence's sum takes in every row's error.  Where the target is likely, that is its exponential's and what additions to it lose: 6e-8 a row (a
+  // plain softmax in fp32: 9e-8), without it 8e-9.  So the target stays out of the sums and comes in in fp64.
+  Part part = pl_sums<T, NT, G, false, true>(body, (int)sp.nv, ie == t ? -INFINITY : xe, false,
+                                             t >= sp.head && t < sp.head + sp.nv * S::E ? (int)(t - sp.head) : -1);
+  part.join_warp();
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = part;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float all = -PL_FAR;
-    double sum = 0.0;
-    for (int k = 0; k < NT / 32; ++k) all = fmaxf(all, sums[k].x);
-    for (int k = 0; k < NT / 32; ++k) sum += (double)pl_moved(sums[k].y, sums[k].x, all);
-    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all) - log(sum);
+    float all = pl_base(xt == xt ? xt : -INFINITY), mean;
+    const double rest_of = pl_join<NT / 32>(sums, all, mean);
+    const double y = (double)xt * (double)PL_L2E - (double)all, e = exp(y * PL_LN2), sum = rest_of + e, most = e / sum;
+    // (the mean of the others, and the target's share)
+    const float of_all = rest_of > 0.0 ? mean + (float)most * (fmaxf((float)y, -256.f) - mean) : (float)y;
+    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all, of_all) + PL_LESS * most - log(sum);
     far = pl_far(all);
   }
   __syncthreads();
   if (!far) return;
   const float m = block_max(pl_far_most<T, NT>(body, (int)sp.nv, xe), red);
-  s = block_sum(pl_far_sum<T, NT>(body, (int)sp.nv, xe, ie >= 0, m), red);
+  const float s = block_sum(pl_far_sum<T, NT>(body, (int)sp.nv, xe, ie >= 0, m), red);
   if (threadIdx.x == 0) rest[r] = make_float4(0.f, m, s, 1.f), lps[r] = (double)xt - (double)m - log((double)s);
 }
 

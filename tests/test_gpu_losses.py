@@ -302,3 +302,65 @@ def test_inputs_on_unlike_devices_are_refused():
     for kw in (dict(targets=torch.zeros(2, dtype=torch.long)), dict(mask=torch.ones(2, dtype=torch.bool)), dict(advantages=torch.zeros(2)), dict(old_logprobs=torch.zeros(2))):
         with pytest.raises(ValueError):
             T.policy_loss(T.Tape(), **{**dict(logits=lg, targets=torch.zeros(2, dtype=torch.long, device=DEV), advantages=torch.zeros(2, device=DEV), scale=1.0), **kw})
+
+
+def test_offsets_past_32_bits():
+    """2.2e9 logits of which the first and the last rows are scored: as those rows on their own, zeros everywhere else."""
+    n, v = 9000, 248320
+    g = torch.Generator(device=DEV).manual_seed(0)
+    lg = torch.empty(n, v, dtype=torch.bfloat16, device=DEV)
+    some = torch.tensor([0, 1, n - 2, n - 1], device=DEV)
+    rows = torch.randn(4, v, generator=g, device=DEV).bfloat16()
+    lg[some] = rows
+    lg[2:n - 2] = NAN
+    targets, mask = torch.full((n,), -5, device=DEV), torch.zeros(n, dtype=torch.bool, device=DEV)
+    targets[some], mask[some] = torch.tensor([0, v - 1, 7, v - 2], device=DEV), True
+    adv = torch.randn(n, generator=g, device=DEV)
+    for pref in (False, True):
+        tape, one = T.Tape(), T.Tape()
+        shape = (lambda t: t.view(2, n // 2, *t.shape[1:])) if pref else (lambda t: t)
+        big, small = shape(lg), rows.view(2, 2, v) if pref else rows
+        tape.watch(big), one.watch(small)
+        if pref:
+            loss, _ = T.preference_loss(tape, big, shape(targets), shape(mask))
+            want, _ = T.preference_loss(one, small, targets[some].view(2, 2))
+        else:
+            loss, terms = T.policy_loss(tape, big, targets, adv, scale=0.25, mask=mask)
+            want, alone = T.policy_loss(one, small, targets[some], adv[some], scale=0.25)
+            assert torch.equal(terms.logprobs[some], alone.logprobs) and int(terms.logprobs.count_nonzero()) == 4
+        assert torch.allclose(loss, want, rtol=1e-6)
+        grad = tape.backward(loss)[id(big)].view(n, v)
+        assert torch.equal(grad[some], one.backward(want)[id(small)].view(4, v))
+        assert not any(part.any() for part in grad[2:n - 2].split(1000))
+        del grad, tape, big
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v,offset", [(5, 1), (700, 0), (4099, 3), (20000, 2), (33000, 0)])
+def test_sums_of_rows_whose_target_is_nearly_certain(v, offset, dtype):
+    """The target at 40, the others at 0: a log-probability of -(v - 1) e^-40.  What is left of it in 64 bits: 1e-16 a number near 1, and the words'
+    mean, which is fp32 (6e-8 of 58, in binary places), times fp32's relative error of log2 e, 2^-24 at most: under 1e-12 a row.  The target's
+    place goes through a vector, a thread's vectors, both ends of the row."""
+    t = 96
+    places = torch.tensor(sorted({*range(min(v, 24)), *range(max(0, v - 24), v), *torch.linspace(0, v - 1, 48).long().tolist()}))
+    targets = places[torch.arange(2 * t) % len(places)].view(2, t).to(DEV)
+    here = torch.zeros(2 * t * v + offset, dtype=dtype, device=DEV)[offset:].view(2, t, v)
+    here.scatter_(-1, targets[..., None], 40.0)
+    _, terms = T.preference_loss(T.Tape(), here, targets)
+    want = -t * (v - 1) * math.exp(-40.0)
+    assert ((terms.logprobs.double().cpu() - want).abs() <= t * 1e-12).all()
+
+
+@pytest.mark.parametrize("v", [513, 33001])
+def test_sums_of_rows_whose_target_is_far_from_the_mean(v):
+    """The target at -80, the others at 0, whose exponentials are 1 exactly: what is left is what rows are given back for the mean of
+    an exponential's error (under 2^-22 as the error is) and fp64's.  A relative error of fp32's log2 e (1.3e-8) in x would be 1e-6 a row."""
+    t = 256
+    here = torch.zeros(2, t, v, device=DEV)
+    here[0, :, 3], here[1, :, 3] = -80.0, 40.0
+    exact = torch.tensor([-80.0 - math.log(v - 1), -(v - 1) * math.exp(-40.0)], dtype=torch.float64)
+    ref = exact.float()[:, None].expand(2, t).contiguous()
+    _, terms = T.preference_loss(T.Tape(), here, torch.full((2, t), 3, device=DEV), ref_logprobs=ref.to(DEV), beta=0.5)
+    off = (exact - ref[:, 0].double()) * t
+    want = 0.5 * float(off[0] - off[1])
+    assert abs(float(terms.margins) - want) <= 0.5 * t * 2 ** -22 / 4 + abs(want) * 2 ** -24
