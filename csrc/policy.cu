@@ -17,6 +17,8 @@
 // (src/tilerl/train.py:805-864).
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "tcgen05.cuh"
 
 namespace {
@@ -231,6 +233,10 @@ __device__ __forceinline__ void pl_each(const uint4* body, int cnt, F f, bool ke
     f(z, i, false);
   }
 }
+// x = -inf if a == b  (written so that arrays of x stay in registers)
+__device__ __forceinline__ void pl_lower(float& x, int a, int b) {
+  asm("{ .reg .pred p; setp.eq.s32 p, %1, %2; @p mov.b32 %0, 0fFF800000; }" : "+f"(x) : "r"(a), "r"(b));
+}
 // A thread's part of a row: of its vectors and the value xe at one of its ends (-inf: none).  SKIP: without value `skip % E` of vector
 // `skip / E` of the row.
 template <typename T, int NT, int G, bool HINT = false, bool SKIP = false>
@@ -248,8 +254,7 @@ __device__ __forceinline__ Part pl_sums(const uint4* body, int cnt, float xe, bo
       if (SKIP && place >= i + k0 * NT && place < i + (k0 + C) * NT) {
         const int which = (place - (i + k0 * NT)) / NT * E + skip % E;
 #pragma unroll
-        for (int k = 0; k < C * E; ++k)              // (written so that v stays in registers)
-          asm("{ .reg .pred p; setp.eq.s32 p, %1, %2; @p mov.b32 %0, 0fFF800000; }" : "+f"(v[k / E][k % E]) : "r"(which), "r"(k));
+        for (int k = 0; k < C * E; ++k) pl_lower(v[k / E][k % E], which, k);
       }
 #pragma unroll
       for (int k = 0; k < C; ++k) {
@@ -320,6 +325,58 @@ __device__ __forceinline__ bool pl_wrote(long long t, long end, int head, int E,
   return t >= 0 && (t == end || (t >= head && tv >= 0 && tv < cnt && tv % NT == k));
 }
 
+// The values of thread k of a short row's NT: N of its vectors; -inf where there are none.
+constexpr int PL_SHORT = 16;
+template <typename T, int NT>
+__device__ __forceinline__ void pl_short_load(const uint4* body, int nv, int k, float (&v)[PL_SHORT]) {
+  constexpr int E = Span<T>::E;
+#pragma unroll
+  for (int i = 0; i < PL_SHORT / E; ++i) {
+    constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;       // -inf
+    float u[E];
+    pl_unpack(k + i * NT < nv ? body[k + i * NT] : make_uint4(low, low, low, low), u);
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[i * E + j] = u[j];
+  }
+}
+// v as 2^((v - less) log2 e), and with the value at an end their sums over the warp.  (The largest value is known before the first exponential here, and the two
+// more instructions of (x - m) log2 e are not what counts.)
+__device__ __forceinline__ Part pl_short_sums(float (&v)[PL_SHORT], float& end, float most, float less) {
+  float s[4] = {}, u[2] = {};
+#pragma unroll
+  for (int i = 0; i < PL_SHORT; ++i) {
+    const float y = (v[i] - less) * PL_L2E;
+    v[i] = pl_exp2(y), s[i & 3] += v[i], u[i & 1] = fmaf(v[i], fmaxf(y, -256.f), u[i & 1]);
+  }
+  const float y = (end - less) * PL_L2E;
+  end = pl_exp2(y);
+  return {most, warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end), warp_sum(u[0] + u[1] + end * fmaxf(y, -256.f))};
+}
+__device__ __forceinline__ float pl_short_most(const float (&v)[PL_SHORT], float end) {
+#pragma unroll
+  for (int i = 0; i < PL_SHORT; i += 2) end = fmaxf(end, fmaxf(v[i], v[i + 1]));
+  return warp_max(end);
+}
+// W parts at the base of their largest values to one at `top` (not below them).  Without a finite value nothing is a number here.
+template <int W>
+__device__ __forceinline__ double pl_short_join(const Part* q, float top, float& u) {
+  double s = 0.0;
+  u = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const float d = fmaxf((q[i].base - top) * PL_L2E, -256.f), f = pl_exp2(d);
+    s += (double)(q[i].s * f), u += fmaf(d, q[i].s, q[i].u) * f;
+  }
+  return s;
+}
+template <int W>
+__device__ __forceinline__ float pl_short_top(const Part* q) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < W; ++i) top = fmaxf(top, q[i].base);
+  return top;
+}
+
 // ---- policy loss -----------------------------------------------------------------------------------------------------------------
 // Up to 4096 values: NT threads a row, which waits in registers, 16 values a thread, as exponentials until its sum and weight are known; the rows of a
 // block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, logarithm and exponentials in fp64) is some 6 us, so what
@@ -331,7 +388,7 @@ __device__ __noinline__ float2 pl_policy_row(const PolicyRow& a, const PolicyIn&
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   using S = Span<T>;
-  constexpr int E = S::E, VPT = 16 / E, N = 16, W = NT / 32, R = 256 / NT;
+  constexpr int E = S::E, VPT = PL_SHORT / E, W = NT / 32, R = 256 / NT;
   __shared__ Part sums[8];                           // (at the base of the largest value itself)
   __shared__ float3 found[R];                        // the largest value, weight over the sum, the target's gradient
   pdl_launch_dependents();                           // (only the sum, which waits for all of this)
@@ -352,41 +409,17 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
   uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
   const long ie = there ? sp.end_of(k) : -1;
-  float v[N], end = scored && ie >= 0 ? pl_float(row[ie]) : -INFINITY;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    constexpr uint32_t low = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;       // -inf
-    float u[E];
-    pl_unpack(scored && k + i * NT < nv ? body[k + i * NT] : make_uint4(low, low, low, low), u);
-#pragma unroll
-    for (int j = 0; j < E; ++j) v[i * E + j] = u[j];
-  }
-  float m = end, s[4] = {}, u[2] = {};
-#pragma unroll
-  for (int i = 0; i < N; i += 2) m = fmaxf(m, fmaxf(v[i], v[i + 1]));
-  // (the largest value is known before the first exponential here, and the two more instructions of (x - m) log2 e are not what counts)
-  const float most = warp_max(m), less = most == -INFINITY ? 0.f : most;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = (v[i] - less) * PL_L2E;
-    v[i] = pl_exp2(y), s[i & 3] += v[i], u[i & 1] = fmaf(v[i], fmaxf(y, -256.f), u[i & 1]);
-  }
-  const float y = (end - less) * PL_L2E;
-  end = pl_exp2(y);
-  const float sum = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) + end), sum_u = warp_sum(u[0] + u[1] + end * fmaxf(y, -256.f));
-  if (threadIdx.x % 32 == 0) sums[warp] = Part{most, sum, sum_u};
+  float v[PL_SHORT], end = scored && ie >= 0 ? pl_float(row[ie]) : -INFINITY;
+  pl_short_load<T, NT>(body, scored ? nv : 0, k, v);
+  const float most = pl_short_most(v, end), less = most == -INFINITY ? 0.f : most;
+  const Part part = pl_short_sums(v, end, most, less);
+  if (threadIdx.x % 32 == 0) sums[warp] = part;
   __syncthreads();
   if (weighs) {
     const Part* q = sums + threadIdx.x * W;
-    float top = -INFINITY, all_u = 0.f;
-    double all = 0.0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) top = fmaxf(top, q[i].base);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {                    // (without a finite value nothing is a number here)
-      const float d = fmaxf((q[i].base - top) * PL_L2E, -256.f), f = pl_exp2(d);
-      all += (double)(q[i].s * f), all_u += fmaf(d, q[i].s, q[i].u) * f;
-    }
+    float all_u;
+    const float top = pl_short_top<W>(q);
+    const double all = pl_short_join<W>(q, top, all_u);
     const float mean = all_u / (float)all, others = 1.f - 1.f / (float)all;        // (the largest value's is 1 exactly)
     const float2 f = pl_policy_row(a, in, rw, (double)xt - (double)top + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)others, all);
     found[threadIdx.x] = make_float3(top, f.x, f.y);
@@ -600,6 +633,78 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   if (threadIdx.x == 0) rest[r] = make_float4(0.f, m, s, 1.f), lps[r] = (double)xt - (double)m - log((double)s);
 }
 
+// Up to 4096 values, as the policy loss has them: NT threads a row.  Of `rest` the largest value and the sum.
+template <typename T, int NT>
+__global__ void __launch_bounds__(256, 5) pl_stats_short_kernel(const T* x, const Rows rows, float4* rest, double* lps) {
+  constexpr int E = Span<T>::E, W = NT / 32, R = 256 / NT;
+  __shared__ Part sums[8];
+  pdl_launch_dependents();
+  const int k = threadIdx.x % NT;
+  const long r0 = (long)blockIdx.x * R, r = r0 + threadIdx.x / NT, rw = r0 + threadIdx.x;
+  const bool scored = r < rows.n && (!rows.mask || rows.mask[r]);
+  const bool forms = threadIdx.x < R && rw < rows.n, weighs = forms && (!rows.mask || rows.mask[rw]);
+  float xt = 0.f;
+  if (weighs) xt = pl_target(x + (size_t)rw * rows.V, rows.target[rw], rows.V, rw);
+  else if (forms) lps[rw] = 0.0;
+  const T* row = x + (size_t)r * rows.V;
+  const Span<T> sp(row, rows.V);
+  const long ie = scored ? sp.end_of(k) : -1;
+  const long long t = scored ? rows.target[r] : -1;
+  float v[PL_SHORT], end = ie >= 0 && ie != t ? pl_float(row[ie]) : -INFINITY;
+  pl_short_load<T, NT>(reinterpret_cast<const uint4*>(row + sp.head), scored ? (int)sp.nv : 0, k, v);
+  if (t >= sp.head && t < sp.head + sp.nv * E && (int)(t - sp.head) / E % NT == k) {       // (the target comes in below)
+    const int which = (int)(t - sp.head) / E / NT * E + (int)(t - sp.head) % E;
+#pragma unroll
+    for (int i = 0; i < PL_SHORT; ++i) pl_lower(v[i], which, i);
+  }
+  const float most = pl_short_most(v, end), less = most == -INFINITY ? 0.f : most;
+  const Part part = pl_short_sums(v, end, most, less);
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = part;
+  __syncthreads();
+  if (!weighs) return;
+  const Part* q = sums + threadIdx.x * W;
+  const float others = pl_short_top<W>(q), top = fmaxf(others, xt);
+  float u;
+  const double rest_of = pl_short_join<W>(q, top, u), low = (double)xt - (double)top, e = exp(low), sum = rest_of + e;
+  const float mean = (u + (float)e * fmaxf((float)low * PL_L2E, -256.f)) / (float)sum;
+  const double rough = rest_of - (others == top ? 1.0 : 0.0);          // (of the sum, from exponentials that are not exact)
+  rest[rw] = make_float4(0.f, top, (float)sum, 1.f);
+  lps[rw] = low + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (rough / sum) - log(sum);
+}
+template <typename T, int NT>
+__global__ void __launch_bounds__(256, 5) pl_grad_short_kernel(const T* x, const Rows rows, const float4* rest, const float* weight, long per, T* grad) {
+  constexpr int E = Span<T>::E, R = 256 / NT;
+  pdl_launch_dependents();
+  pdl_wait();
+  const long r = rows.n - 1 - ((long)blockIdx.x * R + threadIdx.x / NT);
+  const int k = threadIdx.x % NT;
+  if (r < 0) return;
+  const bool scored = !rows.mask || rows.mask[r];
+  const T* row = x + (size_t)r * rows.V;
+  T* out = grad + (size_t)r * rows.V;
+  const Span<T> sp(row, rows.V);
+  const int nv = (int)sp.nv;
+  const long ie = sp.end_of(k);
+  float v[PL_SHORT];
+  pl_short_load<T, NT>(reinterpret_cast<const uint4*>(row + sp.head), scored ? nv : 0, k, v);
+  const float w = scored ? weight[(unsigned)r / (unsigned)per] : 0.f;
+  const float4 st = scored ? rest[r] : make_float4(0.f, 0.f, 1.f, 0.f);
+  const float c = w / st.z;
+  uint4* dst = reinterpret_cast<uint4*>(out + sp.head);
+  auto one = [&](float x) { return pl_exp2((x - st.y) * PL_L2E); };
+#pragma unroll
+  for (int i = 0; i < PL_SHORT / E; ++i) {
+    float u[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) u[j] = scored ? one(v[i * E + j]) * c : 0.f;
+    if (k + i * NT < nv) __stcs(dst + k + i * NT, pl_pack(u));
+  }
+  if (ie >= 0) out[ie] = pl_round<T>(scored ? one(pl_float(row[ie])) * c : 0.f);
+  if (!scored) return;
+  const long long t = rows.target[r];
+  if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>((one(pl_float(row[t])) / st.z - 1.f) * w);
+}
+
 // Gradients: a block a slice of a row.  weight of row r: weight[r / per].  The last rows first: they are what L2 still holds.
 constexpr int PL_SLICE = 4096;                       // vectors a block
 template <typename T>
@@ -692,8 +797,34 @@ __global__ void __launch_bounds__(256) pl_scale_kernel(T* x, const float* up, lo
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) x[i] = pl_round<T>(pl_float(x[i]) * u);
 }
 
+// f(NT as a type) for rows of up to 4096 values, 16 a thread.
+template <typename F>
+int short_form(long V, F f) {
+  if (V <= 512) return f(std::integral_constant<int, 32>());
+  if (V <= 1024) return f(std::integral_constant<int, 64>());
+  if (V <= 2048) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
+}
+constexpr long PL_SHORT_ROW = 4096;
+unsigned short_blocks(long n, int threads) { return (unsigned)((n + 256 / threads - 1) / (256 / threads)); }
+
+template <typename T>
+int stats_launch(const T* x, const Rows& rows, float4* rest, double* lps, cudaStream_t st) {
+  if (rows.V > PL_SHORT_ROW) {
+    pl_stats_kernel<T><<<(unsigned)rows.n, 256, 0, st>>>(x, rows, rest, lps);
+    return (int)cudaGetLastError();
+  }
+  return short_form(rows.V, [&](auto nt) {
+    pl_stats_short_kernel<T, nt.value><<<short_blocks(rows.n, nt.value), 256, 0, st>>>(x, rows, rest, lps);
+    return (int)cudaGetLastError();
+  });
+}
 template <typename T>
 int grad_launch(const void* x, const Rows& rows, const float4* rest, const float* weight, long per, void* grad, cudaStream_t st) {
+  if (rows.V <= PL_SHORT_ROW)
+    return short_form(rows.V, [&](auto nt) {
+      return (int)trl_launch(pl_grad_short_kernel<T, nt.value>, dim3(short_blocks(rows.n, nt.value)), dim3(256), 0, st, (const T*)x, rows, rest, weight, per, (T*)grad);
+    });
   const long nv = rows.V / Span<T>::E, slices = nv < PL_SLICE ? 1 : (nv + PL_SLICE - 1) / PL_SLICE;
   if (rows.n * slices >= 1l << 31) return (int)cudaErrorInvalidValue;
   return (int)trl_launch(pl_grad_kernel<T>, dim3((unsigned)(rows.n * slices)), dim3(256), 0, st, (const T*)x, rows, rest, weight, per, (T*)grad, (int)slices);
@@ -715,14 +846,11 @@ template <typename T>
 int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaStream_t st) {
   constexpr int E = Span<T>::E;
   const long V = rows.V;
-  auto brief = [&](auto kern, int per_block) {
-    kern<<<(unsigned)((rows.n + per_block - 1) / per_block), 256, 0, st>>>(x, rows, grad, a);
-    return (int)cudaGetLastError();
-  };
-  if (V <= 512) return brief(pl_policy_short_kernel<T, 32>, 8);
-  if (V <= 1024) return brief(pl_policy_short_kernel<T, 64>, 4);
-  if (V <= 2048) return brief(pl_policy_short_kernel<T, 128>, 2);
-  if (V <= 4096) return brief(pl_policy_short_kernel<T, 256>, 1);
+  if (V <= PL_SHORT_ROW)
+    return short_form(V, [&](auto nt) {
+      pl_policy_short_kernel<T, nt.value><<<short_blocks(rows.n, nt.value), 256, 0, st>>>(x, rows, grad, a);
+      return (int)cudaGetLastError();
+    });
   // By a row's bytes, since those in work have to stay in L2 (some 50 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
   // us (and the next): 4096 x 8192 57 (two blocks a row 68), 2048 x 32 768 107 (one block of 384 threads 110, two of 192 108), 1024 x 65 536 110 (two of 256 113),
   // 1024 x 248 320 382 (four of 256 415, four blocks an SM in place of three 437); bf16 2048 x 49 999 99 (one of 128 107), 1024 x 131 072 116 (four of 128
@@ -769,8 +897,8 @@ TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, lon
   double* pair_loss = lps + n;
   float* weight = (float*)(pair_loss + pairs);
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
-  if (type) pl_stats_kernel<bf16><<<(int)n, 256, 0, st>>>((const bf16*)x, rows, rest, lps);
-  else pl_stats_kernel<float><<<(int)n, 256, 0, st>>>((const float*)x, rows, rest, lps);
+  const int stated = type ? stats_launch((const bf16*)x, rows, rest, lps, st) : stats_launch((const float*)x, rows, rest, lps, st);
+  if (stated) return stated;
   const cudaError_t paired = trl_launch(pl_pairs_kernel, dim3((unsigned)pairs), dim3(256), 0, st, (const double*)lps, (const float*)ref, rows.mask, T, beta, smooth,
                                         average, scale, (float*)totals, (float*)margins, pair_loss, weight);
   if (paired != cudaSuccess) return (int)paired;

@@ -364,3 +364,10 @@ def test_sums_of_rows_whose_target_is_far_from_the_mean(v):
     off = (exact - ref[:, 0].double()) * t
     want = 0.5 * float(off[0] - off[1])
     assert abs(float(terms.margins) - want) <= 0.5 * t * 2 ** -22 / 4 + abs(want) * 2 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pairs,t,v,offset", [(3, 11, 17, 2), (2, 7, 512, 0), (1, 5, 513, 1), (2, 6, 1024, 0), (1, 9, 1025, 3), (3, 3, 2048, 0), (1, 7, 2049, 1), (2, 3, 4096, 0), (1, 3, 4096, 3), (1, 5, 4097, 0)])
+def test_preference_loss_at_the_borders_of_its_short_rows(pairs, t, v, offset, dtype):
+    """Rows of every number of threads that keep them in registers, and one value to either side."""
+    test_preference_loss(pairs, t, v, offset, dtype)
