@@ -272,6 +272,19 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
   gp_cluster_sync();                                // no CTA leaves while the other's half is being given back
 }
 
+// The log-probability and the entropy of a row whose words' (m, s, u) are joined.
+__device__ __forceinline__ void score_write(const ScoreArgs& p, int to, float xt, float m, float s, float u, float* lp, float* entropy) {
+  const long long t = p.target[to];
+  const double log_s = log((double)s);
+  if (t < 0 || t >= p.V) {
+    trl_set_error(TRL_ERR_BOUNDS, SC_SITE, (int)t, p.V);
+    lp[to] = NAN;
+  } else {
+    lp[to] = (float)((double)xt - (double)m - log_s);
+  }
+  if (entropy) entropy[to] = (float)(log_s - (double)u / (double)s);
+}
+
 // A block a scored row: its tiles together.
 __global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, float* lp, float* entropy) {
   __shared__ float red[32];
@@ -292,90 +305,114 @@ __global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, floa
   s = block_sum(s, red);
   if (entropy) u = block_sum(u, red);
   if (threadIdx.x) return;
+  score_write(p, p.index ? p.index[row] : row, p.xt[row], m, s, u, lp, entropy);
+}
+
+// Few rows, whose logits [n, ldo] are there: a cluster of blocks a row, each goes through its part of the words once and sends the first its (m, s, u).
+constexpr int SC_SPREAD = 8;
+__global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_few_kernel(const float* x, long ldo, const ScoreArgs p, float* lp, float* entropy) {
+  __shared__ float red[32];
+  __shared__ float parts[SC_SPREAD][3];
+  pdl_wait();
+  const int row = blockIdx.x / SC_SPREAD, rank = blockIdx.x % SC_SPREAD, n = p.count ? *p.count : p.n;
+  if (row >= n) return;                              // (the whole cluster)
+  const float* at = x + (size_t)row * ldo;
+  const int nv = (int)(ldo / 4), per = (nv + SC_SPREAD - 1) / SC_SPREAD, end = min(nv, (rank + 1) * per);
+  float m = -INFINITY, s = 0.f, u = 0.f;
+  for (int i = rank * per + threadIdx.x; i < end; i += 4 * 256) {
+    float4 v[4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = i + k * 256;
+      v[k] = j < end ? reinterpret_cast<const float4*>(at)[j] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (j == nv - 1) {                             // (the last vector may reach past the words)
+        if (4 * j + 1 >= p.V) v[k].y = -INFINITY;
+        if (4 * j + 2 >= p.V) v[k].z = -INFINITY;
+        if (4 * j + 3 >= p.V) v[k].w = -INFINITY;
+      }
+      top = fmaxf(top, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
+    }
+    if (top > m) {
+      if (m != -INFINITY) {
+        const float f = expf(m - top);
+        u = f == 0.f ? 0.f : f * (u + s * (m - top)), s *= f;
+      }
+      m = top;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    auto one = [&](float x) {
+      const float d = x - base, e = expf(d);
+      s += e;
+      if (e > 0.f) u += e * d;
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) one(v[k].x), one(v[k].y), one(v[k].z), one(v[k].w);
+  }
+  auto moved = [](float& s, float& u, float from, float to) {
+    const float f = from == -INFINITY ? 0.f : expf(from - to);
+    u = f == 0.f ? 0.f : f * (u + s * (from - to)), s *= f;
+  };
+  const float most = block_max(m, red);
+  moved(s, u, m, most);
+  s = block_sum(s, red);
+  if (entropy) u = block_sum(u, red);
+  gp_cluster_sync();                                 // all blocks run
+  if (threadIdx.x == 0) {
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_u32(parts[rank])));
+    asm volatile("st.shared::cluster.f32 [%0], %1; st.shared::cluster.f32 [%0 + 4], %2; st.shared::cluster.f32 [%0 + 8], %3;" ::"r"(to), "f"(most), "f"(s), "f"(u) : "memory");
+  }
+  gp_cluster_sync();
+  if (rank || threadIdx.x) return;
+  m = -INFINITY, s = 0.f, u = 0.f;
+  for (int k = 0; k < SC_SPREAD; ++k) m = fmaxf(m, parts[k][0]);
+  for (int k = 0; k < SC_SPREAD; ++k) {
+    float sk = parts[k][1], uk = parts[k][2];
+    moved(sk, uk, parts[k][0], m);
+    s += sk, u += uk;
+  }
   const int to = p.index ? p.index[row] : row;
   const long long t = p.target[to];
-  const double log_s = log((double)s);
-  if (t < 0 || t >= p.V) {
-    trl_set_error(TRL_ERR_BOUNDS, SC_SITE, (int)t, p.V);
-    lp[to] = NAN;
-  } else {
-    lp[to] = (float)((double)p.xt[row] - (double)m - log_s);
-  }
-  if (entropy) entropy[to] = (float)(log_s - (double)u / (double)s);
+  score_write(p, to, t >= 0 && t < p.V ? at[t] : 0.f, m, s, u, lp, entropy);
 }
 
-// Few rows: their logits [n, ldo] are there; a block a row and SC_PART words of it.
-constexpr int SC_PART = 4096;
-__global__ void __launch_bounds__(256) score_part_kernel(const float* x, long ldo, const ScoreArgs p) {
-  __shared__ float red[32];
-  pdl_wait();
-  const int row = blockIdx.y, n = p.count ? *p.count : p.n;
-  if (row >= n) return;
-  const int c0 = blockIdx.x * SC_PART + threadIdx.x * 4;
-  const float* at = x + (size_t)row * ldo + c0;
-  float4 v[4];
-  float m = -INFINITY, s = 0.f, u = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int c = c0 + k * 1024;
-    v[k] = c < p.V ? *reinterpret_cast<const float4*>(at + k * 1024) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    if (c + 1 >= p.V) v[k].y = -INFINITY;            // (the last vector of a row may reach past it)
-    if (c + 2 >= p.V) v[k].z = -INFINITY;
-    if (c + 3 >= p.V) v[k].w = -INFINITY;
-    m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
-  }
-  m = block_max(m, red);
-  const float base = m == -INFINITY ? 0.f : m;
-  auto one = [&](float x) {
-    const float d = x - base, e = expf(d);
-    s += e;
-    if (e > 0.f) u += e * d;
-  };
-#pragma unroll
-  for (int k = 0; k < 4; ++k) one(v[k].x), one(v[k].y), one(v[k].z), one(v[k].w);
-  s = block_sum(s, red);
-  if (p.part_u) u = block_sum(u, red);
-  if (threadIdx.x) return;
-  const size_t o = (size_t)row * p.parts + blockIdx.x;
-  p.part[o] = make_float2(m, s);
-  if (p.part_u) p.part_u[o] = u;
-  const long long t = p.target[p.index ? p.index[row] : row];
-  if (t >= 0 && t < p.V && t / SC_PART == blockIdx.x) p.xt[row] = x[(size_t)row * ldo + t];
-}
-
-// Indices of the scored rows in order, and their number; results of the others are 0.  One block.
-__global__ void __launch_bounds__(1024) score_rows_kernel(const unsigned char* mask, int n, int* index, int* count, float* lp, float* entropy) {
-  __shared__ int sums[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0;
-  for (int i0 = 0; i0 < n; i0 += 1024) {
-    const int i = i0 + threadIdx.x;
-    const bool on = i < n && mask[i];
-    if (i < n && !on) {
+// The scored rows in bf16, one behind the other in order, their indices, and their number; results of the others are 0.  A block a row: it counts the
+// scored ones before it for itself (some KB of mask bytes from L2 each; one block that counted for all took 8 us on its own: 4096
+// rows, half of them, 32 768 x 1024, 112 us with entropies, 125 before).
+template <typename T>
+__global__ void __launch_bounds__(256) score_pack_kernel(const T* h, bf16* out, int n, int H, const unsigned char* mask, int* index, int* count, float* lp, float* entropy) {
+  __shared__ int sums[8];
+  const int i = blockIdx.x;
+  int row = i;
+  if (mask) {
+    const bool on = mask[i];
+    if (!on && threadIdx.x == 0) {
       lp[i] = 0.f;
       if (entropy) entropy[i] = 0.f;
     }
-    const unsigned vote = __ballot_sync(0xffffffffu, on);
-    if (lane == 0) sums[warp] = __popc(vote);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
+    if (!on && i != n - 1) return;
+    int before = 0;
+    if (reinterpret_cast<uintptr_t>(mask) % 4 == 0) {
+      const uint32_t* four = reinterpret_cast<const uint32_t*>(mask);
+      for (int k = threadIdx.x; k < i / 4; k += 256) before += __popc(__vsetne4(four[k], 0u));
+      if (threadIdx.x < i % 4) before += mask[i / 4 * 4 + threadIdx.x] != 0;
+    } else {
+      for (int k = threadIdx.x; k < i; k += 256) before += mask[k] != 0;
     }
-    if (on) index[base + before + __popc(vote & ((1u << lane) - 1u))] = i;
-    base += all;
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = before;
     __syncthreads();
+    row = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) row += sums[w];
+    if (threadIdx.x == 0) {
+      if (on) index[row] = i;
+      if (i == n - 1) *count = row + on;
+    }
+    if (!on) return;
   }
-  if (threadIdx.x == 0) *count = base;
-}
-// The scored rows in bf16, one behind the other.
-template <typename T>
-__global__ void __launch_bounds__(256) score_pack_kernel(const T* h, bf16* out, int n, int H, const int* index, const int* count) {
-  pdl_wait();
-  const int row = blockIdx.x;
-  if (count && row >= *count) return;
-  const T* src = h + (size_t)(index ? index[row] : row) * H;
+  const T* src = h + (size_t)i * H;
   bf16* dst = out + (size_t)row * H;
   for (int c = threadIdx.x * 8; c < H; c += 2048) {
     uint4 v;
@@ -449,7 +486,7 @@ int score_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& 
 
 // Up to so many rows the head's kernel for decode ticks streams the words (its MMA has them as rows, and as many columns as there are hidden rows), and
 // their logits, 1 MB a row of 248 320, go through L2: an MMA of 256 rows here, most of them empty, takes longer than the words from memory.  Pairs and
-// this, us: 248 320 x 5120 1 row 562, 388 (389 to read W), 32 rows 441, 411, 40 rows 445, 431, 64 rows 449, 445; 32 768 x 1024 1 row 40, 30, 33 rows 34, 34.
+// this, us: 248 320 x 5120 1 row 562, 388 (389 to read W), 32 rows 441, 411, 40 rows 445, 431, 64 rows 449, 445; 32 768 x 1024 1 row 40, 28, 33 rows 34, 32.
 constexpr int SC_FEW = 32;
 int score_parts(int V) { return (V + SC_WORDS - 1) / SC_WORDS * 2; }
 
@@ -459,9 +496,9 @@ TRL_API int trl_head_bf16_after(const void* x, const void* w, void* out, long ld
 
 // Bytes of workspace for n rows (of which the scored ones are gathered, `packed`), a multiple of 256.
 TRL_API long trl_score_workspace(int n, int H, int V, int packed, int entropy) {
-  long b = (long)n * score_parts(V) * (entropy ? 12 : 8) + 4l * n * 2 + 512;
+  long b = 4l * n * 2 + 512;
   if (packed) b += 2l * n * H + 512;
-  if (n <= SC_FEW) b += 4l * n * ((V + 3) / 4 * 4) + 512;
+  b += n <= SC_FEW ? 4l * n * ((V + 3) / 4 * 4) : (long)n * score_parts(V) * (entropy ? 12 : 8);
   return (b + 255) / 256 * 256;
 }
 // h [n, H] (type 0: fp32, 1: bf16), w [V, H] bf16, both contiguous and 16-byte aligned, H % 8 == 0; target int64 [n]; mask bytes [n] or null; lp and entropy
@@ -480,26 +517,25 @@ TRL_API int trl_score(const void* h, int type, const void* w, const void* target
     at += (bytes + 15) / 16 * 16;
     return r;
   };
-  float2* part = (float2*)take(8l * n * parts);
-  float* part_u = entropy ? (float*)take(4l * n * parts) : nullptr;
-  float* xt = (float*)take(4l * n);
   int* index = mask ? (int*)take(4l * n) : nullptr;
   int* count = mask ? (int*)take(4) : nullptr;
   bf16* rows = packed ? (bf16*)take(2l * n * H) : nullptr;
-  if (mask) score_rows_kernel<<<1, 1024, 0, st>>>((const unsigned char*)mask, n, index, count, (float*)lp, (float*)entropy);
   if (packed) {
-    const cudaError_t rc = type == 0 ? trl_launch(score_pack_kernel<float>, dim3(n), dim3(256), 0, st, (const float*)h, rows, n, H, (const int*)index, (const int*)count)
-                                     : trl_launch(score_pack_kernel<bf16>, dim3(n), dim3(256), 0, st, (const bf16*)h, rows, n, H, (const int*)index, (const int*)count);
+    if (type == 0) score_pack_kernel<float><<<n, 256, 0, st>>>((const float*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
+    else score_pack_kernel<bf16><<<n, 256, 0, st>>>((const bf16*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
+    const cudaError_t rc = cudaGetLastError();
     if (rc != cudaSuccess) return (int)rc;
   }
   if (n <= SC_FEW) {
     const long ldo = (V + 3) / 4 * 4;
     float* logits = (float*)take(4l * n * ldo);
-    const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, 0, 0, (V + SC_PART - 1) / SC_PART, 0};
-    int rc = trl_head_bf16_after(packed ? rows : h, w, logits, ldo, n, V, H, stream);
-    if (!rc) rc = (int)trl_launch(score_part_kernel, dim3(p.parts, n), dim3(256), 0, st, (const float*)logits, ldo, p);
-    return rc ? rc : (int)trl_launch(score_join_kernel, dim3(n), dim3(128), 0, st, p, (float*)lp, (float*)entropy);
+    const ScoreArgs p{count, index, (const long long*)target, nullptr, nullptr, nullptr, n, V, 0, 0, 0, 0};
+    const int rc = trl_head_bf16_after(packed ? rows : h, w, logits, ldo, n, V, H, stream);
+    return rc ? rc : (int)trl_launch(score_few_kernel, dim3(SC_SPREAD * n), dim3(256), 0, st, (const float*)logits, ldo, p, (float*)lp, (float*)entropy);
   }
+  float2* part = (float2*)take(8l * n * parts);
+  float* part_u = entropy ? (float*)take(4l * n * parts) : nullptr;
+  float* xt = (float*)take(4l * n);
   CUtensorMap mh, mw;
   if (!score_map(&mh, packed ? rows : h, n, H) || !score_map(&mw, w, V, H)) return (int)cudaErrorInvalidValue;
   const ScoreArgs p{count, index, (const long long*)target, part, part_u, xt, n, V, (H + SC_KT - 1) / SC_KT, v_tiles, parts, (H + SC_SEGMENT - 1) / SC_SEGMENT};

@@ -37,7 +37,7 @@ def test_scoring(rows, hidden, vocab):
     want, went = _exact(h, w, tg)
     before = native.launch_count
     lp, ent = T.linear_logprobs(h, w, tg, entropy=True)
-    assert native.launch_count == before + (3 if tg.numel() <= score.FEW else 2) and score.takes(h, w)
+    assert native.launch_count == before + 2 and score.takes(h, w)
     assert ((lp - want).abs() <= 2 * _bound(h, w) + want.abs() * 2 ** -23).all()
     # a logit's error moves the entropy by p (log p + H) of it, whose sum over the words is the deviation of log p: below 1 + log(vocab) here
     assert ((ent - went).abs() <= 10 * _bound(h, w) + went.abs() * 2 ** -22).all()
@@ -117,3 +117,36 @@ def test_calls_of_many_rows_streams_and_graphs(monkeypatch):
     for _ in range(50):                                   # the same bits every time
         assert torch.equal(T.linear_logprobs(h, w, tg, mask=mask), want)
     assert native.read_error()[0] == 0
+
+
+@pytest.mark.parametrize("n", [1, 3, 20, 32, 33, 255, 300])
+def test_masks_that_begin_anywhere(n):
+    """The scored rows' places are counted from the mask's words or bytes, by where it begins: none, all, the first, the last, some."""
+    h, w, tg, _ = _inputs((n,), 64, 300, n)
+    lp, ent = T.linear_logprobs(h, w, tg, entropy=True)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    for offset in range(4):
+        mask = torch.zeros(n + offset, dtype=torch.bool, device=DEV)[offset:]
+        for on in (mask, ~mask, torch.arange(n, device=DEV) == 0, torch.arange(n, device=DEV) == n - 1, torch.rand(n, generator=g, device=DEV) < 0.5):
+            mask.copy_(on)
+            for x in (h, h.float()):
+                got, gent = T.linear_logprobs(x, w, tg, mask=mask, entropy=True)
+                assert torch.equal(got, torch.where(on, lp, 0.0)) and torch.equal(gent, torch.where(on, ent, 0.0))
+
+
+@pytest.mark.parametrize("vocab", [1, 31, 1024, 32768, 33001])
+def test_few_rows_with_values_without_a_number(vocab):
+    """Logits of infinity and NaN of a hidden row's, words on their own far above the others, in every block's part of the words."""
+    w = torch.zeros(vocab, 16, device=DEV)
+    w[:, 0] = 1.0
+    places = sorted({0, vocab // 3, vocab // 2, vocab - 1})
+    for k, c in enumerate(places):
+        w[c, 1 + k] = 1.0
+    h = torch.zeros(len(places) + 2, 16, device=DEV)
+    for k in range(len(places)):
+        h[k, 1 + k] = 60.0                    # the word is all of the row: e^-60 for each of the others
+    h[-2, 0], h[-1, 0] = NAN, float("inf")
+    tg = torch.tensor(places + [0, 0], device=DEV)
+    lp, ent = T.linear_logprobs(h.bfloat16(), w.bfloat16(), tg, entropy=True)
+    assert (lp[:-2].abs() <= 1e-15).all() and (ent[:-2].abs() <= 1e-15).all() if vocab > 1 else not lp[:-2].any()
+    assert lp[-2:].isnan().all() and ent[-2:].isnan().all()

@@ -32,13 +32,13 @@ def policy(logits, targets, mask, adv, old, ref, *, lo: float, hi: float, kl: fl
     x, n = logits.contiguous(), targets.numel()
     with N.on(x.device):
         # one piece of memory: what the kernels keep (n doubles), the terms, the loss
-        some, clipped = torch.empty(6 * n + 1, dtype=torch.float32, device=x.device), torch.empty(targets.shape, dtype=torch.bool, device=x.device)
+        some, clipped = torch.empty(6 * n + 1, dtype=torch.float32, device=x.device), torch.empty_like(targets, dtype=torch.bool)
         grad, at = _like(x) if want_grad else None, some.data_ptr()
         N.check(N.lib().trl_policy_loss(x.data_ptr(), TYPES[x.dtype], n, x.shape[-1], targets.data_ptr(), N.ptr(mask), adv.data_ptr(), n // adv.numel(),
                                         N.ptr(old), N.ptr(ref), lo, hi, kl, scale, at + 8 * n, clipped.data_ptr(), at + 24 * n, N.ptr(grad), at,
                                         N.stream()), "policy_loss")
     N.count(2)
-    return some[6 * n], some[2 * n:6 * n].view(4, *targets.shape).unbind(0), clipped, grad
+    return some[6 * n], some.as_strided((4, *targets.shape), (n, *targets.stride()), 2 * n).unbind(0), clipped, grad
 
 
 def preference(logits, targets, mask, ref: Optional[torch.Tensor], *, beta: float, smooth: float, average: bool, scale: float, want_grad: bool):

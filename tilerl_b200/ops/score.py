@@ -34,14 +34,14 @@ def score(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[to
         n, kind = h.shape[0], int(h.dtype == torch.bfloat16)
         lp = torch.empty(n, dtype=torch.float32, device=h.device)
         ent = torch.empty_like(lp) if entropy else None
+        packed = int(mask is not None or not kind)
         for a in range(0, n, ROWS):
-            some = slice(a, min(n, a + ROWS))
-            m = some.stop - a
-            packed = int(mask is not None or not kind)
+            m = min(n - a, ROWS)
+            piece = (lambda t: t) if m == n else (lambda t: None if t is None else t[a:a + m])
             work = torch.empty(lib.trl_score_workspace(m, hidden, v, packed, int(entropy)), dtype=torch.uint8, device=h.device)
-            N.check(lib.trl_score(h[some].data_ptr(), kind, w.data_ptr(), targets[some].data_ptr(), None if mask is None else mask[some].data_ptr(), m, hidden, v,
-                                  lp[some].data_ptr(), ent[some].data_ptr() if entropy else None, work.data_ptr(), N.stream()), "score")
-            N.count(2 + packed + int(mask is not None) + int(m <= FEW))
+            N.check(lib.trl_score(piece(h).data_ptr(), kind, w.data_ptr(), piece(targets).data_ptr(), N.ptr(piece(mask)), m, hidden, v, piece(lp).data_ptr(),
+                                  N.ptr(piece(ent)), work.data_ptr(), N.stream()), "score")
+            N.count(2 + packed)
     return lp, ent
 
 

@@ -701,7 +701,8 @@ def _loss_inputs(what: str, logits, targets, mask, **floats):
 def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
     if grad is None:
         return
-    grad = grad.view(logits.shape)
+    if grad.shape != logits.shape:
+        grad = grad.view(logits.shape)
 
     def bwd(g):
         if g is _ONE:
