@@ -23,8 +23,8 @@ MOST = float.fromhex("0x1.020406p+121")      # the largest scale 127 times which
 
 
 def _empty(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty(x.shape, dtype=torch.int8, device=x.device),
-            torch.empty(*x.shape[:-1], -(-x.shape[-1] // GROUP), dtype=torch.float32, device=x.device))
+    like = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    return like, torch.empty(*x.shape[:-1], -(-x.shape[-1] // GROUP), dtype=torch.float32, device=x.device)
 
 
 def pack(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -68,7 +68,7 @@ class Kept8:
         if not (q.is_cuda and q.numel() and N.has("trl_keep_unpack")):
             return unpack(q, self.scale)
         with N.on(q.device):
-            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+            out = torch.empty_like(q, dtype=torch.float32)
             N.check(N.lib().trl_keep_unpack(q.data_ptr(), self.scale.data_ptr(), out.data_ptr(), q.numel() // q.shape[-1], q.shape[-1], N.stream()), "keep_unpack")
         N.count()
         return out
@@ -106,7 +106,7 @@ def swiglu(gu: torch.Tensor) -> Tuple[torch.Tensor, Kept8]:
 def swiglu_grad(kept: Kept8, g: torch.Tensor) -> torch.Tensor:
     g, q = g.float().contiguous(), kept.q
     with N.on(q.device):
-        d = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        d = torch.empty_like(q, dtype=torch.float32)
         N.check(N.lib().trl_keep_swiglu_grad(q.data_ptr(), kept.scale.data_ptr(), g.data_ptr(), d.data_ptr(), q.numel() // q.shape[-1], q.shape[-1], N.stream()),
                 "keep_swiglu_grad")
     N.count()
