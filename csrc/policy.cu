@@ -199,7 +199,7 @@ __device__ __forceinline__ double pl_block_sum(double v, double* red) {
 
 // ---- the two passes over a row --------------------------------------------------------------------------------------------------
 // G vectors a thread at a time, NT threads apart: f(vectors, first one's place, whether all are there).  Those past the end are -inf.
-// HINT: L2 is told whether it should keep them (the second pass reads them again: 1024 x 248 320 388 -> 382 us, bf16 217 -> 213) or they are not needed
+// HINT: L2 is told whether it should keep them (the second pass reads them again: 1.5 % less time at 1024 x 248 320) or they are not needed
 // any more.
 __device__ __forceinline__ uint64_t pl_policy_of(bool keep) {
   uint64_t last, first;
@@ -852,7 +852,7 @@ int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaS
       return (int)cudaGetLastError();
     });
   // By a row's bytes, since those in work have to stay in L2 (some 50 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
-  // us (and the next): 4096 x 8192 57 (two blocks a row 68), 2048 x 32 768 107 (one block of 384 threads 110, two of 192 108), 1024 x 65 536 110 (two of 256 113),
+  // us, before the pass summed the mean too, which takes 2 % (and the next): 4096 x 8192 57 (two blocks a row 68), 2048 x 32 768 107 (one block of 384 threads 110, two of 192 108), 1024 x 65 536 110 (two of 256 113),
   // 1024 x 248 320 382 (four of 256 415, four blocks an SM in place of three 437); bf16 2048 x 49 999 99 (one of 128 107), 1024 x 131 072 116 (four of 128
   // 118), 1024 x 248 320 213 (eight of 256 222).
   const long bytes = V * (long)sizeof(T);
