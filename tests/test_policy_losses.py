@@ -324,3 +324,15 @@ def test_swiglu_with_its_pairs_in_8_bits(shape):
 def test_packed_bytes_by_hand():
     q, scale = keep.pack(torch.tensor([[127.0, -63.5, 0.4, 0.5, 1.5, -126.6]]))
     assert q.tolist() == [[127, -64, 0, 0, 2, -127]] and scale.tolist() == [[1.0]]        # ties go to the even one
+
+
+def test_a_segment_that_hands_on_its_input():
+    """What goes in is what comes out: the tape lets go of both, and the gradient goes on to the op that made it."""
+    x = torch.randn(3, 200, generator=torch.Generator().manual_seed(1))
+    tape = T.Tape()
+    tape.watch(x)
+    h = T.scale(tape, x, 2.0)
+    y = tape.checkpoint(lambda t, z: z, h, bits=8)
+    z = T.scale(tape, tape.checkpoint(lambda t, z: z, y, bits=8), 3.0)
+    grads = tape.backward(z, torch.ones_like(z))
+    assert torch.equal(grads[id(x)], torch.full_like(x, 6.0))

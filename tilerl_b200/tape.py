@@ -82,13 +82,15 @@ class Tape:
         return known[1] if known is not None and known[0]() is t else t
 
     def _swap(self, old, new) -> None:
+        if id(old) in self.made:
+            self.made.discard(id(old)), self.made.add(id(new))
         for n in reversed(self.nodes):
+            through = any(t is old for t in n.inputs)
             n.inputs = tuple(new if t is old else t for t in n.inputs)
             if any(t is old for t in n.outputs):
                 n.outputs = tuple(new if t is old else t for t in n.outputs)
-                if id(old) in self.made:
-                    self.made.discard(id(old)), self.made.add(id(new))
-                break
+                if not through:               # (an op may hand on what it was given)
+                    break
 
     def let_go(self, t: torch.Tensor) -> None:
         """Hold ``t`` no longer, for ops that keep another form of what they need of it; gradients still pass.  (A watched tensor stays.)"""
