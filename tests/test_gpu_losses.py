@@ -371,3 +371,17 @@ def test_sums_of_rows_whose_target_is_far_from_the_mean(v):
 def test_preference_loss_at_the_borders_of_its_short_rows(pairs, t, v, offset, dtype):
     """Rows of every number of threads that keep them in registers, and one value to either side."""
     test_preference_loss(pairs, t, v, offset, dtype)
+
+
+@pytest.mark.parametrize("v", [11, 5000])
+def test_one_row_without_dimensions_before_the_vocabulary(v):
+    logits, here, targets, _, adv, old, refs = _inputs((1,), v, torch.float32, v)
+    kw = dict(scale=1.0, kl_coef=0.1)
+    whole, row = T.Tape(), T.Tape()
+    whole.watch(here)
+    loss, terms = T.policy_loss(whole, here, targets.to(DEV), adv.to(DEV), old_logprobs=old.to(DEV), ref_logprobs=refs.to(DEV), **kw)
+    one = here[0].clone()
+    row.watch(one)
+    got, some = T.policy_loss(row, one, targets[0].to(DEV), adv[0].to(DEV), old_logprobs=old[0].to(DEV), ref_logprobs=refs[0].to(DEV), **kw)
+    assert torch.equal(got, loss) and all(torch.equal(a, b[0]) and a.shape == () for a, b in zip(some, terms))
+    assert torch.equal(row.backward(got)[id(one)], whole.backward(loss)[id(here)][0])

@@ -170,8 +170,8 @@ register("any", "sm100", {
     "train_cross_entropy": Kernel("tr_lse_kernel + tr_ce_grad_kernel", "csrc/train.cu", "trl_train_lse", "tilerl_b200.ops.train_kernels"),
     "train_policy_loss": Kernel("pl_policy_kernel + pl_policy_short_kernel + pl_sum_kernel", "csrc/policy.cu", "trl_policy_loss", "tilerl_b200.ops.loss_kernels",
                                 note="clipped policy loss with a KL term, fp32 or bf16 logits"),
-    "train_preference_loss": Kernel("pl_stats_kernel + pl_pairs_kernel + pl_grad_kernel", "csrc/policy.cu", "trl_preference_loss", "tilerl_b200.ops.loss_kernels"),
-    "score_tokens": Kernel("score_kernel + score_join_kernel", "csrc/score.cu", "trl_score", "tilerl_b200.ops.score",
+    "train_preference_loss": Kernel("pl_stats_kernel + pl_stats_short_kernel + pl_pairs_kernel + pl_grad_kernel + pl_grad_short_kernel", "csrc/policy.cu", "trl_preference_loss", "tilerl_b200.ops.loss_kernels"),
+    "score_tokens": Kernel("score_pack_kernel + score_kernel + score_join_kernel + score_few_kernel", "csrc/score.cu", "trl_score", "tilerl_b200.ops.score",
                            note="log-probabilities and entropies from hidden rows and the head, logits in TMEM; only scored rows"),
     "keep_8bit": Kernel("kp_kernel", "csrc/keep.cu", "trl_keep_pack", "tilerl_b200.ops.keep", note="activations in 8 bits, groups of 128; SwiGLU from and to them"),
     "train_gdn": Kernel("gt_prep_kernel + gt_chunk_kernel + gt_scan_kernel + gt_norm_kernel", "csrc/gdn_train.cu", "trl_gdn_train_forward", "tilerl_b200.ops.gdn_train",
