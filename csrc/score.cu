@@ -93,6 +93,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ 
   gp_cluster_sync();                                // both halves are allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();                          // (the joining blocks, which wait for all of this)
   pdl_wait();                                       // (the rows and their number come from the kernels before)
   const int n = p.count ? min(*p.count, p.n) : p.n, r_tiles = (n + 2 * SC_ROWS - 1) / (2 * SC_ROWS), units = r_tiles * p.v_tiles;
 
@@ -285,27 +286,48 @@ __device__ __forceinline__ void score_write(const ScoreArgs& p, int to, float xt
   if (entropy) entropy[to] = (float)(log_s - (double)u / (double)s);
 }
 
-// A block a scored row: its tiles together.
+// (s, u) of values whose largest is `from` as those of values whose largest is `to`, not below it
+__device__ __forceinline__ void score_move(float& s, float& u, float from, float to) {
+  const float f = from == -INFINITY ? 0.f : expf(from - to);
+  u = f == 0.f ? 0.f : f * (u + s * (from - to)), s *= f;
+}
+
+// A block a scored row: its tiles together, those of up to 131 072 words in registers.
 __global__ void __launch_bounds__(128) score_join_kernel(const ScoreArgs p, float* lp, float* entropy) {
+  constexpr int U = 8;
   __shared__ float red[32];
   pdl_wait();
   const int row = blockIdx.x, n = p.count ? *p.count : p.n;
   if (row >= n) return;
   const float2* part = p.part + (size_t)row * p.parts;
+  const float* part_u = p.part_u + (size_t)row * p.parts;
+  const int to = threadIdx.x || !p.index ? row : p.index[row];
+  const float xt = threadIdx.x ? 0.f : p.xt[row];
   float m = -INFINITY, s = 0.f, u = 0.f;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < p.parts; i += 128) m = fmaxf(m, part[i].x);
-  m = block_max(m, red);
-  for (int i = threadIdx.x; i < p.parts; i += 128) {
-    const float2 v = part[i];
-    const float f = expf(v.x - m);
-    s += v.y * f;
-    if (entropy && v.y != 0.f) u += f * (p.part_u[(size_t)row * p.parts + i] + v.y * (v.x - m));
+  for (int i = threadIdx.x; i < p.parts; i += U * 128) {
+    float2 v[U];
+    float w[U], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const bool there = i + k * 128 < p.parts;
+      v[k] = there ? part[i + k * 128] : make_float2(-INFINITY, 0.f);
+      w[k] = there && entropy ? part_u[i + k * 128] : 0.f;
+      top = fmaxf(top, v[k].x);
+    }
+    if (top > m) score_move(s, u, m, top), m = top;
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float f = expf(v[k].x - base);
+      s += v[k].y * f;
+      if (entropy && v[k].y != 0.f) u += f * (w[k] + v[k].y * (v[k].x - base));
+    }
   }
+  const float most = block_max(m, red);
+  score_move(s, u, m, most);
   s = block_sum(s, red);
   if (entropy) u = block_sum(u, red);
-  if (threadIdx.x) return;
-  score_write(p, p.index ? p.index[row] : row, p.xt[row], m, s, u, lp, entropy);
+  if (threadIdx.x == 0) score_write(p, to, xt, most, s, u, lp, entropy);
 }
 
 // Few rows, whose logits [n, ldo] are there: a cluster of blocks a row, each goes through its part of the words once and sends the first its (m, s, u).
@@ -334,10 +356,7 @@ __global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_f
       top = fmaxf(top, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
     }
     if (top > m) {
-      if (m != -INFINITY) {
-        const float f = expf(m - top);
-        u = f == 0.f ? 0.f : f * (u + s * (m - top)), s *= f;
-      }
+      score_move(s, u, m, top);
       m = top;
     }
     const float base = m == -INFINITY ? 0.f : m;
@@ -349,12 +368,8 @@ __global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_f
 #pragma unroll
     for (int k = 0; k < 4; ++k) one(v[k].x), one(v[k].y), one(v[k].z), one(v[k].w);
   }
-  auto moved = [](float& s, float& u, float from, float to) {
-    const float f = from == -INFINITY ? 0.f : expf(from - to);
-    u = f == 0.f ? 0.f : f * (u + s * (from - to)), s *= f;
-  };
   const float most = block_max(m, red);
-  moved(s, u, m, most);
+  score_move(s, u, m, most);
   s = block_sum(s, red);
   if (entropy) u = block_sum(u, red);
   gp_cluster_sync();                                 // all blocks run
@@ -369,7 +384,7 @@ __global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_f
   for (int k = 0; k < SC_SPREAD; ++k) m = fmaxf(m, parts[k][0]);
   for (int k = 0; k < SC_SPREAD; ++k) {
     float sk = parts[k][1], uk = parts[k][2];
-    moved(sk, uk, parts[k][0], m);
+    score_move(sk, uk, parts[k][0], m);
     s += sk, u += uk;
   }
   const int to = p.index ? p.index[row] : row;
@@ -377,44 +392,51 @@ __global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_f
   score_write(p, to, t >= 0 && t < p.V ? at[t] : 0.f, m, s, u, lp, entropy);
 }
 
-// The scored rows in bf16, one behind the other in order, their indices, and their number; results of the others are 0.  A block a row: it counts the
-// scored ones before it for itself (some KB of mask bytes from L2 each; one block that counted for all took 8 us on its own: 4096
-// rows, half of them, 32 768 x 1024, 112 us with entropies, 125 before).
+// The scored rows in bf16, one behind the other in order, their indices, and their number; results of the others are 0.  A warp a row; a block counts
+// the scored rows before its own for itself (some KB of mask bytes from L2; one block that counted for all took 8 us on its own, a block a row
+// with the copy 9).
+constexpr int SC_PACK = 8;                           // rows a block
 template <typename T>
-__global__ void __launch_bounds__(256) score_pack_kernel(const T* h, bf16* out, int n, int H, const unsigned char* mask, int* index, int* count, float* lp, float* entropy) {
-  __shared__ int sums[8];
-  const int i = blockIdx.x;
+__global__ void __launch_bounds__(SC_PACK * 32) score_pack_kernel(const T* h, bf16* out, int n, int H, const unsigned char* mask, int* index, int* count, float* lp, float* entropy) {
+  __shared__ int sums[SC_PACK];
+  pdl_launch_dependents();
+  const int first = blockIdx.x * SC_PACK, warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = first + warp;
   int row = i;
   if (mask) {
-    const bool on = mask[i];
-    if (!on && threadIdx.x == 0) {
-      lp[i] = 0.f;
-      if (entropy) entropy[i] = 0.f;
-    }
-    if (!on && i != n - 1) return;
+    const unsigned on = __ballot_sync(0xffffffffu, lane < SC_PACK && first + lane < n && mask[first + lane]);
     int before = 0;
-    if (reinterpret_cast<uintptr_t>(mask) % 4 == 0) {
-      const uint32_t* four = reinterpret_cast<const uint32_t*>(mask);
-      for (int k = threadIdx.x; k < i / 4; k += 256) before += __popc(__vsetne4(four[k], 0u));
-      if (threadIdx.x < i % 4) before += mask[i / 4 * 4 + threadIdx.x] != 0;
-    } else {
-      for (int k = threadIdx.x; k < i; k += 256) before += mask[k] != 0;
-    }
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = before;
-    __syncthreads();
-    row = 0;
+    if (on || first + SC_PACK >= n) {                // (the last block says how many there are)
+      if (reinterpret_cast<uintptr_t>(mask) % 4 == 0) {
+        const uint32_t* four = reinterpret_cast<const uint32_t*>(mask);
+#pragma unroll 4
+        for (int k = threadIdx.x; k < first / 4; k += SC_PACK * 32) before += __popc(__vsetne4(four[k], 0u));
+      } else {
+        for (int k = threadIdx.x; k < first; k += SC_PACK * 32) before += mask[k] != 0;
+      }
+      before = __reduce_add_sync(0xffffffffu, before);
+      if (lane == 0) sums[warp] = before;
+      __syncthreads();
+      before = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) row += sums[w];
-    if (threadIdx.x == 0) {
-      if (on) index[row] = i;
-      if (i == n - 1) *count = row + on;
+      for (int w = 0; w < SC_PACK; ++w) before += sums[w];
     }
-    if (!on) return;
+    if (first + SC_PACK >= n && threadIdx.x == 0) *count = before + __popc(on);
+    if (i >= n) return;
+    if (!(on >> warp & 1u)) {
+      if (lane == 0) {
+        lp[i] = 0.f;
+        if (entropy) entropy[i] = 0.f;
+      }
+      return;
+    }
+    row = before + __popc(on & ((1u << warp) - 1u));
+    if (lane == 0) index[row] = i;
   }
+  if (i >= n) return;
   const T* src = h + (size_t)i * H;
   bf16* dst = out + (size_t)row * H;
-  for (int c = threadIdx.x * 8; c < H; c += 2048) {
+#pragma unroll 4
+  for (int c = lane * 8; c < H; c += 256) {
     uint4 v;
     if (sizeof(T) == 2) {
       v = *reinterpret_cast<const uint4*>(src + c);
@@ -521,8 +543,8 @@ TRL_API int trl_score(const void* h, int type, const void* w, const void* target
   int* count = mask ? (int*)take(4) : nullptr;
   bf16* rows = packed ? (bf16*)take(2l * n * H) : nullptr;
   if (packed) {
-    if (type == 0) score_pack_kernel<float><<<n, 256, 0, st>>>((const float*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
-    else score_pack_kernel<bf16><<<n, 256, 0, st>>>((const bf16*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
+    if (type == 0) score_pack_kernel<float><<<(n + SC_PACK - 1) / SC_PACK, SC_PACK * 32, 0, st>>>((const float*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
+    else score_pack_kernel<bf16><<<(n + SC_PACK - 1) / SC_PACK, SC_PACK * 32, 0, st>>>((const bf16*)h, rows, n, H, (const unsigned char*)mask, index, count, (float*)lp, (float*)entropy);
     const cudaError_t rc = cudaGetLastError();
     if (rc != cudaSuccess) return (int)rc;
   }
