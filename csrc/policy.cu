@@ -152,32 +152,46 @@ __device__ __forceinline__ float pl_target(const T* row, long long t, long V, lo
   return pl_float(row[t]);
 }
 
-// What a scored row's terms need, and they from its target's logit, less what the sum's exponentials have less, and the sum.  The exponentials do not wait for the logarithm.
+// What a scored row's terms need, and they from its target's logit, less what the sum's exponentials have less, and the sum.  Two warps share the
+// chain: the three exponentials go side by side over a warp's lanes and give the weight, which every thread waits for; the logarithm, which only the written
+// terms need, is another warp's.  8192 x 4000 83 us, 2048 x 32 768 103 (one thread for
+// all of it 95, 108; all of it in fp32 81, 101).
 struct PolicyIn {
   float adv, old, ref;
-  __device__ PolicyIn() {}
+  __device__ PolicyIn() : adv(0.f), old(0.f), ref(0.f) {}
   __device__ PolicyIn(const PolicyRow& a, long r) : adv(a.adv[a.adv_rows == 1 ? (unsigned)r : (unsigned)r / (unsigned)a.adv_rows]), old(a.old ? a.old[r] : 0.f), ref(a.ref ? a.ref[r] : 0.f) {}
 };
-struct PolicyOut {
-  float weight, target;                              // of the row's gradient, and its target's: weight (p - 1)
-  double part;                                       // 1 / sum
+struct PolicyMid {                                   // of a row, in shared memory
+  double low, log_sum, rho, kle;                     // kle: e^d
+  float adv, ref;
 };
-__device__ __forceinline__ PolicyOut pl_policy(const PolicyRow& a, const PolicyIn& in, long r, double low, double sum, bool write = true) {
-  const double A = (double)in.adv, part = 1.0 / sum;
-  const double lp = low - log(sum), p = exp(low) * part;
-  const double rho = a.old ? exp(low - (double)in.old) * part : 1.0;
-  const bool clip = (rho > a.hi && A > 0.0) || (rho < a.lo && A < 0.0);
-  // (an advantage of nothing has no part in the loss, whatever the ratio)
-  double w = A == 0.0 ? 0.0 : clip ? 0.0 : A * rho, loss = A == 0.0 ? 0.0 : clip ? -A * (A > 0.0 ? a.hi : a.lo) : -A * rho, kl = 0.0;
-  if (lp != lp) w = loss = lp;                       // (NaN stays where the advantage or the clipping would hide it)
-  if (a.ref) {
-    const double d = (double)in.ref - lp, e = exp((double)in.ref - low) * sum;      // (1e-16 of cancellation in kl: d^2 / 2 from |d| of 1e-5 on)
-    kl = e - d - 1.0;
-    if (a.kl != 0.0) w += a.kl * (e - 1.0), loss += a.kl * kl;
-  }
+__device__ __forceinline__ bool pl_clips(const PolicyRow& a, double A, double rho) { return (rho > a.hi && A > 0.0) || (rho < a.lo && A < 0.0); }
+// By a whole warp, four lanes a row, all of which have its values: (weight over the sum, the target's gradient weight (p - 1)).
+// (Inlined: a function of its own would read the kernel's arguments through memory: 2048 x 32 768 120 us.)
+__device__ __forceinline__ float2 pl_weigh(const PolicyRow& a, const PolicyIn in, double low, double sum, PolicyMid* mid, float* weight_of) {
+  const int lane = threadIdx.x & 31, j = lane & 3, lead = lane & ~3;
+  const double A = (double)in.adv, part = 1.0 / sum, e = exp(j == 1 ? low - (double)in.old : j == 2 ? (double)in.ref - low : low);
+  const double p = __shfl_sync(0xffffffffu, e, lead) * part, by_old = __shfl_sync(0xffffffffu, e, lead + 1), by_ref = __shfl_sync(0xffffffffu, e, lead + 2);
+  const double rho = a.old ? by_old * part : 1.0, kle = by_ref * sum;      // (1e-16 of cancellation in kl: d^2 / 2 from |d| of 1e-5 on)
+  // (an advantage of nothing has no part in the loss, whatever the ratio; NaN stays where the advantage or the clipping would hide it)
+  double w = A == 0.0 || pl_clips(a, A, rho) ? 0.0 : A * rho;
+  if (low != low || sum != sum) w = low + sum;
+  if (a.ref && a.kl != 0.0) w += a.kl * (kle - 1.0);
   const float weight = (float)(w * a.scale);
-  if (write) a.lp[r] = (float)lp, a.ratio[r] = (float)rho, a.klv[r] = (float)kl, a.weight[r] = weight, a.clipped[r] = clip, a.loss[r] = loss;
-  return {weight, (float)((p - 1.0) * (double)weight), part};
+  if (j == 0 && mid) mid->low = low, mid->rho = rho, mid->kle = kle, mid->adv = in.adv, mid->ref = in.ref, *weight_of = weight;
+  return make_float2((float)((double)weight * part), (float)((p - 1.0) * (double)weight));
+}
+// The rest of a row's terms, written.
+__device__ __forceinline__ void pl_write(const PolicyRow& a, long r, const PolicyMid& mid) {
+  const double A = (double)mid.adv, lp = mid.low - mid.log_sum, rho = mid.rho;
+  const bool clip = pl_clips(a, A, rho);
+  double loss = A == 0.0 ? 0.0 : clip ? -A * (A > 0.0 ? a.hi : a.lo) : -A * rho, kl = 0.0;
+  if (lp != lp) loss = lp;
+  if (a.ref) {
+    kl = mid.kle - ((double)mid.ref - lp) - 1.0;
+    if (a.kl != 0.0) loss += a.kl * kl;
+  }
+  a.lp[r] = (float)lp, a.ratio[r] = (float)rho, a.klv[r] = (float)kl, a.clipped[r] = clip, a.loss[r] = loss;
 }
 __device__ __forceinline__ void pl_policy_skip(const PolicyRow& a, long r) {
   a.lp[r] = a.ratio[r] = a.klv[r] = a.weight[r] = 0.f, a.clipped[r] = 0, a.loss[r] = 0.0;
@@ -379,29 +393,31 @@ __device__ __forceinline__ float pl_short_top(const Part* q) {
 
 // ---- policy loss -----------------------------------------------------------------------------------------------------------------
 // Up to 4096 values: NT threads a row, which waits in registers, 16 values a thread, as exponentials until its sum and weight are known; the rows of a
-// block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, logarithm and exponentials in fp64) is some 6 us, so what
-// counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us.)
-__device__ __noinline__ float2 pl_policy_row(const PolicyRow& a, const PolicyIn& in, long r, double low, double sum) {       // (apart: its fp64 registers beside a row's values would halve the warps)
-  const PolicyOut o = pl_policy(a, in, r, low, sum);
-  return make_float2((float)((double)o.weight * o.part), o.target);
-}
+// block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, exponentials in fp64) is some 5 us, so what
+// counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us, this 50.)
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
   using S = Span<T>;
   constexpr int E = S::E, VPT = PL_SHORT / E, W = NT / 32, R = 256 / NT;
   __shared__ Part sums[8];                           // (at the base of the largest value itself)
   __shared__ float3 found[R];                        // the largest value, weight over the sum, the target's gradient
+  __shared__ PolicyMid mid[R];
   pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const int k = threadIdx.x % NT, mine = threadIdx.x / NT, warp = threadIdx.x >> 5;
   const long r0 = (long)blockIdx.x * R, r = r0 + mine;
   const bool there = r < rows.n, scored = there && (!rows.mask || rows.mask[r]);
-  // thread i < R looks after row r0 + i
-  const long rw = r0 + threadIdx.x;
-  const bool forms = threadIdx.x < R && rw < rows.n, weighs = forms && (!rows.mask || rows.mask[rw]);
+  // lanes 4 i .. of the first warp, and lane i of the second, look after row r0 + i
+  const int q = warp == 0 ? threadIdx.x / 4 : threadIdx.x % 32;
+  const long rw = r0 + q;
+  const bool forms = warp < 2 && q < R && rw < rows.n, weighs = forms && (!rows.mask || rows.mask[rw]);
   PolicyIn in;
   float xt = 0.f;
-  if (weighs) in = PolicyIn(a, rw), xt = pl_target(x + (size_t)rw * rows.V, rows.target[rw], rows.V, rw);
-  else if (forms) pl_policy_skip(a, rw);
+  if (weighs) {
+    if (warp == 0) in = PolicyIn(a, rw);
+    const long long t = rows.target[rw];
+    if (warp == 1) pl_target(x + (size_t)rw * rows.V, t, rows.V, rw);
+    xt = t >= 0 && t < rows.V ? pl_float(x[(size_t)rw * rows.V + t]) : NAN;
+  }
   const T* row = x + (size_t)r * rows.V;
   T* out = grad + (size_t)r * rows.V;
   const S sp(row, rows.V);
@@ -415,18 +431,27 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   const Part part = pl_short_sums(v, end, most, less);
   if (threadIdx.x % 32 == 0) sums[warp] = part;
   __syncthreads();
-  if (weighs) {
-    const Part* q = sums + threadIdx.x * W;
-    float all_u;
-    const float top = pl_short_top<W>(q);
-    const double all = pl_short_join<W>(q, top, all_u);
-    const float mean = all_u / (float)all, others = 1.f - 1.f / (float)all;        // (the largest value's is 1 exactly)
-    const float2 f = pl_policy_row(a, in, rw, (double)xt - (double)top + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)others, all);
-    found[threadIdx.x] = make_float3(top, f.x, f.y);
+  if (warp < 2) {
+    double low = 0.0, all = 1.0;
+    float top = 0.f;
+    if (weighs) {
+      const Part* of = sums + q * W;
+      float all_u;
+      top = pl_short_top<W>(of), all = pl_short_join<W>(of, top, all_u);
+      const float mean = all_u / (float)all, others = 1.f - 1.f / (float)all;      // (the largest value's is 1 exactly)
+      low = (double)xt - (double)top + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)others;
+    }
+    if (warp == 0) {
+      const float2 f = pl_weigh(a, in, low, all, weighs ? mid + q : nullptr, a.weight + rw);
+      if (weighs && threadIdx.x % 4 == 0) found[q] = make_float3(top, f.x, f.y);
+    } else if (weighs) {
+      mid[q].log_sum = log(all);
+    }
   }
-  if (!grad) return;
   __syncthreads();
-  if (!there) return;
+  if (weighs && warp == 1) pl_write(a, rw, mid[q]);
+  else if (forms && warp == 1) pl_policy_skip(a, rw);
+  if (!grad || !there) return;
   const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
   const float c = scored ? pl_exp2((less - f.x) * PL_L2E) * f.y : 0.f;
 #pragma unroll
@@ -483,7 +508,7 @@ struct PolicyPart {
 
 // A far row.  All blocks of its cluster come here, behind the same barriers.
 template <typename T, int CL, int NT>
-__device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad, const PolicyRow& a, long r, Part* sums, Part* peers, float4* found) {
+__device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad, const PolicyRow& a, long r, Part* sums, Part* peers, float4* found, PolicyMid* mid) {
   const PolicyPart<T, CL> p(x, grad, r, rows.V);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto meet = [&] {
@@ -512,11 +537,13 @@ __device__ __noinline__ void pl_policy_far(const T* x, const Rows& rows, T* grad
   const float m = join(pl_far_most<T, NT>(p.body, p.cnt, xe), [](float v) { return warp_max(v); }, [](float v, float w) { return fmaxf(v, w); }, -INFINITY);
   const float sum = join(pl_far_sum<T, NT>(p.body, p.cnt, xe, p.ie >= 0, m), [](float v) { return warp_sum(v); }, [](float v, float w) { return v + w; }, 0.f);
   const long long t = rows.target[r];
-  if (tid == 0) {
-    const PolicyOut o = pl_policy(a, PolicyIn(a, r), r, (double)pl_target(p.row, t, rows.V, r) - (double)m, (double)sum, p.rank == 0);
-    *found = make_float4(0.f, (float)((double)o.weight * o.part), o.target, 0.f);
+  if (warp == 0) {
+    const float xt = t >= 0 && t < rows.V ? pl_float(p.row[t]) : NAN;
+    const float2 f = pl_weigh(a, PolicyIn(a, r), (double)xt - (double)m, (double)sum, mid, a.weight + r);
+    if (tid == 0) *found = make_float4(0.f, f.x, f.y, 0.f), mid->log_sum = log((double)sum);
   }
   __syncthreads();
+  if (tid == 0 && p.rank == 0) pl_write(a, r, *mid);
   if (grad) {
     pl_far_grads<T, NT>(p.body, p.dst, p.cnt, m, found->y);
     if (p.ie >= 0) p.out[p.ie] = pl_round<T>(expf(xe - m) * found->y);
@@ -530,6 +557,7 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   constexpr int W = NT / 32;
   __shared__ Part sums[W], peers[CL];
   __shared__ float4 found;                           // base, weight over the sum, the target's gradient, whether the row is far
+  __shared__ PolicyMid mid;
   pdl_launch_dependents();                           // (only the sum, which waits for all of this)
   const long r = blockIdx.x / CL;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -546,7 +574,8 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   const long long t = rows.target[r];
   PolicyIn in;
   float xt = 0.f;
-  if (tid == 0) in = PolicyIn(a, r), xt = pl_target(p.row, t, rows.V, r);
+  if (warp == 0) in = PolicyIn(a, r), xt = t >= 0 && t < rows.V ? pl_float(p.row[t]) : NAN;
+  if (tid == 0 && p.rank == 0) pl_target(p.row, t, rows.V, r);
   const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
   Part part = pl_sums<T, NT, G, true>(p.body, p.cnt, xe, grad != nullptr);
   part.join_warp();
@@ -566,21 +595,25 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
     }
   }
   if (CL > 1) pl_cluster_arrive(), pl_cluster_wait();
-  if (tid == 0) {
+  else __syncthreads();
+  if (warp < 2) {
     float all = -PL_FAR, mean;
     const double sum = pl_join<CL>(peers, all, mean);
     if (pl_far(all)) {
-      found.w = 1.f;
-    } else {
-      const PolicyOut o = pl_policy(a, in, r, pl_low(xt, all, mean), sum, p.rank == 0);
-      found = make_float4(all, (float)((double)o.weight * o.part), o.target, 0.f);
+      if (tid == 0) found.w = 1.f;
+    } else if (warp == 0) {
+      const float2 f = pl_weigh(a, in, pl_low(xt, all, mean), sum, &mid, a.weight + r);
+      if (lane == 0) found = make_float4(all, f.x, f.y, 0.f);
+    } else if (lane == 0 && p.rank == 0) {
+      mid.log_sum = log(sum);
     }
   }
   __syncthreads();
   if (found.w != 0.f) {
-    pl_policy_far<T, CL, NT>(x, rows, grad, a, r, sums, peers, &found);
+    pl_policy_far<T, CL, NT>(x, rows, grad, a, r, sums, peers, &found, &mid);
     return;
   }
+  if (tid == 32 && p.rank == 0) pl_write(a, r, mid);
   if (!grad) return;
   pl_grads<T, NT, G, true>(p.body, p.dst, p.cnt, found.x, found.y);
   if (p.ie >= 0) p.out[p.ie] = pl_round<T>(pl_exp(xe, found.x) * found.y);
