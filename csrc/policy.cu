@@ -782,11 +782,13 @@ __global__ void __launch_bounds__(1024) pl_sum_kernel(const double* v, long n, d
 }
 
 // A block a pair: rows [2p T, 2p T + T) chosen, the T behind them rejected.  Results: sums of log-probabilities, margins, a pair's
-// loss, and each sequence's weight for its rows' gradients.
+// loss, and each sequence's weight for its rows' gradients.  `whole` (few pairs: the blocks are one cluster): the sum of the losses too, in place of a launch more.
+constexpr int PL_PAIRS = 8;
 __global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const float* ref, const unsigned char* mask, long T, double beta, double smooth,
-                                                       int average, double scale, float* totals, float* margins, double* loss, float* weight) {
-  __shared__ double red[8][6];
+                                                       int average, double scale, float* totals, float* margins, double* loss, float* weight, float* whole) {
+  __shared__ double red[8][6], losses[PL_PAIRS];
   pdl_launch_dependents();
+  if (whole) pl_cluster_arrive();
   pdl_wait();
   const long p = blockIdx.x;
   double v[6] = {};                                  // log-probabilities, their differences to the reference's, scored tokens; chosen, rejected
@@ -804,22 +806,32 @@ __global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const 
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32][q] = v[q];
   }
   __syncthreads();
-  if (threadIdx.x) return;
+  if (threadIdx.x == 0) {
 #pragma unroll
-  for (int q = 0; q < 6; ++q) {
-    v[q] = 0.0;
-    for (int w = 0; w < 8; ++w) v[q] += red[w][q];
+    for (int q = 0; q < 6; ++q) {
+      v[q] = 0.0;
+      for (int w = 0; w < 8; ++w) v[q] += red[w][q];
+    }
+    const double by0 = average ? 1.0 / fmax(v[2], 1.0) : 1.0, by1 = average ? 1.0 / fmax(v[5], 1.0) : 1.0;
+    const double z = beta * (v[1] * by0 - v[4] * by1), e = smooth;
+    // with u = e^-|z|: sigmoid(|z|) = 1 / (1 + u), -log of it log(1 + u), and |z| more the other way round
+    const double u = exp(-fabs(z)), l = log1p(u), near = 1.0 / (1.0 + u), up = z >= 0.0 ? near : u * near, down = z >= 0.0 ? u * near : near;
+    const double dz = z == z ? e * up - (1.0 - e) * down : z;
+    totals[2 * p] = (float)(v[0] * by0), totals[2 * p + 1] = (float)(v[3] * by1);
+    margins[p] = (float)z;
+    const double of = (1.0 - e) * (l + fmax(-z, 0.0)) + (e != 0.0 ? e * (l + fmax(z, 0.0)) : 0.0);
+    loss[p] = losses[0] = of;
+    // (the row's gradient is weight (p - onehot): minus that of its log-probability)
+    weight[2 * p] = (float)(-dz * scale * beta * by0), weight[2 * p + 1] = (float)(dz * scale * beta * by1);
   }
-  const double by0 = average ? 1.0 / fmax(v[2], 1.0) : 1.0, by1 = average ? 1.0 / fmax(v[5], 1.0) : 1.0;
-  const double z = beta * (v[1] * by0 - v[4] * by1), e = smooth;
-  // with u = e^-|z|: sigmoid(|z|) = 1 / (1 + u), -log of it log(1 + u), and |z| more the other way round
-  const double u = exp(-fabs(z)), l = log1p(u), near = 1.0 / (1.0 + u), up = z >= 0.0 ? near : u * near, down = z >= 0.0 ? u * near : near;
-  const double dz = z == z ? e * up - (1.0 - e) * down : z;
-  totals[2 * p] = (float)(v[0] * by0), totals[2 * p + 1] = (float)(v[3] * by1);
-  margins[p] = (float)z;
-  loss[p] = (1.0 - e) * (l + fmax(-z, 0.0)) + (e != 0.0 ? e * (l + fmax(z, 0.0)) : 0.0);
-  // (the row's gradient is weight (p - onehot): minus that of its log-probability)
-  weight[2 * p] = (float)(-dz * scale * beta * by0), weight[2 * p + 1] = (float)(dz * scale * beta * by1);
+  if (!whole) return;
+  pl_cluster_wait();                                 // every block runs
+  if (threadIdx.x == 0 && p) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(pl_map(smem_u32(&losses[p]), 0)), "d"(losses[0]) : "memory");
+  pl_cluster_arrive(), pl_cluster_wait();
+  if (p || threadIdx.x) return;
+  double sum = 0.0;
+  for (long k = 0; k < gridDim.x; ++k) sum += losses[k];
+  *whole = (float)(sum * scale);
 }
 
 // x times *up; no pass over the values where that is 1.
@@ -932,13 +944,22 @@ TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, lon
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
   const int stated = type ? stats_launch((const bf16*)x, rows, rest, lps, st) : stats_launch((const float*)x, rows, rest, lps, st);
   if (stated) return stated;
-  const cudaError_t paired = trl_launch(pl_pairs_kernel, dim3((unsigned)pairs), dim3(256), 0, st, (const double*)lps, (const float*)ref, rows.mask, T, beta, smooth,
-                                        average, scale, (float*)totals, (float*)margins, pair_loss, weight);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)pairs), cfg.blockDim = dim3(256), cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = g_trl_use_pdl ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)pairs, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = pairs <= PL_PAIRS ? 2 : 1;
+  const cudaError_t paired = cudaLaunchKernelEx(&cfg, pl_pairs_kernel, (const double*)lps, (const float*)ref, rows.mask, T, beta, smooth, average, scale,
+                                                (float*)totals, (float*)margins, pair_loss, weight, pairs <= PL_PAIRS ? (float*)loss : nullptr);
   if (paired != cudaSuccess) return (int)paired;
   if (grad) {
     const int rc = type ? grad_launch<bf16>(x, rows, rest, weight, T, grad, st) : grad_launch<float>(x, rows, rest, weight, T, grad, st);
     if (rc) return rc;
   }
+  if (pairs <= PL_PAIRS) return 0;
   return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, pair_loss, pairs, scale, (float*)loss);
 }
 

@@ -136,3 +136,9 @@ def test_offsets_past_32_bits():
     one.watch(small)
     z = T.swiglu(one, small, bits=8)
     assert torch.equal(y[-3:], z) and torch.equal(grad[-3:], one.backward(z, torch.ones_like(z))[id(small)])
+
+
+@pytest.mark.parametrize("shape", [(3, 8), (300, 3000), (5, 34816)])
+def test_the_forward_pass_is_that_without_8_bits(shape):
+    x = torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV) * 3
+    assert torch.equal(T.swiglu(T.Tape(), x, bits=8), T.swiglu(T.Tape(), x))

@@ -385,3 +385,10 @@ def test_one_row_without_dimensions_before_the_vocabulary(v):
     got, some = T.policy_loss(row, one, targets[0].to(DEV), adv[0].to(DEV), old_logprobs=old[0].to(DEV), ref_logprobs=refs[0].to(DEV), **kw)
     assert torch.equal(got, loss) and all(torch.equal(a, b[0]) and a.shape == () for a, b in zip(some, terms))
     assert torch.equal(row.backward(got)[id(one)], whole.backward(loss)[id(here)][0])
+
+
+@pytest.mark.parametrize("pairs", [5, 7, 8, 9, 33])
+@pytest.mark.parametrize("v", [40, 5000])
+def test_losses_of_few_pairs_and_of_many(pairs, v):
+    """Up to eight pairs' losses are added up where they are formed, more by a kernel of their own."""
+    test_preference_loss(pairs, 3, v, 0, torch.float32)

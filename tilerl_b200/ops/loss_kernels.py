@@ -51,7 +51,7 @@ def preference(logits, targets, mask, ref: Optional[torch.Tensor], *, beta: floa
         N.check(N.lib().trl_preference_loss(x.data_ptr(), TYPES[x.dtype], seqs // 2, t, x.shape[-1], targets.data_ptr(), N.ptr(mask), N.ptr(ref), beta, smooth,
                                             int(average), scale, at + 4 * keep, at + 4 * (keep + seqs), at + 4 * (keep + seqs + seqs // 2), N.ptr(grad), at,
                                             N.stream()), "preference_loss")
-    N.count(4 if want_grad else 3)
+    N.count(2 + int(want_grad) + int(seqs > 16))
     return some[-1], some[keep:keep + seqs], some[keep + seqs:-1], grad
 
 
