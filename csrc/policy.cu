@@ -339,6 +339,21 @@ __device__ __forceinline__ bool pl_wrote(long long t, long end, int head, int E,
   return t >= 0 && (t == end || (t >= head && tv >= 0 && tv < cnt && tv % NT == k));
 }
 
+__device__ __forceinline__ uint32_t pl_map(uint32_t addr, int cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ void pl_cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void pl_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  __syncwarp();
+}
+
 // The values of thread k of a short row's NT: N of its vectors; -inf where there are none.
 constexpr int PL_SHORT = 16;
 template <typename T, int NT>
@@ -396,7 +411,7 @@ __device__ __forceinline__ float pl_short_top(const Part* q) {
 // block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, exponentials in fp64) is some 5 us, so what
 // counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us, this 50.)
 template <typename T, int NT>
-__global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a) {
+__global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a, float* whole) {
   using S = Span<T>;
   constexpr int E = S::E, VPT = PL_SHORT / E, W = NT / 32, R = 256 / NT;
   __shared__ Part sums[8];                           // (at the base of the largest value itself)
@@ -451,42 +466,37 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   __syncthreads();
   if (weighs && warp == 1) pl_write(a, rw, mid[q]);
   else if (forms && warp == 1) pl_policy_skip(a, rw);
-  if (!grad || !there) return;
-  const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
-  const float c = scored ? pl_exp2((less - f.x) * PL_L2E) * f.y : 0.f;
+  if (whole) pl_cluster_arrive();
+  if (grad && there) {
+    const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
+    const float c = scored ? pl_exp2((less - f.x) * PL_L2E) * f.y : 0.f;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    float u[E];
+    for (int i = 0; i < VPT; ++i) {
+      float u[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) u[j] = scored ? v[i * E + j] * c : 0.f;
-    if (k + i * NT < nv) __stcs(dst + k + i * NT, pl_pack(u));
+      for (int j = 0; j < E; ++j) u[j] = scored ? v[i * E + j] * c : 0.f;
+      if (k + i * NT < nv) __stcs(dst + k + i * NT, pl_pack(u));
+    }
+    if (ie >= 0) out[ie] = pl_round<T>(scored ? end * c : 0.f);
+    if (scored) {
+      const long long t = rows.target[r];
+      if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>(f.z);
+    }
   }
-  if (ie >= 0) out[ie] = pl_round<T>(scored ? end * c : 0.f);
-  if (scored) {
-    const long long t = rows.target[r];
-    if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>(f.z);
-  }
+  if (!whole) return;
+  pl_cluster_wait();                                 // (every row's loss is written)
+  if (blockIdx.x || warp) return;
+  double sum = 0.0;
+  for (long i = threadIdx.x; i < rows.n; i += 32) sum += a.loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (threadIdx.x == 0) *whole = (float)(sum * a.scale);
 }
 
 // Longer rows: a cluster of CL blocks goes through a row twice, for its sum and for its gradient; the second time the row is still in L2, as long as
 // those in work fit there.  Between the passes the blocks send each other their (B, s, u); each adds them up in a fixed order and forms the row's weight for
 // itself.  The cluster's first barrier is passed before another block's shared memory is touched, no block's is after the second.  Both end:
 // every thread of a scored row's cluster comes to them, and nothing before them waits.
-__device__ __forceinline__ uint32_t pl_map(uint32_t addr, int cta) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
-  return r;
-}
-__device__ __forceinline__ void pl_cluster_arrive() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-}
-__device__ __forceinline__ void pl_cluster_wait() {
-  __syncwarp();
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-  __syncwarp();
-}
-
 // What a block works on: its vectors of a row, and its threads' values at the row's ends.
 template <typename T, int CL>
 struct PolicyPart {
@@ -653,10 +663,11 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   if (threadIdx.x == 0) {
     float all = pl_base(xt == xt ? xt : -INFINITY), mean;
     const double rest_of = pl_join<NT / 32>(sums, all, mean);
-    const double y = (double)xt * (double)PL_L2E - (double)all, e = exp(y * PL_LN2), sum = rest_of + e, most = e / sum;
+    const double y = (double)xt * (double)PL_L2E - (double)all, e = exp(y * PL_LN2), sum = rest_of + e;
+    const float most = (float)e / (float)sum;
     // (the mean of the others, and the target's share)
-    const float of_all = rest_of > 0.0 ? mean + (float)most * (fmaxf((float)y, -256.f) - mean) : (float)y;
-    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all, of_all) + PL_LESS * most - log(sum);
+    const float of_all = rest_of > 0.0 ? mean + most * (fmaxf((float)y, -256.f) - mean) : (float)y;
+    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all, of_all) + PL_LESS * (double)most - log(sum);
     far = pl_far(all);
   }
   __syncthreads();
@@ -700,9 +711,9 @@ __global__ void __launch_bounds__(256, 5) pl_stats_short_kernel(const T* x, cons
   float u;
   const double rest_of = pl_short_join<W>(q, top, u), low = (double)xt - (double)top, e = exp(low), sum = rest_of + e;
   const float mean = (u + (float)e * fmaxf((float)low * PL_L2E, -256.f)) / (float)sum;
-  const double rough = rest_of - (others == top ? 1.0 : 0.0);          // (of the sum, from exponentials that are not exact)
+  const float rough = (float)(rest_of - (others == top ? 1.0 : 0.0)) / (float)sum;       // (what exponentials that are not exact have of the sum)
   rest[rw] = make_float4(0.f, top, (float)sum, 1.f);
-  lps[rw] = low + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (rough / sum) - log(sum);
+  lps[rw] = low + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)rough - log(sum);
 }
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_grad_short_kernel(const T* x, const Rows rows, const float4* rest, const float* weight, long per, T* grad) {
@@ -784,9 +795,9 @@ __global__ void __launch_bounds__(1024) pl_sum_kernel(const double* v, long n, d
 // A block a pair: rows [2p T, 2p T + T) chosen, the T behind them rejected.  Results: sums of log-probabilities, margins, a pair's
 // loss, and each sequence's weight for its rows' gradients.  `whole` (few pairs: the blocks are one cluster): the sum of the losses too, in place of a launch more.
 constexpr int PL_PAIRS = 8;
-__global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const float* ref, const unsigned char* mask, long T, double beta, double smooth,
+__global__ void __launch_bounds__(1024) pl_pairs_kernel(const double* lps, const float* ref, const unsigned char* mask, long T, double beta, double smooth,
                                                        int average, double scale, float* totals, float* margins, double* loss, float* weight, float* whole) {
-  __shared__ double red[8][6], losses[PL_PAIRS];
+  __shared__ double red[32][6], losses[PL_PAIRS];
   pdl_launch_dependents();
   if (whole) pl_cluster_arrive();
   pdl_wait();
@@ -796,7 +807,7 @@ __global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const 
   for (int k = 0; k < 2; ++k) {
     const long at = (2 * p + k) * T;
 #pragma unroll 4
-    for (long i = threadIdx.x; i < T; i += 256)
+    for (long i = threadIdx.x; i < T; i += blockDim.x)
       if (!mask || mask[at + i]) v[3 * k] += lps[at + i], v[3 * k + 1] += lps[at + i] - (ref ? (double)ref[at + i] : 0.0), v[3 * k + 2] += 1.0;
   }
 #pragma unroll
@@ -810,7 +821,7 @@ __global__ void __launch_bounds__(256) pl_pairs_kernel(const double* lps, const 
 #pragma unroll
     for (int q = 0; q < 6; ++q) {
       v[q] = 0.0;
-      for (int w = 0; w < 8; ++w) v[q] += red[w][q];
+      for (int w = 0; w < (int)blockDim.x / 32; ++w) v[q] += red[w][q];
     }
     const double by0 = average ? 1.0 / fmax(v[2], 1.0) : 1.0, by1 = average ? 1.0 / fmax(v[5], 1.0) : 1.0;
     const double z = beta * (v[1] * by0 - v[4] * by1), e = smooth;
@@ -888,13 +899,21 @@ int policy_launch(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cud
 }
 // The form by a row's length.
 template <typename T>
-int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, cudaStream_t st) {
+int policy_rows(const T* x, const Rows& rows, T* grad, const PolicyRow& a, float* loss, bool& summed, cudaStream_t st) {
   constexpr int E = Span<T>::E;
   const long V = rows.V;
   if (V <= PL_SHORT_ROW)
     return short_form(V, [&](auto nt) {
-      pl_policy_short_kernel<T, nt.value><<<short_blocks(rows.n, nt.value), 256, 0, st>>>(x, rows, grad, a);
-      return (int)cudaGetLastError();
+      // (few blocks are a cluster, which adds the rows' losses up as well: a launch less)
+      const unsigned blocks = short_blocks(rows.n, nt.value);
+      summed = blocks <= 8;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(256), cfg.stream = st;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = blocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr, cfg.numAttrs = summed ? 1 : 0;
+      return (int)cudaLaunchKernelEx(&cfg, pl_policy_short_kernel<T, nt.value>, x, rows, grad, a, summed ? loss : nullptr);
     });
   // By a row's bytes, since those in work have to stay in L2 (some 50 MB) and blocks to be many: the longer a row, the more blocks share it.  Measured best,
   // us, before the pass summed the mean too, which takes 2 % (and the next): 4096 x 8192 57 (two blocks a row 68), 2048 x 32 768 107 (one block of 384 threads 110, two of 192 108), 1024 x 65 536 110 (two of 256 113),
@@ -924,8 +943,9 @@ TRL_API int trl_policy_loss(const void* x, int type, long n, long V, const void*
   const Rows rows{(const unsigned char*)mask, (const long long*)target, n, V};
   const PolicyRow a{(const float*)adv, (const float*)old, (const float*)ref, (int)adv_rows, lo, hi, kl, scale, f, f + n, f + 2 * n, f + 3 * n,
                     (unsigned char*)clipped, row_loss};
-  const int rc = type ? policy_rows((const bf16*)x, rows, (bf16*)grad, a, st) : policy_rows((const float*)x, rows, (float*)grad, a, st);
-  if (rc) return rc;
+  bool summed = false;
+  const int rc = type ? policy_rows((const bf16*)x, rows, (bf16*)grad, a, (float*)loss, summed, st) : policy_rows((const float*)x, rows, (float*)grad, a, (float*)loss, summed, st);
+  if (rc || summed) return rc;
   return (int)trl_launch(pl_sum_kernel, dim3(1), dim3(1024), 0, st, row_loss, n, scale, (float*)loss);
 }
 
@@ -945,7 +965,7 @@ TRL_API int trl_preference_loss(const void* x, int type, long pairs, long T, lon
   const int stated = type ? stats_launch((const bf16*)x, rows, rest, lps, st) : stats_launch((const float*)x, rows, rest, lps, st);
   if (stated) return stated;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)pairs), cfg.blockDim = dim3(256), cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)pairs), cfg.blockDim = dim3(T > 4096 ? 1024 : 256), cfg.stream = st;       // (a pair of 2 x 32 768 rows of 500: 103 us, with 256 threads 128; of 2 x 2048 rows of 2000 34, 30)
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = g_trl_use_pdl ? 1 : 0;

@@ -392,3 +392,23 @@ def test_one_row_without_dimensions_before_the_vocabulary(v):
 def test_losses_of_few_pairs_and_of_many(pairs, v):
     """Up to eight pairs' losses are added up where they are formed, more by a kernel of their own."""
     test_preference_loss(pairs, 3, v, 0, torch.float32)
+
+
+@pytest.mark.parametrize("v,rows,launches", [(300, 64, 1), (300, 65, 2), (512, 57, 1), (700, 32, 1), (700, 33, 2), (1500, 16, 1), (1500, 17, 2), (4000, 8, 1), (4000, 9, 2),
+                                             (4097, 5, 2)])
+def test_policy_losses_of_few_rows_and_of_many(v, rows, launches):
+    """Up to eight blocks of short rows add their losses up themselves, to either side of that."""
+    test_policy_loss((rows,), v, 0, torch.float32)
+    lg = torch.zeros(rows, v, device=DEV)
+    off, _ = T.policy_loss(T.Tape(), lg, torch.zeros(rows, dtype=torch.long, device=DEV), torch.ones(rows, device=DEV), scale=0.5,
+                           mask=torch.zeros(rows, dtype=torch.bool, device=DEV))
+    assert float(off) == 0.0
+    before = native.launch_count
+    loss, _ = T.policy_loss(T.Tape(), lg, torch.zeros(rows, dtype=torch.long, device=DEV), torch.ones(rows, device=DEV), scale=0.5)       # (without a gradient)
+    assert float(loss) == -0.5 * rows and native.launch_count == before + launches
+
+
+@pytest.mark.parametrize("t", [255, 2500, 4096, 4097, 9000])
+def test_preference_loss_of_long_sequences(t):
+    """More tokens than a pair's block has threads."""
+    test_preference_loss(2, t, 40, 0, torch.float32)

@@ -37,7 +37,8 @@ def policy(logits, targets, mask, adv, old, ref, *, lo: float, hi: float, kl: fl
         N.check(N.lib().trl_policy_loss(x.data_ptr(), TYPES[x.dtype], n, x.shape[-1], targets.data_ptr(), N.ptr(mask), adv.data_ptr(), n // adv.numel(),
                                         N.ptr(old), N.ptr(ref), lo, hi, kl, scale, at + 8 * n, clipped.data_ptr(), at + 24 * n, N.ptr(grad), at,
                                         N.stream()), "policy_loss")
-    N.count(2)
+    v = x.shape[-1]
+    N.count(1 if v <= 4096 and n <= 64 >> max(0, (v - 1).bit_length() - 9) else 2)      # (up to eight blocks of short rows sum their losses themselves)
     return some[6 * n], some.as_strided((4, *targets.shape), (n, *targets.stride()), 2 * n).unbind(0), clipped, grad
 
 
