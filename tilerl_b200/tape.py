@@ -683,21 +683,24 @@ def _loss_inputs(what: str, logits, targets, mask, **floats):
     """Shapes, types and devices of what a loss over rows of logits takes; the tensors as its kernels read them."""
     if not logits.is_floating_point() or logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"{what}: logits are [..., vocab] in floating point, got {tuple(logits.shape)} {logits.dtype}")
-    rows = tuple(logits.shape[:-1])
-    if tuple(targets.shape) != rows or targets.is_floating_point() or targets.dtype == torch.bool:
-        raise ValueError(f"{what}: targets are token ids {rows}, got {tuple(targets.shape)} {targets.dtype}")
-    if mask is not None and (tuple(mask.shape) != rows or mask.dtype != torch.bool):
-        raise ValueError(f"{what}: the mask is bool {rows}, got {tuple(mask.shape)} {mask.dtype}")
-    for name, t in floats.items():
-        if t is not None and (tuple(t.shape) != rows or not t.is_floating_point()):
-            raise ValueError(f"{what}: {name} is floating point {rows}, got {tuple(t.shape)} {t.dtype}")
-    dev = logits.device
-    for t in (targets, mask, *floats.values()):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: logits are on {logits.device}, another input on {t.device}")
+    rows, dev = logits.shape[:-1], logits.device
+    if targets.shape != rows or targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"{what}: targets are token ids {tuple(rows)}, got {tuple(targets.shape)} {targets.dtype}")
+    if mask is not None and (mask.shape != rows or mask.dtype != torch.bool):
+        raise ValueError(f"{what}: the mask is bool {tuple(rows)}, got {tuple(mask.shape)} {mask.dtype}")
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
-    ready = lambda t, dtype: t if t is None or (t.dtype == dtype and t.is_contiguous()) else t.to(dtype).contiguous()
-    return (ready(targets, torch.int64), ready(mask, torch.bool)) + tuple(ready(t, wide) for t in floats.values())
+    for name, t in floats.items():
+        if t is not None and (t.shape != rows or not t.is_floating_point()):
+            raise ValueError(f"{what}: {name} is floating point {tuple(rows)}, got {tuple(t.shape)} {t.dtype}")
+    ready = []
+    for t, dtype in ((targets, torch.int64), (mask, torch.bool), *((t, wide) for t in floats.values())):
+        if t is not None:
+            if t.device != dev:
+                raise ValueError(f"{what}: logits are on {dev}, another input on {t.device}")
+            if t.dtype != dtype or not t.is_contiguous():
+                t = t.to(dtype).contiguous()
+        ready.append(t)
+    return ready
 
 
 def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
@@ -739,7 +742,7 @@ def policy_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, advanta
     if tape.tp_world > 1:
         raise ValueError("policy_loss takes whole rows of logits: with a sharded vocabulary use cross_entropy_tp")
     tg, mk, old, refs = _loss_inputs("policy_loss", logits, targets, mask, old_logprobs=old_logprobs, ref_logprobs=ref_logprobs)
-    if tuple(advantages.shape) not in (tuple(targets.shape), tuple(targets.shape[:1])) or not advantages.is_floating_point() or advantages.device != logits.device:
+    if advantages.shape not in (targets.shape, targets.shape[:1]) or not advantages.is_floating_point() or advantages.device != logits.device:
         raise ValueError(f"policy_loss: advantages are floating point {tuple(targets.shape)} or {tuple(targets.shape[:1])} on {logits.device}, "
                          f"got {tuple(advantages.shape)} {advantages.dtype} on {advantages.device}")
     adv = advantages.to(torch.float64 if logits.dtype == torch.float64 else torch.float32).contiguous()
@@ -864,18 +867,22 @@ def linear_logprobs(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, 
     A target outside of the vocabulary in a scored row gives NaN and sets the device's error word; on the CPU it is an error."""
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or not w.is_floating_point() or not h.is_floating_point() or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1:
         raise ValueError(f"linear_logprobs: h [..., H] and a dense w [vocab, H], got {tuple(h.shape)} and {tuple(w.shape)}")
-    rows = tuple(h.shape[:-1])
-    if tuple(targets.shape) != rows or targets.is_floating_point() or targets.dtype == torch.bool:
-        raise ValueError(f"linear_logprobs: targets are token ids {rows}, got {tuple(targets.shape)} {targets.dtype}")
-    if mask is not None and (tuple(mask.shape) != rows or mask.dtype != torch.bool):
-        raise ValueError(f"linear_logprobs: the mask is bool {rows}, got {tuple(mask.shape)} {mask.dtype}")
-    if any(t is not None and t.device != h.device for t in (w, targets, mask)):
+    rows, dev = h.shape[:-1], h.device
+    if targets.shape != rows or targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"linear_logprobs: targets are token ids {tuple(rows)}, got {tuple(targets.shape)} {targets.dtype}")
+    if mask is not None and (mask.shape != rows or mask.dtype != torch.bool):
+        raise ValueError(f"linear_logprobs: the mask is bool {tuple(rows)}, got {tuple(mask.shape)} {mask.dtype}")
+    if w.device != dev or targets.device != dev or (mask is not None and mask.device != dev):
         raise ValueError("linear_logprobs: all inputs are on one device")
-    tg, mk = targets.reshape(-1).long().contiguous(), None if mask is None else mask.reshape(-1).contiguous()
-    hf = h.reshape(-1, h.shape[-1])
+    hf, tg, mk = h, targets, mask
+    if len(rows) != 1:
+        hf, tg, mk = h.reshape(-1, h.shape[-1]), targets.reshape(-1), None if mask is None else mask.reshape(-1)
+    tg, mk = tg.long().contiguous(), None if mk is None else mk.contiguous()
     wc = w.to(torch.bfloat16) if h.is_cuda else w
     lp, ent = (score.score if score.takes(hf, wc) else score.score_torch)(hf, wc, tg, mk, entropy)
-    return (lp.view(rows), ent.view(rows)) if entropy else lp.view(rows)
+    if len(rows) != 1:
+        lp, ent = lp.view(rows), ent.view(rows) if entropy else None
+    return (lp, ent) if entropy else lp
 
 
 @_nograd
