@@ -412,3 +412,18 @@ def test_policy_losses_of_few_rows_and_of_many(v, rows, launches):
 def test_preference_loss_of_long_sequences(t):
     """More tokens than a pair's block has threads."""
     test_preference_loss(2, t, 40, 0, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+def test_targets_outside_of_the_vocabulary_in_the_torch_form(dtype):
+    """Logits in types that the kernels do not take: a row without a number, as from the kernels, but for the error word."""
+    lg = torch.randn(4, 30, generator=torch.Generator().manual_seed(0)).to(DEV, dtype)
+    for t in (-1, 30, 1 << 40):
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.policy_loss(tape, lg, torch.tensor([0, t, 1, 2], device=DEV), torch.ones(4, device=DEV), scale=1.0)
+        grad = tape.backward(loss)[id(lg)]
+        assert loss.isnan() and terms.logprobs.isnan().tolist() == [False, True, False, False] == grad.isnan().any(-1).tolist()
+        loss, _ = T.preference_loss(T.Tape(), lg.view(4, 1, 30), torch.tensor([[0], [t], [1], [2]], device=DEV))
+        assert loss.isnan()
+    assert native.read_error()[0] == 0

@@ -150,3 +150,18 @@ def test_few_rows_with_values_without_a_number(vocab):
     lp, ent = T.linear_logprobs(h.bfloat16(), w.bfloat16(), tg, entropy=True)
     assert (lp[:-2].abs() <= 1e-15).all() and (ent[:-2].abs() <= 1e-15).all() if vocab > 1 else not lp[:-2].any()
     assert lp[-2:].isnan().all() and ent[-2:].isnan().all()
+
+
+def test_targets_outside_of_the_vocabulary_in_the_torch_form():
+    """As from the kernels, but for the error word: nothing is indexed with such a target."""
+    for hidden, dtype in ((20, torch.bfloat16), (64, torch.float16), (64, torch.float64)):
+        h, w, tg, _ = _inputs((300,), hidden, 50, 5)
+        h = h.to(dtype)
+        assert not score.takes(h, w)
+        want, went = T.linear_logprobs(h, w, tg, entropy=True)
+        for t in (-1, 50, 1 << 40):
+            bad = tg.clone()
+            bad[7], bad[299] = t, t
+            lp, ent = T.linear_logprobs(h, w, bad, entropy=True)
+            assert lp.isnan().nonzero()[:, 0].tolist() == [7, 299] and torch.equal(torch.where(lp.isnan(), want, lp), want) and torch.equal(ent, went)
+    assert native.read_error()[0] == 0

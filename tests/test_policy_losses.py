@@ -336,3 +336,37 @@ def test_a_segment_that_hands_on_its_input():
     z = T.scale(tape, tape.checkpoint(lambda t, z: z, y, bits=8), 3.0)
     grads = tape.backward(z, torch.ones_like(z))
     assert torch.equal(grads[id(x)], torch.full_like(x, 6.0))
+
+
+def test_targets_outside_of_the_vocabulary_in_the_torch_forms(monkeypatch):
+    """Where an index out of range is no error (the torch forms on a GPU, for types and widths that the kernels do not take) nothing is indexed with one:
+    its row has no number, in the losses and the log-probabilities, and no other row differs."""
+    from tilerl_b200.ops import ref
+    g = torch.Generator().manual_seed(0)
+    logits, adv, mask = torch.randn(6, 9, generator=g, dtype=torch.float64), torch.randn(6, generator=g, dtype=torch.float64), torch.tensor([1, 1, 1, 0, 1, 1]).bool()
+    targets, h, w = torch.tensor([0, 8, 3, 4, 5, 1]), torch.randn(6, 7, generator=g), torch.randn(9, 7, generator=g)
+
+    def forms(tg):
+        tape, pairs = T.Tape(), logits.view(2, 3, 9)
+        tape.watch(logits, pairs)
+        loss, terms = T.policy_loss(tape, logits, tg, adv, scale=0.5, mask=mask)
+        grad = tape.backward(loss)[id(logits)]
+        pref, seen = T.preference_loss(tape, pairs, tg.view(2, 3), mask.view(2, 3))
+        return loss, terms, grad, pref, seen, tape.backward(pref)[id(pairs)], *T.linear_logprobs(h, w, tg, mask=mask, entropy=True)
+
+    loss, terms, grad, pref, seen, pgrad, lp, ent = forms(targets)
+    for bad in (-1, 9, 1 << 40):
+        tg = targets.clone()
+        tg[1], tg[3] = bad, bad                           # (row 3 is not scored)
+        with pytest.raises((IndexError, RuntimeError)):
+            forms(tg)
+        with monkeypatch.context() as m:
+            m.setattr(ref, "index_raises", lambda t: False)
+            got = forms(tg)
+        assert got[0].isnan() and got[1].logprobs.isnan().tolist() == [False, True] + [False] * 4 == got[2].isnan().any(-1).tolist()
+        rest = [0, 2, 3, 4, 5]
+        assert torch.equal(got[2][rest], grad[rest]) and torch.equal(got[1].logprobs[rest], terms.logprobs[rest]) and got[2][1].isnan().all()
+        assert got[3].isnan() and got[4].logprobs.isnan().tolist() == [True, False] and got[5][mask.view(2, 3)].isnan().all() and not got[5][~mask.view(2, 3)].any()
+        assert torch.equal(got[4].logprobs[1], seen.logprobs[1])
+        assert got[6].isnan().tolist() == [False, True] + [False] * 4 and torch.equal(got[6][rest], lp[rest]) and torch.equal(got[7], ent)
+    assert ref.within(targets, 9) == (targets, None)

@@ -517,17 +517,33 @@ def cross_entropy_sharded(logits_shards, targets, weights, vocab_starts):
 
 
 # ---- losses of policy and preference training ---------------------------------------------------------
+def index_raises(t) -> bool:
+    """Whether an index out of range is an error here; on a GPU it is a failed assert, after which nothing runs there any more."""
+    return not t.is_cuda
+
+
+def within(targets, vocab: int):
+    """Targets that may be indexed with, and where they were outside of the vocabulary (None: indexing says so itself)."""
+    if index_raises(targets):
+        return targets, None
+    bad = (targets < 0) | (targets >= vocab)
+    return torch.where(bad, 0, targets), bad
+
+
 def _scored_rows(logits, targets, mask):
     """``(e, s, log-probabilities in 64 bits)`` of rows of logits: exponentials below the largest and their sum.  Rows that are not scored are
-    taken as zeros, so that nothing in them is seen."""
+    taken as zeros, so that nothing in them is seen; the log-probability of a target outside of the vocabulary is NaN."""
     x = logits if logits.dtype == torch.float64 else logits.float()
     targets = targets.long()[:, None]
     if mask is not None:
         x, targets = torch.where(mask[:, None], x, 0.0), torch.where(mask[:, None], targets, 0)
+    targets, bad = within(targets, x.shape[-1])
     m = x.amax(-1, keepdim=True)
     e = torch.exp(x - m)
     s = e.sum(-1, keepdim=True)
     lp = (x.gather(-1, targets).double() - m.double() - torch.log(s.double()))[:, 0]
+    if bad is not None:
+        lp = torch.where(bad[:, 0], float("nan"), lp)
     return e, s, targets, lp if mask is None else torch.where(mask, lp, 0.0)
 
 

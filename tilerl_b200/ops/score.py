@@ -6,6 +6,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import native as N
+from . import ref
 
 N.register("trl_score_workspace", [N.I] * 5, N.L)
 N.register("trl_score", [N.P, N.I, N.P, N.P, N.P] + [N.I] * 3 + [N.P] * 4)
@@ -46,7 +47,8 @@ def score(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[to
 
 
 def score_torch(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """The same in torch, a few rows of logits at a time; on the GPU with bf16 operands and fp32 results, on the CPU in fp32."""
+    """The same in torch, a few rows of logits at a time; on the GPU with bf16 operands and fp32 results, on the CPU in fp32.  (The error word is the
+    kernels'.)"""
     cd = torch.bfloat16 if h.is_cuda else torch.float64 if h.dtype == torch.float64 else torch.float32
     wide = torch.float64 if cd == torch.float64 else torch.float32
     wc = w.to(cd)
@@ -55,12 +57,14 @@ def score_torch(h, w, targets, mask, entropy: bool) -> Tuple[torch.Tensor, Optio
     for a in range(0, h.shape[0], CHUNK):
         some = slice(a, a + CHUNK)
         x = h[some].to(cd).to(wide) @ wc.t().to(wide)
-        tg = targets[some] if mask is None else torch.where(mask[some], targets[some], 0)
+        tg, bad = ref.within(targets[some] if mask is None else torch.where(mask[some], targets[some], 0), x.shape[-1])
         m = x.amax(-1, keepdim=True)
         low = x - m
         e = torch.exp(low)
         s = e.sum(-1).double()
         got = low.gather(-1, tg[:, None])[:, 0].double() - torch.log(s)
+        if bad is not None:
+            got = torch.where(bad, float("nan"), got)
         lp[some] = (got if mask is None else torch.where(mask[some], got, 0.0)).to(wide)
         if entropy:
             got = torch.log(s) - torch.where(e > 0, e * low, 0.0).sum(-1).double() / s

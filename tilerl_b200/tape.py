@@ -734,7 +734,7 @@ def policy_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, advanta
 
     The logits' gradient has their type (fp32, bf16) and is formed here, so they may be written into afterwards.  Rows that are not scored get zeros, whatever
     their logits (NaN among them) and targets are.  A target outside of the vocabulary in a scored row makes the loss and the row's gradient NaN and
-    sets the device's error word; on the CPU it is an error."""
+    sets the device's error word (not where torch forms the loss: logits in fp16 or fp64); on the CPU it is an error."""
     if clip_eps < 0 or (clip_eps_high is not None and clip_eps_high < 0) or not math.isfinite(scale) or not math.isfinite(kl_coef):
         raise ValueError("policy_loss: clip_eps is not negative, scale and kl_coef are finite")
     if kl_coef and ref_logprobs is None:
@@ -864,7 +864,8 @@ def linear_logprobs(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, 
     hold and cost nothing.  ``entropy``: also the entropies of the rows, as a second result.  fp32; on CUDA the product has bf16 operands and fp32
     sums, as :func:`linear`'s.  It is no op of a tape: gradients through the head are :func:`linear_cross_entropy`'s.
 
-    A target outside of the vocabulary in a scored row gives NaN and sets the device's error word; on the CPU it is an error."""
+    A target outside of the vocabulary in a scored row gives NaN and sets the device's error word (not where torch forms the product: ``H`` no
+    multiple of 8, rows in fp16 or fp64); on the CPU it is an error."""
     if not isinstance(w, torch.Tensor) or w.dim() != 2 or not w.is_floating_point() or not h.is_floating_point() or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1:
         raise ValueError(f"linear_logprobs: h [..., H] and a dense w [vocab, H], got {tuple(h.shape)} and {tuple(w.shape)}")
     rows, dev = h.shape[:-1], h.device
