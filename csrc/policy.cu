@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   if (whole) pl_cluster_arrive();
   if (grad && there) {
     const float3 f = scored ? found[mine] : make_float3(0.f, 0.f, 0.f);
-    const float c = scored ? pl_exp2((less - f.x) * PL_L2E) * f.y : 0.f;
+    // (a warp that saw no word that can be has exponentials of 0 at a base of 0, which may lie above f.x by more than a float holds)
+    const float c = scored ? pl_exp2((most - f.x) * PL_L2E) * f.y : 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float u[E];

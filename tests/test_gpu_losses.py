@@ -427,3 +427,37 @@ def test_targets_outside_of_the_vocabulary_in_the_torch_form(dtype):
         loss, _ = T.preference_loss(T.Tape(), lg.view(4, 1, 30), torch.tensor([[0], [t], [1], [2]], device=DEV))
         assert loss.isnan()
     assert native.read_error()[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [600, 900, 2000, 4000, 4099, 40000])
+def test_rows_of_few_words_that_can_be(v, dtype):
+    """-inf everywhere but at three words, which few of a row's threads see, in rows that lie anywhere.  Against 64 bits, as rows far from zero."""
+    g = torch.Generator().manual_seed(v)
+    rows = [(level, place) for level in (0.0, -100.0, 100.0, -1e6, 1e6) for place in (0, 130, v // 2, v - 3)]
+    x, targets = torch.full((len(rows), v), float("-inf")), torch.tensor([place + 1 for _, place in rows])
+    for row, (level, place) in zip(x, rows):
+        row[place:place + 3] = level + torch.randn(3, generator=g)
+    x = x.to(dtype)
+    wide, tape64 = x.double(), T.Tape()
+    tape64.watch(wide)
+    want, terms64 = T.policy_loss(tape64, wide, targets, torch.ones(len(rows)), scale=1.0)
+    wgrad = tape64.backward(want)[id(wide)]
+    here, tape = x.to(DEV), T.Tape()
+    tape.watch(here)
+    loss, terms = T.policy_loss(tape, here, targets.to(DEV), torch.ones(len(rows), device=DEV), scale=1.0)
+    grad = tape.backward(loss)[id(here)].cpu()
+    spread = (wide.amax(-1) - wide.gather(-1, targets[:, None])[:, 0]).abs()
+    assert ((terms.logprobs.cpu() - terms64.logprobs).abs() <= spread * 2 ** -22 + _adds(v) * 2 ** -24 + terms64.logprobs.abs() * 2 ** -23).all()
+    bound = _grad_bounds(x, terms64.weights.double(), torch.zeros(len(rows), dtype=torch.float64), v)
+    assert torch.isfinite(grad).all() and ((grad.double() - wgrad).abs() <= bound).all() and not grad[x == float("-inf")].any()
+    pairs = here.view(len(rows), 1, v)
+    tape.watch(pairs)
+    pref, seen = T.preference_loss(tape, pairs, targets.to(DEV)[:, None])
+    pgrad = tape.backward(pref)[id(pairs)].view(len(rows), v).cpu()
+    assert torch.isfinite(pref) and torch.isfinite(pgrad).all() and not pgrad[x == float("-inf")].any()
+    assert torch.allclose(seen.logprobs, terms.logprobs, rtol=2 ** -22, atol=2 * _adds(v) * 2 ** -24)
+    here.fill_(float("-inf"))                             # no word can be: no number
+    tape.watch(here)
+    loss, terms = T.policy_loss(tape, here, targets.to(DEV), torch.ones(len(rows), device=DEV), scale=1.0)
+    assert loss.isnan() and terms.logprobs.isnan().all() and tape.backward(loss)[id(here)].isnan().all()
