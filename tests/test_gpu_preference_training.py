@@ -93,3 +93,37 @@ def test_swiglu_rows_are_let_go_of(model):
         del lg, tape
     rows = ids.numel() * 2 * cfg.ffn * cfg.n_layers
     assert held[0] - held[1] >= 0.9 * rows * (4 - 1 - 4 / 128)
+
+
+def test_a_policy_scored_as_its_own_reference():
+    """Adapters that add nothing, a head whose logits reach 20: a row's log-probabilities are the reference's but for the order of two fp32 sums of
+    ``hidden`` products, each addition off by 2^-23 of the row's sum of |h w| at most (hidden / 16 + 2 of them in either form), as scoring is tested."""
+    from tilerl_b200.factory import build_model, make_ops
+    m = build_model(small_gpu(), DEV, seed=1, ops=make_ops(DEV))
+    m.add_lora(rank=4, alpha=8.0)
+    head = m.params["embed" if m.cfg.tie_embeddings else "lm_head"]
+    ids, plens, slens = _batch(m, 4, 70)
+    tape = T.Tape()
+    tape.enabled = False
+    with torch.no_grad():
+        h, w, _ = m.forward_dense(tape, ids, return_hidden=True)
+        head.mul_(20.0 / float((h.bfloat16().float() @ w.float().t()).abs().max()))
+        size = (h.bfloat16().double().abs() @ w.double().abs().t()).amax(-1)
+    off = 4 * size * (h.shape[-1] / 16 + 2) * 2 ** -23 + 1e-5      # of a log-probability: its logit's and the sum's, in both forms
+    assert float(off.max()) < 0.02
+    mask = rl._scored_mask(ids, plens, slens).to(DEV)
+    refs = rl.sequence_logprobs(m, ids, plens, slens, adapters=False)
+    assert torch.equal(refs, rl.sequence_logprobs(m, ids, plens, slens))
+    lg = m.forward_dense(T.Tape(), ids)
+    assert 19.0 < float(lg.abs().max()) < 21.0
+    _, terms = T.policy_loss(T.Tape(), lg, torch.roll(ids, -1, 1), torch.ones(4, device=DEV), scale=1.0, mask=mask, old_logprobs=refs, ref_logprobs=refs)
+    d = (terms.logprobs - refs).abs()
+    assert (d <= off).all() and (terms.kl <= off * off).all() and ((terms.ratio - 1).abs()[mask] <= 2 * off[mask]).all()
+    st = rl.policy_step(m, ids, plens, slens, torch.ones(4), None, old_logprobs=refs, ref_logprobs=refs, kl_coef=0.1)
+    assert st["kl"] <= float(off.max()) ** 2 and st["clipped"] == 0
+    st = rl.preference_step(m, ids, plens, slens, None, ref_logprobs=refs, beta=0.1)
+    assert abs(st["margin"]) <= 0.1 * float((off * mask).sum())
+    # (each product of the chunked head is as long as that of the whole one)
+    tape = T.Tape()
+    _, lp = T.linear_cross_entropy(tape, h, w, torch.roll(ids, -1, 1), torch.zeros_like, chunk=100)
+    assert ((lp - refs).abs()[mask] <= off[mask]).all()

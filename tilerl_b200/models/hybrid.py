@@ -377,4 +377,4 @@ class HybridModel:
         frozen = id(w) not in tape.leaves
         if return_hidden:          # the caller fuses the head with its loss (never forms [T, vocab])
             return h, w, frozen
-        return T.linear(tape, h, w, frozen=frozen)
+        return T.linear(tape, h, w, frozen=frozen, wide=True)

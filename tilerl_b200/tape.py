@@ -282,12 +282,17 @@ def set_dequant(fn: Optional[Callable]) -> None:
     DEQUANT_BF16 = fn
 
 
+def _wide_product(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    """``x @ w^T`` of two bf16 tensors on CUDA, the fp32 sums as they are."""
+    return torch.mm(x.reshape(-1, x.shape[-1]), w.t(), out_dtype=torch.float32).view(*x.shape[:-1], w.shape[0])
+
+
 @_nograd
-def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False) -> torch.Tensor:
+def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = False) -> torch.Tensor:
     """``y = x @ W^T``.  ``w`` is a dense master tensor (dX and dW) or a quantised
     weight / ``frozen=True`` dense tensor (dX only, the LoRA-on-frozen-base mode).
-    On CUDA the three GEMMs run in bf16 with fp32 accumulation; on CPU everything is fp32
-    (the oracle path)."""
+    On CUDA the three GEMMs run in bf16 with fp32 accumulation, y rounded to bf16 (``wide``: not rounded, as logits are, since
+    a rounding of 2^-9 of a logit of 20 is 0.04 of a log-probability); on CPU everything is fp32 (the oracle path)."""
     dense = isinstance(w, torch.Tensor)
     if x.is_cuda:
         if dense:
@@ -297,7 +302,7 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False) -> torch.Tensor
         else:
             wf = w.dequant().to(x.device, torch.bfloat16)
         xb = x.to(torch.bfloat16)
-        out = (xb @ wf.t()).float()
+        out = _wide_product(xb, wf) if wide else (xb @ wf.t()).float()
 
         def bwd(g):
             gb = g.to(torch.bfloat16)
@@ -821,7 +826,7 @@ def linear_cross_entropy(tape: Tape, h: torch.Tensor, w: torch.Tensor, targets: 
     ``weights_fn(logprobs [T]) -> weights [T]`` (SFT mask / N, or the PPO-clip weight times the
     advantage) turns them into per-token weights, pass 2 recomputes each chunk's logits and
     immediately folds ``w_i (softmax - onehot)`` into dH (and dW when the head is trainable).
-    Returns ``(loss, logprobs)``; the gradients are final, backward only scales them.
+    Returns ``(loss, logprobs)``; the gradients are final, backward only scales them.  Logits are those of ``linear(wide=True)``.
 
     Parity: the reference forms the full logits and overwrites them with the gradient
     (``tilerl_kernels/backend.py:1651-1672``, ``reference.py:1511-1603``)."""
@@ -831,9 +836,10 @@ def linear_cross_entropy(tape: Tape, h: torch.Tensor, w: torch.Tensor, targets: 
     n = hf.shape[0]
     cd = torch.bfloat16 if h.is_cuda else torch.float32
     wc = w if w.dtype == cd else w.to(cd)
+    product = _wide_product if h.is_cuda else lambda x, w: x @ w.t()
     lp = torch.empty(n, dtype=torch.float32, device=h.device)
     for a in range(0, n, chunk):
-        lg = (hf[a:a + chunk].to(cd) @ wc.t()).float()
+        lg = product(hf[a:a + chunk].to(cd), wc)
         lp[a:a + chunk] = lg.gather(-1, tg[a:a + chunk, None]).squeeze(-1) - torch.logsumexp(lg, -1)
     wts = weights_fn(lp.view(t_shape)).reshape(-1).float().to(h.device)
     loss = -(wts * lp).sum()
@@ -841,7 +847,7 @@ def linear_cross_entropy(tape: Tape, h: torch.Tensor, w: torch.Tensor, targets: 
     dw = None if frozen else torch.zeros(w.shape, dtype=torch.float32, device=h.device)
     for a in range(0, n, chunk):
         hc = hf[a:a + chunk].to(cd)
-        lg = (hc @ wc.t()).float()
+        lg = product(hc, wc)
         g = torch.softmax(lg, -1)
         g[torch.arange(g.shape[0], device=g.device), tg[a:a + chunk]] -= 1.0
         g = (g * wts[a:a + chunk, None]).to(cd)
@@ -862,7 +868,8 @@ def linear_logprobs(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, 
     """Log-probabilities of ``targets [...]`` under ``softmax(h W^T)`` from hidden rows ``h [..., H]`` and a dense head ``w [vocab, H]``, without the
     logits: how a frozen policy (a reference, the one that sampled) is scored.  ``mask`` (bool): the rows to score, the others give 0 whatever they
     hold and cost nothing.  ``entropy``: also the entropies of the rows, as a second result.  fp32; on CUDA the product has bf16 operands and fp32
-    sums, as :func:`linear`'s.  It is no op of a tape: gradients through the head are :func:`linear_cross_entropy`'s.
+    sums, as that of the training forward's logits (:func:`linear` with ``wide``): a policy and its reference with the same weights differ by the
+    order of those sums.  Rows in fp16 or fp64 are rounded to bf16 there too.  It is no op of a tape: gradients through the head are :func:`linear_cross_entropy`'s.
 
     A target outside of the vocabulary in a scored row gives NaN and sets the device's error word (not where torch forms the product: ``H`` no
     multiple of 8, rows in fp16 or fp64); on the CPU it is an error."""
