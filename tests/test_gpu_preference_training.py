@@ -127,3 +127,22 @@ def test_a_policy_scored_as_its_own_reference():
     tape = T.Tape()
     _, lp = T.linear_cross_entropy(tape, h, w, torch.roll(ids, -1, 1), torch.zeros_like, chunk=100)
     assert ((lp - refs).abs()[mask] <= off[mask]).all()
+
+
+def test_a_reference_with_a_quantised_head():
+    """The head of a training forward may be quantised; its words are scored as what it stands for."""
+    import dataclasses
+    from tilerl_b200.factory import build_model, make_ops
+    m = build_model(dataclasses.replace(small_gpu(), lm_head_quant="nvfp4"), DEV, seed=0, ops=make_ops(DEV))
+    m.add_lora(rank=4, alpha=8.0)
+    ids, plens, slens = _batch(m)
+    tape = T.Tape()
+    tape.enabled = False
+    h, w, _ = m.forward_dense(tape, ids, return_hidden=True)
+    assert hasattr(w, "wq")
+    mask, targets = rl._scored_mask(ids, plens, slens).to(DEV), torch.roll(ids, -1, 1)
+    want, went = T.linear_logprobs(h, w.dequant().to(DEV, torch.bfloat16), targets, mask=mask, entropy=True)
+    got, gent = rl.sequence_logprobs(m, ids, plens, slens, adapters=False, entropy=True)
+    assert torch.equal(got, want) and torch.equal(gent, went)
+    st = next(iter(rl.preference_loop(m, [([1, 2], [3, 4, 5], [6, 7])], None, steps=1, device=DEV)))
+    assert abs(st["margin"]) < 1e-3

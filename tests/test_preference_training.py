@@ -170,3 +170,25 @@ def test_train_preference_command(tmp_path, capsys, monkeypatch):
     for bad in (base, base[:-2], base + ["--rl"], base[:-3] + ["--kl-reference", "base"]):
         with pytest.raises(SystemExit):
             cli.main(bad + ["--force"])
+
+
+def test_a_reference_with_a_quantised_head():
+    """The head that a training forward takes may be quantised: its words are scored as what it stands for."""
+    import dataclasses
+    model = HybridModel.build_random(dataclasses.replace(tiny_hybrid(), lm_head_quant="nvfp4", tie_embeddings=False), seed=4)
+    model.add_lora(rank=2)
+    head = model.params["lm_head"]
+    assert hasattr(head, "wq")
+    ids, plens, slens = _batch(model.cfg)
+    mask, tape = rl._scored_mask(ids, plens, slens), T.Tape()
+    lp, ent = rl.sequence_logprobs(model, ids, plens, slens, adapters=False, entropy=True, micro=3)
+    want = torch.log_softmax(model.forward_dense(tape, ids), -1)
+    assert torch.allclose(lp, torch.where(mask, want.gather(-1, torch.roll(ids, -1, 1)[..., None])[..., 0], 0.0), atol=1e-5)
+    assert torch.allclose(ent, torch.where(mask, -(want.exp() * want).sum(-1), 0.0), atol=1e-5)
+    m = next(iter(rl.preference_loop(model, [([1, 2], [3, 4, 5], [6])], None, steps=1)))
+    assert abs(m["margin"]) < 1e-4
+    h = torch.zeros(2, head.shape[1])
+    assert torch.equal(T.linear_logprobs(h, head, torch.tensor([0, 1])), T.linear_logprobs(h, head.dequant(), torch.tensor([0, 1])))
+    for x, w in ((h[:, :-1], head), (h, None), (h, [[0.0]]), (h, head.to("meta"))):       # (another width, no weight, another device)
+        with pytest.raises(ValueError):
+            T.linear_logprobs(x, w, torch.tensor([0, 1]))

@@ -269,14 +269,15 @@ def sequence_logprobs(model, ids: torch.Tensor, prompt_lens, seq_lens, *, adapte
     no logits are formed (``tape.linear_logprobs``)."""
     if model.tp > 1:
         raise ValueError("sequence_logprobs scores with whole vocabularies: give it a model that is not sharded")
-    mask, targets, out = _scored_mask(ids, prompt_lens, seq_lens).to(ids.device), torch.roll(ids, -1, 1), []
+    mask, targets, out, head = _scored_mask(ids, prompt_lens, seq_lens).to(ids.device), torch.roll(ids, -1, 1), [], None
     for s in range(0, len(ids), micro or max(1, len(ids))):
         sl = slice(s, s + (micro or len(ids)))
         tape = T.Tape()
         tape.enabled = False
         with contextlib.nullcontext() if adapters else model.without_adapters():
             h, w, _ = model.forward_dense(tape, ids[sl], return_hidden=True)
-        out.append(T.linear_logprobs(h, w, targets[sl], mask=mask[sl], entropy=entropy))
+        head = T.dense_weight(w, h.device) if head is None else head      # (a quantised one is decoded once)
+        out.append(T.linear_logprobs(h, head, targets[sl], mask=mask[sl], entropy=entropy))
     if not out:
         raise ValueError("sequence_logprobs: no sequences")
     return tuple(torch.cat(o) for o in zip(*out)) if entropy else torch.cat(out)

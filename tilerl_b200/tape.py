@@ -282,6 +282,15 @@ def set_dequant(fn: Optional[Callable]) -> None:
     DEQUANT_BF16 = fn
 
 
+def dense_weight(w, device: torch.device) -> torch.Tensor:
+    """What a product on ``device`` multiplies with: a dense tensor, or what a quantised one stands for (bf16 on CUDA, fp32 on the CPU)."""
+    if isinstance(w, torch.Tensor):
+        return w
+    if device.type != "cuda":
+        return w.dequant().to(device)
+    return DEQUANT_BF16(w) if DEQUANT_BF16 is not None and hasattr(w, "wq") else w.dequant().to(device, torch.bfloat16)
+
+
 def _wide_product(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """``x @ w^T`` of two bf16 tensors on CUDA, the fp32 sums as they are."""
     return torch.mm(x.reshape(-1, x.shape[-1]), w.t(), out_dtype=torch.float32).view(*x.shape[:-1], w.shape[0])
@@ -294,13 +303,9 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
     On CUDA the three GEMMs run in bf16 with fp32 accumulation, y rounded to bf16 (``wide``: not rounded, as logits are, since
     a rounding of 2^-9 of a logit of 20 is 0.04 of a log-probability); on CPU everything is fp32 (the oracle path)."""
     dense = isinstance(w, torch.Tensor)
+    wf = dense_weight(w, x.device)
     if x.is_cuda:
-        if dense:
-            wf = w if w.dtype == torch.bfloat16 else w.to(torch.bfloat16)
-        elif DEQUANT_BF16 is not None and hasattr(w, "wq"):
-            wf = DEQUANT_BF16(w)
-        else:
-            wf = w.dequant().to(x.device, torch.bfloat16)
+        wf = wf.to(torch.bfloat16)
         xb = x.to(torch.bfloat16)
         out = _wide_product(xb, wf) if wide else (xb @ wf.t()).float()
 
@@ -314,7 +319,7 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
 
         tape.record("linear", (x, w) if dense and not frozen else (x,), (out,), bwd)
         return out
-    wf = w.float() if dense else w.dequant().to(x.device)
+    wf = wf.float()
     out = x.float() @ wf.t()
 
     def bwd(g):
@@ -864,17 +869,24 @@ def linear_cross_entropy(tape: Tape, h: torch.Tensor, w: torch.Tensor, targets: 
 
 
 @_nograd
-def linear_logprobs(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, *, mask: Optional[torch.Tensor] = None, entropy: bool = False):
-    """Log-probabilities of ``targets [...]`` under ``softmax(h W^T)`` from hidden rows ``h [..., H]`` and a dense head ``w [vocab, H]``, without the
-    logits: how a frozen policy (a reference, the one that sampled) is scored.  ``mask`` (bool): the rows to score, the others give 0 whatever they
+def linear_logprobs(h: torch.Tensor, w, targets: torch.Tensor, *, mask: Optional[torch.Tensor] = None, entropy: bool = False):
+    """Log-probabilities of ``targets [...]`` under ``softmax(h W^T)`` from hidden rows ``h [..., H]`` and a head ``w [vocab, H]``, dense or quantised
+    (as :func:`linear` takes it, decoded whole), without the logits: how a frozen policy (a reference, the one that sampled) is scored.  ``mask`` (bool): the rows to score, the others give 0 whatever they
     hold and cost nothing.  ``entropy``: also the entropies of the rows, as a second result.  fp32; on CUDA the product has bf16 operands and fp32
     sums, as that of the training forward's logits (:func:`linear` with ``wide``): a policy and its reference with the same weights differ by the
     order of those sums.  Rows in fp16 or fp64 are rounded to bf16 there too.  It is no op of a tape: gradients through the head are :func:`linear_cross_entropy`'s.
 
     A target outside of the vocabulary in a scored row gives NaN and sets the device's error word (not where torch forms the product: ``H`` no
     multiple of 8, rows in fp16 or fp64); on the CPU it is an error."""
-    if not isinstance(w, torch.Tensor) or w.dim() != 2 or not w.is_floating_point() or not h.is_floating_point() or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1:
-        raise ValueError(f"linear_logprobs: h [..., H] and a dense w [vocab, H], got {tuple(h.shape)} and {tuple(w.shape)}")
+    if not isinstance(w, torch.Tensor):
+        coded = getattr(w, "wq", getattr(w, "w8", None))
+        if coded is None:
+            raise ValueError(f"linear_logprobs: w is a tensor or a quantised weight, got {type(w).__name__}")
+        if coded.device != h.device:
+            raise ValueError("linear_logprobs: all inputs are on one device")
+        w = dense_weight(w, h.device)
+    if w.dim() != 2 or not w.is_floating_point() or not h.is_floating_point() or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"linear_logprobs: h [..., H] and w [vocab, H] in floating point, got {tuple(h.shape)} {h.dtype} and {tuple(w.shape)} {w.dtype}")
     rows, dev = h.shape[:-1], h.device
     if targets.shape != rows or targets.is_floating_point() or targets.dtype == torch.bool:
         raise ValueError(f"linear_logprobs: targets are token ids {tuple(rows)}, got {tuple(targets.shape)} {targets.dtype}")
