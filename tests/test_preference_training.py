@@ -192,3 +192,29 @@ def test_a_reference_with_a_quantised_head():
     for x, w in ((h[:, :-1], head), (h, None), (h, [[0.0]]), (h, head.to("meta"))):       # (another width, no weight, another device)
         with pytest.raises(ValueError):
             T.linear_logprobs(x, w, torch.tensor([0, 1]))
+
+
+def test_adapters_stay_in_place_while_the_base_model_is_scored():
+    """What other threads compute, and what is read of the adapters or added to them meanwhile, is as outside of the block."""
+    import threading
+    model = _adapters(HybridModel.build_random(tiny_hybrid(), seed=4))
+    ids, plens, slens = _batch(model.cfg)
+    run = lambda: rl.sequence_logprobs(model, ids, plens, slens)
+    own, base, names, seen = run(), rl.sequence_logprobs(model, ids, plens, slens, adapters=False), set(model.trainable()), []
+    with model.without_adapters():
+        other = threading.Thread(target=lambda: seen.append(run()))
+        other.start()
+        other.join()
+        assert torch.equal(run(), base) and set(model.trainable()) == names and all(".lora_" in k for k in names)
+        with model.without_adapters():
+            assert torch.equal(run(), base)
+        assert torch.equal(run(), base)                   # (the inner block's end is not the outer one's)
+        model.add_lora(rank=1, targets=["down"], seed=1)
+        assert torch.equal(run(), base)
+    assert torch.equal(seen[0], own)
+    narrow = [k for k, v in model.lora.items() if v[0].shape[0] == 1]
+    assert narrow and all(k.endswith("down") for k in narrow) and not torch.equal(run(), own)      # (added adapters are there)
+    with pytest.raises(ZeroDivisionError):
+        with model.without_adapters():
+            1 / 0
+    assert not torch.equal(run(), base)

@@ -26,6 +26,7 @@ Parity: reference ``src/tilerl/model.py`` -- ``param_specs:38``,
 from __future__ import annotations
 
 import contextlib
+import contextvars
 import math
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -108,6 +109,10 @@ def random_master(cfg: ModelConfig, seed: int = 0, device="cpu", dtype=torch.flo
     return out
 
 
+#: ids of the models whose forward passes go without adapters in this thread (``without_adapters``)
+_BARE: contextvars.ContextVar = contextvars.ContextVar("models_without_adapters", default=frozenset())
+
+
 class HybridModel:
     def __init__(self, cfg: ModelConfig, params: Dict[str, object], tp_rank: int = 0,
                  tp: int = 1):
@@ -185,16 +190,17 @@ class HybridModel:
         return keys
 
     def _lora(self, name: str):
-        return self.lora.get(name)
+        return None if id(self) in _BARE.get() else self.lora.get(name)
 
     @contextlib.contextmanager
     def without_adapters(self):
-        """The base model while the block runs (training forward): the policy that adapters started from."""
-        kept, self.lora = self.lora, {}
+        """The base model for the forward passes of this thread while the block runs: the policy that adapters started from.  The adapters stay where
+        they are, for other threads and for all that reads or adds some."""
+        before = _BARE.set(_BARE.get() | {id(self)})
         try:
             yield self
         finally:
-            self.lora = kept
+            _BARE.reset(before)
 
     # ---- serving forward ------------------------------------------------------------------
     def forward(self, batch, ops, kv_pool, state_pool, *, last_only: bool = True,
@@ -297,7 +303,7 @@ class HybridModel:
     def _tlinear(self, tape, x, name: str):
         from .. import tape as T
         w, frozen = self._w(name)
-        lo = self.lora.get(name)
+        lo = self._lora(name)
         if lo is not None:
             return T.linear_lora(tape, x, w, frozen, lo[0], lo[1], lo[2])
         return T.linear(tape, x, w, frozen=frozen)
