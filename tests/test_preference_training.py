@@ -218,3 +218,19 @@ def test_adapters_stay_in_place_while_the_base_model_is_scored():
         with model.without_adapters():
             1 / 0
     assert not torch.equal(run(), base)
+
+
+def test_weights_that_a_sharded_trainer_holds_are_not_scored():
+    from tilerl_b200.parallel.zero3 import Zero3
+    whole, model = (HybridModel.build_random(tiny_hybrid(), seed=4, keep_master=True) for _ in range(2))
+    Zero3(model)
+    ids, plens, slens = _batch(model.cfg)
+    with pytest.raises(ValueError, match="sharded trainer"):
+        rl.sequence_logprobs(model, ids, plens, slens)
+    assert (rl._reference_logprobs(whole, model, ids, plens, slens)[rl._scored_mask(ids, plens, slens)] < 0).all()
+    adapted = _adapters(HybridModel.build_random(tiny_hybrid(), seed=4))
+    base = rl.sequence_logprobs(adapted, ids, plens, slens, adapters=False)
+    Zero3(adapted, mode="lora")                           # (the adapters alone: the base model is whole)
+    with pytest.raises(ValueError, match="sharded trainer"):
+        rl.sequence_logprobs(adapted, ids, plens, slens)
+    assert torch.equal(rl.sequence_logprobs(adapted, ids, plens, slens, adapters=False), base)

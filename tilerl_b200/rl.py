@@ -269,6 +269,8 @@ def sequence_logprobs(model, ids: torch.Tensor, prompt_lens, seq_lens, *, adapte
     no logits are formed (``tape.linear_logprobs``)."""
     if model.tp > 1:
         raise ValueError("sequence_logprobs scores with whole vocabularies: give it a model that is not sharded")
+    if any(isinstance(t, torch.Tensor) and not t.numel() for k, t in model.params.items() if adapters or ".lora_" not in k):
+        raise ValueError("sequence_logprobs: a sharded trainer holds this model's weights between its steps: give it a whole model, a frozen copy say")
     mask, targets, out, head = _scored_mask(ids, prompt_lens, seq_lens).to(ids.device), torch.roll(ids, -1, 1), [], None
     for s in range(0, len(ids), micro or max(1, len(ids))):
         sl = slice(s, s + (micro or len(ids)))
