@@ -234,3 +234,19 @@ def test_weights_that_a_sharded_trainer_holds_are_not_scored():
     with pytest.raises(ValueError, match="sharded trainer"):
         rl.sequence_logprobs(adapted, ids, plens, slens)
     assert torch.equal(rl.sequence_logprobs(adapted, ids, plens, slens, adapters=False), base)
+
+
+def test_models_whose_forward_pass_keeps_32_bits_only():
+    """A model of one's own, with the forward pass that training steps have always asked for."""
+    class Own(HybridModel):
+        def forward_dense(self, tape, ids, *, checkpoint_layers=False, positions=None, hook=None, cp=None, return_hidden=False):
+            return super().forward_dense(tape, ids, checkpoint_layers=checkpoint_layers, positions=positions, hook=hook, cp=cp, return_hidden=return_hidden)
+
+    model, own = (_adapters(cls.build_random(tiny_hybrid(), seed=4)) for cls in (HybridModel, Own))
+    assert type(own) is Own
+    ids, plens, slens = _batch(model.cfg)
+    for fused in (False, True):
+        want, got = (rl.policy_step(m, ids, plens, slens, torch.ones(4), None, return_grads=True, fused_ce=fused) for m in (model, own))
+        assert want["loss"] == got["loss"] and all(torch.equal(g, got["grads"][k]) for k, g in want["grads"].items())
+    with pytest.raises(TypeError):
+        rl.policy_step(own, ids, plens, slens, torch.ones(4), None, activation_bits=8)

@@ -152,12 +152,15 @@ def forward_backward(model, ids: torch.Tensor, targets: torch.Tensor, weights_fn
     what the forward pass keeps (``HybridModel.forward_dense``)."""
     tp = T.Tape(tp_group, tp_world)
     tp.watch(*trainable.values())
+    kw = dict(checkpoint_layers=checkpoint_layers, hook=hook)
+    if activation_bits != 32:            # (a model of one's own need not know of it)
+        kw["activation_bits"] = activation_bits
     if fused_ce and tp_world == 1:
-        h, w, frozen = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook, return_hidden=True, activation_bits=activation_bits)
+        h, w, frozen = model.forward_dense(tp, ids, return_hidden=True, **kw)
         loss, lp = T.linear_cross_entropy(tp, h, w, targets, lp_weights_fn, frozen=frozen)
         grads = tp.backward(loss, on_grad=on_grad)
         return float(loss), _named_grads(trainable, grads), lp
-    logits = model.forward_dense(tp, ids, checkpoint_layers=checkpoint_layers, hook=hook, activation_bits=activation_bits)
+    logits = model.forward_dense(tp, ids, **kw)
     if tp_world > 1:
         # vocab-parallel logits: the loss and the weights come from the sharded CE
         if lp_weights_fn is None:
