@@ -461,3 +461,27 @@ def test_rows_of_few_words_that_can_be(v, dtype):
     tape.watch(here)
     loss, terms = T.policy_loss(tape, here, targets.to(DEV), torch.ones(len(rows), device=DEV), scale=1.0)
     assert loss.isnan() and terms.logprobs.isnan().all() and tape.backward(loss)[id(here)].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("preference", [False, True])
+def test_a_captured_backward_pass_of_an_eager_loss(preference, dtype):
+    """Replayed, it gives the gradient times the loss's own again, not times that once more."""
+    logits, here, targets, mask, adv, _, _ = _inputs((2, 5), 900, dtype, 3)
+    grads, up = [], torch.tensor(0.5, device=DEV)
+    for _ in range(2):
+        tape = T.Tape()
+        tape.watch(here)
+        loss, _ = T.preference_loss(tape, here, targets.to(DEV)) if preference else T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=1.0)
+        if not grads:
+            grads.append(tape.backward(loss, up)[id(here)].clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = tape.backward(loss, up)[id(here)]
+    assert out.dtype == dtype
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, grads[0])                 # (half of a value is exact)
+    up.fill_(2.0)
+    graph.replay()
+    assert torch.equal(out, grads[0] * 4)

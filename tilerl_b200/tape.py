@@ -723,7 +723,8 @@ def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
         if g is _ONE:
             return (grad,)
         if K is not None and g.numel() == 1 and g.device == grad.device:
-            return (K.scale_grad(grad, g),)
+            # in place, but not where the pass is captured: each replay would multiply what the one before left
+            return (grad * g.reshape(()) if torch.cuda.is_current_stream_capturing() else K.scale_grad(grad, g),)
         return (grad * g,)
 
     bwd.takes_one = True
