@@ -632,7 +632,8 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
 }
 
 // ---- preference loss: a row's weight needs its whole sequence -------------------------------------------------------------------
-// A block a row: what its gradient needs into `rest` (base; of far rows the largest value; sum; whether the row is far), and its log-probability.
+// A block a row: what its gradient needs into `rest`, and its log-probability.  `rest`: base, p - 1 of the target, sum, 0; of far rows p - 1, the largest
+// value, sum, 1.  p - 1 is the others' share, formed as that: a quotient less 1 would have fp32's rounding of 1, 6 % of a share of 1e-6.
 template <typename T>
 __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows rows, float4* rest, double* lps) {
   using S = Span<T>;
@@ -668,17 +669,20 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
     const float most = (float)e / (float)sum;
     // (the mean of the others, and the target's share)
     const float of_all = rest_of > 0.0 ? mean + most * (fmaxf((float)y, -256.f) - mean) : (float)y;
-    rest[r] = make_float4(all, 0.f, (float)sum, 0.f), lps[r] = pl_low(xt, all, of_all) + PL_LESS * (double)most - log(sum);
+    rest[r] = make_float4(all, (float)(-rest_of / sum), (float)sum, 0.f), lps[r] = pl_low(xt, all, of_all) + PL_LESS * (double)most - log(sum);
     far = pl_far(all);
   }
   __syncthreads();
   if (!far) return;
   const float m = block_max(pl_far_most<T, NT>(body, (int)sp.nv, xe), red);
   const float s = block_sum(pl_far_sum<T, NT>(body, (int)sp.nv, xe, ie >= 0, m), red);
-  if (threadIdx.x == 0) rest[r] = make_float4(0.f, m, s, 1.f), lps[r] = (double)xt - (double)m - log((double)s);
+  if (threadIdx.x == 0) {
+    const double low = (double)xt - (double)m;
+    rest[r] = make_float4((float)(exp(low) / (double)s - 1.0), m, s, 1.f), lps[r] = low - log((double)s);
+  }
 }
 
-// Up to 4096 values, as the policy loss has them: NT threads a row.  Of `rest` the largest value and the sum.
+// Up to 4096 values, as the policy loss has them: NT threads a row.  `rest` as of far rows.
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_stats_short_kernel(const T* x, const Rows rows, float4* rest, double* lps) {
   constexpr int E = Span<T>::E, W = NT / 32, R = 256 / NT;
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(256, 5) pl_stats_short_kernel(const T* x, cons
   const double rest_of = pl_short_join<W>(q, top, u), low = (double)xt - (double)top, e = exp(low), sum = rest_of + e;
   const float mean = (u + (float)e * fmaxf((float)low * PL_L2E, -256.f)) / (float)sum;
   const float rough = (float)(rest_of - (others == top ? 1.0 : 0.0)) / (float)sum;       // (what exponentials that are not exact have of the sum)
-  rest[rw] = make_float4(0.f, top, (float)sum, 1.f);
+  rest[rw] = make_float4((float)(-rest_of / sum), top, (float)sum, 1.f);
   lps[rw] = low + PL_OFF * PL_LN2 * (double)mean - PL_LESS * (double)rough - log(sum);
 }
 template <typename T, int NT>
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(256, 5) pl_grad_short_kernel(const T* x, const
   if (ie >= 0) out[ie] = pl_round<T>(scored ? one(pl_float(row[ie])) * c : 0.f);
   if (!scored) return;
   const long long t = rows.target[r];
-  if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>((one(pl_float(row[t])) / st.z - 1.f) * w);
+  if (t < rows.V && pl_wrote(t, ie, sp.head, E, 0, nv, k, NT)) out[t] = pl_round<T>(st.x * w);
 }
 
 // Gradients: a block a slice of a row.  weight of row r: weight[r / per].  The last rows first: they are what L2 still holds.
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(256, 4) pl_grad_kernel(const T* x, const Rows 
   if (st.w != 0.f) pl_far_grads<T, NT>(body, dst, cnt, st.y, c);
   else pl_grads<T, NT, G>(body, dst, cnt, st.x, c);
   if (ie >= 0) out[ie] = pl_round<T>(one(pl_float(row[ie])) * c);
-  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, k, NT)) out[t] = pl_round<T>((one(pl_float(row[t])) / st.z - 1.f) * w);
+  if (t < rows.V && pl_wrote(t, ie, sp.head, S::E, lo, cnt, k, NT)) out[t] = pl_round<T>((st.w != 0.f ? st.x : st.y) * w);
 }
 
 // ---- sums over rows, and pairs of sequences ----------------------------------------------------------------------------------

@@ -485,3 +485,25 @@ def test_a_captured_backward_pass_of_an_eager_loss(preference, dtype):
     up.fill_(2.0)
     graph.replay()
     assert torch.equal(out, grads[0] * 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v,offset", [(5, 1), (700, 0), (4096, 0), (4099, 3), (33000, 0)])
+def test_gradients_of_targets_that_are_nearly_certain(v, offset, dtype):
+    """The target's gradient is weight (p - 1), which is the others' share of the sum: relative to itself it has the roundings of that share's sum, of
+    the quotient, the weight and the product (2^-24 each, 8 with what the weight is of), and the result's."""
+    levels = torch.tensor([math.log((v - 1) / rest) for rest in (1e-1, 1e-3, 1e-5, 1e-7)])
+    targets = torch.tensor([0, v - 1, v // 2, v // 3] * 2).view(2, 4)
+    logits = torch.zeros(2, 4, v)
+    logits.scatter_(-1, targets[..., None], levels[None, :, None].expand(2, 4, 1))
+    logits = logits.to(dtype)
+    here = torch.empty(logits.numel() + offset, dtype=dtype, device=DEV)[offset:].view(logits.shape).copy_(logits)
+    tape, cpu, wide = T.Tape(), T.Tape(), logits.double()
+    tape.watch(here), cpu.watch(wide)
+    loss, _ = T.preference_loss(tape, here, targets.to(DEV), beta=0.5)
+    want, _ = T.preference_loss(cpu, wide, targets, beta=0.5)
+    grad, wgrad = tape.backward(loss)[id(here)].cpu().double(), cpu.backward(want)[id(wide)]
+    # 64 bits of p - 1 leave 1e-16 of 1, 1e-9 of 1e-7
+    got, exact = (t.gather(-1, targets[..., None]) for t in (grad, wgrad))
+    half = 0.0 if dtype == torch.float32 else 2 ** -8
+    assert ((got - exact).abs() <= exact.abs() * ((_adds(v) + 8) * 2 ** -24 + 2e-9 + half)).all()
