@@ -370,3 +370,14 @@ def test_targets_outside_of_the_vocabulary_in_the_torch_forms(monkeypatch):
         assert torch.equal(got[4].logprobs[1], seen.logprobs[1])
         assert got[6].isnan().tolist() == [False, True] + [False] * 4 and torch.equal(got[6][rest], lp[rest]) and torch.equal(got[7], ent)
     assert ref.within(targets, 9) == (targets, None)
+
+
+@pytest.mark.parametrize("mask", [None, torch.zeros(4, 0, dtype=torch.bool)])
+@pytest.mark.parametrize("average", [False, True])
+def test_pairs_of_sequences_without_tokens(average, mask):
+    """Log ratios of 0, sums as means: log 2 a pair."""
+    tape, logits = T.Tape(), torch.zeros(4, 0, 5)
+    tape.watch(logits)
+    loss, terms = T.preference_loss(tape, logits, torch.zeros(4, 0, dtype=torch.long), mask, average=average)
+    assert abs(float(loss) - math.log(2.0)) < 1e-6 and terms.logprobs.tolist() == [0.0] * 4 and terms.margins.tolist() == [0.0] * 2
+    assert tape.backward(loss)[id(logits)].shape == (4, 0, 5)

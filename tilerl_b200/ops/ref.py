@@ -595,7 +595,7 @@ def preference_loss(logits, targets, mask, ref, *, beta, smooth, average, scale,
         gap = torch.where(flat, gap, 0.0)
     count = torch.ones(n, dtype=torch.float64, device=lp.device)
     if average:
-        count = count * t if mask is None else mask.sum(-1).clamp_min(1).double()
+        count = count * max(1, t) if mask is None else mask.sum(-1).clamp_min(1).double()
     total, gap = lp.view(n, t).sum(-1) / count, gap.view(n, t).sum(-1) / count
     z = beta * (gap[0::2] - gap[1::2])
     loss = ((1 - smooth) * F.softplus(-z) + smooth * F.softplus(z)).sum() * scale
