@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(1024) pl_pairs_kernel(const double* lps, const
     const double dz = z == z ? e * up - (1.0 - e) * down : z;
     totals[2 * p] = (float)(v[0] * by0), totals[2 * p + 1] = (float)(v[3] * by1);
     margins[p] = (float)z;
-    const double of = (1.0 - e) * (l + fmax(-z, 0.0)) + (e != 0.0 ? e * (l + fmax(z, 0.0)) : 0.0);
+    const double of = z != z ? z : (e != 1.0 ? (1.0 - e) * (l + fmax(-z, 0.0)) : 0.0) + (e != 0.0 ? e * (l + fmax(z, 0.0)) : 0.0);
     loss[p] = losses[0] = of;
     // (the row's gradient is weight (p - onehot): minus that of its log-probability)
     weight[2 * p] = (float)(-dz * scale * beta * by0), weight[2 * p + 1] = (float)(dz * scale * beta * by1);

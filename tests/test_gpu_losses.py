@@ -507,3 +507,22 @@ def test_gradients_of_targets_that_are_nearly_certain(v, offset, dtype):
     got, exact = (t.gather(-1, targets[..., None]) for t in (grad, wgrad))
     half = 0.0 if dtype == torch.float32 else 2 ** -8
     assert ((got - exact).abs() <= exact.abs() * ((_adds(v) + 8) * 2 ** -24 + 2e-9 + half)).all()
+
+
+@pytest.mark.parametrize("v", [9, 5000])
+def test_margins_without_bounds(v):
+    """A chosen or rejected word that cannot be (-inf): the side of the loss that has no share counts nothing, the other is infinite or 0."""
+    inf = float("inf")
+    for side, smooth, want in ((1, 0.0, 0.0), (1, 1.0, inf), (1, 0.5, inf), (0, 0.0, inf), (0, 1.0, 0.0), (0, 0.5, inf)):
+        lg = torch.zeros(2, 3, v, device=DEV)
+        lg[side, 1, 4] = -inf
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.preference_loss(tape, lg, torch.full((2, 3), 4, device=DEV), beta=0.5, label_smoothing=smooth)
+        assert float(loss) == want and float(terms.margins) == (inf if side else -inf)
+        grad = tape.backward(loss)[id(lg)]
+        assert torch.isfinite(grad).all() and bool(grad.any()) == (want == inf)
+    lg[0, 0, 0] = NAN
+    for smooth in (0.0, 0.5, 1.0):
+        loss, terms = T.preference_loss(T.Tape(), lg, torch.full((2, 3), 4, device=DEV), label_smoothing=smooth)
+        assert loss.isnan() and terms.margins.isnan().all()

@@ -381,3 +381,21 @@ def test_pairs_of_sequences_without_tokens(average, mask):
     loss, terms = T.preference_loss(tape, logits, torch.zeros(4, 0, dtype=torch.long), mask, average=average)
     assert abs(float(loss) - math.log(2.0)) < 1e-6 and terms.logprobs.tolist() == [0.0] * 4 and terms.margins.tolist() == [0.0] * 2
     assert tape.backward(loss)[id(logits)].shape == (4, 0, 5)
+
+
+def test_margins_without_bounds():
+    """A chosen or rejected word that cannot be (-inf): the side of the loss that has no share counts nothing, the other is infinite or 0."""
+    inf = float("inf")
+    for side, smooth, want in ((1, 0.0, 0.0), (1, 1.0, inf), (1, 0.5, inf), (0, 0.0, inf), (0, 1.0, 0.0), (0, 0.5, inf)):
+        lg = torch.zeros(2, 3, 9)
+        lg[side, 1, 4] = -inf
+        tape = T.Tape()
+        tape.watch(lg)
+        loss, terms = T.preference_loss(tape, lg, torch.full((2, 3), 4), beta=0.5, label_smoothing=smooth)
+        assert float(loss) == want and float(terms.margins) == (inf if side else -inf)
+        grad = tape.backward(loss)[id(lg)]
+        assert torch.isfinite(grad).all() and bool(grad.any()) == (want == inf)
+    lg[0, 0, 0] = NAN
+    for smooth in (0.0, 0.5, 1.0):
+        loss, terms = T.preference_loss(T.Tape(), lg, torch.full((2, 3), 4), label_smoothing=smooth)
+        assert loss.isnan() and terms.margins.isnan().all()

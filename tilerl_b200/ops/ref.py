@@ -598,7 +598,8 @@ def preference_loss(logits, targets, mask, ref, *, beta, smooth, average, scale,
         count = count * max(1, t) if mask is None else mask.sum(-1).clamp_min(1).double()
     total, gap = lp.view(n, t).sum(-1) / count, gap.view(n, t).sum(-1) / count
     z = beta * (gap[0::2] - gap[1::2])
-    loss = ((1 - smooth) * F.softplus(-z) + smooth * F.softplus(z)).sum() * scale
+    part = lambda factor, y: factor * F.softplus(y) if factor else torch.where(z.isnan(), z, 0.0)      # (nothing of an infinite loss is nothing)
+    loss = (part(1 - smooth, -z) + part(smooth, z)).sum() * scale
     dz = (smooth * torch.sigmoid(z) - (1 - smooth) * torch.sigmoid(-z)) * scale
     w = (torch.stack([-dz, dz], -1).reshape(-1) * beta / count)[:, None].expand(n, t).reshape(-1)
     if flat is not None:
