@@ -250,3 +250,26 @@ def test_models_whose_forward_pass_keeps_32_bits_only():
         assert want["loss"] == got["loss"] and all(torch.equal(g, got["grads"][k]) for k, g in want["grads"].items())
     with pytest.raises(TypeError):
         rl.policy_step(own, ids, plens, slens, torch.ones(4), None, activation_bits=8)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("watched", [True, False])
+def test_a_segment_that_is_given_an_input_twice(bits, watched):
+    """x^2 + 3 x from one tensor as two inputs, and a leaf that is an input and a parameter: gradients are not counted again."""
+    g = torch.Generator().manual_seed(0)
+    leaf, w = torch.randint(-127, 128, (3, 128), generator=g).float(), torch.randn(4, 128, generator=g)
+    leaf[:, 0] = 127.0                                    # (whole steps of 1: what 8 bits stand for is the values)
+    tape = T.Tape()
+    tape.watch(leaf, w)
+    x = leaf if watched else T.scale(tape, leaf, 1.0)
+
+    def segment(tape, a, b, c):
+        out = a * b
+        tape.record("product", (a, b), (out,), lambda g: (g * b, g * a))
+        return T.linear(tape, T.add(tape, out, T.scale(tape, a, 3.0)), c)
+
+    y = tape.checkpoint(segment, x, x, w, params=(w,), bits=bits)
+    up = torch.randn(3, 4, generator=g)
+    grads = tape.backward(y, up)
+    assert torch.allclose(grads[id(w)], up.t() @ (leaf * leaf + 3 * leaf), rtol=1e-5)
+    assert torch.allclose(grads[id(leaf)], (up @ w) * (2 * leaf + 3), rtol=1e-4, atol=1e-2)

@@ -172,7 +172,7 @@ class Tape:
                 sub.leaves[id(t)] = t
             y = fn(sub, *again)
             gs = sub.backward(y, g)
-            return tuple(gs.get(id(t)) for t in again + params)
+            return tuple(gs.pop(id(t), None) for t in again + params)      # (one that is given twice has its whole gradient the first time)
 
         self.record("checkpoint", inputs + params, (out,), bwd)
         for t, k in zip(inputs, kept):
