@@ -144,7 +144,7 @@ __device__ __forceinline__ double pl_join(const Part* parts, float& base, float&
 }
 
 template <typename T>
-__device__ __forceinline__ float pl_target(const T* row, long long t, long V, long r) {
+__device__ __forceinline__ float pl_target(const T* row, long long t, long V) {
   if (t < 0 || t >= V) {
     trl_set_error(TRL_ERR_BOUNDS, PL_SITE, (int)t, (int)V);
     return NAN;
@@ -408,7 +408,7 @@ __device__ __forceinline__ float pl_short_top(const Part* q) {
 
 // ---- policy loss -----------------------------------------------------------------------------------------------------------------
 // Up to 4096 values: NT threads a row, which waits in registers, 16 values a thread, as exponentials until its sum and weight are known; the rows of a
-// block have theirs formed side by side, a thread a row.  A row's chain (target, its logit, exponentials in fp64) is some 5 us, so what
+// block have theirs formed side by side, four lanes of a warp and a lane of another a row.  A row's chain (target, its logit, exponentials in fp64) is some 5 us, so what
 // counts is how many are on their way: 40 warps an SM.  (A warp a row, 32 values a lane, each its own weight: 16 384 x 1000 69 us, this 50.)
 template <typename T, int NT>
 __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, const Rows rows, T* grad, const __grid_constant__ PolicyRow a, float* whole) {
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(256, 5) pl_policy_short_kernel(const T* x, con
   if (weighs) {
     if (warp == 0) in = PolicyIn(a, rw);
     const long long t = rows.target[rw];
-    if (warp == 1) pl_target(x + (size_t)rw * rows.V, t, rows.V, rw);
+    if (warp == 1) pl_target(x + (size_t)rw * rows.V, t, rows.V);
     xt = t >= 0 && t < rows.V ? pl_float(x[(size_t)rw * rows.V + t]) : NAN;
   }
   const T* row = x + (size_t)r * rows.V;
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(NT, BLOCKS) pl_policy_kernel(const T* x, const
   PolicyIn in;
   float xt = 0.f;
   if (warp == 0) in = PolicyIn(a, r), xt = t >= 0 && t < rows.V ? pl_float(p.row[t]) : NAN;
-  if (tid == 0 && p.rank == 0) pl_target(p.row, t, rows.V, r);
+  if (tid == 0 && p.rank == 0) pl_target(p.row, t, rows.V);
   const float xe = p.ie >= 0 ? pl_float(p.row[p.ie]) : -INFINITY;
   Part part = pl_sums<T, NT, G, true>(p.body, p.cnt, xe, grad != nullptr);
   part.join_warp();
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(256, 4) pl_stats_kernel(const T* x, const Rows
   const uint4* body = reinterpret_cast<const uint4*>(row + sp.head);
   float xt = 0.f;
   const long long t = rows.target[r];
-  if (threadIdx.x == 0) xt = pl_target(row, t, rows.V, r);
+  if (threadIdx.x == 0) xt = pl_target(row, t, rows.V);
   const long ie = sp.end_of(threadIdx.x);
   const float xe = ie >= 0 ? pl_float(row[ie]) : -INFINITY;
   // A sequence's sum takes in every row's error.  Where the target is likely, that is its exponential's and what additions to it lose: 6e-8 a row (a
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(256, 5) pl_stats_short_kernel(const T* x, cons
   const bool scored = r < rows.n && (!rows.mask || rows.mask[r]);
   const bool forms = threadIdx.x < R && rw < rows.n, weighs = forms && (!rows.mask || rows.mask[rw]);
   float xt = 0.f;
-  if (weighs) xt = pl_target(x + (size_t)rw * rows.V, rows.target[rw], rows.V, rw);
+  if (weighs) xt = pl_target(x + (size_t)rw * rows.V, rows.target[rw], rows.V);
   else if (forms) lps[rw] = 0.0;
   const T* row = x + (size_t)r * rows.V;
   const Span<T> sp(row, rows.V);

@@ -337,7 +337,7 @@ __global__ void __cluster_dims__(SC_SPREAD, 1, 1) __launch_bounds__(256) score_f
   __shared__ float parts[SC_SPREAD][3];
   pdl_wait();
   const int row = blockIdx.x / SC_SPREAD, rank = blockIdx.x % SC_SPREAD, n = p.count ? *p.count : p.n;
-  if (row >= n) return;                              // (the whole cluster)
+  if (row >= n) return;                              // (the whole cluster, before its first barrier)
   const float* at = x + (size_t)row * ldo;
   const int nv = (int)(ldo / 4), per = (nv + SC_SPREAD - 1) / SC_SPREAD, end = min(nv, (rank + 1) * per);
   float m = -INFINITY, s = 0.f, u = 0.f;
@@ -508,7 +508,9 @@ int score_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& 
 
 // Up to so many rows the head's kernel for decode ticks streams the words (its MMA has them as rows, and as many columns as there are hidden rows), and
 // their logits, 1 MB a row of 248 320, go through L2: an MMA of 256 rows here, most of them empty, takes longer than the words from memory.  Pairs and
-// this, us: 248 320 x 5120 1 row 562, 388 (389 to read W), 32 rows 441, 411, 40 rows 445, 431, 64 rows 449, 445; 32 768 x 1024 1 row 40, 28, 33 rows 34, 32.
+// this, us, in turn: 248 320 x 5120 1 row 562, 379 (389 to read W at the measured copy rate), 33 rows 467 to 488, 445, 64 rows 543 to 591, 472; 128 000 x 4096
+// 33 rows 190, 190, 64 rows 223 to 236, 203; 32 768 x 1024 1 row 40, 29, 33 rows 27, 29, 48 rows 24, 25, 64 rows 22, 26.  Above 32 rows, up to
+// the 64 that the head's kernel takes, small heads are better off with pairs and large ones with this: a rule by rows alone ends where neither loses much.
 constexpr int SC_FEW = 32;
 int score_parts(int V) { return (V + SC_WORDS - 1) / SC_WORDS * 2; }
 

@@ -12,13 +12,14 @@ __device__ __forceinline__ uint32_t gp_map(uint32_t addr, int cta) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
   return r;
 }
-// What a CTA waits for without a limit, and why it ends.  A cluster barrier takes the place of __syncthreads for two to six CTAs
-// that the hardware starts together; shared memory of another CTA may only be touched once one has been passed, and no CTA may
-// leave before the last access to its own, so an mbarrier with a limit can stand in for neither the first nor the last.  Every thread
-// comes to each of them: no path returns early, and all waits in between (the ring, the accumulators, the producers' tail) have
-// a limit, after which they leave their loop.  The allocation of TMEM waits for the other CTA's, right behind the first barrier, and
-// for columns to be free: a CTA leaves too little shared memory on its SM for any other kernel that holds some (each takes
-// 190 KB or more, and gives its columns back on every path).  The release waits for the other CTA's, behind a barrier too.
+// What a CTA waits for without a limit, and why it ends.  A cluster barrier takes the place of __syncthreads for CTAs that the
+// hardware starts together; shared memory of another CTA may only be touched once one has been passed, and no CTA may
+// leave before the last access to its own, so an mbarrier with a limit can stand in for neither the first nor the last.  What a kernel has
+// to hold to: either every thread of a cluster comes to all of its barriers or none comes to any (a whole cluster may return before the
+// first), and all waits in between (rings, accumulators, producers' tails) have a limit, after which they leave their loop.
+// Kernels with TMEM: the allocation waits for the other CTA's, right behind the first barrier, and for columns to be free, so a CTA leaves too
+// little shared memory on its SM for any other kernel that holds some (each takes 190 KB or more, and gives its columns back on every
+// path).  The release waits for the other CTA's, behind a barrier too.
 // Not the .aligned forms: the warps come here from loops and branches that their lanes left at different times, and a warp
 // that is not converged would count more than once.
 __device__ __forceinline__ void gp_cluster_sync() {

@@ -12,7 +12,6 @@ N.register("trl_score_workspace", [N.I] * 5, N.L)
 N.register("trl_score", [N.P, N.I, N.P, N.P, N.P] + [N.I] * 3 + [N.P] * 4)
 
 ROWS = 8192               # a call: the tiles' parts of as many rows over 248 320 words are 127 MB
-FEW = 32                  # rows that go through the decode ticks' head and a pass over their logits
 CHUNK = 256               # rows of logits that the torch form has at a time
 
 
