@@ -121,10 +121,10 @@ struct Part {
     s = warp_sum(s), u = warp_sum(u);
   }
 };
-// The log-probability of a value x but for the logarithm of the sum, in fp64.
+// The log-probability of a value x but for the logarithm of the sum, in fp64.  (x itself goes in as it is: a target at the type's lowest value has
+// an old log-probability as low, and 1e-16 of 1e38 between them would be a ratio of infinity.)
 __device__ __forceinline__ double pl_low(float x, float base, float mean) {
-  const double y = (double)x * (double)PL_L2E - (double)base;
-  return (y - PL_OFF * (y - (double)mean)) * PL_LN2 - PL_LESS;
+  return (double)x + (PL_OFF * (double)mean - (double)base) * (1.0 / (double)PL_L2E) - PL_LESS;
 }
 // N parts, in order: the sum and, through it, a value's pl_low.  base: at first one that the result's is not to be below.
 template <int N>

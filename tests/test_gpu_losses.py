@@ -526,3 +526,30 @@ def test_margins_without_bounds(v):
     for smooth in (0.0, 0.5, 1.0):
         loss, terms = T.preference_loss(T.Tape(), lg, torch.full((2, 3), 4, device=DEV), label_smoothing=smooth)
         assert loss.isnan() and terms.margins.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [40, 900, 5000, 40000, 150000, 270000])
+def test_targets_that_are_masked_with_a_low_value(v, dtype):
+    """A target far below its row, with old and reference log-probabilities as low: the ratio is e to the minus of the other words' log-sum, of which
+    64-bit numbers of that size keep something (2e-6 at 1e10) or nothing: at most 2, as a row's sum is of exponentials below the next power
+    of two.  No weight but one of that size, no gradient without a number, and none of the target's p."""
+    g = torch.Generator().manual_seed(v)
+    x = torch.randn(6, v, generator=g).to(dtype)
+    targets = torch.tensor([0, 1, 17, v // 2, v - 2, v - 1])
+    for low in (-1e10, -1e30, torch.finfo(dtype).min):
+        x[torch.arange(6), targets] = low
+        same = x[torch.arange(6), targets].float().to(DEV)
+        here, tape = x.to(DEV), T.Tape()
+        tape.watch(here)
+        loss, terms = T.policy_loss(tape, here, targets.to(DEV), torch.tensor([1.0, -1.0] * 3, device=DEV), scale=1.0, old_logprobs=same, ref_logprobs=same, kl_coef=0.1)
+        grad = tape.backward(loss)[id(here)].cpu().double()
+        rest = torch.logsumexp(x.double(), -1)
+        assert torch.isfinite(loss) and (terms.logprobs.cpu() - same.cpu()).abs().le(same.cpu().abs() * 2 ** -23).all()
+        assert (terms.ratio <= 2).all() and (terms.kl.abs() <= 1e6).all()
+        if low == -1e10:
+            assert torch.allclose(terms.ratio.cpu().double(), torch.exp(-rest), rtol=1e-5)
+        w = terms.weights.cpu().double()
+        p = torch.softmax(x.double(), -1)
+        p[torch.arange(6), targets] -= 1.0
+        assert torch.isfinite(w).all() and ((grad - w[:, None] * p).abs() <= _grad_bounds(x, w, w * 0, v)).all()
