@@ -466,25 +466,32 @@ def test_rows_of_few_words_that_can_be(v, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("preference", [False, True])
 def test_a_captured_backward_pass_of_an_eager_loss(preference, dtype):
-    """Replayed, it gives the gradient times the loss's own again, not times that once more."""
+    """Its gradient is multiplied in place, again at every replay, and its memory is the tape's, which lets go of it: refused.  Captured as a
+    whole a pass gives the same at every replay."""
     logits, here, targets, mask, adv, _, _ = _inputs((2, 5), 900, dtype, 3)
-    grads, up = [], torch.tensor(0.5, device=DEV)
-    for _ in range(2):
+    targets, adv, up = targets.to(DEV), adv.to(DEV), torch.tensor(0.5, device=DEV)
+
+    def loss():
         tape = T.Tape()
         tape.watch(here)
-        loss, _ = T.preference_loss(tape, here, targets.to(DEV)) if preference else T.policy_loss(tape, here, targets.to(DEV), adv.to(DEV), scale=1.0)
-        if not grads:
-            grads.append(tape.backward(loss, up)[id(here)].clone())
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        out = tape.backward(loss, up)[id(here)]
-    assert out.dtype == dtype
-    for _ in range(3):
-        graph.replay()
-        assert torch.equal(out, grads[0])                 # (half of a value is exact)
+        return tape, (T.preference_loss(tape, here, targets) if preference else T.policy_loss(tape, here, targets, adv, scale=1.0))[0]
+
+    tape, l = loss()
+    want = tape.backward(l, up)[id(here)].clone()
+    for grad in (None, up):
+        tape, l = loss()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="captured with the forward pass"):
+                tape.backward(l, grad)
+            tape, l = loss()
+            out = tape.backward(l, up)[id(here)]
+        for _ in range(3):
+            graph.replay()
+            assert torch.equal(out, want)
     up.fill_(2.0)
     graph.replay()
-    assert torch.equal(out, grads[0] * 4)
+    assert torch.equal(out, want * 4)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

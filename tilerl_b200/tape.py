@@ -713,18 +713,24 @@ def _loss_inputs(what: str, logits, targets, mask, **floats):
     return ready
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def _record_loss(tape: "Tape", name: str, logits, loss, grad, K) -> None:
     if grad is None:
         return
     if grad.shape != logits.shape:
         grad = grad.view(logits.shape)
+    captured = _capturing(logits)
 
     def bwd(g):
+        if not captured and _capturing(grad):
+            raise RuntimeError(f"{name}: its backward pass is captured with the forward pass, which forms the gradient; that of a loss formed before goes with the tape")
         if g is _ONE:
             return (grad,)
         if K is not None and g.numel() == 1 and g.device == grad.device:
-            # in place, but not where the pass is captured: each replay would multiply what the one before left
-            return (grad * g.reshape(()) if torch.cuda.is_current_stream_capturing() else K.scale_grad(grad, g),)
+            return (K.scale_grad(grad, g),)
         return (grad * g,)
 
     bwd.takes_one = True
@@ -743,7 +749,8 @@ def policy_loss(tape: Tape, logits: torch.Tensor, targets: torch.Tensor, advanta
     ``advantages`` too, or one value for each of the first dimension.  ``clip_eps_high`` defaults to ``clip_eps``; ``scale`` is mostly one over the
     number of scored tokens of the whole batch.  A reference with ``kl_coef`` 0 is measured only.  An advantage of 0 contributes nothing.
 
-    The logits' gradient has their type (fp32, bf16) and is formed here, so they may be written into afterwards.  Rows that are not scored get zeros, whatever
+    The logits' gradient has their type (fp32, bf16) and is formed here, so they may be written into afterwards, and a backward pass is captured into a graph
+    together with this or not at all.  Rows that are not scored get zeros, whatever
     their logits (NaN among them) and targets are.  A target outside of the vocabulary in a scored row makes the loss and the row's gradient NaN and
     sets the device's error word (not where torch forms the loss: logits in fp16 or fp64); on the CPU it is an error."""
     if clip_eps < 0 or (clip_eps_high is not None and clip_eps_high < 0) or not math.isfinite(scale) or not math.isfinite(kl_coef):
