@@ -1,0 +1,40 @@
+// What the kernels of 8-bit integer projections share: the arithmetic of a row's integers and the order in which a row's squares are
+// added up, so that a row has the same integers and the same scale, bit for bit, in whichever kernel it is quantised.
+#pragma once
+#include "common.cuh"
+
+namespace {
+
+constexpr float I8_MOST = 127.f;          // of activations and weights
+constexpr float I16_MOST = 32512.f;       // of gradients, two digits of 8 bits: 127 * 256
+constexpr float I8_LEAST = 0x1p-110f;     // rows whose largest magnitude is below count as zeros: (1 / m) * 32512 is finite above
+
+// What a row's values are multiplied with; 0 for a row of zeros, one with an infinity or NaN too.  Magnitudes are compared as the integers
+// that their bits are, in which a NaN is the largest.
+__device__ __forceinline__ float i8_factor(uint32_t most_bits, float most_int) {
+  const float m = __uint_as_float(most_bits);
+  return most_bits >= 0x7f800000u || m < I8_LEAST ? 0.f : __fmul_rn(__frcp_rn(m), most_int);
+}
+// The row's scale (before a norm's factor).  `part` is 1 / most_int rounded to fp32.
+__device__ __forceinline__ float i8_scale(uint32_t most_bits, float part) {
+  const float m = __uint_as_float(most_bits);
+  return most_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : m < I8_LEAST ? 0.f : __fmul_rn(m, part);
+}
+__device__ __forceinline__ uint32_t i8_abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// (A row with an infinity has the factor 0, and 0 times it is NaN: rounds to 0.)
+__device__ __forceinline__ int i8_round(float t, float factor) { return __float2int_rn(__fmul_rn(t, factor)); }
+__device__ __forceinline__ uint32_t i8_pack(int a, int b, int c, int d) {
+  return __byte_perm(__byte_perm((uint32_t)a, (uint32_t)b, 0x0040), __byte_perm((uint32_t)c, (uint32_t)d, 0x0040), 0x5410);
+}
+
+// Order of a row's squares: vectors of eight values one after the other; the 32 vectors of a group of 256 values by halving (xor 16, 8, 4,
+// 2, 1); then the groups, of which lane l of a warp adds l, l + 32, ... in that order before the lanes are halved again.
+constexpr int I8_GROUP = 256;
+__device__ __forceinline__ float i8_groups_sum(const float* groups, int n) {
+  float s = 0.f;
+  for (int g = threadIdx.x & 31; g < n; g += 32) s += groups[g];
+  return warp_sum(s);
+}
+__device__ __forceinline__ uint32_t i8_warp_most(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+}  // namespace

@@ -1,0 +1,247 @@
+"""Projections in 8-bit integers on the CPU: the format, the reference backend, the tape's op, checkpoints, shards, refusals."""
+import dataclasses
+import json
+
+import pytest
+import torch
+
+from tilerl_b200 import formats as F
+from tilerl_b200 import tape as T
+from tilerl_b200.config import get_config
+from tilerl_b200.models.hybrid import HybridModel, linear_names, random_master
+from tilerl_b200.ops import ref
+from tilerl_b200.ops.backend import RefOps
+
+
+def _rows(t, k, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, k, generator=g)
+    x[:, ::13] *= 9.0
+    return x
+
+
+def test_integers_are_the_nearest_and_the_largest_is_127():
+    w = _rows(7, 48)
+    w[3] = 0.0
+    q = F.quantize_int8(w)
+    assert q.w8.dtype == torch.int8 and q.wscale.dtype == torch.float32 and q.shape == (7, 48)
+    amax = w.abs().amax(-1)
+    assert torch.equal(q.w8.abs().amax(-1)[amax > 0], torch.full((6,), 127, dtype=torch.int8))
+    # half a step, and the rounding of the quotient, the product and the scale (three halves of 2^-23 at 127 steps)
+    step = amax.double() / 127
+    assert ((q.dequant().double() - w.double()).abs() <= (step * (0.5 + 127 * 6 * 2.0 ** -24))[:, None]).all()
+    assert q.wscale[3] == 0 and not q.w8[3].any()
+    assert F.nbytes("int8", (7, 48)) == q.nbytes() == 7 * 48 + 28
+    again = F.quantize_int8(q.dequant())
+    assert torch.equal(again.w8, q.w8)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_rows_with_an_infinity_or_nan_are_nan_as_a_whole(bad):
+    x = _rows(3, 32)
+    x[1, 5] = bad
+    q, s = F.quantize_act_int8(x)
+    assert torch.isnan(s[1]) and torch.isfinite(s[[0, 2]]).all() and not q[1].any()
+    y = ref.linear_int8(x, F.quantize_int8(_rows(5, 32, 1)))
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[[0, 2]]).all()
+
+
+def test_the_norms_factor_goes_into_the_scale_alone():
+    x, w = _rows(5, 64), torch.rand(64) + 0.5
+    q, s = F.quantize_act_int8(x, w, 1e-6)
+    plain, _ = F.quantize_act_int8(x * w)
+    assert torch.equal(q, plain)
+    h = ref.rmsnorm(x, w, 1e-6)
+    assert ((q.double() * s.double()[:, None] - h.double()).abs() <= h.abs().amax(-1, keepdim=True).double() / 127 * 0.501).all()
+
+
+def test_products_in_16_bits_of_a_gradient():
+    g = torch.Generator().manual_seed(3)
+    up, w = torch.randn(4, 30, generator=g), F.quantize_int8(_rows(30, 16, 4))
+    up[2] = 0.0
+    q, s = F.quantize_grad_int16(up, w.wscale)
+    assert int(q.abs().max()) == 32512
+    u = up.double() * w.wscale.double()
+    assert ((q.double() * s.double()[:, None] - u).abs() <= (u.abs().amax(-1) / 32512 * (0.5 + 32512 * 8 * 2.0 ** -24))[:, None]).all()
+    # digits of 8 bits put together again
+    hi = (q + 128) >> 8
+    assert int(hi.abs().max()) <= 127 and int((q - 256 * hi).max()) <= 127 and int((q - 256 * hi).min()) >= -128
+    want = u @ w.w8.double()
+    off = (u.abs().amax(-1, keepdim=True) / 32512 * 0.51) * w.w8.double().abs().sum(0)
+    assert ((ref.linear_int8_grad(up, w).double() - want).abs() <= off + want.abs() * 2.0 ** -20).all()
+
+
+def test_tape_gradient_against_the_formula_and_differences():
+    """On rows that lie on the grid the product is linear, so differences over whole steps are the gradient."""
+    w = F.quantize_int8(_rows(12, 32, 5))
+    g = torch.Generator().manual_seed(6)
+    x = torch.randint(-90, 90, (2, 3, 32), generator=g).float()
+    x[..., 7] = 127.0                                # the largest stays where it is
+    up = torch.randn(2, 3, 12, generator=g)
+    tape = T.Tape()
+    tape.watch(x)
+    out = T.linear(tape, x, w, frozen=True)
+    assert out.shape == (2, 3, 12) and out.dtype == torch.float32
+    dx = tape.backward(out, up)[id(x)]
+    want = up.double() @ w.dequant().double()
+    # half a 16-bit step of u for each channel
+    off = ((up * w.wscale).double().abs().amax(-1, keepdim=True) / 32512 * 0.51) * w.w8.double().abs().sum(0) + want.abs() * 2.0 ** -20
+    assert ((dx.double() - want).abs() <= off).all()
+    for at in ((0, 0, 0), (1, 2, 31), (0, 1, 8)):
+        hi, lo = x.clone(), x.clone()
+        hi[at] += 5
+        lo[at] -= 5
+        diff = ((T.linear(T.Tape(), hi, w).double() - T.linear(T.Tape(), lo, w).double()) * up.double()).sum() / 10
+        scale = (T.linear(T.Tape(), hi, w).double().abs() * up.double().abs()).sum() / 10
+        assert abs(float(diff - dx[at])) <= float(off[at] + scale * 8 * 2.0 ** -23)
+
+
+def test_adapters_over_integers():
+    w, a, b = F.quantize_int8(_rows(8, 16, 7)), torch.randn(4, 16), torch.randn(8, 4)
+    x, up = _rows(3, 16, 8), torch.randn(3, 8)
+    tape = T.Tape()
+    tape.watch(x, a, b)
+    y = T.linear_lora(tape, x, w, True, a, b, 0.5)
+    assert torch.allclose(y, ref.linear_int8(x, w) + x @ a.t() @ b.t() * 0.5, rtol=1e-5, atol=1e-5)
+    grads = tape.backward(y, up)
+    assert torch.allclose(grads[id(x)], ref.linear_int8_grad(up, w) + up @ b @ a * 0.5, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("lead", [(), (0,), (2, 0)])
+def test_rows_without_tokens_and_one_row(lead):
+    w = F.quantize_int8(_rows(6, 16, 9))
+    x = torch.randn(*lead, 16)
+    tape = T.Tape()
+    tape.watch(x)
+    y = T.linear(tape, x, w)
+    assert y.shape == (*lead, 6)
+    assert tape.backward(y, torch.randn(*lead, 6))[id(x)].shape == x.shape
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="int8"):
+        F.INT8Tensor(torch.zeros(4, 16), torch.zeros(4))
+    with pytest.raises(ValueError, match="scales"):
+        F.INT8Tensor(torch.zeros(4, 16, dtype=torch.int8), torch.zeros(3))
+    with pytest.raises(ValueError, match=r"\[N, K\]"):
+        F.quantize_int8(torch.zeros(4))
+    from tilerl_b200.ops import gemm_int8
+    w = F.quantize_int8(_rows(4, 16))
+    assert not gemm_int8.takes(w)                    # (kernels read weights on a GPU)
+    with pytest.raises(ValueError, match="INT8 products"):
+        gemm_int8.linear(None, torch.zeros(2, 16), w, torch.zeros(2, 4))
+    with pytest.raises(ValueError, match="quantize_"):
+        gemm_int8.quantize_(torch.zeros(4, 16), w)
+
+
+def _tiny(name="tiny"):
+    return dataclasses.replace(get_config(name), quant="int8")
+
+
+def test_reference_backend_serves_and_the_training_forward_gives_the_same_projection():
+    cfg = _tiny()
+    m = HybridModel.build_random(cfg, keep_master=False)
+    assert all(isinstance(m.params[n], F.INT8Tensor) for n in linear_names(cfg))
+    assert m.served_bytes() == sum(v.nbytes() if hasattr(v, "w8") else v.numel() * v.element_size() for v in m.params.values())
+    ops = RefOps()
+    w, nw = m.params["L0.qkv"], m.params["L0.norm1"] * 1.3
+    x = _rows(5, cfg.hidden, 10)
+    y = ops.norm_linear(x, nw, w, cfg.rms_eps)
+    # the tape norms first: the same integers but where rounding puts a value on the other side of a half
+    h = ref.rmsnorm(x, nw, cfg.rms_eps)
+    z = T.linear(T.Tape(), h, w)
+    step = h.abs().amax(-1, keepdim=True) / 127 * w.dequant().abs().amax(-1)
+    assert ((y - z).abs() <= step * 3 + z.abs() * 1e-6).all()
+    act = ops.norm_linear_swiglu(x, nw, m.params["L0.gate_up"], cfg.rms_eps)
+    gu = ref.linear_int8(x, m.params["L0.gate_up"], nw, cfg.rms_eps)
+    assert torch.equal(act, ref.swiglu(gu))
+
+
+def test_training_model_has_gradients_and_requantises():
+    cfg = _tiny()
+    m = HybridModel.build_random(cfg, keep_master=True)
+    before = m.params["L0.o"].w8.clone()
+    m.params["master.L0.o"].mul_(-1)
+    m.requantize_()
+    assert torch.equal(m.params["L0.o"].w8, -before)
+    lora = HybridModel.build_random(cfg)
+    lora.add_lora(4)
+    tape = T.Tape()
+    tape.watch(*lora.trainable().values())
+    y = lora.forward_dense(tape, torch.randint(0, cfg.vocab, (1, 9)))
+    assert len(tape.backward(y)) == len(lora.trainable())
+
+
+@pytest.mark.parametrize("leaf", ["L0.qkv", "L0.o", "L0.gate_up", "L0.down"])
+def test_shards_hold_the_integers_of_the_whole(leaf):
+    from tilerl_b200.parallel.mesh import shard_param
+    cfg = _tiny()
+    full = F.quantize_int8(random_master(cfg)[leaf])
+    parts = [shard_param(cfg, leaf, full, r, 2) for r in range(2)]
+    dense = [shard_param(cfg, leaf, full.dequant(), r, 2) for r in range(2)]
+    for p, d in zip(parts, dense):
+        assert isinstance(p, F.INT8Tensor) and torch.equal(p.dequant(), d) and p.w8.is_contiguous()
+
+
+def test_checkpoints_keep_the_integers(tmp_path):
+    from tilerl_b200.checkpoint import load_checkpoint, save_checkpoint
+    cfg = _tiny()
+    m = HybridModel.build_random(cfg)
+    save_checkpoint(m, str(tmp_path))
+    assert json.load(open(tmp_path / "config.json"))["quant"] == "int8"
+    again = load_checkpoint(cfg, str(tmp_path))
+    for n in linear_names(cfg):
+        assert torch.equal(again.params[n].w8, m.params[n].w8) and torch.equal(again.params[n].wscale, m.params[n].wscale)
+
+
+@pytest.mark.parametrize("scales", ["rows", "column", "one"])
+def test_int8_files_are_taken_as_they_are(tmp_path, scales):
+    """Projections of an exported file with its own scales: adopted by a model served in this format, decoded for any other."""
+    from safetensors.torch import save_file
+    from test_checkpoint import _hf_tensors
+    from tilerl_b200.checkpoint import CheckpointError, load_checkpoint
+    cfg = _tiny("tiny-hybrid")
+    tensors = _hf_tensors(cfg, random_master(cfg, seed=3), "bf16")
+    fn = str(tmp_path / "model.safetensors")
+    g = torch.Generator().manual_seed(2)
+    for k in [k for k in tensors if k.endswith("down_proj.weight") or k.endswith("gate_proj.weight") or k.endswith("up_proj.weight")]:
+        n, kk = tensors[k].shape
+        tensors[k] = torch.randint(-100, 100, (n, kk), generator=g, dtype=torch.int8)       # (no row reaches 127)
+        s = torch.rand(n, generator=g) * 1e-3
+        tensors[k + "_scale"] = {"rows": s, "column": s[:, None].contiguous(), "one": s[:1]}[scales]
+    save_file(tensors, fn)
+    m = load_checkpoint(cfg, str(tmp_path))
+    down = next(k for k in tensors if k.endswith("layers.0.mlp.down_proj.weight"))
+    assert torch.equal(m.params["L0.down"].w8, tensors[down])
+    assert torch.equal(m.params["L0.down"].wscale, tensors[down + "_scale"].reshape(-1).expand(tensors[down].shape[0]))
+    gate = down.replace("down", "gate")
+    assert torch.equal(m.params["L0.gate_up"].w8[0::2], tensors[gate])
+    dense = load_checkpoint(dataclasses.replace(cfg, quant="bf16"), str(tmp_path))
+    assert torch.equal(dense.params["L0.down"].float(), m.params["L0.down"].dequant())
+    del tensors[down + "_scale"]
+    save_file(tensors, fn)
+    with pytest.raises(CheckpointError, match="weight_scale"):
+        load_checkpoint(cfg, str(tmp_path))
+
+
+def test_resync_writes_integers():
+    from tilerl_b200.parallel.resync import _store
+    dst, src = F.quantize_int8(_rows(4, 16, 1)), F.quantize_int8(_rows(4, 16, 2))
+    at = dst.w8.data_ptr()
+    assert _store(dst, src) == 4 * 16 + 16 and torch.equal(dst.w8, src.w8) and torch.equal(dst.wscale, src.wscale) and dst.w8.data_ptr() == at
+
+
+def test_a_run_of_them_together():
+    """Prompt and decode ticks through the engine choose what the training forward over the same tokens finds largest: the rollout's
+    projections are the trainer's."""
+    from helpers import make_engine
+    from tilerl_b200.engine import SamplingParams
+    cfg = _tiny()
+    eng = make_engine(cfg)
+    prompt = [5, 17, 200, 31, 9, 77]
+    got = eng.generate([prompt], SamplingParams(max_tokens=8, temperature=0.0))[0]
+    tokens = list(getattr(got, "tokens", got))[-8:]
+    logits = eng.model.forward_dense(T.Tape(), torch.tensor([prompt + tokens]))[0]
+    for i, t in enumerate(tokens):
+        row = logits[len(prompt) - 1 + i]
+        assert float(row.max() - row[t]) <= 0.02 * float(row.std()), (i, t)

@@ -10,9 +10,11 @@ parameter dict (TP-sharded if asked):
 * official NVFP4 files: ``.weight`` uint8 + ``.weight_scale`` + ``.weight_scale_2``;
 * FP8 128x128-block files: ``.weight`` e4m3 + ``.weight_scale_inv``; FP8 per-tensor / per-channel:
   ``.weight`` e4m3 + ``.weight_scale``;
+* 8-bit integers per channel: ``.weight`` int8 + ``.weight_scale`` ``[N]``, ``[N, 1]`` or one for all; a model
+  served in this format (``quant="int8"``) takes them as they are;
 * MLX 4-bit: ``.weight`` uint32 (8 nibbles, low first) + ``.scales`` + ``.biases`` per group of 64;
 * AWQ: ``.qweight`` int32 ``[K, N/8]`` (AWQ nibble order) + ``.qzeros`` + ``.scales`` per group;
-* this framework's own dialect: ``<name>.wq / .scale / .tscale``.
+* this framework's own dialect: ``<name>.wq / .scale / .tscale`` (NVFP4), ``<name>.w8 / .wscale`` (8-bit integers).
 
 HF tensor names are mapped onto the fused layouts used here (gate/query interleave for
 ``qkv``, ``[q;k;v;z;a;b]`` for the GDN input projection, interleaved ``gate_up``).  RMSNorm
@@ -38,7 +40,7 @@ from typing import Dict, Optional
 import torch
 
 from .config import ATTN, DeluvikConfig, FetotarConfig, ModelConfig, StreamDesign, TobadraConfig, ZinutarConfig
-from .formats import (FP8BlockTensor, NVFP4Tensor, dequantize_fp8_block, dequantize_nvfp4,
+from .formats import (FP8BlockTensor, INT8Tensor, NVFP4Tensor, dequantize_fp8_block, dequantize_nvfp4,
                       quantize_nvfp4)
 from .models.hybrid import HybridModel, linear_names, quantize_weight
 from .models.deluvik import DeluvikModel
@@ -190,7 +192,29 @@ class _Reader:
                 s = self.get(base + ".weight_scale").float()
                 return w.float() * (s if s.numel() == 1 else s.reshape(-1, 1))
             return w.float()
+        if w.dtype == torch.int8:
+            return self._int8(base, w).dequant()
         return w.float()
+
+    def _int8(self, base: str, w: torch.Tensor) -> INT8Tensor:
+        if not self.has(base + ".weight_scale"):
+            raise CheckpointError(f"{base}: int8 weight without .weight_scale")
+        s = self.get(base + ".weight_scale").float().reshape(-1)
+        if w.dim() != 2 or s.numel() not in (1, w.shape[0]) or self.has(base + ".weight_zero_point") and bool(self.get(base + ".weight_zero_point").any()):
+            raise CheckpointError(f"{base}: int8 weights have a scale per row or one for all and no zero points, got {tuple(w.shape)} with {s.numel()} scales")
+        return INT8Tensor(w, s.expand(w.shape[0]).contiguous())
+
+    def linear(self, base: str, quant: str):
+        """A projection for a model served as ``quant``: its own integers where they are that, else its dense value."""
+        if quant == "int8" and self.has(base + ".weight") and not self.has(base + ".wq"):
+            w = self.get(base + ".weight")
+            if w.dtype == torch.int8:
+                return self._int8(base, w)
+        return self.dense(base)
+
+    def int8(self, base: str) -> Optional[INT8Tensor]:
+        """Integers of the own dialect."""
+        return INT8Tensor(self.get(base + ".w8"), self.get(base + ".wscale").float()) if self.has(base + ".w8") else None
 
     def nvfp4(self, base: str) -> Optional[NVFP4Tensor]:
         """The stored NVFP4 planes when the file already holds them (no requantisation)."""
@@ -208,13 +232,24 @@ def _hf_prefix(reader: _Reader) -> str:
     return ""
 
 
-def _interleave_rows(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+def _interleave_rows(a, b):
+    if isinstance(a, INT8Tensor) and isinstance(b, INT8Tensor):
+        return INT8Tensor(_interleave_rows(a.w8, b.w8), _interleave_rows(a.wscale, b.wscale))
+    a, b = (t.dequant() if isinstance(t, INT8Tensor) else t for t in (a, b))
     return torch.stack([a, b], dim=1).reshape(a.shape[0] * 2, *a.shape[1:])
+
+
+def _cat_rows(*parts):
+    """Projections that share their input, one below the other; integers stay what they are if all parts are."""
+    if all(isinstance(t, INT8Tensor) for t in parts):
+        return INT8Tensor(torch.cat([t.w8 for t in parts]), torch.cat([t.wscale for t in parts]))
+    return torch.cat([t.dequant() if isinstance(t, INT8Tensor) else t for t in parts])
 
 
 def assemble_master(cfg: ModelConfig, reader: _Reader) -> Dict[str, torch.Tensor]:
     """HF tensors -> full (TP=1) master dict in this framework's fused layouts."""
     p = _hf_prefix(reader)
+    lin = lambda base: reader.linear(base, cfg.quant)
     own = reader.has("embed") or reader.has("embed.weight")
     out: Dict[str, torch.Tensor] = {}
 
@@ -239,24 +274,22 @@ def assemble_master(cfg: ModelConfig, reader: _Reader) -> Dict[str, torch.Tensor
         if t == ATTN:
             a = L + "self_attn."
             # HF q_proj rows are already [query(D); gate(D)] per head when gated
-            out[q + "qkv"] = torch.cat([reader.dense(a + "q_proj"), reader.dense(a + "k_proj"),
-                                        reader.dense(a + "v_proj")])
-            out[q + "o"] = reader.dense(a + "o_proj")
+            out[q + "qkv"] = _cat_rows(lin(a + "q_proj"), lin(a + "k_proj"), lin(a + "v_proj"))
+            out[q + "o"] = lin(a + "o_proj")
             out[q + "q_norm"] = norm(a + "q_norm.weight")
             out[q + "k_norm"] = norm(a + "k_norm.weight")
         else:
             g = L + "linear_attn."
-            out[q + "in"] = torch.cat([reader.dense(g + "in_proj_qkv"), reader.dense(g + "in_proj_z"),
-                                       reader.dense(g + "in_proj_a"), reader.dense(g + "in_proj_b")])
-            out[q + "out"] = reader.dense(g + "out_proj")
+            out[q + "in"] = _cat_rows(lin(g + "in_proj_qkv"), lin(g + "in_proj_z"), lin(g + "in_proj_a"), lin(g + "in_proj_b"))
+            out[q + "out"] = lin(g + "out_proj")
             conv = reader.get(g + "conv1d.weight").float()
             out[q + "conv"] = conv.reshape(conv.shape[0], -1)
             out[q + "dt_bias"] = reader.get(g + "dt_bias").float()
             out[q + "a_log"] = reader.get(g + "A_log").float()
             out[q + "gdn_norm"] = reader.get(g + "norm.weight").float()
         m = L + "mlp."
-        out[q + "gate_up"] = _interleave_rows(reader.dense(m + "gate_proj"), reader.dense(m + "up_proj"))
-        out[q + "down"] = reader.dense(m + "down_proj")
+        out[q + "gate_up"] = _interleave_rows(lin(m + "gate_proj"), lin(m + "up_proj"))
+        out[q + "down"] = lin(m + "down_proj")
     return out
 
 
@@ -307,14 +340,14 @@ def load_checkpoint(cfg: ModelConfig, path: str, *, device="cpu", tp_rank: int =
 
 
 def _load_own(cfg, reader: _Reader, device, tp_rank, tp, keep_master) -> HybridModel:
-    """Own dialect: NVFP4 planes are adopted bit for bit (no requantisation)."""
+    """Own dialect: NVFP4 planes and 8-bit integers are adopted bit for bit (no requantisation)."""
     from .parallel.mesh import shard_param
     params: Dict[str, object] = {}
     lin = set(linear_names(cfg))
-    names = {k.rsplit(".", 1)[0] if k.endswith((".wq", ".scale", ".tscale")) else k for k in reader.index}
+    names = {k.rsplit(".", 1)[0] if k.endswith((".wq", ".scale", ".tscale", ".w8", ".wscale")) else k for k in reader.index}
     act = torch.bfloat16 if torch.device(device).type == "cuda" else torch.float32
     for name in sorted(names):
-        q = reader.nvfp4(name)
+        q = reader.nvfp4(name) or reader.int8(name)
         if q is not None:
             v = shard_param(cfg, name, q, tp_rank, tp).to(device)
         else:
@@ -346,6 +379,8 @@ def save_checkpoint(model: HybridModel, path: str) -> None:
             tensors[k + ".wq"] = v.wq.cpu().contiguous()
             tensors[k + ".scale"] = v.scale.view(torch.uint8).cpu().contiguous()
             tensors[k + ".tscale"] = v.tscale.cpu().contiguous()
+        elif isinstance(v, INT8Tensor):
+            tensors[k + ".w8"], tensors[k + ".wscale"] = v.w8.cpu().contiguous(), v.wscale.cpu().contiguous()
         elif isinstance(v, FP8BlockTensor):
             tensors[k] = v.dequant().to(torch.bfloat16).cpu().contiguous()
         else:

@@ -53,7 +53,7 @@ class ModelConfig:
     rms_eps: float = 1e-6
     max_ctx: int = 262144
     tie_embeddings: bool = False
-    quant: str = "nvfp4"  # "nvfp4" | "fp8" | "bf16": format of the served linears
+    quant: str = "nvfp4"  # "nvfp4" | "fp8" | "int8" | "bf16": format of the served linears
     lm_head_quant: str = "bf16"
 
     def __post_init__(self) -> None:

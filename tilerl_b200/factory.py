@@ -22,7 +22,7 @@ import torch
 
 from .config import DeluvikConfig, FetotarConfig, ModelConfig, StreamDesign, TobadraConfig, ZinutarConfig, get_config
 from .engine import Engine, StepLimits
-from .formats import NVFP4Tensor
+from .formats import INT8Tensor, NVFP4Tensor
 from .kv import NoPrefixStore, PrefixStore, kv_pages, make_kv_pool, make_state_pool
 from .models.deluvik import DeluvikModel
 from .models.fetotar import FetotarModel
@@ -77,8 +77,12 @@ def build_random_streaming(cfg: ModelConfig, device, seed: int = 0, tp_rank: int
                                 torch.empty(1, dtype=torch.float32, device=device))
                 ops.quantize_nvfp4_(full.contiguous(), q)
                 params[name] = shard_param(cfg, name, q, tp_rank, tp)
-            elif cfg.quant == "nvfp4":
-                params[name] = shard_param(cfg, name, quantize_weight(full.float(), "nvfp4"), tp_rank, tp)
+            elif cfg.quant == "int8" and name in lin and device.type == "cuda" and ops is not None:
+                q = INT8Tensor(torch.empty(full.shape, dtype=torch.int8, device=device), torch.empty(full.shape[0], dtype=torch.float32, device=device))
+                ops.quantize_int8_(full, q)
+                params[name] = shard_param(cfg, name, q, tp_rank, tp)
+            elif cfg.quant in ("nvfp4", "int8"):
+                params[name] = shard_param(cfg, name, quantize_weight(full.float(), cfg.quant if name in lin else "nvfp4"), tp_rank, tp)
             else:
                 params[name] = quantize_weight(w.float(), cfg.quant)
             if keep_master:

@@ -1,5 +1,6 @@
-"""Numeric formats: NVFP4 (e2m1 + e4m3 block scales + fp32 tensor scale) and
-block-scaled FP8, as torch reference code plus a byte-accounting registry.
+"""Numeric formats: NVFP4 (e2m1 + e4m3 block scales + fp32 tensor scale),
+block-scaled FP8 and 8-bit integers with a scale per row, as torch reference code plus a
+byte-accounting registry.
 
 The packed layouts here are exactly what the CUDA kernels consume:
 
@@ -207,21 +208,98 @@ def quantize_kv_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return (x.float() / s.unsqueeze(-1)).to(torch.float8_e4m3fn), s
 
 
+# ---- 8-bit integers ------------------------------------------------------------
+INT8_MAX = 127.0
+INT16_MAX = 32512.0                 # of rows in two 8-bit digits: 127 * 256
+INT8_LEAST = 2.0 ** -110            # rows whose largest magnitude is below are zeros: (1 / m) times 32512 stays finite above
+
+
+@dataclass
+class INT8Tensor:
+    """int8 weight ``[N, K]`` with one fp32 scale per row (output channel).  Products with it take their other operand in 8-bit
+    integers too, with a scale per token: the sums are of integers, exact, and the same whatever else is in the batch."""
+    w8: torch.Tensor      # int8 [N, K]
+    wscale: torch.Tensor  # fp32 [N]
+
+    def __post_init__(self):
+        if self.w8.dim() != 2 or self.w8.dtype != torch.int8 or self.wscale.dtype != torch.float32 or self.wscale.shape != self.w8.shape[:1]:
+            raise ValueError(f"INT8 weights are int8 [N, K] with fp32 scales [N], got {tuple(self.w8.shape)} {self.w8.dtype} and "
+                             f"{tuple(self.wscale.shape)} {self.wscale.dtype}")
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return tuple(self.w8.shape)
+
+    def nbytes(self) -> int:
+        return self.w8.numel() + self.wscale.numel() * 4
+
+    def to(self, device) -> "INT8Tensor":
+        return INT8Tensor(self.w8.to(device), self.wscale.to(device))
+
+    def dequant(self) -> torch.Tensor:
+        return dequantize_int8(self)
+
+
+def _row_integers(t: torch.Tensor, most_int: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows -> (integers up to ``most_int``, still fp32; scale per row).  ``q = rint(t * ((1 / m) * most))`` and
+    ``scale = m * (1 / most)`` with every quotient and product rounded to fp32, so that kernels give the same integers.  A row with an
+    infinity or NaN has the scale NaN."""
+    if not t.shape[-1]:
+        return t, t.new_zeros(t.shape[:-1])
+    most = t.abs().amax(-1, keepdim=True)
+    fine = torch.isfinite(most) & (most >= INT8_LEAST)
+    q = torch.where(fine, torch.round(t * (torch.where(fine, most, 1.0).reciprocal() * most_int)), 0.0)
+    part = torch.tensor(1.0 / most_int, dtype=torch.float32, device=t.device)
+    scale = torch.where(torch.isfinite(most), torch.where(fine, most * part, 0.0), float("nan"))
+    return q, scale[..., 0]
+
+
+def quantize_int8(w: torch.Tensor) -> INT8Tensor:
+    """``[N, K]`` -> int8, every row's largest magnitude at 127."""
+    if w.dim() != 2:
+        raise ValueError(f"INT8 needs [N, K], got {tuple(w.shape)}")
+    q, s = _row_integers(w.float(), INT8_MAX)
+    return INT8Tensor(q.to(torch.int8), s.contiguous())
+
+
+def dequantize_int8(t: INT8Tensor) -> torch.Tensor:
+    return t.w8.float() * t.wscale[:, None]
+
+
+def quantize_act_int8(x: torch.Tensor, norm_w: torch.Tensor | None = None, eps: float = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``[..., K]`` -> (int8, fp32 scale per row), of ``rmsnorm(x) * norm_w`` where a norm is given.  The norm's factor of a row is
+    the same for all of it, so it goes into the scale alone: the integers are those of ``x * norm_w``."""
+    xf = x.float()
+    q, s = _row_integers(xf if norm_w is None else xf * norm_w.float(), INT8_MAX)
+    if norm_w is not None:
+        s = s * torch.rsqrt(xf.pow(2).mean(-1) + eps)
+    return q.to(torch.int8), s
+
+
+def quantize_grad_int16(g: torch.Tensor, wscale: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows of an output's gradient times the channels' scales, in 16 bits: (int32 ``[..., N]`` up to 32512, fp32 scale per row).  8 bits,
+    as for activations, would lose what is below 1/254 of a row's largest gradient; 16 bits keep down to 1/65024, and go through the tensor
+    cores as two digits of 8 bits."""
+    q, s = _row_integers(g.float() * wscale.float(), INT16_MAX)
+    return q.to(torch.int32), s
+
+
 # ---- byte accounting ------------------------------------------------------------
 @dataclass(frozen=True)
 class Format:
     """Prices a tensor: ``bits`` per element plus scale planes given as
-    (elements-per-scale, bytes-per-scale)."""
+    (elements-per-scale, bytes-per-scale), plus ``per_row_bytes`` for every row of the last dimension."""
     name: str
     bits: int
     scales: Tuple[Tuple[int, int], ...] = ()
     per_tensor_bytes: int = 0
+    per_row_bytes: int = 0
 
     def nbytes(self, shape: Iterable[int]) -> int:
-        n = 1
+        n = rows = 1
         for d in shape:
-            n *= int(d)
-        total = (n * self.bits + 7) // 8 + self.per_tensor_bytes
+            n, rows = n * int(d), n
+        total = (n * self.bits + 7) // 8 + self.per_tensor_bytes + rows * self.per_row_bytes
         for per, b in self.scales:
             total += (n + per - 1) // per * b
         return total
@@ -233,6 +311,7 @@ FORMATS: Dict[str, Format] = {
     "nvfp4": Format("nvfp4", 4, ((FP4_BLOCK, 1),), 4),
     "fp8_block": Format("fp8_block", 8, ((FP8_BLOCK * FP8_BLOCK, 4),)),
     "fp8": Format("fp8", 8, (), 4),
+    "int8": Format("int8", 8, per_row_bytes=4),
     "kv_bf16": Format("kv_bf16", 16),
     "kv_fp8": Format("kv_fp8", 8, ((1 << 30, 0),)),
 }
@@ -256,7 +335,7 @@ def weight_specs(cfg) -> Dict[str, Tuple[Tuple[int, ...], str]]:
     if isinstance(cfg, StreamDesign):
         return {n: (s, "bf16" if k == "w" else "f32") for n, (s, k) in cfg.layout.param_shapes(cfg).items()}
     q = cfg.quant
-    lin = {"nvfp4": "nvfp4", "fp8": "fp8_block", "bf16": "bf16"}[q]
+    lin = {"nvfp4": "nvfp4", "fp8": "fp8_block", "int8": "int8", "bf16": "bf16"}[q]
     h = cfg.hidden
     out: Dict[str, Tuple[Tuple[int, ...], str]] = {
         "embed": ((cfg.vocab, h), "bf16"),

@@ -42,7 +42,7 @@ class Row:
 
 
 def _lin_format(cfg: ModelConfig) -> str:
-    return {"nvfp4": "nvfp4", "fp8": "fp8_block", "bf16": "bf16"}[cfg.quant]
+    return {"nvfp4": "nvfp4", "fp8": "fp8_block", "int8": "int8", "bf16": "bf16"}[cfg.quant]
 
 
 def _linear(name: str, count: int, m: int, n: int, k: int, fmt: str, comm: float = 0.0) -> Row:

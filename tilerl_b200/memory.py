@@ -215,7 +215,7 @@ def train_plan(cfg: ModelConfig, *, mode: str = "lora", rank: int = 16, zero: in
     if mode == "lora":
         shapes = []
         for name, (shape, fmt) in weight_specs(cfg).items():
-            if fmt in ("nvfp4", "fp8_block") and len(shape) == 2 and name not in ("lm_head",):
+            if fmt in ("nvfp4", "fp8_block", "int8") and len(shape) == 2 and name not in ("lm_head",):
                 shapes += [(rank, shape[1]), (shape[0], rank)]
         lora = sum(a * b for a, b in shapes)
         rows["adapters (fp32)"] = lora * 4

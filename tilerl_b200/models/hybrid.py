@@ -33,7 +33,7 @@ from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 import torch
 
 from ..config import ATTN, GDN, ModelConfig
-from ..formats import (FP8BlockTensor, NVFP4Tensor, quantize_fp8_block, quantize_nvfp4)
+from ..formats import (FP8BlockTensor, INT8Tensor, NVFP4Tensor, quantize_fp8_block, quantize_int8, quantize_nvfp4)
 
 LINEAR_KEYS_ATTN = ("qkv", "o")
 LINEAR_KEYS_GDN = ("in", "out")
@@ -83,6 +83,8 @@ def quantize_weight(w: torch.Tensor, quant: str):
         return quantize_nvfp4(w)
     if quant == "fp8":
         return quantize_fp8_block(w)
+    if quant == "int8":
+        return quantize_int8(w)
     return w
 
 
@@ -138,11 +140,16 @@ class HybridModel:
             ws = shard_param(cfg, name, w, tp_rank, tp)
             if device is not None:
                 ws = ws.to(device)
-            if name in lin or (name == "lm_head" and cfg.lm_head_quant == "nvfp4"):
-                if quant == "nvfp4" or name == "lm_head":
+            if isinstance(ws, INT8Tensor):            # (a checkpoint's own integers)
+                params[name] = ws
+                if keep_master:
+                    params["master." + name] = ws.dequant()
+            elif name in lin or (name == "lm_head" and cfg.lm_head_quant == "nvfp4"):
+                if quant in ("nvfp4", "int8") or name == "lm_head":
                     # quantise the FULL tensor, then cut the packed planes: every TP degree
                     # serves exactly the same quantised values
-                    q = shard_param(cfg, name, quantize_nvfp4(w.float()), tp_rank, tp)
+                    q = quantize_nvfp4(w.float()) if name == "lm_head" else quantize_weight(w.float(), quant)
+                    q = shard_param(cfg, name, q, tp_rank, tp)
                     params[name] = q.to(device) if device is not None else q
                 else:
                     params[name] = quantize_weight(ws.float(), quant)
@@ -181,7 +188,7 @@ class HybridModel:
             w = self.params[n]
             nn, kk = w.shape
             dev = w.wq.device if isinstance(w, formats.NVFP4Tensor) else (
-                w.w8.device if isinstance(w, formats.FP8BlockTensor) else w.device)
+                w.w8.device if isinstance(w, (formats.FP8BlockTensor, formats.INT8Tensor)) else w.device)
             a = (torch.randn(rank, kk, generator=g) / math.sqrt(rank)).to(dev, dtype)
             b = torch.zeros(nn, rank, dtype=dtype, device=dev)
             self.params[n + ".lora_a"], self.params[n + ".lora_b"] = a, b
@@ -260,7 +267,7 @@ class HybridModel:
             cur = self.params[n]
             if isinstance(cur, NVFP4Tensor):
                 cur.wq.copy_(new.wq), cur.scale.copy_(new.scale), cur.tscale.copy_(new.tscale)
-            elif isinstance(cur, FP8BlockTensor):
+            elif isinstance(cur, (FP8BlockTensor, INT8Tensor)):
                 cur.w8.copy_(new.w8), cur.wscale.copy_(new.wscale)
             else:
                 cur.copy_(new)

@@ -17,6 +17,7 @@ from typing import Optional
 
 import torch
 
+from ..formats import INT8Tensor
 from . import ref
 from .ref_mixers import RefMixers
 
@@ -60,13 +61,15 @@ class RefOps(RefMixers):
             y = y + (x.float() @ a.float().t()) @ b.float().t() * s
         return y
 
-    def norm_linear(self, x, norm_w, w, eps, lora=None):
+    def _norm_linear(self, x, norm_w, w, eps, lora=None):
         h = ref.rmsnorm(x, norm_w, eps)
-        return self._lora(ref.linear(h, w), h, lora).to(self.act_dtype)
+        return self._lora(ref.linear_int8(x, w, norm_w, eps) if isinstance(w, INT8Tensor) else ref.linear(h, w), h, lora)
+
+    def norm_linear(self, x, norm_w, w, eps, lora=None):
+        return self._norm_linear(x, norm_w, w, eps, lora).to(self.act_dtype)
 
     def norm_linear_swiglu(self, x, norm_w, w, eps, lora=None):
-        h = ref.rmsnorm(x, norm_w, eps)
-        return ref.swiglu(self._lora(ref.linear(h, w), h, lora)).to(self.act_dtype)
+        return ref.swiglu(self._norm_linear(x, norm_w, w, eps, lora)).to(self.act_dtype)
 
     def device_alive(self) -> bool:
         return True
@@ -167,8 +170,7 @@ class RefOps(RefMixers):
 
     def lm_head(self, x, norm_w, w, eps):
         """Final norm + vocab(-parallel) head; returns full-vocab fp32 logits."""
-        h = ref.rmsnorm(x, norm_w, eps)
-        return self.all_gather_last(ref.linear(h, w))
+        return self.all_gather_last(self._norm_linear(x, norm_w, w, eps))
 
     def full_logits(self, logits):
         return logits

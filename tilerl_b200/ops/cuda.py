@@ -24,7 +24,7 @@ from typing import Dict, Optional
 
 import torch
 
-from ..formats import FP8BlockTensor, NVFP4Tensor
+from ..formats import FP8BlockTensor, INT8Tensor, NVFP4Tensor
 from . import native as N
 from .cuda_blocks import BlockOps
 from .cuda_gated import GatedOps
@@ -286,6 +286,9 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
         elif isinstance(w, FP8BlockTensor):
             from . import gemm_fp8
             gemm_fp8.gemv(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
+        elif isinstance(w, INT8Tensor):
+            from . import gemm_int8
+            gemm_int8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
         else:
             raise TypeError(f"no GEMV for weight type {type(w)}")
 
@@ -311,6 +314,11 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
             from . import gemm_fp8
             self.settle()
             gemm_fp8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
+            return
+        if isinstance(w, INT8Tensor):
+            from . import gemm_int8
+            self.settle()
+            gemm_int8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
             return
         if (self._tc(w, t) and self.gemv_mma and t <= self.mma_tokens and x.shape[1] <= self.mma_kmax
                 and not self.decode_tc and x.stride(0) % 8 == 0):
@@ -626,7 +634,7 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
             self._gemv(x.contiguous(), w, logits, norm_w=self._f32(norm_w), eps=eps, epi=EPI_STORE_F32)
         else:
             xc = x.contiguous()
-            if (isinstance(w, NVFP4Tensor) and self.use_tc_gemm) or isinstance(w, FP8BlockTensor):
+            if (isinstance(w, NVFP4Tensor) and self.use_tc_gemm) or isinstance(w, (FP8BlockTensor, INT8Tensor)):
                 self._linear(xc, w, logits, norm_w=self._f32(norm_w), eps=eps, epi=EPI_STORE_F32)
             else:
                 h = self._rmsnorm(xc, norm_w, eps, name="h_head")
@@ -764,6 +772,11 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
                           torch.empty(1, dtype=torch.float32, device=self.device))
         self.quantize_nvfp4_(w.contiguous(), dst)
         return dst
+
+    def quantize_int8_(self, w: torch.Tensor, dst: INT8Tensor) -> None:
+        """Re-pack ``w`` (fp32 or bf16 ``[N, K]``) into ``dst`` in place."""
+        from . import gemm_int8
+        gemm_int8.quantize_(w, dst)
 
     def read_device_error(self, clear: bool = True):
         """``(code, a, b, c)`` of the device error word: non-zero code when a bounded wait of a kernel

@@ -1,0 +1,132 @@
+"""Projections over weights in 8-bit integers (``formats.INT8Tensor``): ``csrc/rows_i8.cu``, ``csrc/gemm_i8.cu``.
+
+Served (``linear``, behind the projections of :class:`~tilerl_b200.ops.cuda.CudaOps`): a tick's rows are quantised per token with the
+RMSNorm folded in, multiplied in integers, and leave through the same epilogues as the other formats'.  Trained (``forward`` and
+``grad``, behind ``tape.linear``): the same product of fp32 rows, not rounded, and its input's gradient from rows in 16 bits.
+
+Sums are of integers, so neither the other rows of a batch nor the kernel that is taken for their number change a row's result: a
+token has the same bits in a prompt, in a decode tick and in training.
+
+The reference multiplies in FP8 (``linear_fp8``, packages/tilerl-kernels/src/tilerl_kernels/kernels_linear.py:1442-1813); it has no integer form.
+"""
+from __future__ import annotations
+
+import torch
+
+from ..formats import INT8Tensor
+from . import native as N
+
+EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
+TYPES = {torch.float32: 0, torch.bfloat16: 1}
+MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
+
+N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.P])
+N.register("trl_gemm_i8", [N.P, N.L, N.P, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.I, N.P])
+N.register("trl_gemm_i8_grad", [N.P, N.L, N.P, N.L, N.P, N.P, N.L, N.I, N.I, N.I, N.P])
+
+
+def there() -> bool:
+    """The library has these kernels (one that serves a single architecture has not)."""
+    return N.has("trl_gemm_i8")
+
+
+def takes(w: INT8Tensor) -> bool:
+    """Weights that the kernels read: rows of whole 16-byte pieces, on such a boundary, and sums that 32 bits hold."""
+    n, k = w.shape
+    return (w.w8.is_cuda and w.wscale.device == w.w8.device and w.wscale.is_contiguous() and 0 < k <= MOST and 0 < n <= MOST and k % 16 == 0
+            and w.w8.stride(1) == 1 and w.w8.stride(0) % 16 == 0 and w.w8.stride(0) >= k and w.w8.data_ptr() % 16 == 0)
+
+
+def _refuse(x: torch.Tensor, w: INT8Tensor, y=None, norm_w=None, residual=None, epi=EPI_STORE) -> None:
+    if not takes(w):
+        raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, up to {MOST} rows and columns, on "
+                         f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
+    if x.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype not in TYPES or x.device != w.w8.device or x.stride(1) != 1 and x.shape[1] > 1:
+        raise ValueError(f"INT8 products take fp32 or bf16 rows [T, {w.shape[1]}] on the weight's device, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    t, (n, k) = x.shape[0], w.shape
+    if epi == EPI_SWIGLU and n % 2:
+        raise ValueError(f"SwiGLU takes rows in (gate, up) pairs, got {n}")
+    kind = torch.float32 if epi == EPI_STORE_F32 else torch.bfloat16
+    if tuple(y.shape) != (t, n // 2 if epi == EPI_SWIGLU else n) or y.dtype != kind or y.device != x.device or t and y.stride(1) != 1 and y.shape[1] > 1:
+        raise ValueError(f"the output of {t} rows by {n} channels is {kind} with channels side by side, got {tuple(y.shape)} {y.dtype} on {y.device}")
+    if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and (
+            residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.device != x.device or residual.stride(1) != 1 and n > 1):
+        raise ValueError("a residual is bf16 rows of the output's shape, given where one is added")
+    if norm_w is not None and (norm_w.shape != (k,) or norm_w.dtype != torch.float32 or norm_w.device != x.device or not norm_w.is_contiguous()):
+        raise ValueError(f"a norm's weight is fp32 [{k}] on the rows' device, got {tuple(norm_w.shape)} {norm_w.dtype} on {norm_w.device}")
+
+
+def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None) -> None:
+    """Rows ``x [T, K]`` into ``q`` (int8 ``[T, >= K]``) and ``s`` (fp32 ``[T]``); with ``channels`` (a gradient's scales) into two rows of digits
+    a row of ``x``."""
+    N.check(N.lib().trl_rows_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(channels if norm_w is None else norm_w), int(norm_w is not None), eps,
+                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, N.stream()), "rows_i8")
+    N.count()
+
+
+def _gemm(w, q, s, y, residual, epi) -> None:
+    n, k = w.shape
+    N.check(N.lib().trl_gemm_i8(w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(), q.data_ptr(), q.stride(0), s.data_ptr(), N.ptr(residual),
+                                residual.stride(0) if residual is not None else 0, y.data_ptr(), y.stride(0), q.shape[0], n, k, epi, N.stream()), "gemm_i8")
+    N.count()
+
+
+def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) -> None:
+    """``y = epi(norm(x) @ W^T)``; ``y`` may be the residual."""
+    _refuse(x, w, y, norm_w, residual, epi)
+    t, (n, k) = x.shape[0], w.shape
+    if t == 0:
+        return
+    with N.on(x.device):
+        q, s = ops.ws.get("int8_q", (t, k), torch.int8), ops.ws.get("int8_s", (t,), torch.float32)
+        quant_rows(x, q, s, norm_w=norm_w, eps=eps)
+        _gemm(w, q, s, y, residual, epi)
+
+
+# ---- the training tape ------------------------------------------------------------------------------------
+def train_takes(x: torch.Tensor, w: INT8Tensor) -> bool:
+    """Rows that the kernels take as they are; the torch forms serve the rest."""
+    return x.is_cuda and there() and takes(w) and x.dtype in TYPES and x.device == w.w8.device and x.dim() >= 1 and x.shape[-1] == w.shape[1]
+
+
+def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
+    """``x [..., K]`` -> fp32 ``[..., N]``."""
+    n, k = w.shape
+    rows = x.reshape(-1, k)
+    if rows.stride(1) != 1:
+        rows = rows.contiguous()
+    with N.on(x.device):
+        out = torch.empty(*x.shape[:-1], n, dtype=torch.float32, device=x.device)
+        if rows.shape[0]:
+            q, s = torch.empty(rows.shape, dtype=torch.int8, device=x.device), torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
+            quant_rows(rows, q, s)
+            _gemm(w, q, s, out.view(-1, n), None, EPI_STORE_F32)
+    return out
+
+
+def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
+    """Gradient of ``forward``'s input, the rounding of ``x`` taken for none: ``g [..., N]`` -> fp32 ``[..., K]``."""
+    n, k = w.shape
+    rows = (g if g.dtype in TYPES else g.float()).reshape(-1, n)
+    if rows.stride(1) != 1:
+        rows = rows.contiguous()
+    t = rows.shape[0]
+    with N.on(g.device):
+        dx = torch.empty(*g.shape[:-1], k, dtype=torch.float32, device=g.device)
+        if t:
+            q, s = torch.empty(2 * t, -(-n // 16) * 16, dtype=torch.int8, device=g.device), torch.empty(t, dtype=torch.float32, device=g.device)
+            quant_rows(rows, q, s, channels=w.wscale)
+            N.check(N.lib().trl_gemm_i8_grad(w.w8.data_ptr(), w.w8.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), dx.data_ptr(), k, t, n, k, N.stream()),
+                    "gemm_i8_grad")
+            N.count()
+    return dx
+
+
+# ---- weights ---------------------------------------------------------------------------------------------------
+def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
+    """fp32 or bf16 ``[N, K]`` into ``dst`` in place, as ``formats.quantize_int8`` gives it."""
+    if not takes(dst) or src.shape != dst.w8.shape or src.dtype not in TYPES or src.device != dst.w8.device:
+        raise ValueError(f"quantize_ takes fp32 or bf16 of {dst.shape} on the weight's device, got {tuple(src.shape)} {src.dtype} on {src.device}")
+    src = src if src.stride(1) == 1 else src.contiguous()
+    with N.on(src.device):
+        quant_rows(src, dst.w8, dst.wscale)

@@ -29,6 +29,8 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from ..formats import INT8Tensor, quantize_act_int8, quantize_grad_int16
+
 KV_BLOCK = 16  # tokens per KV page
 
 
@@ -475,8 +477,24 @@ def dequant_weight(w) -> torch.Tensor:
 
 
 def linear(x, w, residual=None):
-    y = _f(x) @ dequant_weight(w).t().to(x.device)
+    if isinstance(w, INT8Tensor):
+        y = linear_int8(x, w)
+    else:
+        y = _f(x) @ dequant_weight(w).t().to(x.device)
     return y if residual is None else y + _f(residual)
+
+
+def linear_int8(x, w, norm_w=None, eps=0.0):
+    """Product of 8-bit integers: rows (of ``rmsnorm(x)`` where a norm is given) quantised per token; exact sums."""
+    q, s = quantize_act_int8(x, norm_w, eps)
+    acc = q.to(torch.float64) @ w.w8.to(x.device, torch.float64).t()
+    return (acc.float() * (s[..., None] * w.wscale.to(x.device)))
+
+
+def linear_int8_grad(g, w):
+    """Gradient of ``linear_int8``'s input, its rounding taken for none, from rows in 16 bits."""
+    q, s = quantize_grad_int16(g, w.wscale.to(g.device))
+    return (q.to(torch.float64) @ w.w8.to(g.device, torch.float64)).float() * s[..., None]
 
 
 # ---- loss / sampling -----------------------------------------------------------------------------

@@ -94,6 +94,8 @@ register("any", "cpu", {op: Kernel(fn, _MIX) for op, fn in {
 register("any", "cpu", {
     "quantize_nvfp4": Kernel("quantize_nvfp4", "tilerl_b200/formats.py"),
     "dequantize_nvfp4": Kernel("dequantize_nvfp4", "tilerl_b200/formats.py"),
+    "quant_int8": Kernel("quantize_act_int8", "tilerl_b200/formats.py"),
+    "linear_int8": Kernel("linear_int8", _REF), "linear_int8_grad": Kernel("linear_int8_grad", _REF),
 })
 
 register("nvfp4", "sm100", {
@@ -134,6 +136,12 @@ register("fp8", "sm100", {
     "paged_attention_decode": Kernel("attn_decode_fp8_kernel / attn_split_fp8_kernel", "csrc/attn_fp8.cu", "trl_attn_paged_fp8",
                                      note="head dim 256 on mma.sync, 64 and 128 on FMAs"),
     "paged_attention_prefill": Kernel("attn_prefill_kernel<true>", "csrc/attn.cu", "trl_attn_prefill_fp8"),
+})
+register("int8", "sm100", {
+    "linear_int8": Kernel("i8_simple_kernel", "csrc/gemm_i8.cu", "trl_gemm_i8", "tilerl_b200.ops.gemm_int8"),
+    "linear_int8_grad": Kernel("i8_simple_kernel", "csrc/gemm_i8.cu", "trl_gemm_i8_grad", "tilerl_b200.ops.gemm_int8", note="rows in two digits of 8 bits"),
+    "quant_int8": Kernel("rows_i8_kernel", "csrc/rows_i8.cu", "trl_rows_i8", "tilerl_b200.ops.gemm_int8",
+                         note="RMSNorm + int8 with one scale per token; weights by channel; gradients in 16 bits"),
 })
 register("any", "sm100", {
     "embed": Kernel("embedding_kernel", "csrc/misc.cu", "trl_embedding"),

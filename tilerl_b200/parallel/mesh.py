@@ -142,10 +142,10 @@ def tp_dims(cfg: ModelConfig, tp: int) -> TPDims:
 
 def check_alignment(cfg: ModelConfig, tp: int) -> None:
     """Refuse shard shapes the quantised kernels cannot address: NVFP4 needs the
-    reduction dim of every shard to be a multiple of 16 (one scale block), the
-    block-scaled FP8 format a multiple of 128."""
+    reduction dim of every shard to be a multiple of 16 (one scale block), 8-bit integers of 16 (the
+    copy engine's step), the block-scaled FP8 format a multiple of 128."""
     d = tp_dims(cfg, tp)
-    need = {"nvfp4": 16, "fp8": 128}.get(cfg.quant, 1)
+    need = {"nvfp4": 16, "fp8": 128, "int8": 16}.get(cfg.quant, 1)
     for name, k in (("o", d.n_q * cfg.head_dim), ("out", d.gdn_nv * cfg.gdn_head_dim), ("down", d.ffn)):
         if k and k % need:
             raise ValueError(f"tp={tp}: reduction dim {k} of '{name}' is not a multiple of {need}")
@@ -248,10 +248,12 @@ def shard_param(cfg: ModelConfig, name: str, w, rank: int, tp: int):
     spec = shard_spec(cfg, name, rank, tp)
     if spec[0] == "full":
         return w
-    from ..formats import FP8BlockTensor, NVFP4Tensor
+    from ..formats import FP8BlockTensor, INT8Tensor, NVFP4Tensor
     if isinstance(w, NVFP4Tensor):
         sc = apply_spec(w.scale.view(torch.uint8), spec, 16).view(torch.float8_e4m3fn)
         return NVFP4Tensor(apply_spec(w.wq, spec, 2), sc, w.tscale.clone())
+    if isinstance(w, INT8Tensor):          # (a channel's scale belongs to its whole row)
+        return INT8Tensor(apply_spec(w.w8, spec), w.wscale.clone() if spec[0] == "cols" else apply_spec(w.wscale, spec))
     if isinstance(w, FP8BlockTensor):
         raise NotImplementedError("block-scaled FP8 weights are sharded before quantisation")
     return apply_spec(w, spec)

@@ -21,7 +21,7 @@ from typing import Callable, Dict, Optional
 
 import torch
 
-from ..formats import NVFP4Tensor, quantize_nvfp4
+from ..formats import INT8Tensor, NVFP4Tensor, quantize_int8, quantize_nvfp4
 from ..models.hybrid import linear_names
 from .mesh import shard_param
 
@@ -33,6 +33,9 @@ def _store(dst, src) -> int:
         dst.scale.copy_(src.scale)
         dst.tscale.copy_(src.tscale)
         return dst.wq.numel() + dst.scale.numel() + 4
+    if isinstance(dst, INT8Tensor):
+        dst.w8.copy_(src.w8), dst.wscale.copy_(src.wscale)
+        return dst.nbytes()
     dst.copy_(src.to(dst.dtype))
     return dst.numel() * dst.element_size()
 
@@ -41,7 +44,8 @@ def resync(zero, rollout, *, quantize: Optional[Callable] = None, refresh: Optio
            engine=None) -> Dict[str, float]:
     """Write the trainer's current weights into ``rollout`` (a served ``HybridModel`` of TP
     degree ``rollout.tp``).  ``quantize(w_full) -> NVFP4Tensor`` defaults to the torch
-    quantiser (a CUDA backend passes its kernel); ``refresh(param)`` is called for every
+    quantiser (a CUDA backend passes its kernel); weights served in 8-bit integers take theirs from
+    ``formats.quantize_int8``; ``refresh(param)`` is called for every
     rewritten quantised tensor (the CUDA backend re-tiles its GEMM copies there)."""
     cfg = rollout.cfg
     quantize = quantize or (lambda w: quantize_nvfp4(w.float()))
@@ -64,6 +68,8 @@ def resync(zero, rollout, *, quantize: Optional[Callable] = None, refresh: Optio
                     nbytes += _store(dst, q)
                     if refresh is not None:
                         refresh(dst)
+                elif base in lin and isinstance(dst, INT8Tensor):
+                    nbytes += _store(dst, shard_param(cfg, base, quantize_int8(w.float()), rollout.tp_rank, rollout.tp))
                 else:
                     src = shard_param(cfg, base, w, rollout.tp_rank, rollout.tp)
                     nbytes += _store(dst, src)

@@ -26,7 +26,8 @@ from typing import Callable, Dict, List, NamedTuple, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
-from .ops import keep, ref, score
+from .formats import INT8Tensor
+from .ops import gemm_int8, keep, ref, score
 from .ops.keep import Kept8, keep8
 
 
@@ -301,7 +302,11 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
     """``y = x @ W^T``.  ``w`` is a dense master tensor (dX and dW) or a quantised
     weight / ``frozen=True`` dense tensor (dX only, the LoRA-on-frozen-base mode).
     On CUDA the three GEMMs run in bf16 with fp32 accumulation, y rounded to bf16 (``wide``: not rounded, as logits are, since
-    a rounding of 2^-9 of a logit of 20 is 0.04 of a log-probability); on CPU everything is fp32 (the oracle path)."""
+    a rounding of 2^-9 of a logit of 20 is 0.04 of a log-probability); on CPU everything is fp32 (the oracle path).
+    Weights in 8-bit integers: the product that serves them, rows quantised per token, y not rounded; the gradient takes that rounding of
+    x for none and its own rows in 16 bits (``ops/gemm_int8.py``)."""
+    if isinstance(w, INT8Tensor):
+        return _linear_int8(tape, x, w)
     dense = isinstance(w, torch.Tensor)
     wf = dense_weight(w, x.device)
     if x.is_cuda:
@@ -331,6 +336,20 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
         return (dx,)
 
     tape.record("linear", (x, w) if dense and not frozen else (x,), (out,), bwd)
+    return out
+
+
+def _linear_int8(tape: Tape, x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
+    takes = gemm_int8.train_takes(x, w)
+    out = gemm_int8.forward(x, w) if takes else ref.linear_int8(x, w)
+    like = _Like(out.shape, out.device)
+
+    def bwd(g):
+        if takes and g.shape == like.shape and g.device == like.device:
+            return (gemm_int8.grad(g, w),)
+        return (ref.linear_int8_grad(g, w),)
+
+    tape.record("linear", (x,), (out,), bwd)
     return out
 
 
