@@ -1,101 +1,482 @@
-// Products of 8-bit integers with a scale for each token and each channel.
+// Products of 8-bit integers with a scale for each token and each channel, on pairs of SMs (tcgen05.mma.cta_group::2.kind::i8).
 //
 //   y[t, n]  = epi((sum_k q[t, k] W[n, k]) * s[t] * ws[n])                              (W: int8 [N, K], q: rows_i8.cu)
 //   dx[t, k] = s[t] * (256 sum_n hi[t, n] W[n, k] + sum_n lo[t, n] W[n, k])             (gradient of y's input, rows in two digits)
 //
-// Simple form: a block 64 x 64 results, 64 bytes of the summed dimension at a time through shared memory, dp4a.
+// Sums are of 32-bit integers: exact, whatever the order, so K may be shared between SMs without a change of the result.
+//
+// A tile is 256 features x BN columns.  Features are the A operand: 128 of them a SM, of y's rows of W (K-major), of dx's columns of W
+// (M-major: the same copies of 128 x 128 bytes, read across, so the gradient needs no second layout of the weight).  Columns are tokens,
+// two a token for dx (high and low digit side by side, put together in the epilogue); each SM holds half of them and the MMA hands them to
+// both.  A stage is 128 bytes of the summed dimension: 16 KB of W and BN / 2 x 128 bytes of q a SM, one copy each, four MMAs.  Two
+// accumulators in TMEM: the epilogue of a tile runs beside the next one's MMAs.  It turns the values round through shared memory, so that
+// they leave as 16-byte pieces of a token's row.  With fewer tiles than pairs, two to four pairs of a cluster share a tile along the summed
+// dimension and add their parts through each other's shared memory.
 //
 // The reference has no integer product; in the place of its `linear_fp8` (packages/tilerl-kernels/src/tilerl_kernels/
 // kernels_linear.py:1777-1813) for weights in this format.
 #include "int8.cuh"
+#include "tcgen05_pair.cuh"
 
 namespace {
 
-enum { I8_STORE = 0, I8_RESIDUAL = 1, I8_SWIGLU = 2, I8_STORE_F32 = 3 };
+constexpr int GI_ROWS = 128;                      // features a SM
+constexpr int GI_KT = 128;                        // bytes of the summed dimension a stage
+constexpr int GI_THREADS = 320;
+constexpr int GI_TR_STRIDE = 36;                  // words a token in a warp's turning piece: 32 features, and 4 so that reads spread
+constexpr int GI_TR_BYTES = 16 * GI_TR_STRIDE * 4;
+constexpr int GI_MAX_PARTS = 4;
+
+template <int BN>
+struct I8Cfg {
+  static constexpr int A_BYTES = GI_ROWS * GI_KT, B_BYTES = BN / 2 * GI_KT, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 200 * 1024 / STAGE < 9 ? 200 * 1024 / STAGE : 9;
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int SMEM = (RING < 160 * 1024 ? 160 * 1024 : RING) + 8 * GI_TR_BYTES + 512 + 1024;
+  static constexpr int TMEM_COLS = BN <= 64 ? 128 : BN <= 128 ? 256 : 512;
+  static_assert(SMEM <= 227 * 1024 && 2 * BN <= TMEM_COLS && STAGE % 1024 == 0, "layout");
+  static_assert(SMEM > 227 * 1024 / 2 + 1024, "no other kernel with TMEM fits beside it on an SM");
+  static_assert(BN * GI_ROWS * 4 <= RING, "parts of a shared tile lie in the ring");
+};
 
 struct I8Params {
-  const int8_t* w;       // [N, K]
   const float* ws;       // [N]
-  const int8_t* q;       // [T, ldq]
   const float* s;        // [T]
   const bf16* residual;
   void* out;
-  long long ldw, ldq, ldr, ldo;
-  int T, N, K, epi;
+  long long ldr, ldo;
+  int features, tokens, depth, nk, r_tiles, c_tiles, epi;
+  int vec;               // 8 features of a token are one aligned vector of the output (of SwiGLU four results) and of the residual
+  int parts;             // pairs that share a tile (a cluster), each a part of the summed dimension; 1: a pair goes through whole tiles
 };
 
-__device__ __forceinline__ void i8_out(const I8Params& p, int t, int n, float v, float up) {
-  const size_t at = (size_t)t * p.ldo;
-  if (p.epi == I8_SWIGLU) {
-    if (!(n & 1)) reinterpret_cast<bf16*>(p.out)[at + (n >> 1)] = __float2bfloat16(__fdividef(v, 1.f + __expf(-v)) * up);
+__device__ __forceinline__ void gi_mma(uint32_t d_tmem, uint32_t alo, uint32_t blo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 da, db;\n"
+      "  mov.b64 da, {%1, %3}; mov.b64 db, {%2, %3};\n"
+      "  setp.ne.b32 p, %5, 0;\n"
+      "  tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, p; }\n"
+      ::"r"(d_tmem), "r"(alo), "r"(blo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ int4 gi_ld_cluster(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Eight features of a token out (v: results before the residual); those past the last one are left out.
+__device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8]) {
+  if (tok >= p.tokens || f >= p.features) return;
+  const size_t at = (size_t)tok * p.ldo;
+  if (p.epi == I8_SWIGLU) {                          // features in (gate, up) pairs
+    bf16* o = reinterpret_cast<bf16*>(p.out) + at + (f >> 1);
+    const float a = i8_swiglu(v[0], v[1]), b = i8_swiglu(v[2], v[3]), c = i8_swiglu(v[4], v[5]), d = i8_swiglu(v[6], v[7]);
+    if (p.vec) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(f2_to_bf162_bits(a, b), f2_to_bf162_bits(c, d));
+    } else {
+      const float y[4] = {a, b, c, d};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (f + 2 * i < p.features) o[i] = __float2bfloat16(y[i]);
+    }
   } else if (p.epi == I8_STORE_F32) {
-    reinterpret_cast<float*>(p.out)[at + n] = v;
+    float* o = reinterpret_cast<float*>(p.out) + at + f;
+    if (p.vec) {
+      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (f + i < p.features) o[i] = v[i];
+    }
   } else {
-    if (p.epi == I8_RESIDUAL) v += __bfloat162float(__ldcg(p.residual + (size_t)t * p.ldr + n));
-    reinterpret_cast<bf16*>(p.out)[at + n] = __float2bfloat16(v);
+    bf16* o = reinterpret_cast<bf16*>(p.out) + at + f;
+    const bf16* r = p.residual + (size_t)tok * p.ldr + f;
+    const bool res = p.epi == I8_RESIDUAL;
+    if (p.vec) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = v[i];
+      if (res) {
+        const uint4 u = __ldcg(reinterpret_cast<const uint4*>(r));
+        const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
+        y[0] = __fadd_rn(y[0], a.x), y[1] = __fadd_rn(y[1], a.y), y[2] = __fadd_rn(y[2], b.x), y[3] = __fadd_rn(y[3], b.y);
+        y[4] = __fadd_rn(y[4], c.x), y[5] = __fadd_rn(y[5], c.y), y[6] = __fadd_rn(y[6], d.x), y[7] = __fadd_rn(y[7], d.y);
+      }
+      *reinterpret_cast<uint4*>(o) = make_uint4(f2_to_bf162_bits(y[0], y[1]), f2_to_bf162_bits(y[2], y[3]), f2_to_bf162_bits(y[4], y[5]), f2_to_bf162_bits(y[6], y[7]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (f + i < p.features) o[i] = __float2bfloat16(res ? __fadd_rn(v[i], __bfloat162float(__ldcg(r + i))) : v[i]);
+    }
   }
 }
 
-// GRAD: results are [T, K], summed over N; q has two rows a token.
-template <bool GRAD>
-__global__ void __launch_bounds__(256) i8_simple_kernel(const I8Params p) {
-  __shared__ int ws_[16][65], qs[16][65], ql[GRAD ? 16 : 1][65];       // [4-byte step][feature or token]
+// GRAD: results are dx; two columns a token.  SPLIT: a cluster's pairs share a tile.
+template <int BN, bool GRAD, bool SPLIT>
+__global__ void __launch_bounds__(GI_THREADS, 1)
+gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const I8Params p) {
+  using C = I8Cfg<BN>;
+  constexpr int STAGES = C::STAGES, J = GRAD ? 2 : 1;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* turn = smem + C::RING;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(turn + 8 * GI_TR_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int part = SPLIT ? pair % p.parts : 0, even = 2 * part;          // even: the cluster's CTA that issues for this pair
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };                              // the even SM's counts both SMs' copies
+  auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };   // of the even SM: both SMs' epilogue warps
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int b = 0; b < 2; ++b) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 16);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // (TMEM of a pair is taken by both SMs together: only once both CTAs are known to run)
+  gp_cluster_sync();
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  gp_cluster_sync();                                // both halves are allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();
-  pdl_wait();
-  const int f0 = blockIdx.x * 64, t0 = blockIdx.y * 64, features = GRAD ? p.K : p.N, depth = GRAD ? p.N : p.K;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {}, low[GRAD ? 4 : 1][4] = {};
-  for (int d0 = 0; d0 < depth; d0 += 64) {
-    for (int i = threadIdx.x; i < 16 * 64; i += 256) {
-      const int r = i / 16, j = i % 16;
-      uint32_t w = 0, q = 0, l = 0;
-      for (int b = 0; b < 4; ++b) {
-        const int d = d0 + j * 4 + b, f = f0 + r, t = t0 + r;
-        if (d < depth && f < features) w |= (uint32_t)(uint8_t)(GRAD ? p.w[(size_t)d * p.ldw + f] : p.w[(size_t)f * p.ldw + d]) << (8 * b);
-        if (d < depth && t < p.T) {
-          q |= (uint32_t)(uint8_t)__ldcg(p.q + (size_t)t * (GRAD ? 2 : 1) * p.ldq + d) << (8 * b);
-          if (GRAD) l |= (uint32_t)(uint8_t)__ldcg(p.q + ((size_t)t * 2 + 1) * p.ldq + d) << (8 * b);
+
+  // Whole tiles, every `pairs`-th one; columns run fastest, so that the pairs at work share a few tiles' features and all columns, and the
+  // L2 cache holds both while they do.
+  const int tiles = p.r_tiles * p.c_tiles, tile0 = SPLIT ? pair / p.parts : pair, tile1 = SPLIT ? tile0 + 1 : tiles, tile_step = SPLIT ? 1 : pairs;
+  const int my_tiles = tile1 > tile0 ? (tile1 - tile0 + tile_step - 1) / tile_step : 0;
+  const int k0 = SPLIT ? (int)((long long)part * p.nk / p.parts) : 0, k1 = SPLIT ? (int)((long long)(part + 1) * p.nk / p.parts) : p.nk;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (elect_one()) {
+      const uint32_t smem0 = smem_u32(smem);
+      const int units = my_tiles * (k1 - k0);
+      auto load_w = [&](int rt, int kt, int st) {
+        const uint32_t dst = smem0 + (uint32_t)st * C::STAGE, bar = gp_map(full(st), even);
+        const int f = (rt * 2 + rank) * GI_ROWS;
+        if (rank == 0) mbar_expect_tx(full(st), 2u * C::STAGE);
+        gp_load_2d(dst, &map_w, GRAD ? f : kt * GI_KT, GRAD ? kt * GI_KT : f, bar);
+      };
+      auto load_q = [&](int ct, int kt, int st) {
+        gp_load_2d(smem0 + (uint32_t)st * C::STAGE + C::A_BYTES, &map_q, kt * GI_KT, ct * BN + rank * (BN / 2), gp_map(full(st), even));
+      };
+      int w_tile = tile0, w_rt = tile0 / p.c_tiles, w_kt = k0, q_tile = tile0, q_ct = tile0 % p.c_tiles, q_kt = k0, st = 0;
+      uint32_t ph = 0;
+      auto next_w = [&] { if (++w_kt == k1) w_kt = k0, w_tile += tile_step, w_rt = w_tile / p.c_tiles; };
+      const int pre = min(STAGES, units);
+      for (int u = 0; u < pre; ++u) load_w(w_rt, w_kt, u), next_w();       // weights do not depend on the kernel ahead (rows_i8.cu)
+      pdl_wait();
+      for (int u = 0; u < units; ++u) {
+        if (u >= pre) {
+          if (!mbar_wait(empty(st), ph ^ 1u, abort_flag)) break;
+          load_w(w_rt, w_kt, st), next_w();
+        }
+        load_q(q_ct, q_kt, st);
+        if (++q_kt == k1) q_kt = k0, q_tile += tile_step, q_ct = q_tile % p.c_tiles;
+        if (++st == STAGES) st = 0, ph ^= 1u;
+      }
+      // the last arrivals of the even SM's MMAs on this CTA's barriers, before its memory goes away
+      for (int s = 0; s < pre; ++s) {
+        const int u = units - pre + s;              // the last unit of its stage
+        if (!mbar_wait(empty(u % STAGES), (uint32_t)(u / STAGES) & 1u, abort_flag)) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (for both SMs) ----------------
+    pdl_wait();
+    if (rank == 0 && elect_one()) {
+      // sums of 32 bits, both operands signed; dx: A with the features side by side
+      constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((GRAD ? 1u : 0u) << 15) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((2 * GI_ROWS) >> 4) << 24);
+      // 32 bytes of a row further along K; across, 32 rows of 128 bytes (and 1024 bytes from eight rows to the next eight either way)
+      constexpr uint32_t A_STEP = GRAD ? 32 * GI_KT >> 4 : 2;
+      const uint64_t d_op = desc_sw128(smem_u32(smem));
+      const uint32_t op_lo = (uint32_t)d_op, op_hi = (uint32_t)(d_op >> 32);
+      int st = 0;
+      uint32_t ph = 0;
+      const uint16_t both = (uint16_t)(3u << even);
+      bool ok = true;
+      for (int n = 0; ok && n < my_tiles; ++n) {
+        const int buf = n & 1;
+        if (n >= 2) {
+          ok = mbar_wait(acc_empty(buf), (uint32_t)((n >> 1) - 1) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        const uint32_t acc = tmem_base + (uint32_t)buf * BN;
+        for (int kt = k0; kt < k1; ++kt) {
+          ok = mbar_wait(full(st), ph, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t off = (uint32_t)st * (uint32_t)(C::STAGE >> 4);
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+            gi_mma(acc, op_lo + off + kb * A_STEP, op_lo + off + (C::A_BYTES >> 4) + kb * 2, op_hi, idesc, kt > k0 || kb ? 1u : 0u);
+          gp_commit(empty(st), both);
+          if (++st == STAGES) st = 0, ph ^= 1u;
+        }
+        if (ok) gp_commit(acc_full(buf), both);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue (warps 2..9) ----------------
+    pdl_wait();
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    constexpr int COLS = BN / 2, CHUNKS = COLS / 32, TOK = 32 / J;      // a warp's columns, in pieces of 32
+    int* tr = reinterpret_cast<int*>(turn + (warp - 2) * GI_TR_BYTES);
+    int* sum = reinterpret_cast<int*>(smem);        // parts: [column][128 features] of this CTA's, in the ring, which is through by then
+    const uint32_t even_empty = gp_map(acc_empty(0), even);
+    for (int n = 0; n < my_tiles; ++n) {
+      const int tile = tile0 + n * tile_step, buf = n & 1, rt = tile / p.c_tiles, ct = tile % p.c_tiles;
+      const int f0 = (rt * 2 + rank) * GI_ROWS + quad * 32 + (lane & 3) * 8;      // this lane's features and this warp's tokens as they leave
+      const int tok0 = (ct * BN + half * COLS) / J;
+      float ws[8], s[CHUNKS];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ws[i] = !GRAD && !SPLIT && f0 + i < p.features ? p.ws[f0 + i] : 0.f;
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) s[c] = !SPLIT && lane < TOK && tok0 + c * TOK + lane < p.tokens ? __ldcg(p.s + tok0 + c * TOK + lane) : 0.f;
+      // (the warps of a group do not meet: each has its own barrier phase and its own piece of shared memory)
+      if (!__all_sync(0xffffffffu, mbar_wait(acc_full(buf), (uint32_t)(n >> 1) & 1u, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        uint32_t r[32];
+        tc_ld32(taddr + (uint32_t)(c * 32), r);
+        tc_wait_ld();
+        if (c == CHUNKS - 1) {                       // read out: the accumulator goes back
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_empty + 8u * buf) : "memory");
+        }
+        if (SPLIT) {
+#pragma unroll
+          for (int t = 0; t < 32; ++t) sum[(size_t)(half * COLS + c * 32 + t) * GI_ROWS + quad * 32 + lane] = (int)r[t];
+        } else {
+#pragma unroll
+          for (int i = 0; i < TOK / 8; ++i) {
+            const int t = i * 8 + (lane >> 2);
+            if (i % 2 == 0) {                        // 16 tokens at a time
+              __syncwarp();
+#pragma unroll
+              for (int u = 0; u < 16; ++u) {
+                const int x = i * 8 + u;
+                tr[u * GI_TR_STRIDE + lane] = GRAD ? __float_as_int(fmaf(256.f, (float)(int)r[x * J], (float)(int)r[x * J + J - 1])) : (int)r[x];
+              }
+              __syncwarp();
+            }
+            const float st = __shfl_sync(0xffffffffu, s[c], t);
+            const int* src = tr + (t & 15) * GI_TR_STRIDE + (lane & 3) * 8;
+            const int4 a = reinterpret_cast<const int4*>(src)[0], b = reinterpret_cast<const int4*>(src)[1];
+            const int x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = GRAD ? __fmul_rn(__int_as_float(x[e]), st) : i8_value(x[e], __fmul_rn(st, ws[e]));
+            gi_store8(p, tok0 + c * TOK + t, f0, v);
+          }
         }
       }
-      ws_[j][r] = (int)w, qs[j][r] = (int)q;
-      if (GRAD) ql[j][r] = (int)l;
     }
-    __syncthreads();
-    for (int j = 0; j < 16; ++j)
-      for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < 4; ++b) {
-          acc[a][b] = __dp4a(qs[j][ty * 4 + a], ws_[j][tx * 4 + b], acc[a][b]);
-          if (GRAD) low[a][b] = __dp4a(ql[j][ty * 4 + a], ws_[j][tx * 4 + b], low[a][b]);
+  }
+
+  if constexpr (SPLIT) {
+    // each pair of the cluster adds up its share of the tokens
+    gp_cluster_sync();
+    constexpr int TOKENS = BN / J;
+    const int rt = tile0 / p.c_tiles, ct = tile0 % p.c_tiles, t0 = part * TOKENS / p.parts, t1 = (part + 1) * TOKENS / p.parts;
+    for (int i = t0 * 16 + (int)threadIdx.x; i < t1 * 16; i += GI_THREADS) {
+      const int t = i >> 4, r = (i & 15) * 8, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
+      if (tok >= p.tokens || f >= p.features) continue;
+      int x[J][8] = {};
+      for (int q = 0; q < p.parts; ++q) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const uint32_t src = gp_map(smem_u32(smem) + (uint32_t)((t * J + j) * GI_ROWS + r) * 4u, 2 * q + rank);
+          const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
+          x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
+          x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
         }
-    __syncthreads();
-  }
-  for (int a = 0; a < 4; ++a) {
-    const int t = t0 + ty * 4 + a;
-    if (t >= p.T) continue;
-    const float s = __ldcg(p.s + t);
-    float v[5] = {};
-    for (int b = 0; b < 4; ++b) {
-      const int f = f0 + tx * 4 + b;
-      if (f < features) v[b] = GRAD ? fmaf(256.f, (float)acc[a][b], (float)low[a][b]) * s : (float)acc[a][b] * (s * p.ws[f]);
+      }
+      const float st = __ldcg(p.s + tok);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : f + e < p.features ? i8_value(x[0][e], __fmul_rn(st, p.ws[f + e])) : 0.f;
+      gi_store8(p, tok, f, v);
     }
-    for (int b = 0; b < 4; ++b)
-      if (f0 + tx * 4 + b < features) i8_out(p, t, f0 + tx * 4 + b, v[b], v[b + 1]);
   }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // give copies that are still in flight time to land before the CTAs' memory goes away
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {
+    }
+  }
+  gp_cluster_sync();                                // nothing of the pair is in flight towards the other SM any more
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS) : "memory");
+  gp_cluster_sync();                                // no CTA leaves while the other's half is being given back
+}
+
+typedef CUresult (*EncodeTiledFnI)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// [rows, width] bytes, rows ld apart, in pieces of 128 bytes x box_rows; what lies outside reads as zero
+bool gi_tensor(CUtensorMap* m, const void* base, long long width, long long rows, long long ld, int box_rows) {
+  static EncodeTiledFnI encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn) return false;
+    encode = (EncodeTiledFnI)fn;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {GI_KT, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool GRAD, bool SPLIT>
+cudaError_t gi_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int ctas, int parts, cudaStream_t stream) {
+  auto kern = gemm_i8_kernel<BN, GRAD, SPLIT>;
+  static TrlPerDevice<bool> set;
+  bool& configured = set.here();
+  if (!configured) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, I8Cfg<BN>::SMEM);
+    if (e != cudaSuccess) return e;
+    configured = true;
+  }
+  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(GI_THREADS), cfg.dynamicSmemBytes = I8Cfg<BN>::SMEM, cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2 * parts, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = g_trl_use_pdl ? 2 : 1;
+  return cudaSuccess;
+}
+
+// Clusters of `parts` pairs that fit the GPU at a time.
+int gi_clusters(int parts) {
+  static TrlPerDevice<int> counts[GI_MAX_PARTS + 1];
+  int& known = counts[parts].here();
+  if (known == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (gi_config<64, false, true>(cfg, attr, 2 * parts, parts, nullptr) != cudaSuccess) return 0;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_kernel<64, false, true>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    known = n > 0 ? n : -1;
+  }
+  return known;
+}
+
+struct I8Plan {
+  int bn, parts, pairs;
+};
+
+// Columns a tile and pairs a tile: the least of rounds x stages x (time of a stage) + what putting parts together costs, in stages of 128
+// columns.
+I8Plan gi_plan(int cols, int features, int nk) {
+  int sms = 0, dev = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int pairs = sms / 2, r_tiles = (features + 2 * GI_ROWS - 1) / (2 * GI_ROWS);
+  static const struct { int bn; double unit, exchange; } forms[] = {{64, 0.9, 3}, {128, 1, 5}, {192, 1.5, 8}, {256, 2, 10}};
+  I8Plan best{0, 1, pairs};
+  double least = 0;
+  for (const auto& f : forms) {
+    const long long T = (long long)r_tiles * ((cols + f.bn - 1) / f.bn);
+    for (int S = 1; S <= GI_MAX_PARTS; ++S) {
+      if (S > 1 && (nk < 4 * S || T * S > pairs || T > gi_clusters(S))) break;
+      const double cost = (double)((T + pairs - 1) / pairs) * ((nk + S - 1) / S) * f.unit + (S > 1 ? f.exchange * (S + 2) / 4 : 0);
+      if (!best.bn || cost < least) best = I8Plan{f.bn, S, pairs}, least = cost;
+    }
+    if (cols <= f.bn) break;
+  }
+  return best;
+}
+
+template <int BN, bool GRAD>
+int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int width, int rows, I8Params p, const I8Plan& plan, cudaStream_t stream) {
+  constexpr int J = GRAD ? 2 : 1;
+  CUtensorMap mw, mq;
+  if (!gi_tensor(&mw, w, width, rows, ldw, GI_ROWS) || !gi_tensor(&mq, q, p.depth, (long long)p.tokens * J, ldq, BN / 2)) return (int)cudaErrorInvalidValue;
+  p.r_tiles = (p.features + 2 * GI_ROWS - 1) / (2 * GI_ROWS), p.c_tiles = (p.tokens * J + BN - 1) / BN, p.parts = plan.parts;
+  const long long tiles = (long long)p.r_tiles * p.c_tiles;
+  if (tiles > 0x7fffffffll / p.nk) return (int)cudaErrorInvalidValue;
+  const int pairs = plan.parts > 1 ? (int)tiles * plan.parts : (int)(tiles < plan.pairs ? tiles : plan.pairs);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  const cudaError_t e = plan.parts > 1 ? gi_config<BN, GRAD, true>(cfg, attr, 2 * pairs, plan.parts, stream) : gi_config<BN, GRAD, false>(cfg, attr, 2 * pairs, 1, stream);
+  if (e != cudaSuccess) return (int)e;
+  return (int)(plan.parts > 1 ? cudaLaunchKernelEx(&cfg, gemm_i8_kernel<BN, GRAD, true>, mw, mq, p) : cudaLaunchKernelEx(&cfg, gemm_i8_kernel<BN, GRAD, false>, mw, mq, p));
+}
+
+template <bool GRAD>
+int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int width, int rows, I8Params& p, cudaStream_t stream) {
+  constexpr int J = GRAD ? 2 : 1;
+  p.nk = (p.depth + GI_KT - 1) / GI_KT;
+  const I8Plan plan = gi_plan(p.tokens * J, p.features, p.nk);
+  switch (plan.bn) {
+    case 64: return gi_launch<64, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
+    case 128: return gi_launch<128, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
+    case 192: return gi_launch<192, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
+    default: return gi_launch<256, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
+  }
+}
+
+constexpr int GI_MOST = 131072;                   // 127 * 128 times as many is below 2^31
+bool gi_operands(const void* w, long long ldw, int K, const void* q, long long ldq) {
+  return reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && ldw >= K && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0;
 }
 
 }  // namespace
 
-// out[t, n] = epi(...).  K and N up to 131072 (sums of 32 bits); SwiGLU: N even, rows of w in (gate, up) pairs, out [T, N / 2].
+// out[t, n] = epi(...).  w and q: rows on 16-byte boundaries.  K up to 131072 (sums of 32 bits); SwiGLU: N even, rows of w in (gate, up)
+// pairs, out [T, N / 2].
 TRL_API int trl_gemm_i8(const void* w, long ldw, const void* ws, const void* q, long ldq, const void* s, const void* residual, long ldr, void* out,
                         long ldo, int T, int N, int K, int epi, void* stream) {
-  if (T <= 0 || N <= 0 || K <= 0 || K > 131072 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2)) return (int)cudaErrorInvalidValue;
-  const I8Params p{(const int8_t*)w, (const float*)ws, (const int8_t*)q, (const float*)s, (const bf16*)residual, out, ldw, ldq, ldr, ldo, T, N, K, epi};
-  return (int)trl_launch(i8_simple_kernel<false>, dim3((N + 63) / 64, (T + 63) / 64), dim3(256), 0, (cudaStream_t)stream, p);
+  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
+      (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, q, ldq) || ldq < K)
+    return (int)cudaErrorInvalidValue;
+  I8Params p{};
+  p.ws = (const float*)ws, p.s = (const float*)s, p.residual = (const bf16*)residual, p.out = out, p.ldr = ldr, p.ldo = ldo;
+  p.features = N, p.tokens = T, p.depth = K, p.epi = epi;
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out), r = reinterpret_cast<uintptr_t>(residual);
+  p.vec = N % 8 == 0 && (epi == I8_SWIGLU ? o % 8 == 0 && ldo % 4 == 0 : epi == I8_STORE_F32 ? o % 16 == 0 && ldo % 4 == 0 : o % 16 == 0 && ldo % 8 == 0) &&
+          (epi != I8_RESIDUAL || (r % 16 == 0 && ldr % 8 == 0));
+  return gi_launch<false>(w, ldw, q, ldq, K, N, p, (cudaStream_t)stream);
 }
 
 // dx[t, k], fp32, of rows in two digits: q [2 T, ldq].
 TRL_API int trl_gemm_i8_grad(const void* w, long ldw, const void* q, long ldq, const void* s, void* dx, long ldo, int T, int N, int K, void* stream) {
-  if (T <= 0 || N <= 0 || K <= 0 || N > 131072) return (int)cudaErrorInvalidValue;
-  const I8Params p{(const int8_t*)w, nullptr, (const int8_t*)q, (const float*)s, nullptr, dx, ldw, ldq, 0, ldo, T, N, K, I8_STORE_F32};
-  return (int)trl_launch(i8_simple_kernel<true>, dim3((K + 63) / 64, (T + 63) / 64), dim3(256), 0, (cudaStream_t)stream, p);
+  if (T <= 0 || T > (1 << 29) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || !gi_operands(w, ldw, K, q, ldq) || ldq < N) return (int)cudaErrorInvalidValue;
+  I8Params p{};
+  p.s = (const float*)s, p.out = dx, p.ldo = ldo, p.features = K, p.tokens = T, p.depth = N, p.epi = I8_STORE_F32;
+  p.vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0 && ldo % 4 == 0;
+  return gi_launch<true>(w, ldw, q, ldq, K, N, p, (cudaStream_t)stream);
 }

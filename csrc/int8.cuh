@@ -37,4 +37,11 @@ __device__ __forceinline__ float i8_groups_sum(const float* groups, int n) {
 }
 __device__ __forceinline__ uint32_t i8_warp_most(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
+// A product's result from its sum of integers: the sum in fp32 (rounded above 2^24) times the product of both scales.  The same operations
+// in the same order in every kernel: a row's results do not depend on which one the number of rows leads to.
+__device__ __forceinline__ float i8_value(int acc, float scale) { return __fmul_rn(__int2float_rn(acc), scale); }
+__device__ __forceinline__ float i8_swiglu(float gate, float up) { return __fmul_rn(__fdividef(gate, 1.f + __expf(-gate)), up); }
+
+enum { I8_STORE = 0, I8_RESIDUAL = 1, I8_SWIGLU = 2, I8_STORE_F32 = 3 };
+
 }  // namespace

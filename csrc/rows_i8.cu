@@ -22,6 +22,7 @@ struct RowsParams {
   int K;
   float eps;
   int norm;
+  int weights;           // q and s are a weight: products may read one before they wait for the kernel ahead of them
 };
 
 template <typename T, bool VEC>
@@ -52,9 +53,12 @@ template <typename T, int CH, bool VEC, bool W16>
 __global__ void __launch_bounds__(1024) rows_i8_kernel(const RowsParams p) {
   extern __shared__ float groups[];              // sums of squares of 256 values each
   __shared__ uint32_t most_s[32];
-  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, K = p.K;
+  // A product behind this kernel loads weights before it waits.  So the dependents are let in only once all that came before is through
+  // (it may have written those weights), and by a weight's quantiser not before its end.
+  pdl_enter();
   pdl_wait();
+  if (!p.weights) pdl_trigger();
   const T* x = reinterpret_cast<const T*>(p.x) + (long long)blockIdx.x * p.ldx;
   constexpr int KEEP = CH ? CH : 1;
   float t[KEEP][8];
@@ -156,13 +160,13 @@ cudaError_t rows_launch(const RowsParams& p, long long rows, cudaStream_t stream
 
 // x [rows, K] (type 0: fp32, 1: bf16; rows ldx apart) -> q int8 [rows, ldq], s fp32 [rows].  w: fp32 [K] or null; norm: w is a norm's
 // weight, and the row's 1 / rms goes into s.  digits 2: q has two rows of digits a row, 16 bits in all, and w is not a norm's.
-// ldq and q on 8-byte boundaries.
+// weights: q and s are a weight's.  ldq and q on 8-byte boundaries.
 TRL_API int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K,
-                        int digits, void* stream) {
+                        int digits, int weights, void* stream) {
   if (rows <= 0 || rows > 0x7fffffffl || K <= 0 || ldq < K || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || (type != 0 && type != 1) ||
       (digits != 1 && digits != 2) || (norm && (w == nullptr || digits == 2)))
     return (int)cudaErrorInvalidValue;
-  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, K, eps, norm};
+  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, K, eps, norm, weights};
   cudaStream_t st = (cudaStream_t)stream;
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (type ? 8 : 4) == 0;
   if (type) {

@@ -20,7 +20,7 @@ EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
 
-N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.P])
+N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.P])
 N.register("trl_gemm_i8", [N.P, N.L, N.P, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.I, N.P])
 N.register("trl_gemm_i8_grad", [N.P, N.L, N.P, N.L, N.P, N.P, N.L, N.I, N.I, N.I, N.P])
 
@@ -56,11 +56,11 @@ def _refuse(x: torch.Tensor, w: INT8Tensor, y=None, norm_w=None, residual=None, 
         raise ValueError(f"a norm's weight is fp32 [{k}] on the rows' device, got {tuple(norm_w.shape)} {norm_w.dtype} on {norm_w.device}")
 
 
-def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None) -> None:
+def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None, weights: bool = False) -> None:
     """Rows ``x [T, K]`` into ``q`` (int8 ``[T, >= K]``) and ``s`` (fp32 ``[T]``); with ``channels`` (a gradient's scales) into two rows of digits
-    a row of ``x``."""
+    a row of ``x``.  ``weights``: they are a weight's, which products load before they wait for the launch ahead of them."""
     N.check(N.lib().trl_rows_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(channels if norm_w is None else norm_w), int(norm_w is not None), eps,
-                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, N.stream()), "rows_i8")
+                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, int(weights), N.stream()), "rows_i8")
     N.count()
 
 
@@ -129,4 +129,4 @@ def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
         raise ValueError(f"quantize_ takes fp32 or bf16 of {dst.shape} on the weight's device, got {tuple(src.shape)} {src.dtype} on {src.device}")
     src = src if src.stride(1) == 1 else src.contiguous()
     with N.on(src.device):
-        quant_rows(src, dst.w8, dst.wscale)
+        quant_rows(src, dst.w8, dst.wscale, weights=True)
