@@ -458,7 +458,7 @@ bool gi_operands(const void* w, long long ldw, int K, const void* q, long long l
 
 // out[t, n] = epi(...).  w and q: rows on 16-byte boundaries.  K up to 131072 (sums of 32 bits); SwiGLU: N even, rows of w in (gate, up)
 // pairs, out [T, N / 2].
-TRL_API int trl_gemm_i8(const void* w, long ldw, const void* ws, const void* q, long ldq, const void* s, const void* residual, long ldr, void* out,
+static int gi_linear(const void* w, long ldw, const void* ws, const void* q, long ldq, const void* s, const void* residual, long ldr, void* out,
                         long ldo, int T, int N, int K, int epi, void* stream) {
   if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, q, ldq) || ldq < K)
@@ -473,10 +473,52 @@ TRL_API int trl_gemm_i8(const void* w, long ldw, const void* ws, const void* q, 
 }
 
 // dx[t, k], fp32, of rows in two digits: q [2 T, ldq].
-TRL_API int trl_gemm_i8_grad(const void* w, long ldw, const void* q, long ldq, const void* s, void* dx, long ldo, int T, int N, int K, void* stream) {
+static int gi_grad(const void* w, long ldw, const void* q, long ldq, const void* s, void* dx, long ldo, int T, int N, int K, void* stream) {
   if (T <= 0 || T > (1 << 29) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || !gi_operands(w, ldw, K, q, ldq) || ldq < N) return (int)cudaErrorInvalidValue;
   I8Params p{};
   p.s = (const float*)s, p.out = dx, p.ldo = ldo, p.features = K, p.tokens = T, p.depth = N, p.epi = I8_STORE_F32;
   p.vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0 && ldo % 4 == 0;
   return gi_launch<true>(w, ldw, q, ldq, K, N, p, (cudaStream_t)stream);
+}
+
+int gemv_i8_takes(int T, int N, int K);
+int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long ldx, const void* s, const void* norm_w, float eps, const void* residual,
+                   long ldr, void* out, long ldo, int T, int N, int K, int epi, int quantised, cudaStream_t stream);
+extern "C" int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K, int digits,
+                           int weights, void* scratch, void* stream);
+extern "C" long trl_rows_i8_scratch(long rows, int K, int digits);
+
+// out[t, n] = epi(norm(x) . w): rows of x (type 0: fp32, 1: bf16) quantised, multiplied.  norm_w: a norm's weight, or null.  scratch: T * K
+// bytes for the integers and 4 * T for the scales, on a 16-byte boundary, K % 16 == 0.  Otherwise as above.  Returns minus the number of launches,
+// or an error.
+TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w, float eps, const void* w, long ldw, const void* ws, const void* residual,
+                          long ldr, void* out, long ldo, void* scratch, int T, int N, int K, int epi, void* stream) {
+  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || K % 16 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
+      (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, scratch, K))
+    return (int)cudaErrorInvalidValue;
+  const int few = gemv_i8_takes(T, N, K);
+  const bool whole = type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;
+  if (few == 1 && whole) {
+    const int rc = gemv_i8_launch(w, ldw, ws, x, ldx, nullptr, norm_w, eps, residual, ldr, out, ldo, T, N, K, epi, 0, (cudaStream_t)stream);
+    return rc ? rc : -1;
+  }
+  void* s = (int8_t*)scratch + (size_t)T * K;
+  int rc = trl_rows_i8(x, type, ldx, norm_w, norm_w != nullptr, eps, scratch, K, s, T, K, 1, 0, nullptr, stream);
+  if (rc) return rc;
+  rc = few ? gemv_i8_launch(w, ldw, ws, scratch, K, s, nullptr, 0.f, residual, ldr, out, ldo, T, N, K, epi, 1, (cudaStream_t)stream)
+           : gi_linear(w, ldw, ws, scratch, K, s, residual, ldr, out, ldo, T, N, K, epi, stream);
+  return rc ? rc : -2;
+}
+
+// Bytes of scratch that trl_linear_i8_grad takes: rows in digits, their scales, the row quantiser's own.
+TRL_API long trl_linear_i8_grad_scratch(int T, int N) { return 2l * T * ((N + 15) / 16 * 16) + 4l * T + trl_rows_i8_scratch(T, N, 2); }
+
+// dx[t, k] of g [T, N] (type 0: fp32, 1: bf16).  scratch on a 16-byte boundary.
+TRL_API int trl_linear_i8_grad(const void* g, int type, long ldg, const void* w, long ldw, const void* ws, void* dx, long ldo, void* scratch, int T, int N, int K,
+                               void* stream) {
+  if (T <= 0 || N <= 0 || N > GI_MOST) return (int)cudaErrorInvalidValue;
+  const long ldq = (N + 15) / 16 * 16;
+  char* s = (char*)scratch + 2 * (size_t)T * ldq;
+  const int rc = trl_rows_i8(g, type, ldg, ws, 0, 0.f, scratch, ldq, s, T, N, 2, 0, s + 4 * (size_t)T, stream);
+  return rc ? rc : gi_grad(w, ldw, scratch, ldq, s, dx, ldo, T, N, K, stream);
 }

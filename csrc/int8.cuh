@@ -21,10 +21,11 @@ __device__ __forceinline__ float i8_scale(uint32_t most_bits, float part) {
   return most_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : m < I8_LEAST ? 0.f : __fmul_rn(m, part);
 }
 __device__ __forceinline__ uint32_t i8_abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// (A row with an infinity has the factor 0, and 0 times it is NaN: rounds to 0.)
-__device__ __forceinline__ int i8_round(float t, float factor) { return __float2int_rn(__fmul_rn(t, factor)); }
-__device__ __forceinline__ uint32_t i8_pack(int a, int b, int c, int d) {
-  return __byte_perm(__byte_perm((uint32_t)a, (uint32_t)b, 0x0040), __byte_perm((uint32_t)c, (uint32_t)d, 0x0040), 0x5410);
+// The nearest integer of t * factor (ties to even), in the low bits, of which a signed byte or 16 bits may be taken: behind the sum with 1.5 * 2^23
+// a float's last bit stands for one.
+__device__ __forceinline__ uint32_t i8_round_bits(float t, float factor) { return __float_as_uint(__fadd_rn(__fmul_rn(t, factor), 12582912.f)); }
+__device__ __forceinline__ uint32_t i8_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // Order of a row's squares: vectors of eight values one after the other; the 32 vectors of a group of 256 values by halving (xor 16, 8, 4,

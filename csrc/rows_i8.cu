@@ -3,9 +3,8 @@
 //   t = x * w (w: norm weight or none),  m = max |t|,  q = rint(t * ((1 / m) * 127)),  s = m * (1 / 127) [* rsqrt(mean x^2 + eps)]
 //   u = g * ws,                          m = max |u|,  Q = rint(u * ((1 / m) * 32512)) = 256 hi + lo,  s = m * (1 / 32512)
 //
-// A norm's factor is the same for a whole row, so it cancels out of the integers and goes into the scale alone.  One pass: a block a
-// row, the row stays in registers between its maximum and its integers (up to 8 vectors of 8 values a thread; longer rows are read a
-// second time, out of L2).  Bound by memory for many rows, by latency (two block barriers) for few.
+// A norm's factor is the same for a whole row, so it cancels out of the integers and goes into the scale alone.  One pass: a block takes
+// row after row, which stays in registers between its maximum and its integers.  Bound by memory for many rows, by latency for few.
 //
 // The reference quantises activations per token for its FP8 products (`quant_fp8`, packages/tilerl-kernels/src/tilerl_kernels/
 // kernels_linear.py:1547-1590); it has no integer form.
@@ -18,161 +17,299 @@ struct RowsParams {
   const float* w;        // norm weight, or the channels' scales of a gradient; may be null
   int8_t* q;             // [rows][ldq]; gradients: rows 2r (high digits) and 2r + 1 (low)
   float* s;
-  long long ldx, ldq;
+  long long ldx, ldq, rows;
   int K;
   float eps;
   int norm;
   int weights;           // q and s are a weight: products may read one before they wait for the kernel ahead of them
 };
 
+// Eight values as they lie in memory.
+template <typename T>
+struct RowsRaw {
+  uint4 u[sizeof(T) / 2];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void rows_load(const T* x, int k, int K, float (&v)[8]) {
+__device__ __forceinline__ RowsRaw<T> rows_load(const T* x, int k, int K) {
+  RowsRaw<T> r;
   if (VEC && k + 8 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(x + k));
-      const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
-      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
-    } else {
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(x + k)), b = __ldcg(reinterpret_cast<const float4*>(x + k) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    return;
-  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = 0.f;
-    if (k + i < K) {
-      if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(__ldcg(x + k + i));
-      else v[i] = __ldcg(x + k + i);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = __ldcg(reinterpret_cast<const uint4*>(x + k) + i);
+    return r;
+  }
+  T* v = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? __ldcg(x + k + i) : T(0.f);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void rows_values(const RowsRaw<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const float2 a = bf162_bits_to_f2(r.u[0].x), b = bf162_bits_to_f2(r.u[0].y), c = bf162_bits_to_f2(r.u[0].z), d = bf162_bits_to_f2(r.u[0].w);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+  } else {
+    const uint32_t b[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, r.u[1].x, r.u[1].y, r.u[1].z, r.u[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(b[i]);
   }
 }
 
-// CH: vectors that a thread keeps; 0: a row of any length, read twice.  W16: two digits.
+// The digits of eight values (rounded: bits) out: byte `digit` of each.
+__device__ __forceinline__ void rows_store(int8_t* out, int k, int K, const uint32_t (&q)[8], int digit) {
+  const uint32_t pick = digit ? 0x0051u : 0x0040u;
+  const uint2 b = make_uint2(__byte_perm(__byte_perm(q[0], q[1], pick), __byte_perm(q[2], q[3], pick), 0x5410),
+                             __byte_perm(__byte_perm(q[4], q[5], pick), __byte_perm(q[6], q[7], pick), 0x5410));
+  if (k + 8 <= K) {
+    *reinterpret_cast<uint2*>(out + k) = b;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) out[k + i] = (int8_t)((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
+  }
+}
+template <bool W16>
+__device__ __forceinline__ void rows_give(const RowsParams& p, long long row, int k, const float (&v)[8], float f) {
+  uint32_t q[8] = {};
+  if (f != 0.f) {                                  // (of a row with an infinity or NaN the products would be NaN)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = i8_round_bits(v[i], f);
+  }
+  int8_t* out = p.q + (W16 ? 2 : 1) * row * p.ldq;
+  if constexpr (W16) {
+    rows_store(out + p.ldq, k, p.K, q, 0);         // the low digit is the low byte, a signed one
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] += 128u;      // the high digit goes up where that one is negative
+    rows_store(out, k, p.K, q, 1);
+  } else {
+    rows_store(out, k, p.K, q, 0);
+  }
+}
+
+// CH: vectors of eight that a thread keeps; 0: a row of any length, read twice.  One vector a thread: the next row's values are on their way
+// while this one's maximum is found and its integers leave.  W16: two digits.
 template <typename T, int CH, bool VEC, bool W16>
-__global__ void __launch_bounds__(1024) rows_i8_kernel(const RowsParams p) {
-  extern __shared__ float groups[];              // sums of squares of 256 values each
-  __shared__ uint32_t most_s[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, K = p.K;
-  // A product behind this kernel loads weights before it waits.  So the dependents are let in only once all that came before is through
-  // (it may have written those weights), and by a weight's quantiser not before its end.
-  pdl_enter();
+__global__ void __launch_bounds__(CH == 1 ? 640 : 1024, CH == 1 ? 2 : 1) rows_i8_kernel(const RowsParams p) {
+  extern __shared__ float groups_s[];            // sums of squares of 256 values each, of two rows in turn
+  __shared__ uint32_t most_s[2][32];
+  // (products load weights before they wait for the kernels ahead, so a weight's quantiser lets none of them start before its end)
+  if (!p.weights) pdl_launch_dependents();
   pdl_wait();
-  if (!p.weights) pdl_trigger();
-  const T* x = reinterpret_cast<const T*>(p.x) + (long long)blockIdx.x * p.ldx;
-  constexpr int KEEP = CH ? CH : 1;
-  float t[KEEP][8];
-  uint32_t most = 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, K = p.K, pieces = (K + I8_GROUP - 1) / I8_GROUP;
   const bool squares = !W16 && p.norm;
-  auto weight = [&](int k, float (&v)[8]) {
-    if (p.w == nullptr) return;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? __fmul_rn(v[i], p.w[k + i]) : 0.f;
-  };
-  auto take = [&](int c, float (&v)[8]) {
-    const int k = (c * (int)blockDim.x + (int)threadIdx.x) * 8;
-    rows_load<T, VEC>(x, k, K, v);
-    if (squares) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-      ss = warp_sum(ss);
-      const int g = c * nw + warp;
-      if (lane == 0 && g * I8_GROUP < K) groups[g] = ss;
-    }
-    weight(k, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, i8_abs_bits(v[i]));
-  };
-  const int chunks = CH ? CH : (K + (int)blockDim.x * 8 - 1) / ((int)blockDim.x * 8);
-  if constexpr (CH > 0) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) take(c, t[c]);
-  } else {
-    for (int c = 0; c < chunks; ++c) take(c, t[0]);
-  }
-  most = i8_warp_most(most);
-  if (lane == 0) most_s[warp] = most;
-  __syncthreads();
-  most = i8_warp_most(lane < nw ? most_s[lane] : 0u);
+  constexpr int KEEP = CH ? CH : 1;
   constexpr float MOST = W16 ? I16_MOST : I8_MOST, PART = 1.f / MOST;
-  const float f = i8_factor(most, MOST);
-  auto give = [&](int c, float (&v)[8]) {
-    const int k = (c * (int)blockDim.x + (int)threadIdx.x) * 8;
-    if (k >= K) return;
-    int q[8];
+  const int chunks = CH ? CH : (K + (int)blockDim.x * 8 - 1) / ((int)blockDim.x * 8);
+  auto at = [&](int c) { return (c * (int)blockDim.x + (int)threadIdx.x) * 8; };
+  auto source = [&](long long row) { return reinterpret_cast<const T*>(p.x) + row * p.ldx; };
+  constexpr int HOLD = CH && CH <= 2 ? CH : 0;   // the factors of a thread's values stay too: all blocks read the same few lines of the L2 cache
+  float wreg[HOLD ? HOLD : 1][8];
+  auto factors = [&](int c, float (&w)[8]) { rows_values<float>(rows_load<float, VEC>(p.w, at(c), K), w); };
+  auto weight = [&](int c, float (&v)[8]) {
+    if (p.w == nullptr) return;
+    float w[8];
+    if constexpr (HOLD == 0) factors(c, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = i8_round(v[i], f);
-    auto store = [&](int8_t* out, const int (&d)[8]) {
-      if (k + 8 <= K) {
-        *reinterpret_cast<uint2*>(out + k) = make_uint2(i8_pack(d[0], d[1], d[2], d[3]), i8_pack(d[4], d[5], d[6], d[7]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i < K) out[k + i] = (int8_t)d[i];
-      }
-    };
-    if constexpr (W16) {
-      int hi[8], lo[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = (q[i] + 128) >> 8, lo[i] = q[i] - hi[i] * 256;
-      int8_t* out = p.q + 2ll * blockIdx.x * p.ldq;
-      store(out, hi), store(out + p.ldq, lo);
-    } else {
-      store(p.q + (long long)blockIdx.x * p.ldq, q);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], HOLD ? wreg[HOLD ? c : 0][i] : w[i]);
   };
+  RowsRaw<T> next[KEEP];
   if constexpr (CH > 0) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) give(c, t[c]);
-  } else {
-    for (int c = 0; c < chunks; ++c) {
-      rows_load<T, VEC>(x, (c * (int)blockDim.x + (int)threadIdx.x) * 8, K, t[0]);
-      weight((c * (int)blockDim.x + (int)threadIdx.x) * 8, t[0]);
-      give(c, t[0]);
+    for (int c = 0; c < CH; ++c) next[c] = rows_load<T, VEC>(source(blockIdx.x), at(c), K);
+  }
+  if constexpr (HOLD > 0) {
+    if (p.w != nullptr) {
+#pragma unroll
+      for (int c = 0; c < HOLD; ++c) factors(c, wreg[c]);
     }
   }
-  if (warp == 0) {
-    float s = i8_scale(most, PART);
-    if (squares) s = __fmul_rn(s, rsqrtf(i8_groups_sum(groups, (K + I8_GROUP - 1) / I8_GROUP) / (float)K + p.eps));
-    if (lane == 0) p.s[blockIdx.x] = s;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    float* groups = groups_s + turn * pieces;
+    float t[KEEP][8];
+    uint32_t most = 0;
+    auto take = [&](int c, const RowsRaw<T>& r, float (&v)[8]) {
+      rows_values<T>(r, v);
+      if (squares) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+        ss = warp_sum(ss);
+        const int g = c * nw + warp;
+        if (lane == 0 && g < pieces) groups[g] = ss;
+      }
+      weight(c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = max(most, i8_abs_bits(v[i]));
+    };
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) take(c, next[c], t[c]);
+      if (CH == 1 && row + gridDim.x < p.rows) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) next[c] = rows_load<T, VEC>(source(row + gridDim.x), at(c), K);
+      }
+    } else {
+      for (int c = 0; c < chunks; ++c) take(c, rows_load<T, VEC>(source(row), at(c), K), t[0]);
+    }
+    most = i8_warp_most(most);
+    if (lane == 0) most_s[turn][warp] = most;
+    __syncthreads();                               // (one a row: what the next row writes is the other half)
+    most = i8_warp_most(lane < nw ? most_s[turn][lane] : 0u);
+    const float f = i8_factor(most, MOST);
+    auto give = [&](int c, const float (&v)[8]) {
+      if (at(c) < K) rows_give<W16>(p, row, at(c), v, f);
+    };
+    if constexpr (CH > 0) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) give(c, t[c]);
+      if (CH > 1 && row + gridDim.x < p.rows) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) next[c] = rows_load<T, VEC>(source(row + gridDim.x), at(c), K);
+      }
+    } else {
+      for (int c = 0; c < chunks; ++c) {
+        rows_values<T>(rows_load<T, VEC>(source(row), at(c), K), t[0]);
+        weight(c, t[0]);
+        give(c, t[0]);
+      }
+    }
+    if (warp == 0) {
+      float s = i8_scale(most, PART);
+      if (squares) s = __fmul_rn(s, rsqrtf(i8_groups_sum(groups, pieces) / (float)K + p.eps));
+      if (lane == 0) p.s[row] = s;
+    }
   }
 }
 
-template <typename T, bool VEC, bool W16>
-cudaError_t rows_launch(const RowsParams& p, long long rows, cudaStream_t stream) {
-  const int vecs = (p.K + 7) / 8;
-  // vectors a thread: more of them keep more loads in flight a block, fewer leave more threads for a short row
-  const int ch = vecs <= 256 ? 1 : vecs <= 1280 ? 2 : vecs <= 2560 ? 4 : vecs <= 8192 ? 8 : 0;
-  const int threads = ch ? max(32, ((vecs + ch - 1) / ch + 31) / 32 * 32) : 1024;
-  const size_t smem = (size_t)((p.K + I8_GROUP - 1) / I8_GROUP) * sizeof(float);
+// Long rows in two digits, many of them: what a SM can hold of such a row leaves it idle between the row's maximum and its integers.  So two
+// passes, a block 2048 channels of every few rows, whose factors stay in registers: the maxima of these pieces, then the integers.
+constexpr int RL_THREADS = 256, RL_PIECE = RL_THREADS * 8;
+template <typename T, bool VEC, bool GIVE>
+__global__ void __launch_bounds__(RL_THREADS, 4) rows_long_kernel(const RowsParams p, uint32_t* most) {      // most: [pieces][rows]
+  constexpr int RL_ROWS = GIVE ? 2 : 4;            // rows at a time
+  __shared__ uint32_t most_s[2][RL_ROWS][RL_THREADS / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = blockIdx.x * RL_PIECE + threadIdx.x * 8, K = p.K;
+  float w[8];
+  rows_values<float>(rows_load<float, VEC>(p.w, min(k, K), K), w);
+  int turn = 0;
+  const long long groups = (p.rows + RL_ROWS - 1) / RL_ROWS;
+  for (long long i = blockIdx.y; i < groups; i += gridDim.y, turn ^= 1) {
+    const long long g = GIVE ? groups - 1 - i : i;      // the second pass begins with what the first one read last
+    RowsRaw<T> raw[RL_ROWS];
+    uint32_t part[RL_ROWS];
+#pragma unroll
+    for (int r = 0; r < RL_ROWS; ++r) {
+      const long long row = min(g * RL_ROWS + r, p.rows - 1);
+      raw[r] = rows_load<T, VEC>(reinterpret_cast<const T*>(p.x) + row * p.ldx, min(k, K), K);
+      if (GIVE) {
+        part[r] = 0;
+        for (int j = lane; j < (int)gridDim.x; j += 32) part[r] = max(part[r], __ldcg(most + (size_t)j * p.rows + row));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RL_ROWS; ++r) {
+      const long long row = g * RL_ROWS + r;
+      float v[8];
+      rows_values<T>(raw[r], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(v[e], w[e]);
+      if constexpr (GIVE) {
+        const uint32_t m = i8_warp_most(part[r]);
+        if (row < p.rows && k < K) rows_give<true>(p, row, k, v, i8_factor(m, I16_MOST));
+        if (row < p.rows && blockIdx.x == 0 && threadIdx.x == 0) p.s[row] = i8_scale(m, 1.f / I16_MOST);
+      } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, k < K ? i8_abs_bits(v[e]) : 0u);
+        m = i8_warp_most(m);
+        if (lane == 0) most_s[turn][r][warp] = m;
+      }
+    }
+    if constexpr (!GIVE) {
+      __syncthreads();                               // (the next rows' go into the other half)
+      if (warp < RL_ROWS && g * RL_ROWS + warp < p.rows) {
+        const uint32_t m = i8_warp_most(lane < RL_THREADS / 32 ? most_s[turn][warp][lane] : 0u);
+        if (lane == 0) most[(size_t)blockIdx.x * p.rows + g * RL_ROWS + warp] = m;
+      }
+    }
+  }
+}
+int rows_long_pieces(int K) { return (K + RL_PIECE - 1) / RL_PIECE; }
+// (up to 10240 values a row leaves registers for the next one: one pass)
+bool rows_long(long long rows, int K, int digits) { return digits == 2 && K > 10240 && rows >= 64; }
+
+template <typename T, bool VEC>
+cudaError_t rows_long_launch(const RowsParams& p, void* most, cudaStream_t stream) {
+  int sms = 0, dev = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int pieces = rows_long_pieces(p.K);
+  const dim3 grid(pieces, (unsigned)min((p.rows + 3) / 4, (long long)max(1, sms * 4 / pieces)));
+  const cudaError_t e = trl_launch(rows_long_kernel<T, VEC, false>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
+  return e != cudaSuccess ? e : trl_launch(rows_long_kernel<T, VEC, true>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
+}
+
+template <typename T, int CH, bool VEC, bool W16>
+cudaError_t rows_launch(const RowsParams& p, int threads, cudaStream_t stream) {
+  auto kern = rows_i8_kernel<T, CH, VEC, W16>;
+  const size_t smem = 2 * (size_t)((p.K + I8_GROUP - 1) / I8_GROUP) * sizeof(float);
   if (smem > 48 * 1024) return cudaErrorInvalidValue;
+  // blocks that fit the GPU at a time
+  static TrlPerDevice<int> fit[33];
+  int& known = fit[threads / 32].here();
+  if (known == 0) {
+    int sms = 0, dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0);
+    if (e != cudaSuccess) return e;
+    known = sms * max(n, 1);
+  }
+  return trl_launch(kern, dim3((unsigned)min(p.rows, (long long)known)), dim3(threads), smem, stream, p);
+}
+template <typename T, bool VEC, bool W16>
+cudaError_t rows_launch(const RowsParams& p, cudaStream_t stream) {
+  const int vecs = (p.K + 7) / 8;
+  // Rows up to 5120 values: a vector a thread, two blocks or more a SM, the next row on its way.  Longer ones: as few vectors a thread as there are
+  // threads for.  From 40960 values on a row is read a second time, out of L2.
+  const int ch = vecs <= 640 ? 1 : vecs <= 2048 ? 2 : vecs <= 5120 ? (vecs + 1023) / 1024 : 0, threads = ch ? max(32, ((vecs + ch - 1) / ch + 31) / 32 * 32) : 1024;
   switch (ch) {
-    case 1: return trl_launch(rows_i8_kernel<T, 1, VEC, W16>, dim3((unsigned)rows), dim3(threads), smem, stream, p);
-    case 2: return trl_launch(rows_i8_kernel<T, 2, VEC, W16>, dim3((unsigned)rows), dim3(threads), smem, stream, p);
-    case 4: return trl_launch(rows_i8_kernel<T, 4, VEC, W16>, dim3((unsigned)rows), dim3(threads), smem, stream, p);
-    case 8: return trl_launch(rows_i8_kernel<T, 8, VEC, W16>, dim3((unsigned)rows), dim3(threads), smem, stream, p);
-    default: return trl_launch(rows_i8_kernel<T, 0, VEC, W16>, dim3((unsigned)rows), dim3(threads), smem, stream, p);
+    case 1: return rows_launch<T, 1, VEC, W16>(p, threads, stream);
+    case 2: return rows_launch<T, 2, VEC, W16>(p, threads, stream);
+    case 3: return rows_launch<T, 3, VEC, W16>(p, threads, stream);
+    case 4: return rows_launch<T, 4, VEC, W16>(p, threads, stream);
+    case 5: return rows_launch<T, 5, VEC, W16>(p, threads, stream);
+    default: return rows_launch<T, 0, VEC, W16>(p, threads, stream);
   }
 }
 
 }  // namespace
 
+// Bytes of scratch that trl_rows_i8 takes for so many rows.
+TRL_API long trl_rows_i8_scratch(long rows, int K, int digits) { return rows_long(rows, K, digits) ? 4l * rows_long_pieces(K) * rows : 0; }
+
 // x [rows, K] (type 0: fp32, 1: bf16; rows ldx apart) -> q int8 [rows, ldq], s fp32 [rows].  w: fp32 [K] or null; norm: w is a norm's
-// weight, and the row's 1 / rms goes into s.  digits 2: q has two rows of digits a row, 16 bits in all, and w is not a norm's.
-// weights: q and s are a weight's.  ldq and q on 8-byte boundaries.
+// weight, and the row's 1 / rms goes into s.  digits 2: q has two rows of digits a row, 16 bits in all, and w is the channels' scales.
+// weights: q and s are a weight's.  ldq and q on 8-byte boundaries, scratch on 4.
 TRL_API int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K,
-                        int digits, int weights, void* stream) {
+                        int digits, int weights, void* scratch, void* stream) {
   if (rows <= 0 || rows > 0x7fffffffl || K <= 0 || ldq < K || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || (type != 0 && type != 1) ||
-      (digits != 1 && digits != 2) || (norm && (w == nullptr || digits == 2)))
+      (digits != 1 && digits != 2) || (norm && (w == nullptr || digits == 2)) || (digits == 2 && w == nullptr) ||
+      (scratch == nullptr && trl_rows_i8_scratch(rows, K, digits)))
     return (int)cudaErrorInvalidValue;
-  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, K, eps, norm, weights};
+  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, rows, K, eps, norm, weights};
   cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (type ? 8 : 4) == 0;
-  if (type) {
-    if (digits == 2) return (int)(vec ? rows_launch<bf16, true, true>(p, rows, st) : rows_launch<bf16, false, true>(p, rows, st));
-    return (int)(vec ? rows_launch<bf16, true, false>(p, rows, st) : rows_launch<bf16, false, false>(p, rows, st));
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || ldx % (type ? 8 : 4) == 0) && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+  if (rows_long(rows, K, digits)) {
+    if (type) return (int)(vec ? rows_long_launch<bf16, true>(p, scratch, st) : rows_long_launch<bf16, false>(p, scratch, st));
+    return (int)(vec ? rows_long_launch<float, true>(p, scratch, st) : rows_long_launch<float, false>(p, scratch, st));
   }
-  if (digits == 2) return (int)(vec ? rows_launch<float, true, true>(p, rows, st) : rows_launch<float, false, true>(p, rows, st));
-  return (int)(vec ? rows_launch<float, true, false>(p, rows, st) : rows_launch<float, false, false>(p, rows, st));
+  if (type) {
+    if (digits == 2) return (int)(vec ? rows_launch<bf16, true, true>(p, st) : rows_launch<bf16, false, true>(p, st));
+    return (int)(vec ? rows_launch<bf16, true, false>(p, st) : rows_launch<bf16, false, false>(p, st));
+  }
+  if (digits == 2) return (int)(vec ? rows_launch<float, true, true>(p, st) : rows_launch<float, false, true>(p, st));
+  return (int)(vec ? rows_launch<float, true, false>(p, st) : rows_launch<float, false, false>(p, st));
 }

@@ -74,6 +74,21 @@ def test_rows_give_the_integers_of_the_definition(t, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_one_after_the_other_and_long_ones_in_two_passes(dtype):
+    for t, k in ((1500, 24), (1300, 2056), (700, 10264), (64, 10248), (67, 20487), (130, 34816), (3, 34816)):
+        x, w = _x(t, k, k, dtype), torch.rand(k, device=DEV) + 0.5
+        x[t // 2] = 0.0
+        x[t - 1, k - 1] = float("nan")
+        q, s = _quant(x, channels=w)
+        want, scale = F.quantize_grad_int16(x, w)
+        q = q.view(t, 2, k)
+        assert torch.equal(q[:, 0].int() * 256 + q[:, 1].int(), want) and torch.equal(s.nan_to_num(-1.0), scale.nan_to_num(-1.0)) and torch.isnan(s[-1])
+        q, s = _quant(x, w, 1e-6)
+        want, _ = F._row_integers(x.float() * w, F.INT8_MAX)
+        assert torch.equal(q, want.to(torch.int8)) and torch.isnan(s[-1]) and torch.isfinite(s[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_off_every_boundary_and_apart(dtype):
     base = _x(9, 517, 3, dtype)
     for x in (base[:, 1:], base[::2, :515], base.flatten()[3:3 + 4 * 100].view(4, 100)):

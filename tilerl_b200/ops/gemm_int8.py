@@ -20,14 +20,16 @@ EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
 
-N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.P])
-N.register("trl_gemm_i8", [N.P, N.L, N.P, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.I, N.P])
-N.register("trl_gemm_i8_grad", [N.P, N.L, N.P, N.L, N.P, N.P, N.L, N.I, N.I, N.I, N.P])
+N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.P, N.P])
+N.register("trl_rows_i8_scratch", [N.L, N.I, N.I], N.L)
+N.register("trl_linear_i8_grad_scratch", [N.I, N.I], N.L)
+N.register("trl_linear_i8", [N.P, N.I, N.L, N.P, N.F, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.P, N.I, N.I, N.I, N.I, N.P])
+N.register("trl_linear_i8_grad", [N.P, N.I, N.L, N.P, N.L, N.P, N.P, N.L, N.P, N.I, N.I, N.I, N.P])
 
 
 def there() -> bool:
     """The library has these kernels (one that serves a single architecture has not)."""
-    return N.has("trl_gemm_i8")
+    return N.has("trl_linear_i8")
 
 
 def takes(w: INT8Tensor) -> bool:
@@ -59,28 +61,31 @@ def _refuse(x: torch.Tensor, w: INT8Tensor, y=None, norm_w=None, residual=None, 
 def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None, weights: bool = False) -> None:
     """Rows ``x [T, K]`` into ``q`` (int8 ``[T, >= K]``) and ``s`` (fp32 ``[T]``); with ``channels`` (a gradient's scales) into two rows of digits
     a row of ``x``.  ``weights``: they are a weight's, which products load before they wait for the launch ahead of them."""
+    some = N.lib().trl_rows_i8_scratch(x.shape[0], x.shape[1], 1 if channels is None else 2)
+    scratch = torch.empty(some, dtype=torch.int8, device=x.device) if some else None
     N.check(N.lib().trl_rows_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(channels if norm_w is None else norm_w), int(norm_w is not None), eps,
-                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, int(weights), N.stream()), "rows_i8")
-    N.count()
+                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, int(weights), N.ptr(scratch), N.stream()), "rows_i8")
+    N.count(2 if some else 1)
 
 
-def _gemm(w, q, s, y, residual, epi) -> None:
-    n, k = w.shape
-    N.check(N.lib().trl_gemm_i8(w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(), q.data_ptr(), q.stride(0), s.data_ptr(), N.ptr(residual),
-                                residual.stride(0) if residual is not None else 0, y.data_ptr(), y.stride(0), q.shape[0], n, k, epi, N.stream()), "gemm_i8")
-    N.count()
+def _product(x, w, out, ldo, scratch, norm_w, eps, residual, epi) -> None:
+    n, k = w.w8.shape
+    rc = N.lib().trl_linear_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(norm_w), eps, w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(),
+                               N.ptr(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(), ldo, scratch.data_ptr(),
+                               x.shape[0], n, k, epi, N.stream())
+    if rc >= 0:
+        N.check(rc or -1, "linear_i8")
+    N.count(-rc)
 
 
 def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) -> None:
     """``y = epi(norm(x) @ W^T)``; ``y`` may be the residual."""
     _refuse(x, w, y, norm_w, residual, epi)
-    t, (n, k) = x.shape[0], w.shape
+    t = x.shape[0]
     if t == 0:
         return
     with N.on(x.device):
-        q, s = ops.ws.get("int8_q", (t, k), torch.int8), ops.ws.get("int8_s", (t,), torch.float32)
-        quant_rows(x, q, s, norm_w=norm_w, eps=eps)
-        _gemm(w, q, s, y, residual, epi)
+        _product(x, w, y, y.stride(0), ops.ws.get("int8_rows", (t * (x.shape[1] + 4),), torch.int8), norm_w, eps, residual, epi)
 
 
 # ---- the training tape ------------------------------------------------------------------------------------
@@ -98,9 +103,8 @@ def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     with N.on(x.device):
         out = torch.empty(*x.shape[:-1], n, dtype=torch.float32, device=x.device)
         if rows.shape[0]:
-            q, s = torch.empty(rows.shape, dtype=torch.int8, device=x.device), torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
-            quant_rows(rows, q, s)
-            _gemm(w, q, s, out.view(-1, n), None, EPI_STORE_F32)
+            scratch = torch.empty(rows.shape[0] * (k + 4), dtype=torch.int8, device=x.device)
+            _product(rows, w, out, n, scratch, None, 0.0, None, EPI_STORE_F32)
     return out
 
 
@@ -114,11 +118,10 @@ def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     with N.on(g.device):
         dx = torch.empty(*g.shape[:-1], k, dtype=torch.float32, device=g.device)
         if t:
-            q, s = torch.empty(2 * t, -(-n // 16) * 16, dtype=torch.int8, device=g.device), torch.empty(t, dtype=torch.float32, device=g.device)
-            quant_rows(rows, q, s, channels=w.wscale)
-            N.check(N.lib().trl_gemm_i8_grad(w.w8.data_ptr(), w.w8.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), dx.data_ptr(), k, t, n, k, N.stream()),
-                    "gemm_i8_grad")
-            N.count()
+            scratch = torch.empty(N.lib().trl_linear_i8_grad_scratch(t, n), dtype=torch.int8, device=g.device)
+            N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(),
+                                               dx.data_ptr(), k, scratch.data_ptr(), t, n, k, N.stream()), "linear_i8_grad")
+            N.count(2)
     return dx
 
 
