@@ -18,6 +18,25 @@
 #include "int8.cuh"
 #include "tcgen05_pair.cuh"
 
+typedef CUresult (*EncodeTiledFnI)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A tensor map of [rows, width] bytes, rows ld apart, in pieces of 128 bytes x box_rows; what lies outside reads as zero
+bool i8_tensor(CUtensorMap* m, const void* base, long long width, long long rows, long long ld, int box_rows) {
+  static EncodeTiledFnI encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn) return false;
+    encode = (EncodeTiledFnI)fn;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 constexpr int GI_ROWS = 128;                      // features a SM
@@ -337,25 +356,6 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   gp_cluster_sync();                                // no CTA leaves while the other's half is being given back
 }
 
-typedef CUresult (*EncodeTiledFnI)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// [rows, width] bytes, rows ld apart, in pieces of 128 bytes x box_rows; what lies outside reads as zero
-bool gi_tensor(CUtensorMap* m, const void* base, long long width, long long rows, long long ld, int box_rows) {
-  static EncodeTiledFnI encode = nullptr;
-  if (!encode) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn) return false;
-    encode = (EncodeTiledFnI)fn;
-  }
-  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t box[2] = {GI_KT, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int BN, bool GRAD, bool SPLIT>
 cudaError_t gi_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], int ctas, int parts, cudaStream_t stream) {
   auto kern = gemm_i8_kernel<BN, GRAD, SPLIT>;
@@ -401,10 +401,7 @@ struct I8Plan {
 // Columns a tile and pairs a tile: the least of rounds x stages x (time of a stage) + what putting parts together costs, in stages of 128
 // columns.
 I8Plan gi_plan(int cols, int features, int nk) {
-  int sms = 0, dev = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int pairs = sms / 2, r_tiles = (features + 2 * GI_ROWS - 1) / (2 * GI_ROWS);
+  const int pairs = i8_sms() / 2, r_tiles = (features + 2 * GI_ROWS - 1) / (2 * GI_ROWS);
   static const struct { int bn; double unit, exchange; } forms[] = {{64, 0.9, 3}, {128, 1, 5}, {192, 1.5, 8}, {256, 2, 10}};
   I8Plan best{0, 1, pairs};
   double least = 0;
@@ -424,7 +421,7 @@ template <int BN, bool GRAD>
 int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int width, int rows, I8Params p, const I8Plan& plan, cudaStream_t stream) {
   constexpr int J = GRAD ? 2 : 1;
   CUtensorMap mw, mq;
-  if (!gi_tensor(&mw, w, width, rows, ldw, GI_ROWS) || !gi_tensor(&mq, q, p.depth, (long long)p.tokens * J, ldq, BN / 2)) return (int)cudaErrorInvalidValue;
+  if (!i8_tensor(&mw, w, width, rows, ldw, GI_ROWS) || !i8_tensor(&mq, q, p.depth, (long long)p.tokens * J, ldq, BN / 2)) return (int)cudaErrorInvalidValue;
   p.r_tiles = (p.features + 2 * GI_ROWS - 1) / (2 * GI_ROWS), p.c_tiles = (p.tokens * J + BN - 1) / BN, p.parts = plan.parts;
   const long long tiles = (long long)p.r_tiles * p.c_tiles;
   if (tiles > 0x7fffffffll / p.nk) return (int)cudaErrorInvalidValue;
@@ -481,12 +478,11 @@ static int gi_grad(const void* w, long ldw, const void* q, long ldq, const void*
   return gi_launch<true>(w, ldw, q, ldq, K, N, p, (cudaStream_t)stream);
 }
 
-int gemv_i8_takes(int T, int N, int K);
-int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long ldx, const void* s, const void* norm_w, float eps, const void* residual,
-                   long ldr, void* out, long ldo, int T, int N, int K, int epi, int quantised, cudaStream_t stream);
+bool gemv_i8_takes(int T, int N, int K);
+int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr,
+                   void* out, long ldo, int T, int N, int K, int epi, cudaStream_t stream);
 extern "C" int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K, int digits,
                            int weights, void* scratch, void* stream);
-extern "C" long trl_rows_i8_scratch(long rows, int K, int digits);
 
 // out[t, n] = epi(norm(x) . w): rows of x (type 0: fp32, 1: bf16) quantised, multiplied.  norm_w: a norm's weight, or null.  scratch: T * K
 // bytes for the integers and 4 * T for the scales, on a 16-byte boundary, K % 16 == 0.  Otherwise as above.  Returns minus the number of launches,
@@ -496,24 +492,19 @@ TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w,
   if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || K % 16 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, scratch, K))
     return (int)cudaErrorInvalidValue;
-  const int few = gemv_i8_takes(T, N, K);
   const bool whole = type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;
-  if (few == 1 && whole) {
-    const int rc = gemv_i8_launch(w, ldw, ws, x, ldx, nullptr, norm_w, eps, residual, ldr, out, ldo, T, N, K, epi, 0, (cudaStream_t)stream);
+  if (whole && gemv_i8_takes(T, N, K)) {
+    const int rc = gemv_i8_launch(w, ldw, ws, x, ldx, norm_w, eps, residual, ldr, out, ldo, T, N, K, epi, (cudaStream_t)stream);
     return rc ? rc : -1;
   }
   void* s = (int8_t*)scratch + (size_t)T * K;
   int rc = trl_rows_i8(x, type, ldx, norm_w, norm_w != nullptr, eps, scratch, K, s, T, K, 1, 0, nullptr, stream);
-  if (rc) return rc;
-  rc = few ? gemv_i8_launch(w, ldw, ws, scratch, K, s, nullptr, 0.f, residual, ldr, out, ldo, T, N, K, epi, 1, (cudaStream_t)stream)
-           : gi_linear(w, ldw, ws, scratch, K, s, residual, ldr, out, ldo, T, N, K, epi, stream);
+  if (!rc) rc = gi_linear(w, ldw, ws, scratch, K, s, residual, ldr, out, ldo, T, N, K, epi, stream);
   return rc ? rc : -2;
 }
 
-// Bytes of scratch that trl_linear_i8_grad takes: rows in digits, their scales, the row quantiser's own.
-TRL_API long trl_linear_i8_grad_scratch(int T, int N) { return 2l * T * ((N + 15) / 16 * 16) + 4l * T + trl_rows_i8_scratch(T, N, 2); }
-
-// dx[t, k] of g [T, N] (type 0: fp32, 1: bf16).  scratch on a 16-byte boundary.
+// dx[t, k] of g [T, N] (type 0: fp32, 1: bf16).  scratch on a 16-byte boundary: 2 * T rows of N rounded up to 16 bytes, 4 * T for the scales, and 4 * T
+// for every 2048 channels.
 TRL_API int trl_linear_i8_grad(const void* g, int type, long ldg, const void* w, long ldw, const void* ws, void* dx, long ldo, void* scratch, int T, int N, int K,
                                void* stream) {
   if (T <= 0 || N <= 0 || N > GI_MOST) return (int)cudaErrorInvalidValue;

@@ -45,4 +45,16 @@ __device__ __forceinline__ float i8_swiglu(float gate, float up) { return __fmul
 
 enum { I8_STORE = 0, I8_RESIDUAL = 1, I8_SWIGLU = 2, I8_STORE_F32 = 3 };
 
+// SMs of the current device (host).
+inline int i8_sms() {
+  static TrlPerDevice<int> counts;
+  int& n = counts.here();
+  if (n == 0) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  }
+  return n;
+}
+
 }  // namespace

@@ -242,10 +242,7 @@ bool rows_long(long long rows, int K, int digits) { return digits == 2 && K > 10
 
 template <typename T, bool VEC>
 cudaError_t rows_long_launch(const RowsParams& p, void* most, cudaStream_t stream) {
-  int sms = 0, dev = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int pieces = rows_long_pieces(p.K);
+  const int sms = i8_sms(), pieces = rows_long_pieces(p.K);
   const dim3 grid(pieces, (unsigned)min((p.rows + 3) / 4, (long long)max(1, sms * 4 / pieces)));
   const cudaError_t e = trl_launch(rows_long_kernel<T, VEC, false>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
   return e != cudaSuccess ? e : trl_launch(rows_long_kernel<T, VEC, true>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
@@ -260,12 +257,10 @@ cudaError_t rows_launch(const RowsParams& p, int threads, cudaStream_t stream) {
   static TrlPerDevice<int> fit[33];
   int& known = fit[threads / 32].here();
   if (known == 0) {
-    int sms = 0, dev = 0, n = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int n = 0;
     const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0);
     if (e != cudaSuccess) return e;
-    known = sms * max(n, 1);
+    known = i8_sms() * max(n, 1);
   }
   return trl_launch(kern, dim3((unsigned)min(p.rows, (long long)known)), dim3(threads), smem, stream, p);
 }
@@ -287,17 +282,14 @@ cudaError_t rows_launch(const RowsParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Bytes of scratch that trl_rows_i8 takes for so many rows.
-TRL_API long trl_rows_i8_scratch(long rows, int K, int digits) { return rows_long(rows, K, digits) ? 4l * rows_long_pieces(K) * rows : 0; }
-
 // x [rows, K] (type 0: fp32, 1: bf16; rows ldx apart) -> q int8 [rows, ldq], s fp32 [rows].  w: fp32 [K] or null; norm: w is a norm's
 // weight, and the row's 1 / rms goes into s.  digits 2: q has two rows of digits a row, 16 bits in all, and w is the channels' scales.
-// weights: q and s are a weight's.  ldq and q on 8-byte boundaries, scratch on 4.
+// weights: q and s are a weight's.  scratch: 4 bytes a row for every 2048 of its values (two digits only).  ldq and q on 8-byte boundaries.
 TRL_API int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K,
                         int digits, int weights, void* scratch, void* stream) {
   if (rows <= 0 || rows > 0x7fffffffl || K <= 0 || ldq < K || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || (type != 0 && type != 1) ||
       (digits != 1 && digits != 2) || (norm && (w == nullptr || digits == 2)) || (digits == 2 && w == nullptr) ||
-      (scratch == nullptr && trl_rows_i8_scratch(rows, K, digits)))
+      (scratch == nullptr && digits == 2))
     return (int)cudaErrorInvalidValue;
   RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, rows, K, eps, norm, weights};
   cudaStream_t st = (cudaStream_t)stream;

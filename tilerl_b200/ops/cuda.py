@@ -25,6 +25,7 @@ from typing import Dict, Optional
 import torch
 
 from ..formats import FP8BlockTensor, INT8Tensor, NVFP4Tensor
+from . import gemm_int8
 from . import native as N
 from .cuda_blocks import BlockOps
 from .cuda_gated import GatedOps
@@ -287,7 +288,6 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
             from . import gemm_fp8
             gemm_fp8.gemv(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
         elif isinstance(w, INT8Tensor):
-            from . import gemm_int8
             gemm_int8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
         else:
             raise TypeError(f"no GEMV for weight type {type(w)}")
@@ -307,6 +307,10 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
 
     def _linear(self, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE):
         """``y = epi(norm(x) @ W^T)`` with everything fused into one or two kernels."""
+        if isinstance(w, INT8Tensor):
+            self.settle()
+            gemm_int8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
+            return
         t = x.shape[0]
         if not (t <= GEMV_MAX_M and not self._tc(w, t)):
             self.settle()     # only the GEMV path can finish a pending all-reduce itself
@@ -314,11 +318,6 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
             from . import gemm_fp8
             self.settle()
             gemm_fp8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
-            return
-        if isinstance(w, INT8Tensor):
-            from . import gemm_int8
-            self.settle()
-            gemm_int8.linear(self, x, w, y, norm_w=norm_w, eps=eps, residual=residual, epi=epi)
             return
         if (self._tc(w, t) and self.gemv_mma and t <= self.mma_tokens and x.shape[1] <= self.mma_kmax
                 and not self.decode_tc and x.stride(0) % 8 == 0):
@@ -775,7 +774,6 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
 
     def quantize_int8_(self, w: torch.Tensor, dst: INT8Tensor) -> None:
         """Re-pack ``w`` (fp32 or bf16 ``[N, K]``) into ``dst`` in place."""
-        from . import gemm_int8
         gemm_int8.quantize_(w, dst)
 
     def read_device_error(self, clear: bool = True):

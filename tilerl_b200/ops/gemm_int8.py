@@ -11,6 +11,8 @@ The reference multiplies in FP8 (``linear_fp8``, packages/tilerl-kernels/src/til
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional
+
 import torch
 
 from ..formats import INT8Tensor
@@ -21,8 +23,6 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1}
 MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
 
 N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.P, N.P])
-N.register("trl_rows_i8_scratch", [N.L, N.I, N.I], N.L)
-N.register("trl_linear_i8_grad_scratch", [N.I, N.I], N.L)
 N.register("trl_linear_i8", [N.P, N.I, N.L, N.P, N.F, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.P, N.I, N.I, N.I, N.I, N.P])
 N.register("trl_linear_i8_grad", [N.P, N.I, N.L, N.P, N.L, N.P, N.P, N.L, N.P, N.I, N.I, N.I, N.P])
 
@@ -32,47 +32,81 @@ def there() -> bool:
     return N.has("trl_linear_i8")
 
 
-def takes(w: INT8Tensor) -> bool:
+class _Ready(NamedTuple):
+    """A weight that the kernels read, looked over once."""
+    w8: torch.Tensor
+    wscale: torch.Tensor
+    n: int
+    k: int
+    ptr: int
+    ld: int
+    scales: int
+    device: int
+
+
+def _ready(w: INT8Tensor) -> Optional[_Ready]:
     """Weights that the kernels read: rows of whole 16-byte pieces, on such a boundary, and sums that 32 bits hold."""
-    n, k = w.shape
-    return (w.w8.is_cuda and w.wscale.device == w.w8.device and w.wscale.is_contiguous() and 0 < k <= MOST and 0 < n <= MOST and k % 16 == 0
-            and w.w8.stride(1) == 1 and w.w8.stride(0) % 16 == 0 and w.w8.stride(0) >= k and w.w8.data_ptr() % 16 == 0)
+    r = w.__dict__.get("_ready")
+    if r is not None and r.w8 is w.w8 and r.wscale is w.wscale and r.ptr == r.w8.data_ptr() and r.scales == r.wscale.data_ptr():
+        return r
+    w8, ws = w.w8, w.wscale
+    n, k = w8.shape
+    fits = (w8.is_cuda and ws.device == w8.device and ws.is_contiguous() and 0 < k <= MOST and 0 < n <= MOST and k % 16 == 0
+            and w8.stride(1) == 1 and w8.stride(0) % 16 == 0 and w8.stride(0) >= k and w8.data_ptr() % 16 == 0)
+    r = w.__dict__["_ready"] = _Ready(w8, ws, n, k, w8.data_ptr(), w8.stride(0), ws.data_ptr(), w8.get_device()) if fits else None
+    return r
 
 
-def _refuse(x: torch.Tensor, w: INT8Tensor, y=None, norm_w=None, residual=None, epi=EPI_STORE) -> None:
-    if not takes(w):
+def takes(w: INT8Tensor) -> bool:
+    return _ready(w) is not None
+
+
+def _refuse(x, w, y, norm_w, residual, epi) -> _Ready:
+    r = _ready(w)
+    if r is None:
         raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, up to {MOST} rows and columns, on "
                          f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
-    if x.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype not in TYPES or x.device != w.w8.device or x.stride(1) != 1 and x.shape[1] > 1:
-        raise ValueError(f"INT8 products take fp32 or bf16 rows [T, {w.shape[1]}] on the weight's device, got {tuple(x.shape)} {x.dtype} on {x.device}")
-    t, (n, k) = x.shape[0], w.shape
-    if epi == EPI_SWIGLU and n % 2:
-        raise ValueError(f"SwiGLU takes rows in (gate, up) pairs, got {n}")
-    kind = torch.float32 if epi == EPI_STORE_F32 else torch.bfloat16
-    if tuple(y.shape) != (t, n // 2 if epi == EPI_SWIGLU else n) or y.dtype != kind or y.device != x.device or t and y.stride(1) != 1 and y.shape[1] > 1:
+    shape, n, k, here = x.shape, r.n, r.k, r.device
+    if len(shape) != 2 or shape[1] != k or x.dtype not in TYPES or x.get_device() != here or x.stride(1) != 1 and k > 1:
+        raise ValueError(f"INT8 products take fp32 or bf16 rows [T, {k}] on the weight's device, got {tuple(shape)} {x.dtype} on {x.device}")
+    t, width, kind = shape[0], n, torch.bfloat16
+    if epi == EPI_SWIGLU:
+        if n % 2:
+            raise ValueError(f"SwiGLU takes rows in (gate, up) pairs, got {n}")
+        width = n // 2
+    elif epi == EPI_STORE_F32:
+        kind = torch.float32
+    if y.shape != (t, width) or y.dtype != kind or y.get_device() != here or t and y.stride(1) != 1 and width > 1:
         raise ValueError(f"the output of {t} rows by {n} channels is {kind} with channels side by side, got {tuple(y.shape)} {y.dtype} on {y.device}")
-    if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and (
-            residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.device != x.device or residual.stride(1) != 1 and n > 1):
+    if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and residual is not y and (
+            residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.get_device() != here or residual.stride(1) != 1 and n > 1):
         raise ValueError("a residual is bf16 rows of the output's shape, given where one is added")
-    if norm_w is not None and (norm_w.shape != (k,) or norm_w.dtype != torch.float32 or norm_w.device != x.device or not norm_w.is_contiguous()):
+    if norm_w is not None and (norm_w.shape != (k,) or norm_w.dtype != torch.float32 or norm_w.get_device() != here or not norm_w.is_contiguous()):
         raise ValueError(f"a norm's weight is fp32 [{k}] on the rows' device, got {tuple(norm_w.shape)} {norm_w.dtype} on {norm_w.device}")
+    return r
+
+
+def _scratch(rows: int, width: int, digits: int = 1) -> int:
+    """Bytes that the kernels want for rows in 8 bits or in two digits: the integers, a scale a row, and of long rows in digits the largest of every
+    2048 values."""
+    if digits == 1:
+        return rows * (width + 4)
+    return rows * (2 * (-(-width // 16) * 16) + 4 + 4 * -(-width // 2048))
 
 
 def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None, weights: bool = False) -> None:
     """Rows ``x [T, K]`` into ``q`` (int8 ``[T, >= K]``) and ``s`` (fp32 ``[T]``); with ``channels`` (a gradient's scales) into two rows of digits
     a row of ``x``.  ``weights``: they are a weight's, which products load before they wait for the launch ahead of them."""
-    some = N.lib().trl_rows_i8_scratch(x.shape[0], x.shape[1], 1 if channels is None else 2)
-    scratch = torch.empty(some, dtype=torch.int8, device=x.device) if some else None
+    scratch = None if channels is None else torch.empty(x.shape[0] * -(-x.shape[1] // 2048), dtype=torch.int32, device=x.device)
     N.check(N.lib().trl_rows_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(channels if norm_w is None else norm_w), int(norm_w is not None), eps,
                                 q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, int(weights), N.ptr(scratch), N.stream()), "rows_i8")
-    N.count(2 if some else 1)
+    N.count()
 
 
-def _product(x, w, out, ldo, scratch, norm_w, eps, residual, epi) -> None:
-    n, k = w.w8.shape
-    rc = N.lib().trl_linear_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(norm_w), eps, w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(),
-                               N.ptr(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(), ldo, scratch.data_ptr(),
-                               x.shape[0], n, k, epi, N.stream())
+def _product(x, r: _Ready, out, ldo, scratch, norm_w, eps, residual, epi) -> None:
+    rc = N.lib().trl_linear_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps, r.ptr, r.ld, r.scales,
+                               None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), ldo,
+                               scratch.data_ptr(), x.shape[0], r.n, r.k, epi, N.stream())
     if rc >= 0:
         N.check(rc or -1, "linear_i8")
     N.count(-rc)
@@ -80,47 +114,53 @@ def _product(x, w, out, ldo, scratch, norm_w, eps, residual, epi) -> None:
 
 def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) -> None:
     """``y = epi(norm(x) @ W^T)``; ``y`` may be the residual."""
-    _refuse(x, w, y, norm_w, residual, epi)
+    r = _refuse(x, w, y, norm_w, residual, epi)
     t = x.shape[0]
     if t == 0:
         return
     with N.on(x.device):
-        _product(x, w, y, y.stride(0), ops.ws.get("int8_rows", (t * (x.shape[1] + 4),), torch.int8), norm_w, eps, residual, epi)
+        _product(x, r, y, y.stride(0), ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8), norm_w, eps, residual, epi)
 
 
 # ---- the training tape ------------------------------------------------------------------------------------
 def train_takes(x: torch.Tensor, w: INT8Tensor) -> bool:
     """Rows that the kernels take as they are; the torch forms serve the rest."""
-    return x.is_cuda and there() and takes(w) and x.dtype in TYPES and x.device == w.w8.device and x.dim() >= 1 and x.shape[-1] == w.shape[1]
+    if not x.is_cuda or not there() or x.dtype not in TYPES or x.dim() < 1:
+        return False
+    r = _ready(w)
+    return r is not None and x.get_device() == r.device and x.shape[-1] == r.k
+
+
+def _flat(x: torch.Tensor, width: int) -> torch.Tensor:
+    if x.dim() != 2:
+        x = x.reshape(-1, width)
+    return x if x.stride(1) == 1 else x.contiguous()
 
 
 def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     """``x [..., K]`` -> fp32 ``[..., N]``."""
-    n, k = w.shape
-    rows = x.reshape(-1, k)
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
+    r = _ready(w)
+    rows = _flat(x, r.k)
+    t = rows.shape[0]
     with N.on(x.device):
-        out = torch.empty(*x.shape[:-1], n, dtype=torch.float32, device=x.device)
-        if rows.shape[0]:
-            scratch = torch.empty(rows.shape[0] * (k + 4), dtype=torch.int8, device=x.device)
-            _product(rows, w, out, n, scratch, None, 0.0, None, EPI_STORE_F32)
+        out = torch.empty(*x.shape[:-1], r.n, dtype=torch.float32, device=x.device)
+        if t:
+            _product(rows, r, out, r.n, torch.empty(_scratch(t, r.k), dtype=torch.int8, device=x.device), None, 0.0, None, EPI_STORE_F32)
     return out
 
 
 def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     """Gradient of ``forward``'s input, the rounding of ``x`` taken for none: ``g [..., N]`` -> fp32 ``[..., K]``."""
-    n, k = w.shape
-    rows = (g if g.dtype in TYPES else g.float()).reshape(-1, n)
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
+    r = _ready(w)
+    n, k = r.n, r.k
+    rows = _flat(g if g.dtype in TYPES else g.float(), n)
     t = rows.shape[0]
     with N.on(g.device):
         dx = torch.empty(*g.shape[:-1], k, dtype=torch.float32, device=g.device)
         if t:
-            scratch = torch.empty(N.lib().trl_linear_i8_grad_scratch(t, n), dtype=torch.int8, device=g.device)
-            N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), w.w8.data_ptr(), w.w8.stride(0), w.wscale.data_ptr(),
-                                               dx.data_ptr(), k, scratch.data_ptr(), t, n, k, N.stream()), "linear_i8_grad")
+            scratch = torch.empty(_scratch(t, n, 2), dtype=torch.int8, device=g.device)
+            N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), r.ptr, r.ld, r.scales, dx.data_ptr(), k,
+                                               scratch.data_ptr(), t, n, k, N.stream()), "linear_i8_grad")
             N.count(2)
     return dx
 
@@ -128,7 +168,7 @@ def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
 # ---- weights ---------------------------------------------------------------------------------------------------
 def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
     """fp32 or bf16 ``[N, K]`` into ``dst`` in place, as ``formats.quantize_int8`` gives it."""
-    if not takes(dst) or src.shape != dst.w8.shape or src.dtype not in TYPES or src.device != dst.w8.device:
+    if _ready(dst) is None or src.shape != dst.w8.shape or src.dtype not in TYPES or src.device != dst.w8.device:
         raise ValueError(f"quantize_ takes fp32 or bf16 of {dst.shape} on the weight's device, got {tuple(src.shape)} {src.dtype} on {src.device}")
     src = src if src.stride(1) == 1 else src.contiguous()
     with N.on(src.device):
