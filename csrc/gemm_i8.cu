@@ -83,51 +83,46 @@ __device__ __forceinline__ int4 gi_ld_cluster(uint32_t addr) {
   return v;
 }
 
-// Eight features of a token out (v: results before the residual); those past the last one are left out.
+__device__ __forceinline__ int gi_ld1_cluster(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Eight features of a token out as one vector (v: results before the residual).
 __device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8]) {
   if (tok >= p.tokens || f >= p.features) return;
   const size_t at = (size_t)tok * p.ldo;
   if (p.epi == I8_SWIGLU) {                          // features in (gate, up) pairs
-    bf16* o = reinterpret_cast<bf16*>(p.out) + at + (f >> 1);
-    const float a = i8_swiglu(v[0], v[1]), b = i8_swiglu(v[2], v[3]), c = i8_swiglu(v[4], v[5]), d = i8_swiglu(v[6], v[7]);
-    if (p.vec) {
-      *reinterpret_cast<uint2*>(o) = make_uint2(f2_to_bf162_bits(a, b), f2_to_bf162_bits(c, d));
-    } else {
-      const float y[4] = {a, b, c, d};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (f + 2 * i < p.features) o[i] = __float2bfloat16(y[i]);
-    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.out) + at + (f >> 1)) =
+        make_uint2(f2_to_bf162_bits(i8_swiglu(v[0], v[1]), i8_swiglu(v[2], v[3])), f2_to_bf162_bits(i8_swiglu(v[4], v[5]), i8_swiglu(v[6], v[7])));
   } else if (p.epi == I8_STORE_F32) {
-    float* o = reinterpret_cast<float*>(p.out) + at + f;
-    if (p.vec) {
-      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (f + i < p.features) o[i] = v[i];
-    }
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at + f);
+    o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
-    bf16* o = reinterpret_cast<bf16*>(p.out) + at + f;
-    const bf16* r = p.residual + (size_t)tok * p.ldr + f;
-    const bool res = p.epi == I8_RESIDUAL;
-    if (p.vec) {
-      float y[8];
+    float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = v[i];
-      if (res) {
-        const uint4 u = __ldcg(reinterpret_cast<const uint4*>(r));
-        const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
-        y[0] = __fadd_rn(y[0], a.x), y[1] = __fadd_rn(y[1], a.y), y[2] = __fadd_rn(y[2], b.x), y[3] = __fadd_rn(y[3], b.y);
-        y[4] = __fadd_rn(y[4], c.x), y[5] = __fadd_rn(y[5], c.y), y[6] = __fadd_rn(y[6], d.x), y[7] = __fadd_rn(y[7], d.y);
-      }
-      *reinterpret_cast<uint4*>(o) = make_uint4(f2_to_bf162_bits(y[0], y[1]), f2_to_bf162_bits(y[2], y[3]), f2_to_bf162_bits(y[4], y[5]), f2_to_bf162_bits(y[6], y[7]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (f + i < p.features) o[i] = __float2bfloat16(res ? __fadd_rn(v[i], __bfloat162float(__ldcg(r + i))) : v[i]);
+    for (int i = 0; i < 8; ++i) y[i] = v[i];
+    if (p.epi == I8_RESIDUAL) {
+      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p.residual + (size_t)tok * p.ldr + f));
+      const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
+      y[0] = __fadd_rn(y[0], a.x), y[1] = __fadd_rn(y[1], a.y), y[2] = __fadd_rn(y[2], b.x), y[3] = __fadd_rn(y[3], b.y);
+      y[4] = __fadd_rn(y[4], c.x), y[5] = __fadd_rn(y[5], c.y), y[6] = __fadd_rn(y[6], d.x), y[7] = __fadd_rn(y[7], d.y);
     }
+    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(p.out) + at + f) =
+        make_uint4(f2_to_bf162_bits(y[0], y[1]), f2_to_bf162_bits(y[2], y[3]), f2_to_bf162_bits(y[4], y[5]), f2_to_bf162_bits(y[6], y[7]));
+  }
+}
+// One feature (of SwiGLU a pair, from its even one), for outputs that take no vectors; neighbouring lanes have neighbouring features.
+__device__ __forceinline__ void gi_store1(const I8Params& p, int tok, int f, float v, float up) {
+  if (tok >= p.tokens || f >= p.features) return;
+  const size_t at = (size_t)tok * p.ldo;
+  if (p.epi == I8_SWIGLU) {
+    if (!(f & 1)) reinterpret_cast<bf16*>(p.out)[at + (f >> 1)] = __float2bfloat16(i8_swiglu(v, up));
+  } else if (p.epi == I8_STORE_F32) {
+    reinterpret_cast<float*>(p.out)[at + f] = v;
+  } else {
+    reinterpret_cast<bf16*>(p.out)[at + f] = __float2bfloat16(p.epi == I8_RESIDUAL ? __fadd_rn(v, __bfloat162float(__ldcg(p.residual + (size_t)tok * p.ldr + f))) : v);
   }
 }
 
@@ -261,11 +256,11 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const uint32_t even_empty = gp_map(acc_empty(0), even);
     for (int n = 0; n < my_tiles; ++n) {
       const int tile = tile0 + n * tile_step, buf = n & 1, rt = tile / p.c_tiles, ct = tile % p.c_tiles;
-      const int f0 = (rt * 2 + rank) * GI_ROWS + quad * 32 + (lane & 3) * 8;      // this lane's features and this warp's tokens as they leave
+      const int f32 = (rt * 2 + rank) * GI_ROWS + quad * 32, f0 = f32 + (p.vec ? (lane & 3) * 8 : lane);      // this lane's first feature as they leave
       const int tok0 = (ct * BN + half * COLS) / J;
       float ws[8], s[CHUNKS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ws[i] = !GRAD && !SPLIT && f0 + i < p.features ? p.ws[f0 + i] : 0.f;
+      for (int i = 0; i < 8; ++i) ws[i] = !GRAD && !SPLIT && f0 + i < p.features && (p.vec || i == 0) ? p.ws[f0 + i] : 0.f;
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) s[c] = !SPLIT && lane < TOK && tok0 + c * TOK + lane < p.tokens ? __ldcg(p.s + tok0 + c * TOK + lane) : 0.f;
       // (the warps of a group do not meet: each has its own barrier phase and its own piece of shared memory)
@@ -288,25 +283,35 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           for (int t = 0; t < 32; ++t) sum[(size_t)(half * COLS + c * 32 + t) * GI_ROWS + quad * 32 + lane] = (int)r[t];
         } else {
 #pragma unroll
-          for (int i = 0; i < TOK / 8; ++i) {
-            const int t = i * 8 + (lane >> 2);
-            if (i % 2 == 0) {                        // 16 tokens at a time
-              __syncwarp();
+          for (int h = 0; h < TOK; h += 16) {        // 16 tokens at a time
+            __syncwarp();
 #pragma unroll
-              for (int u = 0; u < 16; ++u) {
-                const int x = i * 8 + u;
-                tr[u * GI_TR_STRIDE + lane] = GRAD ? __float_as_int(fmaf(256.f, (float)(int)r[x * J], (float)(int)r[x * J + J - 1])) : (int)r[x];
-              }
-              __syncwarp();
+            for (int u = 0; u < 16; ++u) {
+              const int x = h + u;
+              tr[u * GI_TR_STRIDE + lane] = GRAD ? __float_as_int(fmaf(256.f, (float)(int)r[x * J], (float)(int)r[x * J + J - 1])) : (int)r[x];
             }
-            const float st = __shfl_sync(0xffffffffu, s[c], t);
-            const int* src = tr + (t & 15) * GI_TR_STRIDE + (lane & 3) * 8;
-            const int4 a = reinterpret_cast<const int4*>(src)[0], b = reinterpret_cast<const int4*>(src)[1];
-            const int x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            float v[8];
+            __syncwarp();
+            auto value = [&](int x, float st, float scale) { return GRAD ? __fmul_rn(__int_as_float(x), st) : i8_value(x, __fmul_rn(st, scale)); };
+            if (p.vec) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = GRAD ? __fmul_rn(__int_as_float(x[e]), st) : i8_value(x[e], __fmul_rn(st, ws[e]));
-            gi_store8(p, tok0 + c * TOK + t, f0, v);
+              for (int i = 0; i < 2; ++i) {
+                const int u = i * 8 + (lane >> 2);
+                const float st = __shfl_sync(0xffffffffu, s[c], h + u);
+                const int* src = tr + u * GI_TR_STRIDE + (lane & 3) * 8;
+                const int4 a = reinterpret_cast<const int4*>(src)[0], b = reinterpret_cast<const int4*>(src)[1];
+                const int x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = value(x[e], st, ws[e]);
+                gi_store8(p, tok0 + c * TOK + h + u, f0, v);
+              }
+            } else {
+#pragma unroll 4
+              for (int u = 0; u < 16; ++u) {
+                const float v = value(tr[u * GI_TR_STRIDE + lane], __shfl_sync(0xffffffffu, s[c], h + u), ws[0]);
+                gi_store1(p, tok0 + c * TOK + h + u, f0, v, __shfl_down_sync(0xffffffffu, v, 1));
+              }
+            }
           }
         }
       }
@@ -318,25 +323,34 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     gp_cluster_sync();
     constexpr int TOKENS = BN / J;
     const int rt = tile0 / p.c_tiles, ct = tile0 % p.c_tiles, t0 = part * TOKENS / p.parts, t1 = (part + 1) * TOKENS / p.parts;
-    for (int i = t0 * 16 + (int)threadIdx.x; i < t1 * 16; i += GI_THREADS) {
-      const int t = i >> 4, r = (i & 15) * 8, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
+    const int per = p.vec ? 8 : p.epi == I8_SWIGLU ? 2 : 1, pieces = GI_ROWS / per;      // features a thread
+    for (int i = t0 * pieces + (int)threadIdx.x; i < t1 * pieces; i += GI_THREADS) {
+      const int t = i / pieces, r = i % pieces * per, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
       if (tok >= p.tokens || f >= p.features) continue;
+      const float st = __ldcg(p.s + tok);
       int x[J][8] = {};
       for (int q = 0; q < p.parts; ++q) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const uint32_t src = gp_map(smem_u32(smem) + (uint32_t)((t * J + j) * GI_ROWS + r) * 4u, 2 * q + rank);
-          const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
-          x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
-          x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
+          if (p.vec) {
+            const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
+            x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
+            x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
+          } else {
+            x[j][0] += gi_ld1_cluster(src);
+            if (per == 2) x[j][1] += gi_ld1_cluster(src + 4);
+          }
         }
       }
-      const float st = __ldcg(p.s + tok);
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : f + e < p.features ? i8_value(x[0][e], __fmul_rn(st, p.ws[f + e])) : 0.f;
-      gi_store8(p, tok, f, v);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0.f;
+        if (e < per) v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : i8_value(x[0][e], __fmul_rn(st, p.ws[f + e]));
+      }
+      if (p.vec) gi_store8(p, tok, f, v);
+      else gi_store1(p, tok, f, v[0], v[1]);
     }
   }
 
@@ -398,18 +412,20 @@ struct I8Plan {
   int bn, parts, pairs;
 };
 
-// Columns a tile and pairs a tile: the least of rounds x stages x (time of a stage) + what putting parts together costs, in stages of 128
-// columns.
+// Columns a tile and pairs a tile, by the least of: what a launch costs (us), rounds x stages x the time of a stage, putting parts together.
+// Measured with the row quantiser, us: 24 rows of 5120 x 17408 with one pair a tile 33.0, two 24.6, three 23.2; of 5120 x 1024 7.4, 8.4, 8.7; 1024 rows of
+// 5120 x 6144 with 64, 128, 192, 256 columns 61.7, 46.0, 41.8, 48.4; 512 rows of 34816 x 5120 125, 86.2, 78.9, 70.9.
 I8Plan gi_plan(int cols, int features, int nk) {
   const int pairs = i8_sms() / 2, r_tiles = (features + 2 * GI_ROWS - 1) / (2 * GI_ROWS);
-  static const struct { int bn; double unit, exchange; } forms[] = {{64, 0.9, 3}, {128, 1, 5}, {192, 1.5, 8}, {256, 2, 10}};
+  static const struct { int bn; double launch, stage; } forms[] = {{64, 5.25, 0.2}, {128, 6, 0.25}, {192, 6.65, 0.33}, {256, 7.35, 0.4}};
+  static const double join[GI_MAX_PARTS + 1] = {0, 0, 2.5, 3.2, 3.8};
   I8Plan best{0, 1, pairs};
   double least = 0;
   for (const auto& f : forms) {
     const long long T = (long long)r_tiles * ((cols + f.bn - 1) / f.bn);
     for (int S = 1; S <= GI_MAX_PARTS; ++S) {
       if (S > 1 && (nk < 4 * S || T * S > pairs || T > gi_clusters(S))) break;
-      const double cost = (double)((T + pairs - 1) / pairs) * ((nk + S - 1) / S) * f.unit + (S > 1 ? f.exchange * (S + 2) / 4 : 0);
+      const double cost = f.launch + (double)((T + pairs - 1) / pairs) * ((nk + S - 1) / S) * f.stage + join[S];
       if (!best.bn || cost < least) best = I8Plan{f.bn, S, pairs}, least = cost;
     }
     if (cols <= f.bn) break;

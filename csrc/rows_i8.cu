@@ -182,70 +182,84 @@ __global__ void __launch_bounds__(CH == 1 ? 640 : 1024, CH == 1 ? 2 : 1) rows_i8
 }
 
 // Long rows in two digits, many of them: what a SM can hold of such a row leaves it idle between the row's maximum and its integers.  So two
-// passes, a block 2048 channels of every few rows, whose factors stay in registers: the maxima of these pieces, then the integers.
-constexpr int RL_THREADS = 256, RL_PIECE = RL_THREADS * 8;
-template <typename T, bool VEC, bool GIVE>
-__global__ void __launch_bounds__(RL_THREADS, 4) rows_long_kernel(const RowsParams p, uint32_t* most) {      // most: [pieces][rows]
-  constexpr int RL_ROWS = GIVE ? 2 : 4;            // rows at a time
+// passes, a block 2048 or 8192 channels of every few rows, whose factors stay in registers: the maxima of pieces of 2048, then the
+// integers.
+constexpr int RL_THREADS = 256, RL_PIECE = RL_THREADS * 8, RL_VECS = 4, RL_ROWS = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(RL_THREADS, 3) rows_most_kernel(const RowsParams p, uint32_t* most) {      // most: [pieces][rows]
   __shared__ uint32_t most_s[2][RL_ROWS][RL_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = blockIdx.x * RL_PIECE + threadIdx.x * 8, K = p.K;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.K, k = min(blockIdx.x * RL_PIECE + threadIdx.x * 8, K);
   float w[8];
-  rows_values<float>(rows_load<float, VEC>(p.w, min(k, K), K), w);
+  rows_values<float>(rows_load<float, VEC>(p.w, k, K), w);
   int turn = 0;
-  const long long groups = (p.rows + RL_ROWS - 1) / RL_ROWS;
-  for (long long i = blockIdx.y; i < groups; i += gridDim.y, turn ^= 1) {
-    const long long g = GIVE ? groups - 1 - i : i;      // the second pass begins with what the first one read last
+  for (long long r0 = blockIdx.y * RL_ROWS; r0 < p.rows; r0 += gridDim.y * RL_ROWS, turn ^= 1) {
     RowsRaw<T> raw[RL_ROWS];
-    uint32_t part[RL_ROWS];
+#pragma unroll
+    for (int r = 0; r < RL_ROWS; ++r) raw[r] = rows_load<T, VEC>(reinterpret_cast<const T*>(p.x) + min(r0 + r, p.rows - 1) * p.ldx, k, K);
 #pragma unroll
     for (int r = 0; r < RL_ROWS; ++r) {
-      const long long row = min(g * RL_ROWS + r, p.rows - 1);
-      raw[r] = rows_load<T, VEC>(reinterpret_cast<const T*>(p.x) + row * p.ldx, min(k, K), K);
-      if (GIVE) {
-        part[r] = 0;
-        for (int j = lane; j < (int)gridDim.x; j += 32) part[r] = max(part[r], __ldcg(most + (size_t)j * p.rows + row));
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < RL_ROWS; ++r) {
-      const long long row = g * RL_ROWS + r;
       float v[8];
       rows_values<T>(raw[r], v);
+      uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(v[e], w[e]);
-      if constexpr (GIVE) {
-        const uint32_t m = i8_warp_most(part[r]);
-        if (row < p.rows && k < K) rows_give<true>(p, row, k, v, i8_factor(m, I16_MOST));
-        if (row < p.rows && blockIdx.x == 0 && threadIdx.x == 0) p.s[row] = i8_scale(m, 1.f / I16_MOST);
-      } else {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, k < K ? i8_abs_bits(v[e]) : 0u);
-        m = i8_warp_most(m);
-        if (lane == 0) most_s[turn][r][warp] = m;
-      }
+      for (int e = 0; e < 8; ++e) m = max(m, i8_abs_bits(__fmul_rn(v[e], w[e])));      // (past the row's end: zeros)
+      m = i8_warp_most(m);
+      if (lane == 0) most_s[turn][r][warp] = m;
     }
-    if constexpr (!GIVE) {
-      __syncthreads();                               // (the next rows' go into the other half)
-      if (warp < RL_ROWS && g * RL_ROWS + warp < p.rows) {
-        const uint32_t m = i8_warp_most(lane < RL_THREADS / 32 ? most_s[turn][warp][lane] : 0u);
-        if (lane == 0) most[(size_t)blockIdx.x * p.rows + g * RL_ROWS + warp] = m;
-      }
+    __syncthreads();                                 // (the next rows' go into the other half)
+    if (warp < RL_ROWS && r0 + warp < p.rows) {
+      const uint32_t m = i8_warp_most(lane < RL_THREADS / 32 ? most_s[turn][warp][lane] : 0u);
+      if (lane == 0) most[(size_t)blockIdx.x * p.rows + r0 + warp] = m;
     }
   }
 }
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(RL_THREADS, 2) rows_digits_kernel(const RowsParams p, const uint32_t* most, int pieces) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, K = p.K;
+  int k[RL_VECS];
+  float w[RL_VECS][8];
+#pragma unroll
+  for (int c = 0; c < RL_VECS; ++c) {
+    k[c] = min((blockIdx.x * RL_VECS + c) * RL_PIECE + (int)threadIdx.x * 8, K);
+    rows_values<float>(rows_load<float, VEC>(p.w, k[c], K), w[c]);
+  }
+  // (from the last row on, which the first pass read last)
+  for (long long row = p.rows - 1 - blockIdx.y; row >= 0; row -= gridDim.y) {
+    RowsRaw<T> raw[RL_VECS];
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+#pragma unroll
+    for (int c = 0; c < RL_VECS; ++c) raw[c] = rows_load<T, VEC>(x, k[c], K);
+    uint32_t m = 0;
+    for (int j = lane; j < pieces; j += 32) m = max(m, __ldcg(most + (size_t)j * p.rows + row));
+    m = i8_warp_most(m);
+    const float f = i8_factor(m, I16_MOST);
+#pragma unroll
+    for (int c = 0; c < RL_VECS; ++c) {
+      float v[8];
+      rows_values<T>(raw[c], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(v[e], w[c][e]);
+      if (k[c] < K) rows_give<true>(p, row, k[c], v, f);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.s[row] = i8_scale(m, 1.f / I16_MOST);
+  }
+}
 int rows_long_pieces(int K) { return (K + RL_PIECE - 1) / RL_PIECE; }
-// (up to 10240 values a row leaves registers for the next one: one pass)
+// (fp32 2000 x 34816: 137 us, 223 in one pass; 1024 x 5120, which one pass holds, 10)
 bool rows_long(long long rows, int K, int digits) { return digits == 2 && K > 10240 && rows >= 64; }
 
 template <typename T, bool VEC>
 cudaError_t rows_long_launch(const RowsParams& p, void* most, cudaStream_t stream) {
-  const int sms = i8_sms(), pieces = rows_long_pieces(p.K);
-  const dim3 grid(pieces, (unsigned)min((p.rows + 3) / 4, (long long)max(1, sms * 4 / pieces)));
-  const cudaError_t e = trl_launch(rows_long_kernel<T, VEC, false>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
-  return e != cudaSuccess ? e : trl_launch(rows_long_kernel<T, VEC, true>, grid, dim3(RL_THREADS), 0, stream, p, (uint32_t*)most);
+  const int pieces = rows_long_pieces(p.K), wide = (pieces + RL_VECS - 1) / RL_VECS;
+  const long long fit = 3 * i8_sms(), fit2 = 2 * i8_sms();
+  const cudaError_t e = trl_launch(rows_most_kernel<T, VEC>, dim3(pieces, (unsigned)min((p.rows + RL_ROWS - 1) / RL_ROWS, max(1ll, fit / pieces))), dim3(RL_THREADS), 0,
+                                   stream, p, (uint32_t*)most);
+  if (e != cudaSuccess) return e;
+  return trl_launch(rows_digits_kernel<T, VEC>, dim3(wide, (unsigned)min(p.rows, max(1ll, fit2 / wide))), dim3(RL_THREADS), 0, stream, p, (const uint32_t*)most, pieces);
 }
 
 template <typename T, int CH, bool VEC, bool W16>
@@ -258,7 +272,7 @@ cudaError_t rows_launch(const RowsParams& p, int threads, cudaStream_t stream) {
   int& known = fit[threads / 32].here();
   if (known == 0) {
     int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem);
     if (e != cudaSuccess) return e;
     known = i8_sms() * max(n, 1);
   }
@@ -267,8 +281,8 @@ cudaError_t rows_launch(const RowsParams& p, int threads, cudaStream_t stream) {
 template <typename T, bool VEC, bool W16>
 cudaError_t rows_launch(const RowsParams& p, cudaStream_t stream) {
   const int vecs = (p.K + 7) / 8;
-  // Rows up to 5120 values: a vector a thread, two blocks or more a SM, the next row on its way.  Longer ones: as few vectors a thread as there are
-  // threads for.  From 40960 values on a row is read a second time, out of L2.
+  // Rows up to 5120 values: a vector a thread, two blocks or more a SM, the next row on its way (2000 x 5120 bf16 13 us; five vectors a thread in
+  // blocks of 128 15).  Longer ones: as few vectors a thread as there are threads for.  From 40960 values on a row is read a second time, out of L2.
   const int ch = vecs <= 640 ? 1 : vecs <= 2048 ? 2 : vecs <= 5120 ? (vecs + 1023) / 1024 : 0, threads = ch ? max(32, ((vecs + ch - 1) / ch + 31) / 32 * 32) : 1024;
   switch (ch) {
     case 1: return rows_launch<T, 1, VEC, W16>(p, threads, stream);
