@@ -462,7 +462,7 @@ int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int wi
   }
 }
 
-constexpr int GI_MOST = 131072;                   // 127 * 128 times as many is below 2^31
+constexpr int GI_MOST = 131072, GI_WIDEST = 1 << 24;      // values a sum: 127 * 128 times as many is below 2^31; channels
 bool gi_operands(const void* w, long long ldw, int K, const void* q, long long ldq) {
   return reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && ldw >= K && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0;
 }
@@ -473,7 +473,7 @@ bool gi_operands(const void* w, long long ldw, int K, const void* q, long long l
 // pairs, out [T, N / 2].
 static int gi_linear(const void* w, long ldw, const void* ws, const void* q, long ldq, const void* s, const void* residual, long ldr, void* out,
                         long ldo, int T, int N, int K, int epi, void* stream) {
-  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
+  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_WIDEST || K <= 0 || K > GI_MOST || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, q, ldq) || ldq < K)
     return (int)cudaErrorInvalidValue;
   I8Params p{};
@@ -505,7 +505,7 @@ extern "C" int trl_rows_i8(const void* x, int type, long ldx, const void* w, int
 // or an error.
 TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w, float eps, const void* w, long ldw, const void* ws, const void* residual,
                           long ldr, void* out, long ldo, void* scratch, int T, int N, int K, int epi, void* stream) {
-  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_MOST || K <= 0 || K > GI_MOST || K % 16 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
+  if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_WIDEST || K <= 0 || K > GI_MOST || K % 16 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, scratch, K))
     return (int)cudaErrorInvalidValue;
   const bool whole = type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;

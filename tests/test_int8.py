@@ -245,3 +245,34 @@ def test_a_run_of_them_together():
     for i, t in enumerate(tokens):
         row = logits[len(prompt) - 1 + i]
         assert float(row.max() - row[t]) <= 0.02 * float(row.std()), (i, t)
+
+
+def test_weights_written_between_the_passes_are_refused():
+    w, x = F.quantize_int8(_rows(8, 16)), _rows(3, 16, 1)
+    tape = T.Tape()
+    tape.watch(x)
+    y = T.linear(tape, x, w)
+    w.w8.neg_()
+    with pytest.raises(RuntimeError, match="changed in place"):
+        tape.backward(y)
+
+
+def test_the_format_by_name_and_by_directory(tmp_path, capsys):
+    from tilerl_b200.checkpoint import save_checkpoint
+    from tilerl_b200.cli import main
+    assert get_config("tiny", "int8").quant == "int8" and get_config("tiny").quant == "bf16"
+    for bad in (("tiny", "int4"), ("deluvik-tiny", "int8")):
+        with pytest.raises(ValueError, match="cannot be served"):
+            get_config(*bad)
+    save_checkpoint(HybridModel.build_random(_tiny()), str(tmp_path))
+    assert get_config(str(tmp_path)) == _tiny()
+    main(["serve", "--model", "qwen38-27b", "--dry-run", "--json", "--quant", "int8"])
+    small = json.loads(capsys.readouterr().out)
+    main(["serve", "--model", "qwen38-27b", "--dry-run", "--json", "--quant", "bf16"])
+    large = json.loads(capsys.readouterr().out)
+    assert small != large
+    cfg = get_config("qwen38-27b", "int8")
+    specs = F.weight_specs(cfg)
+    assert specs["L0.gate_up"][1] == "int8" and F.nbytes("int8", (34816, 5120)) == 34816 * 5124
+    from tilerl_b200.kernel_cost import prefill_rows
+    assert prefill_rows(cfg, 100)

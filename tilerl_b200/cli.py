@@ -20,12 +20,19 @@ def _add_model_flags(p: argparse.ArgumentParser) -> None:
     p.add_argument("--seed", type=int, default=0)
 
 
+def _add_quant_flag(p: argparse.ArgumentParser) -> None:
+    p.add_argument("--quant", default=None, choices=["nvfp4", "fp8", "int8", "bf16"],
+                   help="format of the projections instead of the configuration's own; int8: 8-bit integers with a scale per channel, "
+                        "activations quantised per token")
+
+
 def build_parser() -> argparse.ArgumentParser:
     ap = argparse.ArgumentParser(prog="tilerl_b200")
     sub = ap.add_subparsers(dest="cmd", required=True)
 
     s = sub.add_parser("serve", help="OpenAI / Anthropic compatible HTTP server")
     _add_model_flags(s)
+    _add_quant_flag(s)
     s.add_argument("--host", default="127.0.0.1")
     s.add_argument("--port", type=int, default=8000)
     s.add_argument("--slots", type=int, default=8)
@@ -82,6 +89,7 @@ def build_parser() -> argparse.ArgumentParser:
 
     t = sub.add_parser("train", help="SFT / GRPO / on-policy distillation")
     _add_model_flags(t)
+    _add_quant_flag(t)
     t.add_argument("--recipe", default=None)
     t.add_argument("--rl", action="store_true")
     t.add_argument("--opd", action="store_true")
@@ -161,6 +169,7 @@ def build_parser() -> argparse.ArgumentParser:
 
     b = sub.add_parser("bench", help="prefill / decode throughput, kernel roofline table, calibration")
     _add_model_flags(b)
+    _add_quant_flag(b)
     b.add_argument("--prompt-len", type=int, default=512)
     b.add_argument("--gen", type=int, default=64)
     b.add_argument("--batches", default="1")
@@ -244,7 +253,7 @@ def _draft_window(args) -> int:
 def cmd_serve(args) -> int:
     from . import memory
     from .config import get_config
-    cfg = get_config(args.model)
+    cfg = get_config(args.model, args.quant)
     if args.dry_run:
         fp8 = args.kv_format == "fp8"
         host_pages = args.kv_cold_bytes // memory.kv_block_bytes(cfg, 1, fp8) if args.kv_cold_bytes else 0
@@ -372,7 +381,7 @@ def cmd_train(args) -> int:
         raise SystemExit("--kl-reference base is the model without its adapters: give --rl and --lora-rank")
     if flags.get("allow_short_rollouts"):        # (a smoke recipe runs into its cap on purpose)
         args.allow_short_rollouts = True
-    cfg = get_config(flags.get("model", args.model))
+    cfg = get_config(flags.get("model", args.model), args.quant)
     if isinstance(cfg, StreamDesign):
         raise SystemExit(f"{cfg.architecture} models are served (serve, generate, bench), not trained")
     if not args.dry_run and flags.get("reward") in ("gsm8k", "boxed") and not args.data and (flags.get("rl") or flags.get("opd")):
@@ -635,7 +644,7 @@ def cmd_bench(args) -> int:
             n += 1
         print(f"appended {n} records to {benchrec.store_path()}")
         return 0
-    cfg = get_config(args.model)
+    cfg = get_config(args.model, args.quant)
     if args.calibrate:
         import dataclasses
         pk = calibrate(_device(args))

@@ -888,12 +888,22 @@ def config_from_dir(path: str):
     if arch in ARCHITECTURES:
         return ARCHITECTURES[arch].from_dir(j, path, os.path.basename(os.path.normpath(path)))
     if j.get("name") in _REGISTRY:
-        return _REGISTRY[j["name"]]()
+        cfg = _REGISTRY[j["name"]]()
+        return replace(cfg, quant="int8") if j.get("quant") == "int8" and isinstance(cfg, ModelConfig) else cfg
     raise ValueError(f"{path}/config.json names neither a known architecture ({sorted(ARCHITECTURES)}) nor a known model")
 
 
-def get_config(name: str):
-    """Configuration by registry name, or by a checkpoint directory that holds a ``config.json``."""
+QUANTS = ("nvfp4", "fp8", "int8", "bf16")
+
+
+def get_config(name: str, quant: Optional[str] = None):
+    """Configuration by registry name, or by a checkpoint directory that holds a ``config.json``.  ``quant``: serve its projections in
+    this format instead of the configuration's own."""
+    if quant is not None:
+        cfg = get_config(name)
+        if quant not in QUANTS or not isinstance(cfg, ModelConfig):
+            raise ValueError(f"projections of {name!r} cannot be served as {quant!r}: known formats {QUANTS}, for the hybrid models")
+        return replace(cfg, quant=quant)
     if name in _REGISTRY:
         return _REGISTRY[name]()
     if os.path.exists(os.path.join(name, "config.json")):

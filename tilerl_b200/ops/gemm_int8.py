@@ -51,7 +51,7 @@ def _ready(w: INT8Tensor) -> Optional[_Ready]:
         return r
     w8, ws = w.w8, w.wscale
     n, k = w8.shape
-    fits = (w8.is_cuda and ws.device == w8.device and ws.is_contiguous() and 0 < k <= MOST and 0 < n <= MOST and k % 16 == 0
+    fits = (w8.is_cuda and ws.device == w8.device and ws.is_contiguous() and 0 < k <= MOST and 0 < n <= 1 << 24 and k % 16 == 0
             and w8.stride(1) == 1 and w8.stride(0) % 16 == 0 and w8.stride(0) >= k and w8.data_ptr() % 16 == 0)
     r = w.__dict__["_ready"] = _Ready(w8, ws, n, k, w8.data_ptr(), w8.stride(0), ws.data_ptr(), w8.get_device()) if fits else None
     return r
@@ -64,7 +64,7 @@ def takes(w: INT8Tensor) -> bool:
 def _refuse(x, w, y, norm_w, residual, epi) -> _Ready:
     r = _ready(w)
     if r is None:
-        raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, up to {MOST} rows and columns, on "
+        raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, of up to {MOST}, on "
                          f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
     shape, n, k, here = x.shape, r.n, r.k, r.device
     if len(shape) != 2 or shape[1] != k or x.dtype not in TYPES or x.get_device() != here or x.stride(1) != 1 and k > 1:
@@ -124,11 +124,11 @@ def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) 
 
 # ---- the training tape ------------------------------------------------------------------------------------
 def train_takes(x: torch.Tensor, w: INT8Tensor) -> bool:
-    """Rows that the kernels take as they are; the torch forms serve the rest."""
+    """Rows that the kernels take as they are; the torch forms serve the rest (of so many channels that their sums could pass 32 bits, too)."""
     if not x.is_cuda or not there() or x.dtype not in TYPES or x.dim() < 1:
         return False
     r = _ready(w)
-    return r is not None and x.get_device() == r.device and x.shape[-1] == r.k
+    return r is not None and x.get_device() == r.device and x.shape[-1] == r.k and r.n <= MOST
 
 
 def _flat(x: torch.Tensor, width: int) -> torch.Tensor:
@@ -173,3 +173,6 @@ def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
     src = src if src.stride(1) == 1 else src.contiguous()
     with N.on(src.device):
         quant_rows(src, dst.w8, dst.wscale, weights=True)
+    for t in (dst.w8, dst.wscale):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)

@@ -342,10 +342,11 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
 def _linear_int8(tape: Tape, x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     takes = gemm_int8.train_takes(x, w)
     out = gemm_int8.forward(x, w) if takes else ref.linear_int8(x, w)
-    like = _Like(out.shape, out.device)
+    shape, device, unchanged = out.shape, out.device, _unchanged(w.w8, w.wscale)
 
     def bwd(g):
-        if takes and g.shape == like.shape and g.device == like.device:
+        unchanged()
+        if takes and g.shape == shape and g.device == device:
             return (gemm_int8.grad(g, w),)
         return (ref.linear_int8_grad(g, w),)
 
