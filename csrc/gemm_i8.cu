@@ -508,7 +508,9 @@ TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w,
   if (T <= 0 || T > (1 << 30) || N <= 0 || N > GI_WIDEST || K <= 0 || K > GI_MOST || K % 16 || epi < 0 || epi > 3 || (epi == I8_SWIGLU && N % 2) ||
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, scratch, K))
     return (int)cudaErrorInvalidValue;
-  const bool whole = type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;
+  // (in one launch every block reads all of x, while others write results already: not into the same memory)
+  const char *x0 = (const char*)x, *y0 = (const char*)out, *x1 = x0 + 2 * ((long long)(T - 1) * ldx + K), *y1 = y0 + 4 * ((long long)(T - 1) * ldo + N);
+  const bool whole = (x1 <= y0 || y1 <= x0) && type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;
   if (whole && gemv_i8_takes(T, N, K)) {
     const int rc = gemv_i8_launch(w, ldw, ws, x, ldx, norm_w, eps, residual, ldr, out, ldo, T, N, K, epi, (cudaStream_t)stream);
     return rc ? rc : -1;

@@ -219,6 +219,76 @@ def test_strides_of_weights_rows_and_outputs(ops):
         assert torch.equal(act[:, 3:68], want) and (act[:, :3] == 7).all() and (act[:, 68:] == 7).all()
 
 
+@pytest.mark.parametrize("t", [1, 2, 3, 70])
+def test_rows_that_are_the_residual_themselves(ops, t):
+    """The output in the place of the rows that are multiplied, whole or in part."""
+    from tilerl_b200.ops import gemm_int8
+    w = _weight(1024, 1024)
+    for _ in range(5):
+        x = _x(t, 1024)
+        want = ops.linear_residual(x.clone(), w, x.clone())
+        assert torch.equal(ops.linear_residual(x, w, x), want)
+    both = _x(t + 1, 1024)
+    want = torch.empty(t, 1024, device=DEV, dtype=torch.bfloat16)
+    gemm_int8.linear(ops, both[:t].clone(), w, want)
+    gemm_int8.linear(ops, both[:t], w, both[1:])
+    assert torch.equal(both[1:], want)
+
+
+def test_first_use_inside_a_capture():
+    """Kernels that this process has not launched yet.  (The backend's buffers have their size already: it refuses to grow them in a capture.)"""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from tilerl_b200 import formats as F, tape as T
+from tilerl_b200.ops.cuda import CudaOps
+ops = CudaOps()
+ws = [F.quantize_int8(torch.randn(n, 1040, device="cuda")) for n in (386, 5120)]
+xs = [torch.randn(t, 1040, device="cuda").bfloat16() for t in (1, 2, 33, 700)]
+xf, up, nw = torch.randn(90, 1040, device="cuda"), torch.randn(90, 386, device="cuda"), torch.ones(1040, device="cuda")
+ops.ws.get("proj", (700, 5120), torch.bfloat16), ops.ws.get("int8_rows", (700 * 1044,), torch.int8)
+outs = []
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    for w in ws:
+        for x in xs:
+            outs.append(ops.norm_linear(x, nw, w, 1e-6).clone())
+    tape = T.Tape()
+    tape.watch(xf)
+    y = T.linear(tape, xf, ws[0])
+    outs += [y, tape.backward(y, up)[id(xf)]]
+g.replay()
+torch.cuda.synchronize()
+want = [ops.norm_linear(x, nw, w, 1e-6).clone() for w in ws for x in xs]
+tape = T.Tape()
+tape.watch(xf)
+y = T.linear(tape, xf, ws[0])
+want += [y, tape.backward(y, up)[id(xf)]]
+assert all(torch.equal(a, b) for a, b in zip(outs, want))
+print("the same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert "the same" in r.stdout, r.stderr[-2000:]
+
+
+def test_weights_that_were_just_written(ops):
+    """Products load weights before they wait for the launch ahead of them; a weight's quantiser lets none start before its end."""
+    for n, k, t in ((5120, 1024, 1), (4096, 4096, 1), (4096, 4096, 20), (8192, 2048, 300)):
+        masters = [torch.randn(n, k, device=DEV) for _ in range(2)]
+        want = [F.quantize_int8(m) for m in masters]
+        w = F.INT8Tensor(torch.zeros(n, k, dtype=torch.int8, device=DEV), torch.zeros(n, device=DEV))
+        x, nw = _x(t, k), torch.rand(k, device=DEV) + 0.5
+        right = [ops.norm_linear(x, nw, v, 1e-6).clone() for v in want]
+        torch.cuda.synchronize()
+        for i in (0, 1, 0, 1, 0):
+            ops.quantize_int8_(masters[i], w)
+            assert torch.equal(ops.norm_linear(x, nw, w, 1e-6), right[i])
+
+
 def test_weights_and_outputs_past_32_bits_of_bytes(ops):
     """A weight of more than 2^31 bytes, and an output of as many values."""
     n, k = 20000, 110080
@@ -251,7 +321,7 @@ def test_refusals(ops):
         gemm_int8.linear(ops, x.t().contiguous().t(), w, y)
     with pytest.raises(ValueError, match="pairs"):
         gemm_int8.linear(ops, x, F.INT8Tensor(w.w8[:31], w.wscale[:31]), y, epi=gemm_int8.EPI_SWIGLU)
-    for bad in (y[:1], y[:, :31], y.float(), y.cpu(), y.t().contiguous().t()):
+    for bad in (y[:1], y[:, :31], y.float(), y.cpu(), y.t().contiguous().t(), y[:1].expand(2, 32)):
         with pytest.raises(ValueError, match="output"):
             gemm_int8.linear(ops, x, w, bad)
     with pytest.raises(ValueError, match="residual"):

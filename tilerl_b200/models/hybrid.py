@@ -263,8 +263,8 @@ class HybridModel:
             m = self.params.get("master." + n)
             if m is None:
                 continue
-            new = quantize_weight(m.float(), self.cfg.quant)
             cur = self.params[n]
+            new = quantize_weight(m.float(), "int8" if isinstance(cur, INT8Tensor) else self.cfg.quant)
             if isinstance(cur, NVFP4Tensor):
                 cur.wq.copy_(new.wq), cur.scale.copy_(new.scale), cur.tscale.copy_(new.tscale)
             elif isinstance(cur, (FP8BlockTensor, INT8Tensor)):

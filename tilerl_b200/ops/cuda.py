@@ -394,6 +394,9 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
         return x
 
     def norm_linear(self, x, norm_w, w, eps, lora=None):
+        if lora is None and isinstance(w, INT8Tensor):
+            self.settle()
+            return gemm_int8.served(self, "proj", x, w, norm_w, eps)
         t, n = x.shape[0], w.shape[0]
         y = self.ws.get("proj", (t, n), torch.bfloat16)
         self._linear(x, w, y, norm_w=self._f32(norm_w), eps=eps)
@@ -402,6 +405,9 @@ class CudaOps(StreamOps, MixerOps, BlockOps, GatedOps):
         return y
 
     def norm_linear_swiglu(self, x, norm_w, w, eps, lora=None):
+        if lora is None and isinstance(w, INT8Tensor):
+            self.settle()
+            return gemm_int8.served(self, "act", x, w, norm_w, eps, EPI_SWIGLU)
         t, n = x.shape[0], w.shape[0]
         act = self.ws.get("act", (t, n // 2), torch.bfloat16)
         if lora is None:

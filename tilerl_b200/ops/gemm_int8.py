@@ -61,29 +61,34 @@ def takes(w: INT8Tensor) -> bool:
     return _ready(w) is not None
 
 
-def _refuse(x, w, y, norm_w, residual, epi) -> _Ready:
-    r = _ready(w)
-    if r is None:
-        raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, of up to {MOST}, on "
-                         f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
-    shape, n, k, here = x.shape, r.n, r.k, r.device
-    if len(shape) != 2 or shape[1] != k or x.dtype not in TYPES or x.get_device() != here or x.stride(1) != 1 and k > 1:
+def _refuse_weight(w: INT8Tensor) -> None:
+    raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, of up to {MOST}, on "
+                     f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
+
+
+def _refuse_rows(x, r: _Ready, norm_w) -> None:
+    shape, k = x.shape, r.k
+    if len(shape) != 2 or shape[1] != k or x.dtype not in TYPES or x.get_device() != r.device or x.stride(1) != 1 and k > 1:
         raise ValueError(f"INT8 products take fp32 or bf16 rows [T, {k}] on the weight's device, got {tuple(shape)} {x.dtype} on {x.device}")
-    t, width, kind = shape[0], n, torch.bfloat16
-    if epi == EPI_SWIGLU:
-        if n % 2:
-            raise ValueError(f"SwiGLU takes rows in (gate, up) pairs, got {n}")
-        width = n // 2
-    elif epi == EPI_STORE_F32:
-        kind = torch.float32
-    if y.shape != (t, width) or y.dtype != kind or y.get_device() != here or t and y.stride(1) != 1 and width > 1:
-        raise ValueError(f"the output of {t} rows by {n} channels is {kind} with channels side by side, got {tuple(y.shape)} {y.dtype} on {y.device}")
-    if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and residual is not y and (
-            residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.get_device() != here or residual.stride(1) != 1 and n > 1):
-        raise ValueError("a residual is bf16 rows of the output's shape, given where one is added")
-    if norm_w is not None and (norm_w.shape != (k,) or norm_w.dtype != torch.float32 or norm_w.get_device() != here or not norm_w.is_contiguous()):
+    if norm_w is not None and (norm_w.shape != (k,) or norm_w.dtype != torch.float32 or norm_w.get_device() != r.device or not norm_w.is_contiguous()):
         raise ValueError(f"a norm's weight is fp32 [{k}] on the rows' device, got {tuple(norm_w.shape)} {norm_w.dtype} on {norm_w.device}")
-    return r
+
+
+def _width(r: _Ready, epi: int) -> int:
+    if epi != EPI_SWIGLU:
+        return r.n
+    if r.n % 2:
+        raise ValueError(f"SwiGLU takes rows in (gate, up) pairs, got {r.n}")
+    return r.n // 2
+
+
+def _refuse_out(y, t: int, r: _Ready, residual, epi: int) -> None:
+    width, kind, here = _width(r, epi), torch.float32 if epi == EPI_STORE_F32 else torch.bfloat16, r.device
+    if y.shape != (t, width) or y.dtype != kind or y.get_device() != here or t and y.stride(1) != 1 and width > 1 or t > 1 and y.stride(0) < width:
+        raise ValueError(f"the output of {t} rows by {r.n} channels is {kind} with channels side by side, got {tuple(y.shape)} {y.dtype} on {y.device}")
+    if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and residual is not y and (
+            residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.get_device() != here or residual.stride(1) != 1 and r.n > 1):
+        raise ValueError("a residual is bf16 rows of the output's shape, given where one is added")
 
 
 def _scratch(rows: int, width: int, digits: int = 1) -> int:
@@ -104,6 +109,9 @@ def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None, weights
 
 
 def _product(x, r: _Ready, out, ldo, scratch, norm_w, eps, residual, epi) -> None:
+    if r.device != N._device():
+        with torch.cuda.device(r.device):
+            return _product(x, r, out, ldo, scratch, norm_w, eps, residual, epi)
     rc = N.lib().trl_linear_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), None if norm_w is None else norm_w.data_ptr(), eps, r.ptr, r.ld, r.scales,
                                None if residual is None else residual.data_ptr(), 0 if residual is None else residual.stride(0), out.data_ptr(), ldo,
                                scratch.data_ptr(), x.shape[0], r.n, r.k, epi, N.stream())
@@ -114,12 +122,29 @@ def _product(x, r: _Ready, out, ldo, scratch, norm_w, eps, residual, epi) -> Non
 
 def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) -> None:
     """``y = epi(norm(x) @ W^T)``; ``y`` may be the residual."""
-    r = _refuse(x, w, y, norm_w, residual, epi)
+    r = _ready(w)
+    if r is None:
+        _refuse_weight(w)
+    _refuse_rows(x, r, norm_w)
     t = x.shape[0]
-    if t == 0:
-        return
-    with N.on(x.device):
+    _refuse_out(y, t, r, residual, epi)
+    if t:
         _product(x, r, y, y.stride(0), ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8), norm_w, eps, residual, epi)
+
+
+def served(ops, name: str, x, w, norm_w, eps: float, epi: int = EPI_STORE) -> torch.Tensor:
+    """``linear`` into the backend's own buffer ``name`` (bf16)."""
+    r = _ready(w)
+    if r is None:
+        _refuse_weight(w)
+    _refuse_rows(x, r, norm_w)
+    t, width = x.shape[0], _width(r, epi)
+    y = ops.ws.get(name, (t, width), torch.bfloat16)
+    if y.get_device() != r.device:
+        raise ValueError(f"the weight is on {w.w8.device}, the backend's buffers on {y.device}")
+    if t:
+        _product(x, r, y, width, ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8), norm_w, eps, None, epi)
+    return y
 
 
 # ---- the training tape ------------------------------------------------------------------------------------
@@ -142,11 +167,10 @@ def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     r = _ready(w)
     rows = _flat(x, r.k)
     t = rows.shape[0]
-    with N.on(x.device):
-        out = torch.empty(*x.shape[:-1], r.n, dtype=torch.float32, device=x.device)
-        if t:
-            _product(rows, r, out, r.n, torch.empty(_scratch(t, r.k), dtype=torch.int8, device=x.device), None, 0.0, None, EPI_STORE_F32)
-    return out
+    out = torch.empty((t, r.n), dtype=torch.float32, device=x.device)
+    if t:
+        _product(rows, r, out, r.n, torch.empty(_scratch(t, r.k), dtype=torch.int8, device=x.device), None, 0.0, None, EPI_STORE_F32)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], r.n)
 
 
 def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
@@ -155,14 +179,14 @@ def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     n, k = r.n, r.k
     rows = _flat(g if g.dtype in TYPES else g.float(), n)
     t = rows.shape[0]
-    with N.on(g.device):
-        dx = torch.empty(*g.shape[:-1], k, dtype=torch.float32, device=g.device)
-        if t:
-            scratch = torch.empty(_scratch(t, n, 2), dtype=torch.int8, device=g.device)
+    dx = torch.empty((t, k), dtype=torch.float32, device=g.device)
+    if t:
+        scratch = torch.empty(_scratch(t, n, 2), dtype=torch.int8, device=g.device)
+        with N.on(g.device):
             N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), r.ptr, r.ld, r.scales, dx.data_ptr(), k,
                                                scratch.data_ptr(), t, n, k, N.stream()), "linear_i8_grad")
-            N.count(2)
-    return dx
+        N.count(2)
+    return dx if g.dim() == 2 else dx.view(*g.shape[:-1], k)
 
 
 # ---- weights ---------------------------------------------------------------------------------------------------
