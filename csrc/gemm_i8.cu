@@ -279,11 +279,13 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
             asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_empty + 8u * buf) : "memory");
         }
         if (SPLIT) {
+          if (tok0 + c * TOK >= p.tokens) continue;
 #pragma unroll
           for (int t = 0; t < 32; ++t) sum[(size_t)(half * COLS + c * 32 + t) * GI_ROWS + quad * 32 + lane] = (int)r[t];
         } else {
 #pragma unroll
           for (int h = 0; h < TOK; h += 16) {        // 16 tokens at a time
+            if (tok0 + c * TOK + h >= p.tokens) break;
             __syncwarp();
 #pragma unroll
             for (int u = 0; u < 16; ++u) {
