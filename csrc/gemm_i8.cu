@@ -83,12 +83,6 @@ __device__ __forceinline__ int4 gi_ld_cluster(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ int gi_ld1_cluster(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // Eight features of a token out as one vector (v: results before the residual).
 __device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8]) {
   if (tok >= p.tokens || f >= p.features) return;
@@ -113,16 +107,31 @@ __device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, con
         make_uint4(f2_to_bf162_bits(y[0], y[1]), f2_to_bf162_bits(y[2], y[3]), f2_to_bf162_bits(y[4], y[5]), f2_to_bf162_bits(y[6], y[7]));
   }
 }
-// One feature (of SwiGLU a pair, from its even one), for outputs that take no vectors; neighbouring lanes have neighbouring features.
-__device__ __forceinline__ void gi_store1(const I8Params& p, int tok, int f, float v, float up) {
-  if (tok >= p.tokens || f >= p.features) return;
-  const size_t at = (size_t)tok * p.ldo;
+// N results out one by one, for outputs that take no vectors: `there` of them, tok_step tokens and f_step features apart.  SwiGLU: v and up are a
+// pair's.  (All values are at hand before the first store: a shuffle or a load between the stores would wait for each of them.)
+template <int N>
+__device__ __forceinline__ void gi_store_each(const I8Params& p, int tok, int tok_step, int f, int f_step, int there, const float (&v)[N], const float (&up)[N]) {
+  const size_t at = (size_t)tok * p.ldo + (p.epi == I8_SWIGLU ? f >> 1 : f);
+  const size_t step = (size_t)tok_step * p.ldo + (p.epi == I8_SWIGLU ? f_step >> 1 : f_step);
   if (p.epi == I8_SWIGLU) {
-    if (!(f & 1)) reinterpret_cast<bf16*>(p.out)[at + (f >> 1)] = __float2bfloat16(i8_swiglu(v, up));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < there) reinterpret_cast<bf16*>(p.out)[at + i * step] = __float2bfloat16(i8_swiglu(v[i], up[i]));
   } else if (p.epi == I8_STORE_F32) {
-    reinterpret_cast<float*>(p.out)[at + f] = v;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < there) reinterpret_cast<float*>(p.out)[at + i * step] = v[i];
+  } else if (p.epi == I8_RESIDUAL) {
+    float r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = i < there ? __bfloat162float(__ldcg(p.residual + (size_t)(tok + i * tok_step) * p.ldr + f + i * f_step)) : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < there) reinterpret_cast<bf16*>(p.out)[at + i * step] = __float2bfloat16(__fadd_rn(v[i], r[i]));
   } else {
-    reinterpret_cast<bf16*>(p.out)[at + f] = __float2bfloat16(p.epi == I8_RESIDUAL ? __fadd_rn(v, __bfloat162float(__ldcg(p.residual + (size_t)tok * p.ldr + f))) : v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < there) reinterpret_cast<bf16*>(p.out)[at + i * step] = __float2bfloat16(v[i]);
   }
 }
 
@@ -308,11 +317,15 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 gi_store8(p, tok0 + c * TOK + h + u, f0, v);
               }
             } else {
-#pragma unroll 4
-              for (int u = 0; u < 16; ++u) {
-                const float v = value(tr[u * GI_TR_STRIDE + lane], __shfl_sync(0xffffffffu, s[c], h + u), ws[0]);
-                gi_store1(p, tok0 + c * TOK + h + u, f0, v, __shfl_down_sync(0xffffffffu, v, 1));
+              float v[16], up[16];
+#pragma unroll
+              for (int u = 0; u < 16; ++u) v[u] = value(tr[u * GI_TR_STRIDE + lane], __shfl_sync(0xffffffffu, s[c], h + u), ws[0]);
+              if (p.epi == I8_SWIGLU) {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) up[u] = __shfl_down_sync(0xffffffffu, v[u], 1);
               }
+              const int tok = tok0 + c * TOK + h;
+              if (f0 < p.features && !(p.epi == I8_SWIGLU && (lane & 1))) gi_store_each<16>(p, tok, 1, f0, 0, p.tokens - tok, v, up);
             }
           }
         }
@@ -325,9 +338,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     gp_cluster_sync();
     constexpr int TOKENS = BN / J;
     const int rt = tile0 / p.c_tiles, ct = tile0 % p.c_tiles, t0 = part * TOKENS / p.parts, t1 = (part + 1) * TOKENS / p.parts;
-    const int per = p.vec ? 8 : p.epi == I8_SWIGLU ? 2 : 1, pieces = GI_ROWS / per;      // features a thread
-    for (int i = t0 * pieces + (int)threadIdx.x; i < t1 * pieces; i += GI_THREADS) {
-      const int t = i / pieces, r = i % pieces * per, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
+    for (int i = t0 * 16 + (int)threadIdx.x; i < t1 * 16; i += GI_THREADS) {
+      const int t = i >> 4, r = (i & 15) * 8, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
       if (tok >= p.tokens || f >= p.features) continue;
       const float st = __ldcg(p.s + tok);
       int x[J][8] = {};
@@ -335,24 +347,23 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const uint32_t src = gp_map(smem_u32(smem) + (uint32_t)((t * J + j) * GI_ROWS + r) * 4u, 2 * q + rank);
-          if (p.vec) {
-            const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
-            x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
-            x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
-          } else {
-            x[j][0] += gi_ld1_cluster(src);
-            if (per == 2) x[j][1] += gi_ld1_cluster(src + 4);
-          }
+          const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
+          x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
+          x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
         }
       }
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = 0.f;
-        if (e < per) v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : i8_value(x[0][e], __fmul_rn(st, p.ws[f + e]));
+      for (int e = 0; e < 8; ++e)
+        v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : f + e < p.features ? i8_value(x[0][e], __fmul_rn(st, p.ws[f + e])) : 0.f;
+      if (p.vec) {
+        gi_store8(p, tok, f, v);
+      } else if (p.epi == I8_SWIGLU) {
+        const float gate[4] = {v[0], v[2], v[4], v[6]}, up[4] = {v[1], v[3], v[5], v[7]};
+        gi_store_each<4>(p, tok, 0, f, 2, (p.features - f + 1) / 2, gate, up);
+      } else {
+        gi_store_each<8>(p, tok, 0, f, 1, p.features - f, v, v);
       }
-      if (p.vec) gi_store8(p, tok, f, v);
-      else gi_store1(p, tok, f, v[0], v[1]);
     }
   }
 
