@@ -157,6 +157,8 @@ def train_takes(x: torch.Tensor, w: INT8Tensor) -> bool:
 
 
 def _flat(x: torch.Tensor, width: int) -> torch.Tensor:
+    if x.requires_grad:
+        x = x.detach()
     if x.dim() != 2:
         x = x.reshape(-1, width)
     return x if x.stride(1) == 1 else x.contiguous()
@@ -167,26 +169,30 @@ def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     r = _ready(w)
     rows = _flat(x, r.k)
     t = rows.shape[0]
-    out = torch.empty((t, r.n), dtype=torch.float32, device=x.device)
+    out = rows.new_empty((t, r.n), dtype=torch.float32)
     if t:
-        _product(rows, r, out, r.n, torch.empty(_scratch(t, r.k), dtype=torch.int8, device=x.device), None, 0.0, None, EPI_STORE_F32)
+        _product(rows, r, out, r.n, rows.new_empty(_scratch(t, r.k), dtype=torch.int8), None, 0.0, None, EPI_STORE_F32)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], r.n)
 
 
 def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     """Gradient of ``forward``'s input, the rounding of ``x`` taken for none: ``g [..., N]`` -> fp32 ``[..., K]``."""
     r = _ready(w)
-    n, k = r.n, r.k
-    rows = _flat(g if g.dtype in TYPES else g.float(), n)
+    rows = _flat(g if g.dtype in TYPES else g.float(), r.n)
     t = rows.shape[0]
-    dx = torch.empty((t, k), dtype=torch.float32, device=g.device)
+    dx = rows.new_empty((t, r.k), dtype=torch.float32)
     if t:
-        scratch = torch.empty(_scratch(t, n, 2), dtype=torch.int8, device=g.device)
-        with N.on(g.device):
-            N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), r.ptr, r.ld, r.scales, dx.data_ptr(), k,
-                                               scratch.data_ptr(), t, n, k, N.stream()), "linear_i8_grad")
-        N.count(2)
-    return dx if g.dim() == 2 else dx.view(*g.shape[:-1], k)
+        _gradient(rows, r, dx, rows.new_empty(_scratch(t, r.n, 2), dtype=torch.int8))
+    return dx if g.dim() == 2 else dx.view(*g.shape[:-1], r.k)
+
+
+def _gradient(rows, r: _Ready, dx, scratch) -> None:
+    if r.device != N._device():
+        with torch.cuda.device(r.device):
+            return _gradient(rows, r, dx, scratch)
+    N.check(N.lib().trl_linear_i8_grad(rows.data_ptr(), TYPES[rows.dtype], rows.stride(0), r.ptr, r.ld, r.scales, dx.data_ptr(), r.k, scratch.data_ptr(),
+                                       rows.shape[0], r.n, r.k, N.stream()), "linear_i8_grad")
+    N.count(2)
 
 
 # ---- weights ---------------------------------------------------------------------------------------------------

@@ -297,7 +297,6 @@ def _wide_product(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return torch.mm(x.reshape(-1, x.shape[-1]), w.t(), out_dtype=torch.float32).view(*x.shape[:-1], w.shape[0])
 
 
-@_nograd
 def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = False) -> torch.Tensor:
     """``y = x @ W^T``.  ``w`` is a dense master tensor (dX and dW) or a quantised
     weight / ``frozen=True`` dense tensor (dX only, the LoRA-on-frozen-base mode).
@@ -305,8 +304,11 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
     a rounding of 2^-9 of a logit of 20 is 0.04 of a log-probability); on CPU everything is fp32 (the oracle path).
     Weights in 8-bit integers: the product that serves them, rows quantised per token, y not rounded; the gradient takes that rounding of
     x for none and its own rows in 16 bits (``ops/gemm_int8.py``)."""
-    if isinstance(w, INT8Tensor):
-        return _linear_int8(tape, x, w)
+    return _linear_int8(tape, x, w) if isinstance(w, INT8Tensor) else _linear_dense(tape, x, w, frozen, wide)
+
+
+@_nograd
+def _linear_dense(tape: Tape, x: torch.Tensor, w, frozen: bool, wide: bool) -> torch.Tensor:
     dense = isinstance(w, torch.Tensor)
     wf = dense_weight(w, x.device)
     if x.is_cuda:
@@ -341,14 +343,14 @@ def linear(tape: Tape, x: torch.Tensor, w, frozen: bool = False, wide: bool = Fa
 
 def _linear_int8(tape: Tape, x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     takes = gemm_int8.train_takes(x, w)
-    out = gemm_int8.forward(x, w) if takes else ref.linear_int8(x, w)
+    out = gemm_int8.forward(x, w) if takes else _nograd(ref.linear_int8)(x, w)
     shape, device, unchanged = out.shape, out.device, _unchanged(w.w8, w.wscale)
 
     def bwd(g):
         unchanged()
         if takes and g.shape == shape and g.device == device:
             return (gemm_int8.grad(g, w),)
-        return (ref.linear_int8_grad(g, w),)
+        return (_nograd(ref.linear_int8_grad)(g, w),)
 
     tape.record("linear", (x,), (out,), bwd)
     return out
