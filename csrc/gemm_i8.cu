@@ -13,6 +13,13 @@
 // they leave as 16-byte pieces of a token's row.  With fewer tiles than pairs, two to four pairs of a cluster share a tile along the summed
 // dimension and add their parts through each other's shared memory.
 //
+// What bounds it.  Many tokens: the tensor cores, at the clocks that the power cap leaves them (2000 x 16 480 x 5120: 116 us alone, tensor pipe 88 % of its
+// active cycles; a second of it 144 us, 2.3 POP/s; on another GPU 175).  An MMA of 128 x 256 x 32 takes 128 clocks, as fp8 does and bf16
+// with half of K.  Few: the read of W (eight rows of 34 816 x 5120: 35 us from an empty L2 cache, 5.1 TB/s; 32 us with the quantiser in a row of
+// products, whose first stages are on their way while the rows between them are quantised).  Measured and not taken: W on its way before TMEM
+// is taken (the quantiser's few loads then wait behind it: 32.8), half a SM a CTA, so that the next product moves in earlier (four
+// stages are too few: 35.6), the head of W fetched into L2 by the quantiser (33.0).
+//
 // The reference has no integer product; in the place of its `linear_fp8` (packages/tilerl-kernels/src/tilerl_kernels/
 // kernels_linear.py:1777-1813) for weights in this format.
 #include "int8.cuh"

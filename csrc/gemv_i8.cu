@@ -7,6 +7,9 @@
 // along K, then down the rows.  Rows of W are the A operand of mma.m16n8k32, tokens B.  Sums go into shared memory by integer atomics: exact, so
 // their order changes nothing.
 //
+// Bound by latency: launch, the row's read, its maximum and its integers (two block barriers), sums, results (1 x 5120 x 1024: 5.1 us, of which the
+// 5 MB take 0.8).
+//
 // The reference's FP8 form for few rows is `linear_fp8_gemv` (packages/tilerl-kernels/src/tilerl_kernels/kernels_linear.py:1442-1494).
 #include <cuda.h>
 

@@ -4,7 +4,8 @@
 //   u = g * ws,                          m = max |u|,  Q = rint(u * ((1 / m) * 32512)) = 256 hi + lo,  s = m * (1 / 32512)
 //
 // A norm's factor is the same for a whole row, so it cancels out of the integers and goes into the scale alone.  One pass: a block takes
-// row after row, which stays in registers between its maximum and its integers.  Bound by memory for many rows, by latency for few.
+// row after row, which stays in registers between its maximum and its integers.  Bound by instructions for many rows (2000 x 5120 bf16: 13 us, 64 % of
+// the issue slots, 31 MB; packed fp32 arithmetic takes 8 % of them away and no time), by latency for few (2.5 us).
 //
 // The reference quantises activations per token for its FP8 products (`quant_fp8`, packages/tilerl-kernels/src/tilerl_kernels/
 // kernels_linear.py:1547-1590); it has no integer form.
