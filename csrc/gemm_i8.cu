@@ -90,8 +90,35 @@ __device__ __forceinline__ int4 gi_ld_cluster(uint32_t addr) {
   return v;
 }
 
-// Eight features of a token out as one vector (v: results before the residual).
-__device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8]) {
+// Eight features of a token (of both its columns, J = 2), summed over the parts; all of them are asked for before the first is added.
+template <int PARTS, int J>
+__device__ __forceinline__ void gi_join(uint32_t at, int rank, int (&y)[J][8]) {
+  int4 x[PARTS][J][2];
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    const uint32_t src = gp_map(at, 2 * q + rank);
+#pragma unroll
+    for (int j = 0; j < J; ++j) x[q][j][0] = gi_ld_cluster(src + j * GI_ROWS * 4), x[q][j][1] = gi_ld_cluster(src + j * GI_ROWS * 4 + 16);
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[j][e] = 0;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      const int4 a = x[q][j][0], b = x[q][j][1];
+      y[j][0] += a.x, y[j][1] += a.y, y[j][2] += a.z, y[j][3] += a.w, y[j][4] += b.x, y[j][5] += b.y, y[j][6] += b.z, y[j][7] += b.w;
+    }
+  }
+}
+
+// The residual's eight features of a token, asked for well before they are added.
+__device__ __forceinline__ uint4 gi_residual8(const I8Params& p, int tok, int f) {
+  if (tok >= p.tokens || f >= p.features) return make_uint4(0u, 0u, 0u, 0u);
+  return __ldcg(reinterpret_cast<const uint4*>(p.residual + (size_t)tok * p.ldr + f));
+}
+// Eight features of a token out as one vector (v: results before the residual u).
+__device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8], const uint4& u) {
   if (tok >= p.tokens || f >= p.features) return;
   const size_t at = (size_t)tok * p.ldo;
   if (p.epi == I8_SWIGLU) {                          // features in (gate, up) pairs
@@ -105,7 +132,6 @@ __device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, con
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = v[i];
     if (p.epi == I8_RESIDUAL) {
-      const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p.residual + (size_t)tok * p.ldr + f));
       const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
       y[0] = __fadd_rn(y[0], a.x), y[1] = __fadd_rn(y[1], a.y), y[2] = __fadd_rn(y[2], b.x), y[3] = __fadd_rn(y[3], b.y);
       y[4] = __fadd_rn(y[4], c.x), y[5] = __fadd_rn(y[5], c.y), y[6] = __fadd_rn(y[6], d.x), y[7] = __fadd_rn(y[7], d.y);
@@ -189,6 +215,17 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const int my_tiles = tile1 > tile0 ? (tile1 - tile0 + tile_step - 1) / tile_step : 0;
   const int k0 = SPLIT ? (int)((long long)part * p.nk / p.parts) : 0, k1 = SPLIT ? (int)((long long)(part + 1) * p.nk / p.parts) : p.nk;
 
+  // Parts of a shared tile: this pair adds up tokens join_t .. join_t1 of it, a thread of the epilogue's eight features of every sixteenth one.  What
+  // that needs besides the parts is asked for before the tile's sums are waited for (a barrier of the cluster waits for loads, too).
+  constexpr int TOKENS = BN / J, JOIN_STEP = (GI_THREADS - 64) / 16;
+  int join_t = 0, join_t1 = 0, join_f = 0;
+  float join_ws[8], join_scale = 0.f;
+  uint4 join_res = make_uint4(0u, 0u, 0u, 0u);
+  auto scale_of = [&](int t) { return t < join_t1 ? __ldcg(p.s + tile0 % p.c_tiles * TOKENS + t) : 0.f; };
+  auto residual_of = [&](int t) {
+    return !GRAD && p.epi == I8_RESIDUAL && p.vec && t < join_t1 ? gi_residual8(p, tile0 % p.c_tiles * TOKENS + t, join_f) : make_uint4(0u, 0u, 0u, 0u);
+  };
+
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (elect_one()) {
@@ -270,6 +307,14 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     int* tr = reinterpret_cast<int*>(turn + (warp - 2) * GI_TR_BYTES);
     int* sum = reinterpret_cast<int*>(smem);        // parts: [column][128 features] of this CTA's, in the ring, which is through by then
     const uint32_t even_empty = gp_map(acc_empty(0), even);
+    if (SPLIT) {
+      const int tokens = min(TOKENS, p.tokens - tile0 % p.c_tiles * TOKENS);
+      join_t = part * tokens / p.parts + (int)((threadIdx.x - 64) >> 4), join_t1 = (part + 1) * tokens / p.parts;
+      join_f = (tile0 / p.c_tiles * 2 + rank) * GI_ROWS + (threadIdx.x & 15) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) join_ws[e] = !GRAD && join_f + e < p.features ? p.ws[join_f + e] : 0.f;
+      join_scale = scale_of(join_t), join_res = residual_of(join_t);
+    }
     for (int n = 0; n < my_tiles; ++n) {
       const int tile = tile0 + n * tile_step, buf = n & 1, rt = tile / p.c_tiles, ct = tile % p.c_tiles;
       const int f32 = (rt * 2 + rank) * GI_ROWS + quad * 32, f0 = f32 + (p.vec ? (lane & 3) * 8 : lane);      // this lane's first feature as they leave
@@ -286,6 +331,12 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         uint32_t r[32];
+        constexpr bool EARLY = BN <= 128;            // (wider tiles have more to do meanwhile)
+        uint4 res[TOK / 8];
+        if (!GRAD && !SPLIT && EARLY && p.epi == I8_RESIDUAL && p.vec) {
+#pragma unroll
+          for (int i = 0; i < TOK / 8; ++i) res[i] = gi_residual8(p, tok0 + c * TOK + i * 8 + (lane >> 2), f0);
+        }
         tc_ld32(taddr + (uint32_t)(c * 32), r);
         tc_wait_ld();
         if (c == CHUNKS - 1) {                       // read out: the accumulator goes back
@@ -321,7 +372,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = value(x[e], st, ws[e]);
-                gi_store8(p, tok0 + c * TOK + h + u, f0, v);
+                if (!GRAD && !EARLY && p.epi == I8_RESIDUAL) res[h / 8 + i] = gi_residual8(p, tok0 + c * TOK + h + u, f0);
+                gi_store8(p, tok0 + c * TOK + h + u, f0, v, res[h / 8 + i]);
               }
             } else {
               float v[16], up[16];
@@ -343,28 +395,19 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   if constexpr (SPLIT) {
     // each pair of the cluster adds up its share of the tokens
     gp_cluster_sync();
-    constexpr int TOKENS = BN / J;
-    const int rt = tile0 / p.c_tiles, ct = tile0 % p.c_tiles, t0 = part * TOKENS / p.parts, t1 = (part + 1) * TOKENS / p.parts;
-    for (int i = t0 * 16 + (int)threadIdx.x; i < t1 * 16; i += GI_THREADS) {
-      const int t = i >> 4, r = (i & 15) * 8, tok = ct * TOKENS + t, f = (rt * 2 + rank) * GI_ROWS + r;
-      if (tok >= p.tokens || f >= p.features) continue;
-      const float st = __ldcg(p.s + tok);
-      int x[J][8] = {};
-      for (int q = 0; q < p.parts; ++q) {
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const uint32_t src = gp_map(smem_u32(smem) + (uint32_t)((t * J + j) * GI_ROWS + r) * 4u, 2 * q + rank);
-          const int4 a = gi_ld_cluster(src), b = gi_ld_cluster(src + 16);
-          x[j][0] += a.x, x[j][1] += a.y, x[j][2] += a.z, x[j][3] += a.w;
-          x[j][4] += b.x, x[j][5] += b.y, x[j][6] += b.z, x[j][7] += b.w;
-        }
-      }
+    for (int t = join_t; warp >= 2 && t < join_t1; t += JOIN_STEP, join_scale = scale_of(t), join_res = residual_of(t)) {
+      const int tok = tile0 % p.c_tiles * TOKENS + t, f = join_f, r = f & (GI_ROWS - 1);
+      int y[J][8];
+      const uint32_t src = smem_u32(smem) + (uint32_t)(t * J * GI_ROWS + r) * 4u;
+      if (p.parts == 2) gi_join<2, J>(src, rank, y);
+      else if (p.parts == 3) gi_join<3, J>(src, rank, y);
+      else gi_join<4, J>(src, rank, y);
+      if (f >= p.features) continue;
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)x[0][e], (float)x[J - 1][e]), st) : f + e < p.features ? i8_value(x[0][e], __fmul_rn(st, p.ws[f + e])) : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)y[0][e], (float)y[J - 1][e]), join_scale) : i8_value(y[0][e], __fmul_rn(join_scale, join_ws[e]));
       if (p.vec) {
-        gi_store8(p, tok, f, v);
+        gi_store8(p, tok, f, v, join_res);
       } else if (p.epi == I8_SWIGLU) {
         const float gate[4] = {v[0], v[2], v[4], v[6]}, up[4] = {v[1], v[3], v[5], v[7]};
         gi_store_each<4>(p, tok, 0, f, 2, (p.features - f + 1) / 2, gate, up);
