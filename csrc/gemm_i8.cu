@@ -72,6 +72,7 @@ struct I8Params {
   void* out;
   long long ldr, ldo;
   int features, tokens, depth, nk, r_tiles, c_tiles, epi;
+  int rows;              // features that a SM's 128 rows hold: fewer, in steps of eight, where the pairs of SMs share W more evenly that way
   int vec;               // 8 features of a token are one aligned vector of the output (of SwiGLU four results) and of the residual
   int parts;             // pairs that share a tile (a cluster), each a part of the summed dimension; 1: a pair goes through whole tiles
 };
@@ -218,6 +219,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   // Parts of a shared tile: this pair adds up tokens join_t .. join_t1 of it, a thread of the epilogue's eight features of every sixteenth one.  What
   // that needs besides the parts is asked for before the tile's sums are waited for (a barrier of the cluster waits for loads, too).
   constexpr int TOKENS = BN / J, JOIN_STEP = (GI_THREADS - 64) / 16;
+  const int join_r = (threadIdx.x & 15) * 8;
   int join_t = 0, join_t1 = 0, join_f = 0;
   float join_ws[8], join_scale = 0.f;
   uint4 join_res = make_uint4(0u, 0u, 0u, 0u);
@@ -233,8 +235,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const int units = my_tiles * (k1 - k0);
       auto load_w = [&](int rt, int kt, int st) {
         const uint32_t dst = smem0 + (uint32_t)st * C::STAGE, bar = gp_map(full(st), even);
-        const int f = (rt * 2 + rank) * GI_ROWS;
-        if (rank == 0) mbar_expect_tx(full(st), 2u * C::STAGE);
+        const int f = (rt * 2 + rank) * p.rows;
+        if (rank == 0) mbar_expect_tx(full(st), 2u * (uint32_t)(p.rows * GI_KT + C::B_BYTES));
         gp_load_2d(dst, &map_w, GRAD ? f : kt * GI_KT, GRAD ? kt * GI_KT : f, bar);
       };
       auto load_q = [&](int ct, int kt, int st) {
@@ -310,14 +312,14 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (SPLIT) {
       const int tokens = min(TOKENS, p.tokens - tile0 % p.c_tiles * TOKENS);
       join_t = part * tokens / p.parts + (int)((threadIdx.x - 64) >> 4), join_t1 = (part + 1) * tokens / p.parts;
-      join_f = (tile0 / p.c_tiles * 2 + rank) * GI_ROWS + (threadIdx.x & 15) * 8;
+      join_f = join_r < p.rows ? (tile0 / p.c_tiles * 2 + rank) * p.rows + join_r : p.features;
 #pragma unroll
       for (int e = 0; e < 8; ++e) join_ws[e] = !GRAD && join_f + e < p.features ? p.ws[join_f + e] : 0.f;
       join_scale = scale_of(join_t), join_res = residual_of(join_t);
     }
     for (int n = 0; n < my_tiles; ++n) {
       const int tile = tile0 + n * tile_step, buf = n & 1, rt = tile / p.c_tiles, ct = tile % p.c_tiles;
-      const int f32 = (rt * 2 + rank) * GI_ROWS + quad * 32, f0 = f32 + (p.vec ? (lane & 3) * 8 : lane);      // this lane's first feature as they leave
+      const int row = quad * 32 + (p.vec ? (lane & 3) * 8 : lane), f0 = row < p.rows ? (rt * 2 + rank) * p.rows + row : p.features;      // this lane's first feature as they leave
       const int tok0 = (ct * BN + half * COLS) / J;
       float ws[8], s[CHUNKS];
 #pragma unroll
@@ -396,9 +398,9 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     // each pair of the cluster adds up its share of the tokens
     gp_cluster_sync();
     for (int t = join_t; warp >= 2 && t < join_t1; t += JOIN_STEP, join_scale = scale_of(t), join_res = residual_of(t)) {
-      const int tok = tile0 % p.c_tiles * TOKENS + t, f = join_f, r = f & (GI_ROWS - 1);
+      const int tok = tile0 % p.c_tiles * TOKENS + t, f = join_f;
       int y[J][8];
-      const uint32_t src = smem_u32(smem) + (uint32_t)(t * J * GI_ROWS + r) * 4u;
+      const uint32_t src = smem_u32(smem) + (uint32_t)(t * J * GI_ROWS + join_r) * 4u;
       if (p.parts == 2) gi_join<2, J>(src, rank, y);
       else if (p.parts == 3) gi_join<3, J>(src, rank, y);
       else gi_join<4, J>(src, rank, y);
@@ -472,24 +474,32 @@ int gi_clusters(int parts) {
 }
 
 struct I8Plan {
-  int bn, parts, pairs;
+  int bn, parts, pairs, rows;
 };
 
 // Columns a tile and pairs a tile, by the least of: what a launch costs (us), rounds x stages x the time of a stage, putting parts together.
 // Measured with the row quantiser, us: 24 rows of 5120 x 17408 with one pair a tile 33.0, two 24.6, three 23.2; of 5120 x 1024 7.4, 8.4, 8.7; 1024 rows of
 // 5120 x 6144 with 64, 128, 192, 256 columns 61.7, 46.0, 41.8, 48.4; 512 rows of 34816 x 5120 125, 86.2, 78.9, 70.9.
-I8Plan gi_plan(int cols, int features, int nk) {
-  const int pairs = i8_sms() / 2, r_tiles = (features + 2 * GI_ROWS - 1) / (2 * GI_ROWS);
+// One tile of columns: a launch reads W once and is over when the pair with the most of it is, so tiles may have 192 to 240 of 256 features: where the
+// tiles are more than pairs (eight rows of 20 000 x 2992 19.3 -> 17.8 us), or few enough that three quarters of the pairs have one afterwards
+// (of 10 000 x 4096 13.9 -> 13.2).  From there on memory is busy, and more pairs are no gain (16 480 x 5120, 224 features on 74 pairs instead of 256 on
+// 65: 18.6 -> 19.0).
+I8Plan gi_plan(int cols, int features, int nk, bool narrow) {
+  const int pairs = i8_sms() / 2;
   static const struct { int bn; double launch, stage; } forms[] = {{64, 5.25, 0.2}, {128, 6, 0.25}, {192, 6.65, 0.33}, {256, 7.35, 0.4}};
   static const double join[GI_MAX_PARTS + 1] = {0, 0, 2.5, 3.2, 3.8};
-  I8Plan best{0, 1, pairs};
+  I8Plan best{0, 1, pairs, GI_ROWS};
   double least = 0;
   for (const auto& f : forms) {
-    const long long T = (long long)r_tiles * ((cols + f.bn - 1) / f.bn);
-    for (int S = 1; S <= GI_MAX_PARTS; ++S) {
-      if (S > 1 && (nk < 4 * S || T * S > pairs || T > gi_clusters(S))) break;
-      const double cost = f.launch + (double)((T + pairs - 1) / pairs) * ((nk + S - 1) / S) * f.stage + join[S];
-      if (!best.bn || cost < least) best = I8Plan{f.bn, S, pairs}, least = cost;
+    for (int R = GI_ROWS; R >= (narrow && cols <= 64 ? 96 : GI_ROWS); R -= 8) {
+      const long long T = (long long)((features + 2 * R - 1) / (2 * R)) * ((cols + f.bn - 1) / f.bn);
+      for (int S = 1; S <= GI_MAX_PARTS; ++S) {
+        if (S > 1 && (nk < 4 * S || T * S > pairs || T > gi_clusters(S))) break;
+        if (R < GI_ROWS && T <= pairs && T * S * 4 > pairs * 3) continue;
+        const double stage = f.stage * (R * GI_KT + f.bn / 2 * GI_KT) / (GI_ROWS * GI_KT + f.bn / 2 * GI_KT);
+        const double cost = f.launch + (double)((T + pairs - 1) / pairs) * ((nk + S - 1) / S) * stage + join[S];
+        if (!best.bn || cost < (R < GI_ROWS ? 0.97 : 1) * least) best = I8Plan{f.bn, S, pairs, R}, least = cost;
+      }
     }
     if (cols <= f.bn) break;
   }
@@ -500,8 +510,8 @@ template <int BN, bool GRAD>
 int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int width, int rows, I8Params p, const I8Plan& plan, cudaStream_t stream) {
   constexpr int J = GRAD ? 2 : 1;
   CUtensorMap mw, mq;
-  if (!i8_tensor(&mw, w, width, rows, ldw, GI_ROWS) || !i8_tensor(&mq, q, p.depth, (long long)p.tokens * J, ldq, BN / 2)) return (int)cudaErrorInvalidValue;
-  p.r_tiles = (p.features + 2 * GI_ROWS - 1) / (2 * GI_ROWS), p.c_tiles = (p.tokens * J + BN - 1) / BN, p.parts = plan.parts;
+  if (!i8_tensor(&mw, w, width, rows, ldw, GRAD ? GI_KT : plan.rows) || !i8_tensor(&mq, q, p.depth, (long long)p.tokens * J, ldq, BN / 2)) return (int)cudaErrorInvalidValue;
+  p.rows = plan.rows, p.r_tiles = (p.features + 2 * p.rows - 1) / (2 * p.rows), p.c_tiles = (p.tokens * J + BN - 1) / BN, p.parts = plan.parts;
   const long long tiles = (long long)p.r_tiles * p.c_tiles;
   if (tiles > 0x7fffffffll / p.nk) return (int)cudaErrorInvalidValue;
   const int pairs = plan.parts > 1 ? (int)tiles * plan.parts : (int)(tiles < plan.pairs ? tiles : plan.pairs);
@@ -516,7 +526,7 @@ template <bool GRAD>
 int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int width, int rows, I8Params& p, cudaStream_t stream) {
   constexpr int J = GRAD ? 2 : 1;
   p.nk = (p.depth + GI_KT - 1) / GI_KT;
-  const I8Plan plan = gi_plan(p.tokens * J, p.features, p.nk);
+  const I8Plan plan = gi_plan(p.tokens * J, p.features, p.nk, !GRAD);
   switch (plan.bn) {
     case 64: return gi_launch<64, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
     case 128: return gi_launch<128, GRAD>(w, ldw, q, ldq, width, rows, p, plan, stream);
