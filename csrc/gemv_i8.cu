@@ -1,4 +1,4 @@
-// Products of 8-bit integers with one row or two: y[t, n] = epi((sum_k q[t, k] W[n, k]) * s[t] * ws[n]), as gemm_i8.cu, bound by the read of
+// Products of 8-bit integers with one to four rows: y[t, n] = epi((sum_k q[t, k] W[n, k]) * s[t] * ws[n]), as gemm_i8.cu, bound by the read of
 // W (reached through trl_linear_i8 there).  The rows are quantised here as rows_i8.cu does it (same integers, same scales), by every
 // block for itself, while its first weights are on their way.
 //
@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int GV_WARPS = 16, GV_THREADS = GV_WARPS * 32, GV_TOKENS = 2, GV_MOST_STAGES = 3;
+constexpr int GV_WARPS = 16, GV_THREADS = GV_WARPS * 32, GV_TOKENS = 4, GV_MOST_STAGES = 3;
 constexpr int GV_ROWS = 32, GV_STEP = 128, GV_UNIT = GV_ROWS * GV_STEP;
 constexpr int GV_PIECES = 2, GV_MOST_K = GV_PIECES * GV_WARPS * I8_GROUP;      // of 256 values, that a warp keeps of a token
 constexpr size_t GV_SMEM = 224 * 1024;
@@ -60,7 +60,7 @@ gemv_i8_kernel(const __grid_constant__ CUtensorMap map32, const __grid_constant_
   const int pieces = (K + I8_GROUP - 1) / I8_GROUP;                      // of 256 values: a warp's lanes have eight each
   unsigned char* ring = smem;                                            // [warp][stage][32 rows x 128 bytes]
   int8_t* xs = reinterpret_cast<int8_t*>(ring + (size_t)GV_WARPS * S * GV_UNIT);      // [T][ldx]
-  int* acc = reinterpret_cast<int*>(xs + (size_t)T * ldx);               // [r8 - r0][2]
+  int* acc = reinterpret_cast<int*>(xs + (size_t)T * ldx);               // [r8 - r0][4]
   float* sums = reinterpret_cast<float*>(acc + (r8 - r0) * GV_TOKENS);   // [T][pieces]
   volatile int* abort_flag = &abort_s;
 
@@ -167,14 +167,15 @@ gemv_i8_kernel(const __grid_constant__ CUtensorMap map32, const __grid_constant_
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const int row = block * GV_ROWS + m * 16 + (lane >> 2), col = (lane & 3) * 2;
-      if (col == 0) {
+      if (col < T) {
+        const bool two = col + 1 < T;
         if (r0 + row < r1) {
-          atomicAdd(&acc[row * GV_TOKENS], c[m][0]);
-          if (T > 1) atomicAdd(&acc[row * GV_TOKENS + 1], c[m][1]);
+          atomicAdd(&acc[row * GV_TOKENS + col], c[m][0]);
+          if (two) atomicAdd(&acc[row * GV_TOKENS + col + 1], c[m][1]);
         }
         if (r0 + row + 8 < r1) {
-          atomicAdd(&acc[(row + 8) * GV_TOKENS], c[m][2]);
-          if (T > 1) atomicAdd(&acc[(row + 8) * GV_TOKENS + 1], c[m][3]);
+          atomicAdd(&acc[(row + 8) * GV_TOKENS + col], c[m][2]);
+          if (two) atomicAdd(&acc[(row + 8) * GV_TOKENS + col + 1], c[m][3]);
         }
       }
       c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0;
@@ -262,11 +263,11 @@ int gv_launch(const CUtensorMap& m32, const CUtensorMap& m8, const GemvI8Params&
 
 bool i8_tensor(CUtensorMap* m, const void* base, long long width, long long rows, long long ld, int box_rows);
 
-// Whether gemv_i8_launch takes T rows.  Weights up to 16 MB: there a launch less counts more than that the pair form's next weights are on their way
+// Whether gemv_i8_launch takes T rows.  Weights up to 16 MB, of three or four rows 8: there a launch less counts more than that the pair form's next weights are on their way
 // while its rows are quantised, for which this form, whose rings fill the SMs, leaves no room (us here and in two launches, one row:
-// 320 x 256 3.8 and 5.1, 5120 x 1024 5.1 and 7.1, 5120 x 5120 11.4 and 10.9, 16480 x 5120 20.6 and 18.5; 5120 x 1024, four rows 6.9 and 7.2, eight 9.4
-// and 7.2).
-bool gemv_i8_takes(int T, int N, int K) { return T <= GV_TOKENS && (long long)N * K <= 16 << 20 && K <= GV_MOST_K && gv_stages(T, N, K) > 0; }
+// 320 x 256 3.8 and 5.1, 5120 x 1024 5.1 and 7.1, 5120 x 5120 11.4 and 10.9, 16480 x 5120 20.6 and 18.5; 5120 x 1024, four rows 6.9 and 6.8, and 2 less of
+// the host's time, eight 9.4 and 6.8; 16000 x 1024, three rows 9.3 and 8.0).
+bool gemv_i8_takes(int T, int N, int K) { return T <= GV_TOKENS && (long long)N * K <= (T > 2 ? 8 : 16) << 20 && K <= GV_MOST_K && gv_stages(T, N, K) > 0; }
 
 // x: bf16 rows, on 16-byte boundaries, quantised here (of rmsnorm(x) * norm_w where that is given).
 int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr,
@@ -274,5 +275,5 @@ int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long 
   CUtensorMap m32, m8;
   if (!i8_tensor(&m32, w, K, N, ldw, GV_ROWS) || !i8_tensor(&m8, w, K, N, ldw, 8)) return (int)cudaErrorInvalidValue;
   GemvI8Params p{(const float*)ws, (const bf16*)x, (const float*)norm_w, (const bf16*)residual, out, ldx, ldr, ldo, T, N, K, epi, gv_stages(T, N, K), eps};
-  return T == 1 ? gv_launch<1>(m32, m8, p, stream) : gv_launch<2>(m32, m8, p, stream);
+  return T == 1 ? gv_launch<1>(m32, m8, p, stream) : T == 2 ? gv_launch<2>(m32, m8, p, stream) : gv_launch<4>(m32, m8, p, stream);
 }

@@ -139,7 +139,7 @@ register("fp8", "sm100", {
 })
 register("int8", "sm100", {
     "linear_int8": Kernel("gemm_i8_kernel", "csrc/gemm_i8.cu", "trl_linear_i8", "tilerl_b200.ops.gemm_int8", note="tcgen05.mma kind::i8 on pairs of SMs"),
-    "linear_int8_gemv": Kernel("gemv_i8_kernel", "csrc/gemv_i8.cu", "trl_linear_i8", "tilerl_b200.ops.gemm_int8", note="up to 8 rows, quantised inside; mma.sync"),
+    "linear_int8_gemv": Kernel("gemv_i8_kernel", "csrc/gemv_i8.cu", "trl_linear_i8", "tilerl_b200.ops.gemm_int8", note="up to 4 rows of weights up to 16 MB, quantised inside; mma.sync"),
     "linear_int8_grad": Kernel("gemm_i8_kernel", "csrc/gemm_i8.cu", "trl_linear_i8_grad", "tilerl_b200.ops.gemm_int8", note="rows in two digits of 8 bits"),
     "quant_int8": Kernel("rows_i8_kernel", "csrc/rows_i8.cu", "trl_rows_i8", "tilerl_b200.ops.gemm_int8",
                          note="RMSNorm + int8 with one scale per token; weights by channel; gradients in 16 bits"),
