@@ -38,6 +38,22 @@ __device__ __forceinline__ RowsRaw<T> rows_load(const T* x, int k, int K) {
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.u[i] = __ldcg(reinterpret_cast<const uint4*>(x + k) + i);
     return r;
   }
+  if constexpr (!VEC && sizeof(T) == 4) {
+    // a row off its boundary (gradients of an odd number of channels): the three aligned vectors that the eight values lie in, where all of
+    // them are the row's.  One by one, 32 bytes from lane to lane, every sector would be asked for eight times.
+    if (k >= 4 && k + 12 <= K) {
+      const int m = (int)(reinterpret_cast<uintptr_t>(x) >> 2 & 3);
+      const uint4* p = reinterpret_cast<const uint4*>(x + k - m);
+      const uint4 a = __ldcg(p), b = __ldcg(p + 1), c = __ldcg(p + 2);
+      switch (m) {
+        case 0: r.u[0] = a, r.u[1] = b; break;
+        case 1: r.u[0] = make_uint4(a.y, a.z, a.w, b.x), r.u[1] = make_uint4(b.y, b.z, b.w, c.x); break;
+        case 2: r.u[0] = make_uint4(a.z, a.w, b.x, b.y), r.u[1] = make_uint4(b.z, b.w, c.x, c.y); break;
+        default: r.u[0] = make_uint4(a.w, b.x, b.y, b.z), r.u[1] = make_uint4(b.w, c.x, c.y, c.z);
+      }
+      return r;
+    }
+  }
   T* v = reinterpret_cast<T*>(&r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = k + i < K ? __ldcg(x + k + i) : T(0.f);
