@@ -478,6 +478,59 @@ def test_captured_training_pass():
         assert torch.equal(a, out) and torch.equal(b, dx)
 
 
+def test_two_threads_at_once_on_one_stream_and_on_two():
+    """The kernels of a call hand each other its integers: no other call's."""
+    import threading
+    ws = [_weight(386, 1040, i) for i in range(2)]
+    xs, ups = [_x(9 + i, 1040, i, torch.float32) for i in range(2)], [_x(9 + i, 386, i, torch.float32) for i in range(2)]
+
+    def step(i):
+        tape = T.Tape()
+        tape.watch(xs[i])
+        out = T.linear(tape, xs[i], ws[i])
+        return out, tape.backward(out, ups[i])[id(xs[i])]
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    for streams in (None, [torch.cuda.Stream() for _ in range(2)]):
+        wrong = []
+
+        def work(i):
+            with torch.cuda.stream(streams[i] if streams else torch.cuda.default_stream()):
+                got = [step(i) for _ in range(200)]
+                torch.cuda.current_stream().synchronize()
+            wrong.extend(1 for g in got if not (torch.equal(g[0], want[i][0]) and torch.equal(g[1], want[i][1])))
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        assert not wrong
+
+
+def test_captured_training_passes_share_nothing():
+    """Two captured passes of one thread, replayed at once on two streams."""
+    w, x, up = _weight(386, 1040), [_x(30, 1040, i, torch.float32) for i in range(2)], _x(30, 386, 3, torch.float32)
+
+    def step(i):
+        tape = T.Tape()
+        tape.watch(x[i])
+        out = T.linear(tape, x[i], w)
+        return out, tape.backward(out, up)[id(x[i])]
+    want = [[t.clone() for t in step(i)] for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, got = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            got.append(step(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        step(0)                                      # (and an eager one beside them)
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+
+
 def test_on_another_stream(ops):
     w, nw = _weight(386, 1040), torch.rand(1040, device=DEV) + 0.5
     side = torch.cuda.Stream()

@@ -11,7 +11,8 @@ The reference multiplies in FP8 (``linear_fp8``, packages/tilerl-kernels/src/til
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+import threading
+from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -156,6 +157,28 @@ def train_takes(x: torch.Tensor, w: INT8Tensor) -> bool:
     return r is not None and x.get_device() == r.device and x.shape[-1] == r.k and r.n <= MOST
 
 
+#: memory for the integers of short calls, for each thread and stream: (an allocation takes as long as a launch)
+_KEPT = threading.local()
+_KEEP = 4 << 20
+
+
+def _workspace(rows: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """Memory that a call's kernels hand to each other.  Up to 4 MB is kept from call to call: calls of one thread on one stream run one
+    after the other, while two threads may launch theirs in between each other.  A captured call has its own, as every other of its tensors."""
+    if nbytes > _KEEP or _capturing():
+        return rows.new_empty(nbytes, dtype=torch.int8)
+    kept: Dict[Tuple[int, int], torch.Tensor] = _KEPT.__dict__
+    key = (rows.get_device(), _raw_stream(rows.get_device()))
+    t = kept.get(key)
+    if t is None:
+        t = kept[key] = rows.new_empty(_KEEP, dtype=torch.int8)
+    return t
+
+
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_raw_stream = N._raw_stream
+
+
 def _flat(x: torch.Tensor, width: int) -> torch.Tensor:
     if x.requires_grad:
         x = x.detach()
@@ -171,7 +194,7 @@ def forward(x: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     t = rows.shape[0]
     out = rows.new_empty((t, r.n), dtype=torch.float32)
     if t:
-        _product(rows, r, out, r.n, rows.new_empty(_scratch(t, r.k), dtype=torch.int8), None, 0.0, None, EPI_STORE_F32)
+        _product(rows, r, out, r.n, _workspace(rows, _scratch(t, r.k)), None, 0.0, None, EPI_STORE_F32)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], r.n)
 
 
@@ -182,7 +205,7 @@ def grad(g: torch.Tensor, w: INT8Tensor) -> torch.Tensor:
     t = rows.shape[0]
     dx = rows.new_empty((t, r.k), dtype=torch.float32)
     if t:
-        _gradient(rows, r, dx, rows.new_empty(_scratch(t, r.n, 2), dtype=torch.int8))
+        _gradient(rows, r, dx, _workspace(rows, _scratch(t, r.n, 2)))
     return dx if g.dim() == 2 else dx.view(*g.shape[:-1], r.k)
 
 
