@@ -118,8 +118,9 @@ __device__ __forceinline__ uint4 gi_residual8(const I8Params& p, int tok, int f)
   if (tok >= p.tokens || f >= p.features) return make_uint4(0u, 0u, 0u, 0u);
   return __ldcg(reinterpret_cast<const uint4*>(p.residual + (size_t)tok * p.ldr + f));
 }
-// Eight features of a token out as one vector (v: results before the residual u).
-__device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8], const uint4& u) {
+// Eight features of a token out as one vector (v: results before the residual, which is u or still to be read).
+template <bool READ>
+__device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, const float (&v)[8], uint4 u) {
   if (tok >= p.tokens || f >= p.features) return;
   const size_t at = (size_t)tok * p.ldo;
   if (p.epi == I8_SWIGLU) {                          // features in (gate, up) pairs
@@ -133,6 +134,7 @@ __device__ __forceinline__ void gi_store8(const I8Params& p, int tok, int f, con
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = v[i];
     if (p.epi == I8_RESIDUAL) {
+      if (!READ) u = gi_residual8(p, tok, f);
       const float2 a = bf162_bits_to_f2(u.x), b = bf162_bits_to_f2(u.y), c = bf162_bits_to_f2(u.z), d = bf162_bits_to_f2(u.w);
       y[0] = __fadd_rn(y[0], a.x), y[1] = __fadd_rn(y[1], a.y), y[2] = __fadd_rn(y[2], b.x), y[3] = __fadd_rn(y[3], b.y);
       y[4] = __fadd_rn(y[4], c.x), y[5] = __fadd_rn(y[5], c.y), y[6] = __fadd_rn(y[6], d.x), y[7] = __fadd_rn(y[7], d.y);
@@ -374,8 +376,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = value(x[e], st, ws[e]);
-                if (!GRAD && !EARLY && p.epi == I8_RESIDUAL) res[h / 8 + i] = gi_residual8(p, tok0 + c * TOK + h + u, f0);
-                gi_store8(p, tok0 + c * TOK + h + u, f0, v, res[h / 8 + i]);
+                gi_store8<EARLY>(p, tok0 + c * TOK + h + u, f0, v, EARLY ? res[h / 8 + i] : make_uint4(0u, 0u, 0u, 0u));
               }
             } else {
               float v[16], up[16];
@@ -409,7 +410,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = GRAD ? __fmul_rn(fmaf(256.f, (float)y[0][e], (float)y[J - 1][e]), join_scale) : i8_value(y[0][e], __fmul_rn(join_scale, join_ws[e]));
       if (p.vec) {
-        gi_store8(p, tok, f, v, join_res);
+        gi_store8<true>(p, tok, f, v, join_res);
       } else if (p.epi == I8_SWIGLU) {
         const float gate[4] = {v[0], v[2], v[4], v[6]}, up[4] = {v[1], v[3], v[5], v[7]};
         gi_store_each<4>(p, tok, 0, f, 2, (p.features - f + 1) / 2, gate, up);
