@@ -248,7 +248,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       uint32_t ph = 0;
       auto next_w = [&] { if (++w_kt == k1) w_kt = k0, w_tile += tile_step, w_rt = w_tile / p.c_tiles; };
       const int pre = min(STAGES, units);
-      for (int u = 0; u < pre; ++u) load_w(w_rt, w_kt, u), next_w();       // weights do not depend on the kernel ahead (rows_i8.cu)
+      for (int u = 0; u < pre; ++u) load_w(w_rt, w_kt, u), next_w();       // the kernel ahead, the rows' quantiser, runs: what wrote the weights has ended (rows_i8.cu)
       pdl_wait();
       for (int u = 0; u < units; ++u) {
         if (u >= pre) {
@@ -572,7 +572,7 @@ bool gemv_i8_takes(int T, int N, int K);
 int gemv_i8_launch(const void* w, long ldw, const void* ws, const void* x, long ldx, const void* norm_w, float eps, const void* residual, long ldr,
                    void* out, long ldo, int T, int N, int K, int epi, cudaStream_t stream);
 extern "C" int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K, int digits,
-                           int weights, void* scratch, void* stream);
+                           void* scratch, void* stream);
 
 // out[t, n] = epi(norm(x) . w): rows of x (type 0: fp32, 1: bf16) quantised, multiplied.  norm_w: a norm's weight, or null.  scratch: T * K
 // bytes for the integers and 4 * T for the scales, on a 16-byte boundary, K % 16 == 0.  Otherwise as above.  Returns minus the number of launches,
@@ -590,7 +590,7 @@ TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w,
     return rc ? rc : -1;
   }
   void* s = (int8_t*)scratch + (size_t)T * K;
-  int rc = trl_rows_i8(x, type, ldx, norm_w, norm_w != nullptr, eps, scratch, K, s, T, K, 1, 0, nullptr, stream);
+  int rc = trl_rows_i8(x, type, ldx, norm_w, norm_w != nullptr, eps, scratch, K, s, T, K, 1, nullptr, stream);
   if (!rc) rc = gi_linear(w, ldw, ws, scratch, K, s, residual, ldr, out, ldo, T, N, K, epi, stream);
   return rc ? rc : -2;
 }
@@ -602,6 +602,6 @@ TRL_API int trl_linear_i8_grad(const void* g, int type, long ldg, const void* w,
   if (T <= 0 || N <= 0 || N > GI_MOST) return (int)cudaErrorInvalidValue;
   const long ldq = (N + 15) / 16 * 16;
   char* s = (char*)scratch + 2 * (size_t)T * ldq;
-  const int rc = trl_rows_i8(g, type, ldg, ws, 0, 0.f, scratch, ldq, s, T, N, 2, 0, s + 4 * (size_t)T, stream);
+  const int rc = trl_rows_i8(g, type, ldg, ws, 0, 0.f, scratch, ldq, s, T, N, 2, s + 4 * (size_t)T, stream);
   return rc ? rc : gi_grad(w, ldw, scratch, ldq, s, dx, ldo, T, N, K, stream);
 }

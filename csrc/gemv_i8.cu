@@ -87,10 +87,10 @@ gemv_i8_kernel(const __grid_constant__ CUtensorMap map32, const __grid_constant_
       for (int r = 0; r < rows; r += 8) tma_load_2d(dst + (uint32_t)r * GV_STEP, &map8, k, row + r, bar);
     }
   };
+  pdl_wait();                                      // (the kernel ahead may have written the weights)
   if (elect_one())
-    for (int u = 0; u < min(S, mine); ++u) load(u, u);      // weights do not depend on the kernel ahead (rows_i8.cu)
+    for (int u = 0; u < min(S, mine); ++u) load(u, u);
   __syncwarp();
-  pdl_wait();
 
   // ---- the rows into integers: a warp has up to two pieces of 256 values of every token, and the norm's factors of those ----
   uint4 raw[GV_PIECES][TOK];

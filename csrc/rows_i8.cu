@@ -22,8 +22,16 @@ struct RowsParams {
   int K;
   float eps;
   int norm;
-  int weights;           // q and s are a weight: products may read one before they wait for the kernel ahead of them
 };
+
+// Products ask for their first weights before they wait for the quantiser of their rows (gemm_i8.cu).  So a quantiser lets them start only once it
+// has itself waited for all that is ahead of it: whatever wrote the weight (a copy, a quantiser of weights, an optimiser) has then ended, and
+// what it wrote can be seen.
+__device__ __forceinline__ void rows_enter() {
+  pdl_enter();
+  pdl_wait();
+  pdl_trigger();
+}
 
 // Eight values as they lie in memory.
 template <typename T>
@@ -108,9 +116,7 @@ template <typename T, int CH, bool VEC, bool W16>
 __global__ void __launch_bounds__(CH == 1 ? 640 : 1024, CH == 1 ? 2 : 1) rows_i8_kernel(const RowsParams p) {
   extern __shared__ float groups_s[];            // sums of squares of 256 values each, of two rows in turn
   __shared__ uint32_t most_s[2][32];
-  // (products load weights before they wait for the kernels ahead, so a weight's quantiser lets none of them start before its end)
-  if (!p.weights) pdl_launch_dependents();
-  pdl_wait();
+  rows_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5, K = p.K, pieces = (K + I8_GROUP - 1) / I8_GROUP;
   const bool squares = !W16 && p.norm;
   constexpr int KEEP = CH ? CH : 1;
@@ -205,8 +211,7 @@ constexpr int RL_THREADS = 256, RL_PIECE = RL_THREADS * 8, RL_VECS = 4, RL_ROWS 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(RL_THREADS, 3) rows_most_kernel(const RowsParams p, uint32_t* most) {      // most: [pieces][rows]
   __shared__ uint32_t most_s[2][RL_ROWS][RL_THREADS / 32];
-  pdl_launch_dependents();
-  pdl_wait();
+  rows_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.K, k = min(blockIdx.x * RL_PIECE + threadIdx.x * 8, K);
   float w[8];
   rows_values<float>(rows_load<float, VEC>(p.w, k, K), w);
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(RL_THREADS, 3) rows_most_kernel(const RowsPara
 }
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(RL_THREADS, 2) rows_digits_kernel(const RowsParams p, const uint32_t* most, int pieces) {
-  pdl_launch_dependents();
+  pdl_launch_dependents();                           // (it runs: the first pass has waited)
   pdl_wait();
   const int lane = threadIdx.x & 31, K = p.K;
   int k[RL_VECS];
@@ -315,14 +320,14 @@ cudaError_t rows_launch(const RowsParams& p, cudaStream_t stream) {
 
 // x [rows, K] (type 0: fp32, 1: bf16; rows ldx apart) -> q int8 [rows, ldq], s fp32 [rows].  w: fp32 [K] or null; norm: w is a norm's
 // weight, and the row's 1 / rms goes into s.  digits 2: q has two rows of digits a row, 16 bits in all, and w is the channels' scales.
-// weights: q and s are a weight's.  scratch: 4 bytes a row for every 2048 of its values (two digits only).  ldq and q on 8-byte boundaries.
+// scratch: 4 bytes a row for every 2048 of its values (two digits only).  ldq and q on 8-byte boundaries.
 TRL_API int trl_rows_i8(const void* x, int type, long ldx, const void* w, int norm, float eps, void* q, long ldq, void* s, long rows, int K,
-                        int digits, int weights, void* scratch, void* stream) {
+                        int digits, void* scratch, void* stream) {
   if (rows <= 0 || rows > 0x7fffffffl || K <= 0 || ldq < K || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || (type != 0 && type != 1) ||
       (digits != 1 && digits != 2) || (norm && (w == nullptr || digits == 2)) || (digits == 2 && w == nullptr) ||
       (scratch == nullptr && digits == 2))
     return (int)cudaErrorInvalidValue;
-  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, rows, K, eps, norm, weights};
+  RowsParams p{x, (const float*)w, (int8_t*)q, (float*)s, ldx, ldq, rows, K, eps, norm};
   cudaStream_t st = (cudaStream_t)stream;
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || ldx % (type ? 8 : 4) == 0) && reinterpret_cast<uintptr_t>(w) % 16 == 0;
   if (rows_long(rows, K, digits)) {

@@ -289,6 +289,35 @@ def test_weights_that_were_just_written(ops):
             assert torch.equal(ops.norm_linear(x, nw, w, 1e-6), right[i])
 
 
+@pytest.mark.parametrize("t", [1, 3, 20, 300])
+def test_weights_that_another_kernel_just_wrote(ops, t):
+    """A copy, an operation in place: kernels that know nothing of the products behind them."""
+    for n, k in ((5120, 1024), (4096, 4096), (8192, 2048)):
+        two = [_weight(n, k, i) for i in range(2)]
+        w = F.INT8Tensor(torch.zeros(n, k, dtype=torch.int8, device=DEV), torch.zeros(n, device=DEV))
+        x, nw, up = _x(t, k), torch.rand(k, device=DEV) + 0.5, _x(t, n, 5, torch.float32)
+
+        def gradient(v):
+            tape = T.Tape()
+            tape.watch(x)
+            return tape.backward(T.linear(tape, x, v), up)[id(x)]
+        right = [(ops.norm_linear(x, nw, v, 1e-6).clone(), T.linear(T.Tape(), x, v), gradient(v)) for v in two]
+        other = ops.norm_linear(x, nw, F.INT8Tensor(-two[0].w8, two[0].wscale), 1e-6).clone()
+        torch.cuda.synchronize()
+        got = []
+        for i in (0, 1, 0, 1):
+            w.w8.zero_(), w.wscale.copy_(two[i].wscale), w.w8.copy_(two[i].w8)
+            a = ops.norm_linear(x, nw, w, 1e-6).clone()
+            w.w8.zero_(), w.w8.copy_(two[i].w8)
+            b = T.linear(T.Tape(), x, w)
+            w.w8.zero_(), w.w8.copy_(two[i].w8)
+            got.append((i, a, b, gradient(w)))
+        w.wscale.copy_(two[0].wscale), w.w8.copy_(two[0].w8), w.w8.neg_()
+        assert torch.equal(ops.norm_linear(x, nw, w, 1e-6), other)
+        for i, *outs in got:
+            assert all(torch.equal(a, b) for a, b in zip(outs, right[i]))
+
+
 def test_weights_and_outputs_past_32_bits_of_bytes(ops):
     """A weight of more than 2^31 bytes, and an output of as many values."""
     n, k = 20000, 110080

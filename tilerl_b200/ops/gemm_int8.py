@@ -23,7 +23,7 @@ EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
 
-N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.I, N.P, N.P])
+N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.P, N.P])
 N.register("trl_linear_i8", [N.P, N.I, N.L, N.P, N.F, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.P, N.I, N.I, N.I, N.I, N.P])
 N.register("trl_linear_i8_grad", [N.P, N.I, N.L, N.P, N.L, N.P, N.P, N.L, N.P, N.I, N.I, N.I, N.P])
 
@@ -100,12 +100,12 @@ def _scratch(rows: int, width: int, digits: int = 1) -> int:
     return rows * (2 * (-(-width // 16) * 16) + 4 + 4 * -(-width // 2048))
 
 
-def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None, weights: bool = False) -> None:
+def quant_rows(x, q, s, *, norm_w=None, eps: float = 0.0, channels=None) -> None:
     """Rows ``x [T, K]`` into ``q`` (int8 ``[T, >= K]``) and ``s`` (fp32 ``[T]``); with ``channels`` (a gradient's scales) into two rows of digits
-    a row of ``x``.  ``weights``: they are a weight's, which products load before they wait for the launch ahead of them."""
+    a row of ``x``."""
     scratch = None if channels is None else torch.empty(x.shape[0] * -(-x.shape[1] // 2048), dtype=torch.int32, device=x.device)
     N.check(N.lib().trl_rows_i8(x.data_ptr(), TYPES[x.dtype], x.stride(0), N.ptr(channels if norm_w is None else norm_w), int(norm_w is not None), eps,
-                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, int(weights), N.ptr(scratch), N.stream()), "rows_i8")
+                                q.data_ptr(), q.stride(0), s.data_ptr(), x.shape[0], x.shape[1], 1 if channels is None else 2, N.ptr(scratch), N.stream()), "rows_i8")
     N.count()
 
 
@@ -225,7 +225,7 @@ def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
         raise ValueError(f"quantize_ takes fp32 or bf16 of {dst.shape} on the weight's device, got {tuple(src.shape)} {src.dtype} on {src.device}")
     src = src if src.stride(1) == 1 else src.contiguous()
     with N.on(src.device):
-        quant_rows(src, dst.w8, dst.wscale, weights=True)
+        quant_rows(src, dst.w8, dst.wscale)
     for t in (dst.w8, dst.wscale):
         if not t.is_inference():
             torch.autograd.graph.increment_version(t)
