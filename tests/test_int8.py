@@ -276,3 +276,38 @@ def test_the_format_by_name_and_by_directory(tmp_path, capsys):
     assert specs["L0.gate_up"][1] == "int8" and F.nbytes("int8", (34816, 5120)) == 34816 * 5124
     from tilerl_b200.kernel_cost import prefill_rows
     assert prefill_rows(cfg, 100)
+
+
+class _Elsewhere:
+    """Memory of a backend on another device, as far as the checks look."""
+    device = torch.device("cuda:1")
+
+    def get_device(self):
+        return 1
+
+
+def _as_if_on_a_gpu(monkeypatch, n, k, buffer):
+    """A weight that passes for one on a device, the products that would be launched, a backend with `buffer`."""
+    import types
+    from tilerl_b200.ops import gemm_int8
+    w = F.quantize_int8(_rows(n, k))
+    launched = []
+    monkeypatch.setattr(gemm_int8, "_ready", lambda w: gemm_int8._Ready(w.w8, w.wscale, n, k, 0, k, 0, -1))
+    monkeypatch.setattr(gemm_int8, "_product", lambda *a: launched.append(a))
+    ops = types.SimpleNamespace(ws=types.SimpleNamespace(get=lambda name, shape, dtype: buffer))
+    return w, ops, launched
+
+
+def test_a_backend_on_another_device_is_refused(monkeypatch):
+    from tilerl_b200.ops import gemm_int8
+    w, ops, launched = _as_if_on_a_gpu(monkeypatch, 8, 16, _Elsewhere())
+    x, y = torch.zeros(2, 16, dtype=torch.bfloat16), torch.zeros(2, 8, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="buffers on cuda:1"):
+        gemm_int8.linear(ops, x, w, y)
+    with pytest.raises(ValueError, match="buffers on cuda:1"):
+        gemm_int8.linear(ops, x, w, y, residual=y, epi=gemm_int8.EPI_RESIDUAL)
+    gemm_int8.linear(ops, x[:0], w, y[:0])
+    assert not launched
+    w, ops, launched = _as_if_on_a_gpu(monkeypatch, 8, 16, torch.zeros(99, dtype=torch.int8))
+    gemm_int8.linear(ops, x, w, y)
+    assert len(launched) == 1

@@ -121,6 +121,14 @@ def _product(x, r: _Ready, out, ldo, scratch, norm_w, eps, residual, epi) -> Non
     N.count(-rc)
 
 
+def _integers(ops, t: int, r: _Ready) -> torch.Tensor:
+    """The backend's memory for a product's integers: its kernels run on the weight's device."""
+    scratch = ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8)
+    if scratch.get_device() != r.device:
+        raise ValueError(f"the weight is on {r.w8.device}, the backend's buffers on {scratch.device}")
+    return scratch
+
+
 def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) -> None:
     """``y = epi(norm(x) @ W^T)``; ``y`` may be the residual."""
     r = _ready(w)
@@ -130,7 +138,7 @@ def linear(ops, x, w, y, *, norm_w=None, eps=0.0, residual=None, epi=EPI_STORE) 
     t = x.shape[0]
     _refuse_out(y, t, r, residual, epi)
     if t:
-        _product(x, r, y, y.stride(0), ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8), norm_w, eps, residual, epi)
+        _product(x, r, y, y.stride(0), _integers(ops, t, r), norm_w, eps, residual, epi)
 
 
 def served(ops, name: str, x, w, norm_w, eps: float, epi: int = EPI_STORE) -> torch.Tensor:
@@ -144,7 +152,7 @@ def served(ops, name: str, x, w, norm_w, eps: float, epi: int = EPI_STORE) -> to
     if y.get_device() != r.device:
         raise ValueError(f"the weight is on {w.w8.device}, the backend's buffers on {y.device}")
     if t:
-        _product(x, r, y, width, ops.ws.get("int8_rows", (_scratch(t, r.k),), torch.int8), norm_w, eps, None, epi)
+        _product(x, r, y, width, _integers(ops, t, r), norm_w, eps, None, epi)
     return y
 
 
