@@ -311,3 +311,32 @@ def test_a_backend_on_another_device_is_refused(monkeypatch):
     w, ops, launched = _as_if_on_a_gpu(monkeypatch, 8, 16, torch.zeros(99, dtype=torch.int8))
     gemm_int8.linear(ops, x, w, y)
     assert len(launched) == 1
+
+
+def test_residuals_that_cross_the_output_are_refused(monkeypatch):
+    """All pairs of views of one small buffer, against the elements that they consist of."""
+    from tilerl_b200.ops import gemm_int8
+    w, ops, launched = _as_if_on_a_gpu(monkeypatch, 3, 16, torch.zeros(99, dtype=torch.int8))
+    x, buffer, seen = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(64, dtype=torch.bfloat16), set()
+    for t in (1, 2, 4):
+        views = [(s, ld) for ld in (3, 5, 8) for s in range(64 - (t - 1) * ld - 2)]
+        place = {v: torch.tensor([v[0] + i * v[1] + j for i in range(t) for j in range(3)]) for v in views}
+        for a in views[::3]:
+            for b in views:
+                y, res = (torch.as_strided(buffer, (t, 3), (ld, 1), s) for s, ld in (a, b))
+                pa, pb = place[a], place[b]
+                bad = bool(((pa[:, None] == pb[None]) & ~torch.eye(len(pa), dtype=torch.bool)).any())
+                if a[1] != b[1] and t > 1 and not bad:
+                    bad = None                       # (may be refused where the ranges cross)
+                    if int(pa[-1]) < int(pb[0]) or int(pb[-1]) < int(pa[0]):
+                        bad = False
+                before = len(launched)
+                try:
+                    gemm_int8.linear(ops, x[:t], w, y, residual=res, epi=gemm_int8.EPI_RESIDUAL)
+                    refused = False
+                except ValueError as e:
+                    assert "residual" in str(e)
+                    refused = True
+                assert refused == (len(launched) == before) and (bad is None or refused == bad), (t, a, b)
+                seen.add((t, refused))
+    assert len(seen) == 6

@@ -83,6 +83,16 @@ def _width(r: _Ready, epi: int) -> int:
     return r.n // 2
 
 
+def _crosses(y: torch.Tensor, residual: torch.Tensor) -> bool:
+    """Whether a result is written over the residual of another one, which another thread may not have read yet.  (Two bf16 tensors of one shape;
+    rows apart by different strides count as crossing wherever their ranges do.)"""
+    (t, n), apart = y.shape, (residual.data_ptr() - y.data_ptr()) // 2
+    ly, lr = (y.stride(0), residual.stride(0)) if t > 1 else (n, n)
+    if not t or apart == 0 and ly == lr or apart >= (t - 1) * ly + n or apart + (t - 1) * lr + n <= 0:
+        return False
+    return ly != lr or apart % ly < n or ly - apart % ly < n
+
+
 def _refuse_out(y, t: int, r: _Ready, residual, epi: int) -> None:
     width, kind, here = _width(r, epi), torch.float32 if epi == EPI_STORE_F32 else torch.bfloat16, r.device
     if y.shape != (t, width) or y.dtype != kind or y.get_device() != here or t and y.stride(1) != 1 and width > 1 or t > 1 and y.stride(0) < width:
@@ -90,6 +100,8 @@ def _refuse_out(y, t: int, r: _Ready, residual, epi: int) -> None:
     if (epi == EPI_RESIDUAL) != (residual is not None) or residual is not None and residual is not y and (
             residual.shape != y.shape or residual.dtype != torch.bfloat16 or residual.get_device() != here or residual.stride(1) != 1 and r.n > 1):
         raise ValueError("a residual is bf16 rows of the output's shape, given where one is added")
+    if residual is not None and residual is not y and _crosses(y, residual):
+        raise ValueError("a residual lies where the output does, each value in the place of its own result, or apart from it")
 
 
 def _scratch(rows: int, width: int, digits: int = 1) -> int:
