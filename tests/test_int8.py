@@ -340,3 +340,46 @@ def test_residuals_that_cross_the_output_are_refused(monkeypatch):
                 assert refused == (len(launched) == before) and (bad is None or refused == bad), (t, a, b)
                 seen.add((t, refused))
     assert len(seen) == 6
+
+
+def test_parts_of_a_fused_projection_that_are_not_integers_leave_the_others_alone(tmp_path):
+    """Exports that keep the recurrent layers' small projections in bf16."""
+    from safetensors.torch import save_file
+    from test_checkpoint import _hf_tensors
+    from tilerl_b200.checkpoint import load_checkpoint
+    cfg = _tiny("tiny-hybrid")
+    tensors = _hf_tensors(cfg, random_master(cfg, seed=3), "bf16")
+    g = torch.Generator().manual_seed(2)
+    dense = ("in_proj_a", "in_proj_b", "k_proj", "up_proj")
+    for k in [k for k in tensors if "_proj" in k and not any(d in k for d in dense)]:
+        tensors[k] = torch.randint(-100, 100, tensors[k].shape, generator=g, dtype=torch.int8)      # (no row reaches 127)
+        tensors[k + "_scale"] = torch.rand(len(tensors[k]), generator=g) * 1e-3 + 1e-5
+    save_file(tensors, str(tmp_path / "model.safetensors"))
+    m = load_checkpoint(cfg, str(tmp_path), keep_master=True)
+
+    def whole(layer, *bases):
+        return [(tensors[f"model.layers.{layer}.{b}.weight"], tensors.get(f"model.layers.{layer}.{b}.weight_scale")) for b in bases]
+
+    def check(rows, scales, master, w, s):
+        if s is not None:
+            assert torch.equal(rows, w) and torch.equal(scales, s) and torch.equal(master, w * s[:, None])
+        else:
+            want = F.quantize_int8(w)
+            assert torch.equal(rows, want.w8) and torch.equal(scales, want.wscale) and torch.equal(master, w.float())
+    for name, parts in (("L0.in", whole(0, *("linear_attn.in_proj_" + n for n in ("qkv", "z", "a", "b")))),
+                        ("L1.qkv", whole(1, *("self_attn." + n + "_proj" for n in "qkv")))):
+        got, master, at = m.params[name], m.params["master." + name], 0
+        for w, s in parts:
+            here = slice(at, at + len(w))
+            check(got.w8[here], got.wscale[here], master[here], w, s)
+            at += len(w)
+        assert at == len(got.w8) == len(master)
+    got, master = m.params["L0.gate_up"], m.params["master.L0.gate_up"]
+    for i, (w, s) in enumerate(whole(0, "mlp.gate_proj", "mlp.up_proj")):
+        check(got.w8[i::2], got.wscale[i::2], master[i::2], w, s)
+    half = load_checkpoint(cfg, str(tmp_path), keep_master=True, tp_rank=1, tp=2)
+    from tilerl_b200.parallel.mesh import shard_param
+    for name in ("L0.in", "L1.qkv", "L0.gate_up", "L0.out"):
+        want = shard_param(cfg, name, m.params[name], 1, 2)
+        assert torch.equal(half.params[name].w8, want.w8) and torch.equal(half.params[name].wscale, want.wscale)
+        assert torch.equal(half.params["master." + name], shard_param(cfg, name, m.params["master." + name], 1, 2))

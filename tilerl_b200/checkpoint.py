@@ -11,7 +11,7 @@ parameter dict (TP-sharded if asked):
 * FP8 128x128-block files: ``.weight`` e4m3 + ``.weight_scale_inv``; FP8 per-tensor / per-channel:
   ``.weight`` e4m3 + ``.weight_scale``;
 * 8-bit integers per channel: ``.weight`` int8 + ``.weight_scale`` ``[N]``, ``[N, 1]`` or one for all; a model
-  served in this format (``quant="int8"``) takes them as they are;
+  served in this format (``quant="int8"``) takes them as they are, also beside parts of a fused projection that are not;
 * MLX 4-bit: ``.weight`` uint32 (8 nibbles, low first) + ``.scales`` + ``.biases`` per group of 64;
 * AWQ: ``.qweight`` int32 ``[K, N/8]`` (AWQ nibble order) + ``.qzeros`` + ``.scales`` per group;
 * this framework's own dialect: ``<name>.wq / .scale / .tscale`` (NVFP4), ``<name>.w8 / .wscale`` (8-bit integers).
@@ -41,7 +41,7 @@ import torch
 
 from .config import ATTN, DeluvikConfig, FetotarConfig, ModelConfig, StreamDesign, TobadraConfig, ZinutarConfig
 from .formats import (FP8BlockTensor, INT8Tensor, NVFP4Tensor, dequantize_fp8_block, dequantize_nvfp4,
-                      quantize_nvfp4)
+                      quantize_int8, quantize_nvfp4)
 from .models.hybrid import HybridModel, linear_names, quantize_weight
 from .models.deluvik import DeluvikModel
 from .models.fetotar import FetotarModel
@@ -233,23 +233,36 @@ def _hf_prefix(reader: _Reader) -> str:
 
 
 def _interleave_rows(a, b):
-    if isinstance(a, INT8Tensor) and isinstance(b, INT8Tensor):
+    if isinstance(a, INT8Tensor) or isinstance(b, INT8Tensor):
+        a, b = _as_int8(a), _as_int8(b)
         return INT8Tensor(_interleave_rows(a.w8, b.w8), _interleave_rows(a.wscale, b.wscale))
-    a, b = (t.dequant() if isinstance(t, INT8Tensor) else t for t in (a, b))
     return torch.stack([a, b], dim=1).reshape(a.shape[0] * 2, *a.shape[1:])
 
 
 def _cat_rows(*parts):
-    """Projections that share their input, one below the other; integers stay what they are if all parts are."""
-    if all(isinstance(t, INT8Tensor) for t in parts):
+    """Projections that share their input, one below the other."""
+    if any(isinstance(t, INT8Tensor) for t in parts):
+        parts = [_as_int8(t) for t in parts]
         return INT8Tensor(torch.cat([t.w8 for t in parts]), torch.cat([t.wscale for t in parts]))
-    return torch.cat([t.dequant() if isinstance(t, INT8Tensor) else t for t in parts])
+    return torch.cat(parts)
 
 
-def assemble_master(cfg: ModelConfig, reader: _Reader) -> Dict[str, torch.Tensor]:
-    """HF tensors -> full (TP=1) master dict in this framework's fused layouts."""
+def _as_int8(t) -> INT8Tensor:
+    """A part of a fused projection whose other parts are integers already: every row has its own scale, so those stay what they are."""
+    return t if isinstance(t, INT8Tensor) else quantize_int8(t)
+
+
+def assemble_master(cfg: ModelConfig, reader: _Reader, masters: Optional[Dict[str, torch.Tensor]] = None) -> Dict[str, torch.Tensor]:
+    """HF tensors -> full (TP=1) master dict in this framework's fused layouts.  ``masters`` takes the dense values of projections that are
+    integers in the file only in part."""
     p = _hf_prefix(reader)
-    lin = lambda base: reader.linear(base, cfg.quant)
+
+    def fuse(name: str, join, *bases: str):
+        parts = [reader.linear(b, cfg.quant) for b in bases]
+        out[name] = join(*parts)
+        if masters is not None and len({type(t) for t in parts}) > 1:
+            masters[name] = join(*(t.dequant() if isinstance(t, INT8Tensor) else t for t in parts))
+
     own = reader.has("embed") or reader.has("embed.weight")
     out: Dict[str, torch.Tensor] = {}
 
@@ -274,22 +287,22 @@ def assemble_master(cfg: ModelConfig, reader: _Reader) -> Dict[str, torch.Tensor
         if t == ATTN:
             a = L + "self_attn."
             # HF q_proj rows are already [query(D); gate(D)] per head when gated
-            out[q + "qkv"] = _cat_rows(lin(a + "q_proj"), lin(a + "k_proj"), lin(a + "v_proj"))
-            out[q + "o"] = lin(a + "o_proj")
+            fuse(q + "qkv", _cat_rows, a + "q_proj", a + "k_proj", a + "v_proj")
+            out[q + "o"] = reader.linear(a + "o_proj", cfg.quant)
             out[q + "q_norm"] = norm(a + "q_norm.weight")
             out[q + "k_norm"] = norm(a + "k_norm.weight")
         else:
             g = L + "linear_attn."
-            out[q + "in"] = _cat_rows(lin(g + "in_proj_qkv"), lin(g + "in_proj_z"), lin(g + "in_proj_a"), lin(g + "in_proj_b"))
-            out[q + "out"] = lin(g + "out_proj")
+            fuse(q + "in", _cat_rows, g + "in_proj_qkv", g + "in_proj_z", g + "in_proj_a", g + "in_proj_b")
+            out[q + "out"] = reader.linear(g + "out_proj", cfg.quant)
             conv = reader.get(g + "conv1d.weight").float()
             out[q + "conv"] = conv.reshape(conv.shape[0], -1)
             out[q + "dt_bias"] = reader.get(g + "dt_bias").float()
             out[q + "a_log"] = reader.get(g + "A_log").float()
             out[q + "gdn_norm"] = reader.get(g + "norm.weight").float()
         m = L + "mlp."
-        out[q + "gate_up"] = _interleave_rows(lin(m + "gate_proj"), lin(m + "up_proj"))
-        out[q + "down"] = lin(m + "down_proj")
+        fuse(q + "gate_up", _interleave_rows, m + "gate_proj", m + "up_proj")
+        out[q + "down"] = reader.linear(m + "down_proj", cfg.quant)
     return out
 
 
@@ -326,7 +339,8 @@ def load_checkpoint(cfg: ModelConfig, path: str, *, device="cpu", tp_rank: int =
     reader = _Reader(path)
     if reader.has("embed"):
         return _load_own(cfg, reader, device, tp_rank, tp, keep_master)
-    master = assemble_master(cfg, reader)
+    masters = {} if keep_master else None
+    master = assemble_master(cfg, reader, masters)
     from .models.hybrid import param_shapes
     shapes = param_shapes(cfg, 1)
     for k, shp in shapes.items():
@@ -336,7 +350,7 @@ def load_checkpoint(cfg: ModelConfig, path: str, *, device="cpu", tp_rank: int =
             raise CheckpointError(f"{k}: checkpoint shape {tuple(master[k].shape)} != expected {tuple(shp)}")
     act = torch.bfloat16 if torch.device(device).type == "cuda" else torch.float32
     return HybridModel.from_master(cfg, master, tp_rank=tp_rank, tp=tp, device=device,
-                                   keep_master=keep_master, act_dtype=act)
+                                   keep_master=keep_master, act_dtype=act, masters=masters)
 
 
 def _load_own(cfg, reader: _Reader, device, tp_rank, tp, keep_master) -> HybridModel:

@@ -130,8 +130,9 @@ class HybridModel:
     @classmethod
     def from_master(cls, cfg: ModelConfig, master: Dict[str, torch.Tensor], *, tp_rank=0, tp=1,
                     device=None, keep_master: bool = False, quant: Optional[str] = None,
-                    act_dtype=torch.bfloat16) -> "HybridModel":
-        """Shard (TP) and quantise a full master dict into serving parameters."""
+                    act_dtype=torch.bfloat16, masters: Optional[Dict[str, torch.Tensor]] = None) -> "HybridModel":
+        """Shard (TP) and quantise a full master dict into serving parameters.  ``masters``: dense values of projections that ``master`` has
+        as integers, for ``keep_master``, where they are not what the integers stand for."""
         from ..parallel.mesh import shard_param
         quant = quant or cfg.quant
         params: Dict[str, object] = {}
@@ -143,7 +144,9 @@ class HybridModel:
             if isinstance(ws, INT8Tensor):            # (a checkpoint's own integers)
                 params[name] = ws
                 if keep_master:
-                    params["master." + name] = ws.dequant()
+                    dense = (masters or {}).get(name)
+                    dense = ws.dequant() if dense is None else shard_param(cfg, name, dense, tp_rank, tp)
+                    params["master." + name] = dense if device is None else dense.to(device)
             elif name in lin or (name == "lm_head" and cfg.lm_head_quant == "nvfp4"):
                 if quant in ("nvfp4", "int8") or name == "lm_head":
                     # quantise the FULL tensor, then cut the packed planes: every TP degree
