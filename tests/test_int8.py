@@ -383,3 +383,40 @@ def test_parts_of_a_fused_projection_that_are_not_integers_leave_the_others_alon
         want = shard_param(cfg, name, m.params[name], 1, 2)
         assert torch.equal(half.params[name].w8, want.w8) and torch.equal(half.params[name].wscale, want.wscale)
         assert torch.equal(half.params["master." + name], shard_param(cfg, name, m.params["master." + name], 1, 2))
+
+
+FORMATS = {"nvfp4": F.NVFP4Tensor, "fp8": F.FP8BlockTensor, "int8": F.INT8Tensor, "bf16": torch.Tensor}
+
+
+@pytest.mark.parametrize("stored", ["nvfp4", "int8", "fp8", "bf16"])
+def test_a_model_serves_the_format_that_its_configuration_names(tmp_path, stored):
+    """Whatever the own dialect's file holds; bit for bit where it is the same."""
+    from tilerl_b200.checkpoint import load_checkpoint, save_checkpoint
+    from tilerl_b200.parallel.mesh import shard_param
+    cfg = dataclasses.replace(get_config("tiny-hybrid"), quant=stored, lm_head_quant="nvfp4", tie_embeddings=False)
+    m = HybridModel.build_random(cfg)
+    save_checkpoint(m, str(tmp_path))
+    dense = {n: m.params[n] if isinstance(m.params[n], torch.Tensor) else m.params[n].dequant() for n in linear_names(cfg)}
+    if stored == "fp8":                              # (written in bf16)
+        dense = {n: w.bfloat16().float() for n, w in dense.items()}
+    for quant, kind in FORMATS.items():
+        served = dataclasses.replace(cfg, quant=quant)
+        for rank, tp in ((0, 1), (1, 2)):
+            if quant == "fp8" and tp > 1:
+                continue
+            again = load_checkpoint(served, str(tmp_path), tp_rank=rank, tp=tp)
+            assert isinstance(again.params["lm_head"], F.NVFP4Tensor)
+            for n in linear_names(cfg):
+                got = again.params[n]
+                assert type(got) is kind, (quant, n)
+                if quant == stored and stored != "fp8":
+                    want = shard_param(cfg, n, m.params[n], rank, tp)
+                elif quant == "fp8":
+                    want = F.quantize_fp8_block(dense[n])
+                elif stored in ("fp8", "bf16") and tp > 1:
+                    continue                         # (dense values of this dialect are cut before they are quantised)
+                else:
+                    want = shard_param(cfg, n, {"nvfp4": F.quantize_nvfp4, "int8": F.quantize_int8, "bf16": lambda w: w}[quant](dense[n]), rank, tp)
+                for field in {"nvfp4": ("wq", "tscale"), "fp8": ("w8", "wscale"), "int8": ("w8", "wscale"), "bf16": ("data",)}[quant]:
+                    a, b = getattr(got, field), getattr(want, field)
+                    assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b), (quant, n, field)

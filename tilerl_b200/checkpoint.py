@@ -354,7 +354,8 @@ def load_checkpoint(cfg: ModelConfig, path: str, *, device="cpu", tp_rank: int =
 
 
 def _load_own(cfg, reader: _Reader, device, tp_rank, tp, keep_master) -> HybridModel:
-    """Own dialect: NVFP4 planes and 8-bit integers are adopted bit for bit (no requantisation)."""
+    """Own dialect: NVFP4 planes and 8-bit integers are adopted bit for bit (no requantisation) by a model that serves its projections in that format;
+    one that serves them in another has them decoded and quantised to its own."""
     from .parallel.mesh import shard_param
     params: Dict[str, object] = {}
     lin = set(linear_names(cfg))
@@ -362,7 +363,13 @@ def _load_own(cfg, reader: _Reader, device, tp_rank, tp, keep_master) -> HybridM
     act = torch.bfloat16 if torch.device(device).type == "cuda" else torch.float32
     for name in sorted(names):
         q = reader.nvfp4(name) or reader.int8(name)
-        if q is not None:
+        if q is not None and name in lin and cfg.quant != ("nvfp4" if isinstance(q, NVFP4Tensor) else "int8"):
+            q = q.dequant()
+            if cfg.quant in ("nvfp4", "int8"):       # (of the whole tensor, as from_master does it)
+                q = quantize_weight(q, cfg.quant)
+            q = shard_param(cfg, name, q, tp_rank, tp)
+            v = (quantize_weight(q, cfg.quant) if isinstance(q, torch.Tensor) else q).to(device)
+        elif q is not None:
             v = shard_param(cfg, name, q, tp_rank, tp).to(device)
         else:
             t = reader.get(name)
