@@ -420,3 +420,18 @@ def test_a_model_serves_the_format_that_its_configuration_names(tmp_path, stored
                 for field in {"nvfp4": ("wq", "tscale"), "fp8": ("w8", "wscale"), "int8": ("w8", "wscale"), "bf16": ("data",)}[quant]:
                     a, b = getattr(got, field), getattr(want, field)
                     assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b), (quant, n, field)
+
+
+@pytest.mark.parametrize("quant", ["nvfp4", "fp8", "int8", "bf16"])
+@pytest.mark.parametrize("name", ["tiny-hybrid", "small-gpu"])
+def test_a_saved_models_directory_names_its_format(tmp_path, name, quant):
+    from tilerl_b200.checkpoint import save_checkpoint
+    cfg = get_config(name, quant)
+    save_checkpoint(HybridModel(cfg, {"final_norm": torch.ones(cfg.hidden)}), str(tmp_path))
+    assert get_config(str(tmp_path)) == cfg and get_config(str(tmp_path), "fp8").quant == "fp8"
+    with open(tmp_path / "config.json") as f:
+        j = json.load(f)
+    j["quant"] = "of another day"
+    with open(tmp_path / "config.json", "w") as f:
+        json.dump(j, f)
+    assert get_config(str(tmp_path)) == get_config(name)

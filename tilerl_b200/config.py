@@ -881,7 +881,7 @@ _REGISTRY = {
 
 def config_from_dir(path: str):
     """The configuration a checkpoint directory describes in its ``config.json``: by ``architecture`` for designs
-    whose file spells every size out, else by the registry name that ``save_checkpoint`` wrote."""
+    whose file spells every size out, else by the registry name and the format of the projections that ``save_checkpoint`` wrote."""
     with open(os.path.join(path, "config.json")) as f:
         j = json.load(f)
     arch = j.get("architecture")
@@ -889,7 +889,7 @@ def config_from_dir(path: str):
         return ARCHITECTURES[arch].from_dir(j, path, os.path.basename(os.path.normpath(path)))
     if j.get("name") in _REGISTRY:
         cfg = _REGISTRY[j["name"]]()
-        return replace(cfg, quant="int8") if j.get("quant") == "int8" and isinstance(cfg, ModelConfig) else cfg
+        return replace(cfg, quant=j["quant"]) if j.get("quant") in QUANTS and isinstance(cfg, ModelConfig) else cfg
     raise ValueError(f"{path}/config.json names neither a known architecture ({sorted(ARCHITECTURES)}) nor a known model")
 
 
