@@ -435,3 +435,17 @@ def test_a_saved_models_directory_names_its_format(tmp_path, name, quant):
     with open(tmp_path / "config.json", "w") as f:
         json.dump(j, f)
     assert get_config(str(tmp_path)) == get_config(name)
+
+
+def test_shards_of_dense_files_hold_the_integers_of_the_whole(tmp_path):
+    """Rows cut along K before they are quantised would have a scale for each part."""
+    from tilerl_b200.checkpoint import load_checkpoint, save_checkpoint
+    from tilerl_b200.parallel.mesh import shard_param
+    cfg = get_config("tiny-hybrid", "bf16")
+    m = HybridModel.build_random(cfg)
+    save_checkpoint(m, str(tmp_path))
+    for rank in range(2):
+        half = load_checkpoint(dataclasses.replace(cfg, quant="int8"), str(tmp_path), tp_rank=rank, tp=2)
+        for n in linear_names(cfg):
+            want = shard_param(cfg, n, F.quantize_int8(m.params[n]), rank, 2)
+            assert torch.equal(half.params[n].w8, want.w8) and torch.equal(half.params[n].wscale, want.wscale), n

@@ -373,8 +373,11 @@ def _load_own(cfg, reader: _Reader, device, tp_rank, tp, keep_master) -> HybridM
             v = shard_param(cfg, name, q, tp_rank, tp).to(device)
         else:
             t = reader.get(name)
-            t = shard_param(cfg, name, t, tp_rank, tp)
-            if name in lin:
+            whole = name in lin and cfg.quant == "int8"        # (a channel's scale is that of its whole row)
+            t = shard_param(cfg, name, quantize_weight(t.float(), "int8") if whole else t, tp_rank, tp)
+            if whole:
+                v = t.to(device)
+            elif name in lin:
                 v = quantize_weight(t.float(), cfg.quant)
                 v = v.to(device) if hasattr(v, "to") else v
             elif name in ("embed", "lm_head"):
