@@ -449,3 +449,51 @@ def test_shards_of_dense_files_hold_the_integers_of_the_whole(tmp_path):
         for n in linear_names(cfg):
             want = shard_param(cfg, n, F.quantize_int8(m.params[n]), rank, 2)
             assert torch.equal(half.params[n].w8, want.w8) and torch.equal(half.params[n].wscale, want.wscale), n
+
+
+def _adopted(cfg, **kw):
+    """A model whose integers came from a file: no row reaches 127."""
+    g = torch.Generator().manual_seed(2)
+    master = random_master(cfg, 3)
+    for n in linear_names(cfg):
+        shape = master[n].shape
+        master[n] = F.INT8Tensor(torch.randint(-100, 100, shape, generator=g, dtype=torch.int8), torch.rand(shape[0], generator=g) * 1e-3 + 1e-5)
+    return HybridModel.from_master(cfg, master, act_dtype=torch.float32, **kw)
+
+
+def test_integers_that_training_left_alone_are_not_rounded_anew():
+    cfg = _tiny("tiny-hybrid")
+    m, before = _adopted(cfg, keep_master=True), _adopted(cfg).params
+    m.requantize_()
+    for n in linear_names(cfg):
+        assert torch.equal(m.params[n].w8, before[n].w8) and torch.equal(m.params[n].wscale, before[n].wscale)
+    moved = m.params["master.L0.down"]
+    moved[3, 5] += 1.0
+    m.requantize_()
+    got, want, was = m.params["L0.down"], F.quantize_int8(moved), before["L0.down"]
+    others = [i for i in range(len(moved)) if i != 3]
+    assert torch.equal(got.w8[others], was.w8[others]) and torch.equal(got.wscale[others], was.wscale[others])
+    assert torch.equal(got.w8[3], want.w8[3]) and got.wscale[3] == want.wscale[3]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tp", [1, 2])
+def test_resync_of_weights_that_did_not_move_keeps_their_integers(tp, dtype):
+    import types
+    from tilerl_b200.parallel.resync import resync
+    cfg = _tiny("tiny-hybrid")
+    trainer = _adopted(cfg, keep_master=True)
+    weights = {n: w.to(dtype) for n, w in trainer.params.items() if n.startswith("master.")}
+    zero = types.SimpleNamespace(units=[0], unit_tensors=lambda i: weights, _prefetch=None, _drop=lambda u: None, device=torch.device("cpu"))
+    for rank in range(tp):
+        rollout, before = (_adopted(cfg, tp_rank=rank, tp=tp) for _ in range(2))
+        resync(zero, rollout)
+        for n in linear_names(cfg):
+            a, b = rollout.params[n], before.params[n]
+            assert torch.equal(a.w8, b.w8) and torch.equal(a.wscale, b.wscale), n
+    weights["master.L0.o" if "master.L0.o" in weights else "master.L0.out"].mul_(2)
+    name = "L0.o" if "master.L0.o" in weights else "L0.out"
+    resync(zero, rollout)
+    from tilerl_b200.parallel.mesh import shard_param
+    want = shard_param(cfg, name, F.quantize_int8(weights["master." + name].float()), rank, tp)
+    assert torch.equal(rollout.params[name].w8, want.w8) and torch.equal(rollout.params[name].wscale, want.wscale)

@@ -262,6 +262,13 @@ def quantize_int8(w: torch.Tensor) -> INT8Tensor:
     return INT8Tensor(q.to(torch.int8), s.contiguous())
 
 
+def keep_int8(new: INT8Tensor, cur: INT8Tensor, w: torch.Tensor) -> INT8Tensor:
+    """``new``, the integers of ``w``, but for rows of ``w`` that are what ``cur`` stands for already (in ``w``'s type), which keep those: a file's own
+    integers, whose rows need not reach 127, are not rounded anew unless training moved them."""
+    same = (cur.dequant().to(w.dtype) == w).all(-1)
+    return INT8Tensor(torch.where(same[:, None], cur.w8, new.w8), torch.where(same, cur.wscale, new.wscale))
+
+
 def dequantize_int8(t: INT8Tensor) -> torch.Tensor:
     return t.w8.float() * t.wscale[:, None]
 

@@ -33,7 +33,7 @@ from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 import torch
 
 from ..config import ATTN, GDN, ModelConfig
-from ..formats import (FP8BlockTensor, INT8Tensor, NVFP4Tensor, quantize_fp8_block, quantize_int8, quantize_nvfp4)
+from ..formats import (FP8BlockTensor, INT8Tensor, NVFP4Tensor, keep_int8, quantize_fp8_block, quantize_int8, quantize_nvfp4)
 
 LINEAR_KEYS_ATTN = ("qkv", "o")
 LINEAR_KEYS_GDN = ("in", "out")
@@ -261,13 +261,16 @@ class HybridModel:
     # ---- weight maintenance -------------------------------------------------------------------
     def requantize_(self) -> None:
         """Re-pack every projection from its master copy *in place* (device
-        addresses stay fixed so captured CUDA graphs keep working)."""
+        addresses stay fixed so captured CUDA graphs keep working).  8-bit integers: rows that
+        training left alone keep theirs."""
         for n in linear_names(self.cfg):
             m = self.params.get("master." + n)
             if m is None:
                 continue
             cur = self.params[n]
             new = quantize_weight(m.float(), "int8" if isinstance(cur, INT8Tensor) else self.cfg.quant)
+            if isinstance(cur, INT8Tensor):
+                new = keep_int8(new, cur, m)
             if isinstance(cur, NVFP4Tensor):
                 cur.wq.copy_(new.wq), cur.scale.copy_(new.scale), cur.tscale.copy_(new.tscale)
             elif isinstance(cur, (FP8BlockTensor, INT8Tensor)):

@@ -21,7 +21,7 @@ from typing import Callable, Dict, Optional
 
 import torch
 
-from ..formats import INT8Tensor, NVFP4Tensor, quantize_int8, quantize_nvfp4
+from ..formats import INT8Tensor, NVFP4Tensor, keep_int8, quantize_int8, quantize_nvfp4
 from ..models.hybrid import linear_names
 from .mesh import shard_param
 
@@ -45,7 +45,7 @@ def resync(zero, rollout, *, quantize: Optional[Callable] = None, refresh: Optio
     """Write the trainer's current weights into ``rollout`` (a served ``HybridModel`` of TP
     degree ``rollout.tp``).  ``quantize(w_full) -> NVFP4Tensor`` defaults to the torch
     quantiser (a CUDA backend passes its kernel); weights served in 8-bit integers take theirs from
-    ``formats.quantize_int8``; ``refresh(param)`` is called for every
+    ``formats.quantize_int8``, but for rows that have not moved; ``refresh(param)`` is called for every
     rewritten quantised tensor (the CUDA backend re-tiles its GEMM copies there)."""
     cfg = rollout.cfg
     quantize = quantize or (lambda w: quantize_nvfp4(w.float()))
@@ -69,7 +69,8 @@ def resync(zero, rollout, *, quantize: Optional[Callable] = None, refresh: Optio
                     if refresh is not None:
                         refresh(dst)
                 elif base in lin and isinstance(dst, INT8Tensor):
-                    nbytes += _store(dst, shard_param(cfg, base, quantize_int8(w.float()), rollout.tp_rank, rollout.tp))
+                    new, part = (shard_param(cfg, base, t, rollout.tp_rank, rollout.tp) for t in (quantize_int8(w.float()), w))
+                    nbytes += _store(dst, keep_int8(new, dst, part))
                 else:
                     src = shard_param(cfg, base, w, rollout.tp_rank, rollout.tp)
                     nbytes += _store(dst, src)
