@@ -497,3 +497,10 @@ def test_resync_of_weights_that_did_not_move_keeps_their_integers(tp, dtype):
     from tilerl_b200.parallel.mesh import shard_param
     want = shard_param(cfg, name, F.quantize_int8(weights["master." + name].float()), rank, tp)
     assert torch.equal(rollout.params[name].w8, want.w8) and torch.equal(rollout.params[name].wscale, want.wscale)
+
+
+def test_a_weight_that_the_kernels_do_not_read_is_named_as_the_cause():
+    from tilerl_b200.ops import gemm_int8
+    w = F.quantize_int8(_rows(37, 40))
+    with pytest.raises(ValueError, match=r"quantize_ takes weights .*multiple of 16 values.*\(37, 40\)"):
+        gemm_int8.quantize_(torch.zeros(37, 40), w)

@@ -62,8 +62,8 @@ def takes(w: INT8Tensor) -> bool:
     return _ready(w) is not None
 
 
-def _refuse_weight(w: INT8Tensor) -> None:
-    raise ValueError(f"INT8 products take weights with rows of a multiple of 16 values on 16-byte boundaries, of up to {MOST}, on "
+def _refuse_weight(w: INT8Tensor, who: str = "INT8 products take") -> None:
+    raise ValueError(f"{who} weights with rows of a multiple of 16 values on 16-byte boundaries, of up to {MOST}, on "
                      f"a GPU with their scales, got {w.shape} with strides {tuple(w.w8.stride())} on {w.w8.device}")
 
 
@@ -241,7 +241,9 @@ def _gradient(rows, r: _Ready, dx, scratch) -> None:
 # ---- weights ---------------------------------------------------------------------------------------------------
 def quantize_(src: torch.Tensor, dst: INT8Tensor) -> None:
     """fp32 or bf16 ``[N, K]`` into ``dst`` in place, as ``formats.quantize_int8`` gives it."""
-    if _ready(dst) is None or src.shape != dst.w8.shape or src.dtype not in TYPES or src.device != dst.w8.device:
+    if not takes(dst):
+        _refuse_weight(dst, "quantize_ takes")
+    if src.shape != dst.w8.shape or src.dtype not in TYPES or src.device != dst.w8.device:
         raise ValueError(f"quantize_ takes fp32 or bf16 of {dst.shape} on the weight's device, got {tuple(src.shape)} {src.dtype} on {src.device}")
     src = src if src.stride(1) == 1 else src.contiguous()
     with N.on(src.device):
