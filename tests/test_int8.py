@@ -504,3 +504,15 @@ def test_a_weight_that_the_kernels_do_not_read_is_named_as_the_cause():
     w = F.quantize_int8(_rows(37, 40))
     with pytest.raises(ValueError, match=r"quantize_ takes weights .*multiple of 16 values.*\(37, 40\)"):
         gemm_int8.quantize_(torch.zeros(37, 40), w)
+
+
+def test_records_of_a_bench_name_a_format_that_is_not_the_models_own(tmp_path, monkeypatch, capsys):
+    """Or the gate would measure one format against the other's best."""
+    from tilerl_b200 import benchrec
+    from tilerl_b200.cli import main
+    monkeypatch.setenv("TRL_BENCH_STORE", str(tmp_path / "m.jsonl"))
+    run = ["bench", "--model", "tiny", "--device", "cpu", "--prompt-len", "8", "--gen", "3", "--record"]
+    for more in ([], ["--quant", "int8"], ["--quant", "bf16"]):
+        assert main(run + more) == 0
+    own, other, again = [r["shape"] for r in benchrec.load(str(tmp_path / "m.jsonl"))]
+    assert "quant" not in own and other == dict(own, quant="int8") and again == own

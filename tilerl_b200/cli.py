@@ -684,6 +684,8 @@ def cmd_bench(args) -> int:
     dev = _device(args)
     ops = make_ops(dev)
     model = build_model(cfg, dev, seed=args.seed, checkpoint=_checkpoint(args), ops=ops if dev != "cpu" else None)
+    # (another format of the projections than the name's own: not measured against those records)
+    served = {"quant": cfg.quant} if hasattr(cfg, "quant") and cfg.quant != get_config(cfg.name).quant else {}
     out = []
     for b in [int(x) for x in args.batches.split(",")]:
         eng = build_engine(model, ops, device=dev, slots=b + 1, max_ctx=args.prompt_len + args.gen + 32, prefix=False)
@@ -701,7 +703,7 @@ def cmd_bench(args) -> int:
         if args.record:
             from . import benchrec
             benchrec.append(benchrec.make_record("decode_tok_s", rec["decode_tok_s"],
-                                                 dict(model=cfg.name, batch=b, ctx=args.prompt_len, tp=args.tp)))
+                                                 dict(model=cfg.name, batch=b, ctx=args.prompt_len, tp=args.tp, **served)))
     print(json.dumps(out))
     return 0
 
