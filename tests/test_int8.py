@@ -516,3 +516,35 @@ def test_records_of_a_bench_name_a_format_that_is_not_the_models_own(tmp_path, m
         assert main(run + more) == 0
     own, other, again = [r["shape"] for r in benchrec.load(str(tmp_path / "m.jsonl"))]
     assert "quant" not in own and other == dict(own, quant="int8") and again == own
+
+
+@pytest.mark.parametrize("dialect", ["own", "export"])
+def test_merges_go_by_what_the_integers_stand_for(tmp_path, dialect):
+    from safetensors.torch import load_file, save_file
+    from tilerl_b200.merge import merge_checkpoints
+    w8, ws = ("p.w8", "p.wscale") if dialect == "own" else ("p.weight", "p.weight_scale")
+    dense = [_rows(6, 32, i) for i in range(3)]
+    dense[1][2], dense[2][2] = dense[0][2], dense[0][2]       # (a row that nobody moved)
+    files = []
+    for i, w in enumerate(dense):
+        q = F.quantize_int8(w)
+        q.w8[2], q.wscale[2] = torch.arange(32) - 9, 0.25      # (and that does not reach 127)
+        (tmp_path / str(i)).mkdir()
+        save_file({w8: q.w8, ws: q.wscale if dialect == "own" else q.wscale[:, None].contiguous(), "norm": torch.full((4,), float(i))},
+                  str(tmp_path / str(i) / "model.safetensors"))
+        files.append(q)
+    merge_checkpoints(str(tmp_path / "0"), [str(tmp_path / "1"), str(tmp_path / "2")], str(tmp_path / "out"))
+    got = load_file(str(tmp_path / "out" / "model.safetensors"))
+    q = F.INT8Tensor(got[w8], got[ws])
+    want = (files[1].dequant().double() + files[2].dequant().double()) / 2
+    # half a step of the merged row, and fp32 sums of three terms
+    step = want.abs().amax(-1, keepdim=True) / 127
+    size = sum(f.dequant().double().abs() for f in files).amax(-1, keepdim=True)
+    assert ((q.dequant().double() - want).abs() <= step * (0.5 + 127 * 6 * 2.0 ** -24) + size * 8 * 2.0 ** -24).all()
+    assert torch.equal(q.w8[2], files[0].w8[2]) and q.wscale[2] == 0.25
+    assert torch.equal(got["norm"], torch.full((4,), 1.5))
+    (tmp_path / "other").mkdir()
+    save_file({"norm": torch.zeros(4)}, str(tmp_path / "other" / "model.safetensors"))
+    merge_checkpoints(str(tmp_path / "0"), [str(tmp_path / "other")], str(tmp_path / "out"))
+    got = load_file(str(tmp_path / "out" / "model.safetensors"))
+    assert torch.equal(got[w8], files[0].w8) and torch.equal(got[ws].reshape(-1), files[0].wscale)

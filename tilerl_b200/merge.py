@@ -5,10 +5,13 @@ Parity: reference ``src/tilerl/merge.py`` (iso / ties / dare / average).
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import Dict, List, Optional, Sequence
 
 import torch
+
+from .formats import INT8Tensor, keep_int8, quantize_int8
 
 
 def merge_average(deltas: Sequence[torch.Tensor], weights: Optional[Sequence[float]] = None) -> torch.Tensor:
@@ -53,16 +56,48 @@ def merge_iso(deltas: Sequence[torch.Tensor]) -> torch.Tensor:
 METHODS = {"average": merge_average, "ties": merge_ties, "dare": merge_dare, "iso": merge_iso}
 
 
+def _integers(f) -> Dict[str, str]:
+    """Projections in 8-bit integers of a file (own dialect, exports) and the names of their scales."""
+    names, out = set(f.keys()), {}
+    for name in names:
+        for tail, of in ((".w8", ".wscale"), (".weight", ".weight_scale")):
+            scale = name[:-len(tail)] + of
+            if name.endswith(tail) and scale in names:
+                w, n = f.get_slice(name), math.prod(f.get_slice(scale).get_shape())
+                if w.get_dtype() == "I8" and len(w.get_shape()) == 2 and n in (1, w.get_shape()[0]):
+                    out[name] = scale
+    return out
+
+
+def _int8(f, name: str, scale: str) -> INT8Tensor:
+    w = f.get_tensor(name)
+    return INT8Tensor(w, f.get_tensor(scale).float().reshape(-1).expand(w.shape[0]).contiguous())
+
+
 def merge_checkpoints(base: str, tuned: List[str], out: str, method: str = "average", **kw) -> int:
-    """Stream safetensors files: ``out = base + merge(tuned_i - base)`` per tensor."""
+    """Stream safetensors files: ``out = base + merge(tuned_i - base)`` per tensor; projections in 8-bit integers by what they stand for."""
     from safetensors import safe_open
     from safetensors.torch import save_file
     fn = METHODS[method]
     f_base = safe_open(os.path.join(base, "model.safetensors"), framework="pt")
     f_tuned = [safe_open(os.path.join(t, "model.safetensors"), framework="pt") for t in tuned]
     result: Dict[str, torch.Tensor] = {}
+    integers = _integers(f_base)
+    scales = set(integers.values())
     for name in f_base.keys():
+        if name in scales:
+            continue
         b = f_base.get_tensor(name)
+        if name in integers:              # neither the integers nor the scales have deltas of their own
+            scale = integers[name]
+            result[name], result[scale] = b, f_base.get_tensor(scale)
+            if all(name in f.keys() and scale in f.keys() for f in f_tuned):
+                base_q = _int8(f_base, name, scale)
+                dense = base_q.dequant()
+                merged = dense + fn([_int8(f, name, scale).dequant() - dense for f in f_tuned], **kw)
+                q = keep_int8(quantize_int8(merged), base_q, merged)
+                result[name], result[scale] = q.w8, q.wscale
+            continue
         if not b.dtype.is_floating_point or b.dtype == torch.float8_e4m3fn or any(name not in f.keys() for f in f_tuned):
             result[name] = b
             continue
