@@ -583,7 +583,8 @@ TRL_API int trl_linear_i8(const void* x, int type, long ldx, const void* norm_w,
       (epi == I8_RESIDUAL) != (residual != nullptr) || !gi_operands(w, ldw, K, scratch, K))
     return (int)cudaErrorInvalidValue;
   // (in one launch every block reads all of x, while others write results already: not into the same memory)
-  const char *x0 = (const char*)x, *y0 = (const char*)out, *x1 = x0 + 2 * ((long long)(T - 1) * ldx + K), *y1 = y0 + 4 * ((long long)(T - 1) * ldo + N);
+  const int width = epi == I8_SWIGLU ? N / 2 : N, size = epi == I8_STORE_F32 ? 4 : 2;
+  const char *x0 = (const char*)x, *y0 = (const char*)out, *x1 = x0 + 2 * ((long long)(T - 1) * ldx + K), *y1 = y0 + size * ((long long)(T - 1) * ldo + width);
   const bool whole = (x1 <= y0 || y1 <= x0) && type == 1 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx % 8 == 0) && reinterpret_cast<uintptr_t>(norm_w) % 16 == 0;
   if (whole && gemv_i8_takes(T, N, K)) {
     const int rc = gemv_i8_launch(w, ldw, ws, x, ldx, norm_w, eps, residual, ldr, out, ldo, T, N, K, epi, (cudaStream_t)stream);

@@ -235,6 +235,25 @@ def test_rows_that_are_the_residual_themselves(ops, t):
     assert torch.equal(both[1:], want)
 
 
+@pytest.mark.parametrize("t", [1, 3])
+def test_rows_right_behind_the_output_go_in_one_launch(ops, t):
+    """As small buffers of one allocator lie; a value further on they are the output's memory, and go in two."""
+    from tilerl_b200.ops import gemm_int8, native
+    n, k = 320, 256
+    w, solid = _weight(n, k), _x(t, k)
+    for epi, dtype, width in ((gemm_int8.EPI_STORE, torch.bfloat16, n), (gemm_int8.EPI_SWIGLU, torch.bfloat16, n // 2), (gemm_int8.EPI_STORE_F32, torch.float32, n)):
+        want = torch.empty(t, width, device=DEV, dtype=dtype)
+        gemm_int8.linear(ops, solid, w, want, epi=epi)
+        size = want.element_size() * t * width
+        for at, launches in ((size, 1), (size - 16, 2)):
+            memory = torch.zeros(size + 2 * t * k, dtype=torch.int8, device=DEV)
+            y, x = memory[:size].view(dtype).view(t, width), memory[at:at + 2 * t * k].view(torch.bfloat16).view(t, k)
+            x.copy_(solid)
+            before = native.launch_count
+            gemm_int8.linear(ops, x, w, y, epi=epi)
+            assert native.launch_count - before == launches and torch.equal(y, want)
+
+
 def test_first_use_inside_a_capture():
     """Kernels that this process has not launched yet.  (The backend's buffers have their size already: it refuses to grow them in a capture.)"""
     import os
