@@ -548,3 +548,18 @@ def test_merges_go_by_what_the_integers_stand_for(tmp_path, dialect):
     merge_checkpoints(str(tmp_path / "0"), [str(tmp_path / "other")], str(tmp_path / "out"))
     got = load_file(str(tmp_path / "out" / "model.safetensors"))
     assert torch.equal(got[w8], files[0].w8) and torch.equal(got[ws].reshape(-1), files[0].wscale)
+
+
+@pytest.mark.parametrize("command", [["serve"], ["bench"], ["train", "--rl", "--reward", "mod7"]])
+def test_dense_projections_are_refused_by_name_on_a_gpu(command, monkeypatch):
+    """Before anything is built: no kernel of the GPU backend serves them."""
+    from tilerl_b200 import cli, factory
+
+    def reached(*a, **k):
+        raise AssertionError("refused too late")
+    for name in ("make_ops", "build_model", "build_engine"):
+        monkeypatch.setattr(factory, name, reached)
+    with pytest.raises(SystemExit, match="--quant bf16"):
+        cli.main(command + ["--model", "small-gpu", "--quant", "bf16", "--device", "cuda"])
+    with pytest.raises(AssertionError, match="too late"):
+        cli.main(command + ["--model", "small-gpu", "--quant", "int8", "--device", "cpu"])

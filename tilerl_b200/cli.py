@@ -23,7 +23,7 @@ def _add_model_flags(p: argparse.ArgumentParser) -> None:
 def _add_quant_flag(p: argparse.ArgumentParser) -> None:
     p.add_argument("--quant", default=None, choices=["nvfp4", "fp8", "int8", "bf16"],
                    help="format of the projections instead of the configuration's own; int8: 8-bit integers with a scale per channel, "
-                        "activations quantised per token")
+                        "activations quantised per token; bf16: on the CPU")
 
 
 def build_parser() -> argparse.ArgumentParser:
@@ -227,6 +227,11 @@ def _device(args) -> str:
     return "cuda" if torch.cuda.is_available() else "cpu"
 
 
+def _refuse_bf16(args, dev: str) -> None:
+    if args.quant == "bf16" and dev.startswith("cuda"):
+        raise SystemExit("--quant bf16: dense projections are served by the reference backend (--device cpu); on a GPU serve nvfp4, fp8 or int8")
+
+
 def _checkpoint(args) -> Optional[str]:
     """``--checkpoint``, or the directory given as ``--model``."""
     return args.checkpoint or (args.model if os.path.isdir(args.model) else None)
@@ -270,6 +275,7 @@ def cmd_serve(args) -> int:
     from .server.app import create_app
     from .tokenizer import load_tokenizer
     dev = _device(args)
+    _refuse_bf16(args, dev)
     if dev != "cpu" and not args.no_card_guard:
         try:
             from .parallel.health import card_guard
@@ -397,6 +403,8 @@ def cmd_train(args) -> int:
             print(f"{k:{width}s} {v / memory.GIB:10.2f} GiB")
         print(f"{'total':{width}s} {sum(rows.values()) / memory.GIB:10.2f} GiB")
         return 0
+    if flags.get("rl") or flags.get("opd"):          # (rollouts are served)
+        _refuse_bf16(args, _device(args))
     if flags.get("indexer_warmup"):
         # the warm-up runs the dense model on the reference backend and trains only the indexer
         from .factory import build_model as _bm
@@ -682,6 +690,7 @@ def cmd_bench(args) -> int:
     from .engine import SamplingParams
     from .factory import build_engine, build_model, make_ops
     dev = _device(args)
+    _refuse_bf16(args, dev)
     ops = make_ops(dev)
     model = build_model(cfg, dev, seed=args.seed, checkpoint=_checkpoint(args), ops=ops if dev != "cpu" else None)
     # (another format of the projections than the name's own: not measured against those records)
