@@ -563,3 +563,15 @@ def test_dense_projections_are_refused_by_name_on_a_gpu(command, monkeypatch):
         cli.main(command + ["--model", "small-gpu", "--quant", "bf16", "--device", "cuda"])
     with pytest.raises(AssertionError, match="too late"):
         cli.main(command + ["--model", "small-gpu", "--quant", "int8", "--device", "cpu"])
+
+
+def test_a_training_run_in_another_format_is_another_run(tmp_path, capsys):
+    """The same command asked twice is handed the finished manifest; with --quant it is not the same."""
+    from tilerl_b200 import cli
+    run = ["train", "--recipe", "grpo-tiny-smoke", "--device", "cpu", "--steps", "1", "--max-tokens", "4", "--prompt-len", "6", "--runs", str(tmp_path)]
+    ids = []
+    for more in ([], ["--quant", "int8"], ["--quant", "int8"], []):
+        assert cli.main(run + more) == 0
+        lines = [json.loads(l) for l in capsys.readouterr().out.splitlines() if l.startswith("{")]
+        ids.append([l["run"] for l in lines if l.get("reused")])
+    assert ids[:2] == [[], []] and len(ids[2]) == len(ids[3]) == 1 and ids[2] != ids[3]

@@ -415,7 +415,7 @@ def cmd_train(args) -> int:
             from .sparse_index import corpus_run, load_spans
             held = load_spans(args.indexer_corpus, "held", args.held_spans)
             control = load_spans(args.indexer_control_corpus, "held", args.held_spans) if args.indexer_control_corpus else None
-            run = Run({"cmd": "train", **flags, "indexer_corpus": args.indexer_corpus, "k_pages": args.k_pages,
+            run = Run({"cmd": "train", **flags, **({"quant": args.quant} if args.quant else {}), "indexer_corpus": args.indexer_corpus, "k_pages": args.k_pages,
                        "q_samples": args.q_samples, "q_min_pos": args.q_min_pos, "di": args.indexer_di, "seed": args.seed,
                        "held_spans": args.held_spans, "control": args.indexer_control_corpus},
                       root=args.runs or runs_dir())
@@ -438,7 +438,7 @@ def cmd_train(args) -> int:
             return 0 if out["passed"] else 1
         g = torch.Generator().manual_seed(args.seed)
         seqs = [torch.randint(0, cfg.vocab, (flags.get("ctx") or 256,), generator=g) for _ in range(4)]
-        run = Run({"cmd": "train", **flags}, root=args.runs or runs_dir())
+        run = Run({"cmd": "train", **flags, **({"quant": args.quant} if args.quant else {})}, root=args.runs or runs_dir())
         hist = warmup(model, ix, seqs, steps=flags["steps"], lr=flags.get("lr") or 3e-3)
         for i, kl in enumerate(hist):
             run.log(step=i, kl=kl)
@@ -461,7 +461,7 @@ def cmd_train(args) -> int:
               "eval_curve_seed": args.eval_curve_seed}
     # (inputs that came later are named only where they are set, so that earlier runs keep their ids)
     inputs.update({k: getattr(args, k) for k, default in (("kl_reference", "none"), ("preference", False), ("beta", 0.1), ("label_smoothing", 0.0),
-                                                          ("checkpoint_layers", False), ("activation_bits", 32)) if getattr(args, k) != default})
+                                                          ("checkpoint_layers", False), ("activation_bits", 32), ("quant", None)) if getattr(args, k) != default})
     fb = {k: getattr(args, k) for k, default in (("checkpoint_layers", False), ("activation_bits", 32)) if getattr(args, k) != default}
     if args.load_adapter and not args.lineage:
         # a run that starts from a saved adapter descends from the run that wrote it (looked up through the
