@@ -575,3 +575,12 @@ def test_a_training_run_in_another_format_is_another_run(tmp_path, capsys):
         lines = [json.loads(l) for l in capsys.readouterr().out.splitlines() if l.startswith("{")]
         ids.append([l["run"] for l in lines if l.get("reused")])
     assert ids[:2] == [[], []] and len(ids[2]) == len(ids[3]) == 1 and ids[2] != ids[3]
+
+
+def test_a_store_of_pages_tells_weights_apart_by_their_scales():
+    """Twice as large a weight has the same integers."""
+    from tilerl_b200.kv_tiers import weights_fingerprint
+    cfg = _tiny("tiny-hybrid")
+    a, b, c = (HybridModel.build_random(cfg) for _ in range(3))
+    b.params["L0.down"].wscale.mul_(2)
+    assert weights_fingerprint(a) == weights_fingerprint(c) != weights_fingerprint(b)

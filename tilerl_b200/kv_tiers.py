@@ -25,6 +25,8 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .formats import INT8Tensor
+
 
 class SpillWriteError(IOError):
     pass
@@ -193,9 +195,11 @@ def weights_fingerprint(model) -> str:
         v = model.params[k]
         t = v.wq if hasattr(v, "wq") else (v.w8 if hasattr(v, "w8") else v)
         h.update(k.encode())
-        h.update(str(tuple(t.shape)).encode())
-        flat = t.reshape(-1)[:: max(1, t.numel() // 64)][:64]
-        h.update(flat.contiguous().view(torch.uint8).cpu().numpy().tobytes())
+        # (every row of 8-bit integers reaches 127, whatever the weight's size: its scales tell weights apart that its integers do not)
+        for t in (t, v.wscale) if isinstance(v, INT8Tensor) else (t,):
+            h.update(str(tuple(t.shape)).encode())
+            flat = t.reshape(-1)[:: max(1, t.numel() // 64)][:64]
+            h.update(flat.contiguous().view(torch.uint8).cpu().numpy().tobytes())
     return h.hexdigest()
 
 
