@@ -15,8 +15,9 @@
 //
 // What bounds it.  Many tokens: the tensor cores, at the clocks that the power cap leaves them (2000 x 16 480 x 5120: 116 us alone, tensor pipe 88 % of its
 // active cycles; a second of it 144 us, 2.3 POP/s; on another GPU 175).  An MMA of 128 x 256 x 32 takes 128 clocks, as fp8 does and bf16
-// with half of K.  Few: the read of W (eight rows of 34 816 x 5120: 35 us from an empty L2 cache, 5.1 TB/s; 32 us with the quantiser in a row of
-// products, whose first stages are on their way while the rows between them are quantised).  Measured and not taken: W on its way before TMEM
+// with half of K.  Few: the read of W (eight rows of 34 816 x 5120: 35 us from an empty L2 cache, 5.1 TB/s; 32.6 us with the quantiser in a row of
+// products, whose first stages are on their way while the rows between them are quantised; it lets them start behind its own wait, for weights
+// that were just written, which costs 0.5 to 1 us).  Measured and not taken: W on its way before TMEM
 // is taken (the quantiser's few loads then wait behind it: 32.8), half a SM a CTA, so that the next product moves in earlier (four
 // stages are too few: 35.6), the head of W fetched into L2 by the quantiser (33.0).
 //
@@ -335,7 +336,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         uint32_t r[32];
-        constexpr bool EARLY = BN <= 128;            // (wider tiles have more to do meanwhile)
+        constexpr bool EARLY = BN <= 128;            // (wider tiles read it where it is added: the other accumulator's MMAs hide the wait behind long sums; behind sums of a few stages nothing does)
         uint4 res[TOK / 8];
         if (!GRAD && !SPLIT && EARLY && p.epi == I8_RESIDUAL && p.vec) {
 #pragma unroll
@@ -536,7 +537,9 @@ int gi_launch(const void* w, long long ldw, const void* q, long long ldq, int wi
   }
 }
 
-constexpr int GI_MOST = 131072, GI_WIDEST = 1 << 24;      // values a sum: 127 * 128 times as many is below 2^31; channels
+// Values a sum: activations go up to 127 and weights to 128 in magnitude, and 127 * 128 times as many is below 2^31.  A gradient's low digits go down
+// to -128, but that of its row's largest value, which is at 127 * 256, is 0, and 128 * 128 times one less is below 2^31 too.
+constexpr int GI_MOST = 131072, GI_WIDEST = 1 << 24;      // (and channels)
 bool gi_operands(const void* w, long long ldw, int K, const void* q, long long ldq) {
   return reinterpret_cast<uintptr_t>(w) % 16 == 0 && ldw % 16 == 0 && ldw >= K && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0;
 }

@@ -7,7 +7,7 @@
 // along K, then down the rows.  Rows of W are the A operand of mma.m16n8k32, tokens B.  Sums go into shared memory by integer atomics: exact, so
 // their order changes nothing.
 //
-// Bound by latency: launch, the row's read, its maximum and its integers (two block barriers), sums, results (1 x 5120 x 1024: 5.1 us, of which the
+// Bound by latency: launch, the row's read, its maximum and its integers (two block barriers), sums, results (1 x 5120 x 1024: 4.9 us, of which the
 // 5 MB take 0.8).
 //
 // The reference's FP8 form for few rows is `linear_fp8_gemv` (packages/tilerl-kernels/src/tilerl_kernels/kernels_linear.py:1442-1494).
@@ -263,10 +263,10 @@ int gv_launch(const CUtensorMap& m32, const CUtensorMap& m8, const GemvI8Params&
 
 bool i8_tensor(CUtensorMap* m, const void* base, long long width, long long rows, long long ld, int box_rows);
 
-// Whether gemv_i8_launch takes T rows.  Weights up to 16 MB, of three or four rows 8: there a launch less counts more than that the pair form's next weights are on their way
-// while its rows are quantised, for which this form, whose rings fill the SMs, leaves no room (us here and in two launches, one row:
-// 320 x 256 3.8 and 5.1, 5120 x 1024 5.1 and 7.1, 5120 x 5120 11.4 and 10.9, 16480 x 5120 20.6 and 18.5; 5120 x 1024, four rows 6.9 and 6.8, and 2 less of
-// the host's time, eight 9.4 and 6.8; 16000 x 1024, three rows 9.3 and 8.0).
+// Whether gemv_i8_launch takes T rows.  Weights up to 16 MB, of three or four rows 8: there a launch less counts more than that the pair form's first weights are on their way
+// while its rows are quantised (us in a row of products here and in two launches, one row: 320 x 256 3.4 and 5.5, 5120 x 1024 4.9 and 7.2,
+// 4096 x 4096 8.3 and 10.7, 5120 x 5120 11.7 and 11.8, 16480 x 5120 19.5 and 19.4; two rows, 5120 x 5120 12.6 and 11.8; three, 5120 x 1600 7.1 and 8.2,
+// 16000 x 1024 9.7 and 9.3; four, 5120 x 1024 6.7 and 7.2, 16480 x 5120 22.1 and 19.2).
 bool gemv_i8_takes(int T, int N, int K) { return T <= GV_TOKENS && (long long)N * K <= (T > 2 ? 8 : 16) << 20 && K <= GV_MOST_K && gv_stages(T, N, K) > 0; }
 
 // x: bf16 rows, on 16-byte boundaries, quantised here (of rmsnorm(x) * norm_w where that is given).

@@ -5,7 +5,9 @@
 //
 // A norm's factor is the same for a whole row, so it cancels out of the integers and goes into the scale alone.  One pass: a block takes
 // row after row, which stays in registers between its maximum and its integers.  Bound by instructions for many rows (2000 x 5120 bf16: 13 us, 64 % of
-// the issue slots, 31 MB; packed fp32 arithmetic takes 8 % of them away and no time), by latency for few (2.5 us).
+// the issue slots, 31 MB; packed fp32 arithmetic takes 8 % of them away and no time), by latency for few (2.5 us).  Bounds of 640 threads twice and of 1024
+// leave 48 and 64 registers a thread, and 38 of the 48 forms spill some of what they hold (aligned fp32 of two vectors 72 bytes stored and 48 read a
+// thread, unaligned fp32 of five 680 and 296).
 //
 // The reference quantises activations per token for its FP8 products (`quant_fp8`, packages/tilerl-kernels/src/tilerl_kernels/
 // kernels_linear.py:1547-1590); it has no integer form.

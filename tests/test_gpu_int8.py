@@ -163,6 +163,44 @@ def test_products_of_all_shapes(ops, n, k):
         _check_served(ops, t, n, k, seed=n)
 
 
+@pytest.mark.parametrize("t", [1, 3, 40])
+def test_adapters_over_served_integers(ops, t):
+    n, k, r, scale = 386, 272, 8, 0.5
+    g = torch.Generator(device=DEV).manual_seed(t)
+    w, x, nw = _weight(n, k), _x(t, k), torch.rand(k, generator=g, device=DEV) + 0.5
+    a, b = torch.randn(r, k, generator=g, device=DEV) / k ** 0.5, torch.randn(n, r, generator=g, device=DEV) * 0.1
+
+    def adapter(h):
+        """What the adapter adds, and the size of all that it adds up."""
+        h, ad, bd = h.double(), a.double(), b.double()
+        return h @ ad.t() @ bd.t() * scale, h.abs() @ ad.abs().t() @ bd.abs().t() * scale
+
+    def room(y, delta, size, e):
+        # the product's error, its rounding and the sum's to bf16; the adapter's sums of k and r terms, a rounding each, in fp32
+        return (y.abs() + (y + delta).abs()) * 2.0 ** -8 * 1.01 + (y.abs() + size) * (e + (k + r + 8) * U) * 1.01
+    q, s = F._row_integers(x.float() * nw, F.INT8_MAX)
+    rstd = 1 / (x.double().square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    y = q.double() @ _ints(w).t() * (s.double()[:, None] * rstd) * w.wscale.double()
+    delta, size = adapter(x.double() * rstd * nw.double())
+    e = _norm_error(k) + 4 * U
+    out = ops.norm_linear(x, nw, w, 1e-6, (a, b, scale)).double()
+    assert ((out - y - delta).abs() <= room(y, delta, size, e)).all()
+    act = ops.norm_linear_swiglu(x, nw, w, 1e-6, (a, b, scale)).double()
+    gu, off = y + delta, room(y, delta, size, e)
+    gate, up = gu[:, 0::2], gu[:, 1::2]
+    silu = gate * torch.sigmoid(gate)
+    # silu's slope is at most 1.1; its own error in fp32 and the result's rounding
+    want = silu * up
+    bound = off[:, 0::2] * 1.1 * (up.abs() + off[:, 1::2]) + silu.abs() * off[:, 1::2] + want.abs() * (2.0 ** -8 + (16 + 2 * gate.abs()) * 2 * U)
+    assert ((act - want).abs() <= bound * 1.01 + 1e-30).all()
+    q, s = F.quantize_act_int8(x)
+    y = q.double() @ _ints(w).t() * s.double()[:, None] * w.wscale.double()
+    delta, size = adapter(x)
+    res = _x(t, n, 3)
+    out = ops.linear_residual(x, w, res.clone(), (a, b, scale)).double()
+    assert ((out - y - delta - res.double()).abs() <= room(y + res.double(), delta, size, 4 * U) + y.abs() * 4 * U).all()
+
+
 @pytest.mark.parametrize("t", [1, 4, 20, 48, 300])
 def test_one_row_has_the_same_bits_in_every_batch(ops, t):
     w, x, nw = _weight(386, 1168), _x(300, 1168), torch.rand(1168, device=DEV) + 0.5

@@ -584,3 +584,61 @@ def test_a_store_of_pages_tells_weights_apart_by_their_scales():
     a, b, c = (HybridModel.build_random(cfg) for _ in range(3))
     b.params["L0.down"].wscale.mul_(2)
     assert weights_fingerprint(a) == weights_fingerprint(c) != weights_fingerprint(b)
+
+
+def test_a_rows_largest_value_has_the_low_digit_zero():
+    """What keeps a gradient's sums of 131072 channels in 32 bits: low digits go down to -128, and so may a file's weights, but one of a row's
+    digits is 0.  For every significand, at magnitudes up to the ends of the range."""
+    m = torch.arange(1 << 23, dtype=torch.int32)
+    for e in (18, 64, 126, 127, 128, 200, 253, 254):          # (the least that counts is 2^-110)
+        v = (m + (e << 23)).view(torch.float32)
+        q, s = F._row_integers(v[:, None], F.INT16_MAX)
+        assert bool((q == 32512).all()) and bool(torch.isfinite(s).all())
+        q, _ = F._row_integers(v[:, None], F.INT8_MAX)
+        assert bool((q == 127).all())
+    assert 131071 * 128 * 128 < 2 ** 31 and 131072 * 127 * 128 < 2 ** 31
+
+
+def _tp_projections(rank, world):
+    """Of two ranks: projections cut along their channels, projections cut along K with the sum over the ranks, and an engine."""
+    import torch.distributed as dist
+    from helpers import rand_prompts
+    from tilerl_b200.engine import Engine, SamplingParams
+    from tilerl_b200.kv import GdnStatePool, PagedKvPool
+    from tilerl_b200.ops.backend import TPContext
+    cfg = _tiny("tiny-hybrid")
+    m = HybridModel.build_random(cfg, seed=1, tp_rank=rank, tp=world)
+    ops = RefOps(TPContext(rank, world, dist.group.WORLD))
+    x, nw = _rows(5, cfg.hidden, 3), torch.rand(cfg.hidden, generator=torch.Generator().manual_seed(4)) + 0.5
+    act = ops.norm_linear_swiglu(x, nw, m.params["L0.gate_up"], cfg.rms_eps)
+    out = ops.linear_residual(act, m.params["L0.down"], x)
+    d = m.dims
+    kv = PagedKvPool(cfg, 64, dtype=torch.float32, n_kv_heads=d.n_kv)
+    st = GdnStatePool(cfg, 6, ring_dtype=torch.float32, n_v_heads=d.gdn_nv, n_k_heads=d.gdn_nk)
+    eng = Engine(m, ops, kv, st)
+    return act, out, [r.tokens for r in eng.generate(rand_prompts(cfg, 2, 24), SamplingParams(max_tokens=8))]
+
+
+def test_two_ranks_serve_the_integers_of_one():
+    from helpers import rand_prompts
+    from tilerl_b200.parallel.mesh import shard_param
+    from world_helpers import run_world
+    cfg = _tiny("tiny-hybrid")
+    whole = HybridModel.build_random(cfg, seed=1)
+    x, nw = _rows(5, cfg.hidden, 3), torch.rand(cfg.hidden, generator=torch.Generator().manual_seed(4)) + 0.5
+    got = run_world(2, _tp_projections)
+    acts, outs, tokens = zip(*got)
+    act = RefOps().norm_linear_swiglu(x, nw, whole.params["L0.gate_up"], cfg.rms_eps)
+    assert torch.equal(torch.cat(acts, -1), act)
+    # each rank's rows have a scale of their own; the sum of two fp32 products and the residual
+    parts = [ref.linear_int8(a, shard_param(cfg, "L0.down", whole.params["L0.down"], r, 2)).double() for r, a in enumerate(acts)]
+    want = parts[0] + parts[1] + x.double()
+    room = (parts[0].abs() + parts[1].abs() + want.abs()) * 2 * 2.0 ** -24
+    assert torch.equal(outs[0], outs[1]) and ((outs[0].double() - want).abs() <= room).all()
+    assert tokens[0] == tokens[1]
+    for prompt, toks in zip(rand_prompts(cfg, 2, 24), tokens[0]):
+        toks = list(toks)[-8:]
+        logits = whole.forward_dense(T.Tape(), torch.tensor([list(prompt) + toks]))[0]
+        for i, t in enumerate(toks):                 # (a token chosen by chance lies some deviations below the largest)
+            row = logits[len(prompt) - 1 + i]
+            assert float(row.max() - row[t]) <= 0.2 * float(row.std()), (i, t)

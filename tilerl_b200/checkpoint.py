@@ -11,7 +11,8 @@ parameter dict (TP-sharded if asked):
 * FP8 128x128-block files: ``.weight`` e4m3 + ``.weight_scale_inv``; FP8 per-tensor / per-channel:
   ``.weight`` e4m3 + ``.weight_scale``;
 * 8-bit integers per channel: ``.weight`` int8 + ``.weight_scale`` ``[N]``, ``[N, 1]`` or one for all; a model
-  served in this format (``quant="int8"``) takes them as they are, also beside parts of a fused projection that are not;
+  served in this format (``quant="int8"``) takes them as they are, also beside parts of a fused projection that are not (int8 without its
+  scale is refused, with zero points or a scale per group too);
 * MLX 4-bit: ``.weight`` uint32 (8 nibbles, low first) + ``.scales`` + ``.biases`` per group of 64;
 * AWQ: ``.qweight`` int32 ``[K, N/8]`` (AWQ nibble order) + ``.qzeros`` + ``.scales`` per group;
 * this framework's own dialect: ``<name>.wq / .scale / .tscale`` (NVFP4), ``<name>.w8 / .wscale`` (8-bit integers).

@@ -21,7 +21,7 @@ from . import native as N
 
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU, EPI_STORE_F32 = 0, 1, 2, 3
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
-MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31
+MOST = 131072             # values that a sum of 32 bits holds: 127 * 128 times as many is below 2^31 (a gradient's low digits: csrc/gemm_i8.cu)
 
 N.register("trl_rows_i8", [N.P, N.I, N.L, N.P, N.I, N.F, N.P, N.L, N.P, N.L, N.I, N.I, N.P, N.P])
 N.register("trl_linear_i8", [N.P, N.I, N.L, N.P, N.F, N.P, N.L, N.P, N.P, N.L, N.P, N.L, N.P, N.I, N.I, N.I, N.I, N.P])
