@@ -521,6 +521,33 @@ def test_adapters_and_checkpointed_layers_over_integers():
         assert float((grads[0][k] - grads[1][k]).norm()) <= 1e-3 * float(grads[0][k].norm()) + 1e-12, k
 
 
+@pytest.mark.parametrize("trainer", [DEV, "cpu"])
+def test_weights_that_did_not_move_keep_a_files_integers(trainer):
+    """Packed again from masters and from a trainer, also one on another device, whose working type is bf16."""
+    import types
+    from tilerl_b200.config import get_config
+    from tilerl_b200.models.hybrid import HybridModel, linear_names, random_master
+    from tilerl_b200.parallel.resync import resync
+    cfg = get_config("tiny-hybrid", "int8")
+    g, master = torch.Generator().manual_seed(2), random_master(cfg, 3)
+    for n in linear_names(cfg):
+        shape = master[n].shape
+        master[n] = F.INT8Tensor(torch.randint(-100, 100, shape, generator=g, dtype=torch.int8), torch.rand(shape[0], generator=g) * 1e-3 + 1e-5)
+    m = HybridModel.from_master(cfg, master, device=DEV, keep_master=True)
+    at = {n: m.params[n].w8.data_ptr() for n in linear_names(cfg)}
+    weights = {n: w.to(trainer, torch.bfloat16) for n, w in m.params.items() if n.startswith("master.")}
+    zero = types.SimpleNamespace(units=[0], unit_tensors=lambda i: weights, _prefetch=None, _drop=lambda u: None, device=torch.device("cpu"))
+    for pack in (m.requantize_, lambda: resync(zero, m)):
+        pack()
+        for n in linear_names(cfg):
+            assert torch.equal(m.params[n].w8.cpu(), master[n].w8) and torch.equal(m.params[n].wscale.cpu(), master[n].wscale) and m.params[n].w8.data_ptr() == at[n]
+    weights["master.L0.down"][1] *= 3
+    resync(zero, m)
+    want = F.quantize_int8(weights["master.L0.down"].float())
+    got = m.params["L0.down"]
+    assert torch.equal(got.w8[1].cpu(), want.w8[1].cpu()) and torch.equal(got.wscale[1].cpu(), want.wscale[1].cpu()) and torch.equal(got.w8[2].cpu(), master["L0.down"].w8[2])
+
+
 # ---- streams, graphs -----------------------------------------------------------------------------------------
 def test_captured_and_replayed(ops):
     """Two captured products that share the backend's workspace, replayed one after the other over new rows; and a training pass."""

@@ -69,7 +69,7 @@ def resync(zero, rollout, *, quantize: Optional[Callable] = None, refresh: Optio
                     if refresh is not None:
                         refresh(dst)
                 elif base in lin and isinstance(dst, INT8Tensor):
-                    new, part = (shard_param(cfg, base, t, rollout.tp_rank, rollout.tp) for t in (quantize_int8(w.float()), w))
+                    new, part = (shard_param(cfg, base, t, rollout.tp_rank, rollout.tp).to(dst.w8.device) for t in (quantize_int8(w.float()), w))
                     nbytes += _store(dst, keep_int8(new, dst, part))
                 else:
                     src = shard_param(cfg, base, w, rollout.tp_rank, rollout.tp)
