@@ -336,7 +336,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
         uint32_t r[32];
-        constexpr bool EARLY = BN <= 128;            // (wider tiles read it where it is added: the other accumulator's MMAs hide the wait behind long sums; behind sums of a few stages nothing does)
+        // (wider tiles read the residual where it is added: behind long sums the other accumulator's MMAs hide that wait, behind a few stages nothing does)
+        constexpr bool EARLY = BN <= 128;
         uint4 res[TOK / 8];
         if (!GRAD && !SPLIT && EARLY && p.epi == I8_RESIDUAL && p.vec) {
 #pragma unroll
