@@ -543,6 +543,12 @@ def test_merges_go_by_what_the_integers_stand_for(tmp_path, dialect):
     assert ((q.dequant().double() - want).abs() <= step * (0.5 + 127 * 6 * 2.0 ** -24) + size * 8 * 2.0 ** -24).all()
     assert torch.equal(q.w8[2], files[0].w8[2]) and q.wscale[2] == 0.25
     assert torch.equal(got["norm"], torch.full((4,), 1.5))
+    if dialect == "export":                          # a dense base, tuned checkpoints in integers
+        (tmp_path / "dense").mkdir()
+        save_file({w8: dense[0]}, str(tmp_path / "dense" / "model.safetensors"))
+        merge_checkpoints(str(tmp_path / "dense"), [str(tmp_path / "1"), str(tmp_path / "2")], str(tmp_path / "out"))
+        got = load_file(str(tmp_path / "out" / "model.safetensors"))[w8]
+        assert ((got.double() - want).abs() <= (size + dense[0].double().abs()) * 8 * 2.0 ** -24).all()
     (tmp_path / "other").mkdir()
     save_file({"norm": torch.zeros(4)}, str(tmp_path / "other" / "model.safetensors"))
     merge_checkpoints(str(tmp_path / "0"), [str(tmp_path / "other")], str(tmp_path / "out"))

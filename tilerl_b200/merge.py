@@ -74,6 +74,10 @@ def _int8(f, name: str, scale: str) -> INT8Tensor:
     return INT8Tensor(w, f.get_tensor(scale).float().reshape(-1).expand(w.shape[0]).contiguous())
 
 
+def _dense(f, name: str, integers: Dict[str, str]) -> torch.Tensor:
+    return _int8(f, name, integers[name]).dequant() if name in integers else f.get_tensor(name).float()
+
+
 def merge_checkpoints(base: str, tuned: List[str], out: str, method: str = "average", **kw) -> int:
     """Stream safetensors files: ``out = base + merge(tuned_i - base)`` per tensor; projections in 8-bit integers by what they stand for."""
     from safetensors import safe_open
@@ -82,7 +86,7 @@ def merge_checkpoints(base: str, tuned: List[str], out: str, method: str = "aver
     f_base = safe_open(os.path.join(base, "model.safetensors"), framework="pt")
     f_tuned = [safe_open(os.path.join(t, "model.safetensors"), framework="pt") for t in tuned]
     result: Dict[str, torch.Tensor] = {}
-    integers = _integers(f_base)
+    integers, tuned_integers = _integers(f_base), [_integers(f) for f in f_tuned]
     scales = set(integers.values())
     for name in f_base.keys():
         if name in scales:
@@ -91,7 +95,7 @@ def merge_checkpoints(base: str, tuned: List[str], out: str, method: str = "aver
         if name in integers:              # neither the integers nor the scales have deltas of their own
             scale = integers[name]
             result[name], result[scale] = b, f_base.get_tensor(scale)
-            if all(name in f.keys() and scale in f.keys() for f in f_tuned):
+            if all(name in i for i in tuned_integers):
                 base_q = _int8(f_base, name, scale)
                 dense = base_q.dequant()
                 merged = dense + fn([_int8(f, name, scale).dequant() - dense for f in f_tuned], **kw)
@@ -101,7 +105,7 @@ def merge_checkpoints(base: str, tuned: List[str], out: str, method: str = "aver
         if not b.dtype.is_floating_point or b.dtype == torch.float8_e4m3fn or any(name not in f.keys() for f in f_tuned):
             result[name] = b
             continue
-        deltas = [f.get_tensor(name).float() - b.float() for f in f_tuned]
+        deltas = [_dense(f, name, i) - b.float() for f, i in zip(f_tuned, tuned_integers)]
         result[name] = (b.float() + fn(deltas, **kw)).to(b.dtype)
     os.makedirs(out, exist_ok=True)
     save_file(result, os.path.join(out, "model.safetensors"))
